@@ -545,6 +545,66 @@ struct GqaArgs {
     uint32_t st_pad;
 };
 
+// ---- a ragged batch's rows (ragged_ops.hip, rows_matmul.hip, paged_attention_rows.hip) ----
+#define CTOX_NO_SLOT 0xffffffffu
+#define CTOX_ROPE_MAX_PAIRS 256
+// Per-head RMS norm and rotary positions on several axes.
+struct RopeAxesArgs {
+    const float *in[2];      // q, k: row t, head h at t * in_row + h * in_head floats
+    float *out[2];
+    const float *norm[2];    // NULL or [hd]: (1 + w) RMS norm first
+    const uint32_t *positions;  // [rows][axes]
+    const uint32_t *row_count;  // NULL, or rows past *row_count are left alone
+    uint64_t in_row[2], in_head[2], out_row[2], out_head[2];
+    uint32_t rows;
+    uint32_t heads[2];
+    uint32_t hd;
+    uint32_t rd;
+    uint32_t axes;
+    uint32_t heads_per_wg;   // consecutive heads (q heads, then k heads) of one workgroup
+    float eps;
+    double turns[CTOX_ROPE_MAX_PAIRS];  // pair i: theta^(-2 i / rd) / (2 pi), turns per position
+    uint8_t axis[CTOX_ROPE_MAX_PAIRS];
+};
+
+// Page descriptors and slot map of a batch's new tokens.
+#define CTOX_PLAN_REQUESTS 4096
+#define CTOX_PLAN_THREADS 512
+struct PagedPlanArgs {
+    const uint32_t *cached;  // [requests]
+    const uint32_t *added;   // [requests]
+    PagedKvDesc *desc;       // [requests][max_pages]
+    const uint32_t *free_slots;
+    uint32_t *row_starts;    // [requests + 1]
+    uint32_t *tokens;        // [requests]
+    uint32_t *page_counts;   // [requests]
+    uint32_t *positions;     // [max_rows]
+    uint32_t *slots;         // [max_rows]
+    uint32_t *status;        // [4]
+    uint32_t requests;
+    uint32_t page_tokens;
+    uint32_t max_pages;
+    uint32_t free_count;
+    uint32_t q4_slots;
+    uint32_t max_rows;
+};
+
+struct KvAppendArgs {
+    uint8_t *q4_pages;
+    const float *keys;
+    const float *values;
+    const uint32_t *slots;   // [rows]: Q4 slot * page_tokens + token in page, or CTOX_NO_SLOT
+    uint64_t key_stride;     // floats between rows
+    uint64_t value_stride;
+    uint64_t q4_page_bytes;
+    uint32_t rows;
+    uint32_t component_values;
+    uint32_t page_tokens;
+    uint32_t slot_limit;     // q4 slots * page_tokens
+    uint32_t rows_per_wg;
+    uint32_t vec;            // rows and strides allow 16-byte loads
+};
+
 // Decode engine helpers (engine_ops.hip).
 struct FillArgs {
     void *ptr;

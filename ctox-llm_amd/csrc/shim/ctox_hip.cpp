@@ -152,7 +152,7 @@ struct ctox_hip_backend {
                   gqa_combine = nullptr, fill = nullptr, embed = nullptr, norm_rows = nullptr, attn_gate = nullptr,
                   swiglu_rows = nullptr, copy_rows = nullptr, write_words = nullptr, norm_prep = nullptr,
                   prep_x = nullptr, finite = nullptr, gather = nullptr, topk_part = nullptr, topk_final = nullptr, stream_read = nullptr,
-                  write_segments = nullptr;
+                  write_segments = nullptr, rope_axes[2] = {}, plan = nullptr, kv_append = nullptr;
     // Batch-1 slice kernels per dtype [Q2, Q4]: [0] walks the slices, [n]
     // requests all n slices up front (n <= 3: more slices up front measured
     // slower than walking them).
@@ -938,7 +938,9 @@ extern "C" ctox_status ctox_hip_backend_create(int device, ctox_hip_backend **ou
                {&b->gdn_k4[1][0], "ctox_gdn_fused1_k4_gfx950"}, {&b->gdn_k4[1][1], "ctox_gdn_fused1_blk_k4_gfx950"},
                {&b->finite, "ctox_finite_check_gfx950"}, {&b->gather, "ctox_gather_rows_gfx950"}, {&b->stream_read, "ctox_stream_read_gfx950"},
                {&b->write_segments, "ctox_write_segments_gfx950"},
-               {&b->topk_part, "ctox_topk_part_gfx950"}, {&b->topk_final, "ctox_topk_final_gfx950"}};
+               {&b->topk_part, "ctox_topk_part_gfx950"}, {&b->topk_final, "ctox_topk_final_gfx950"},
+               {&b->rope_axes[0], "ctox_rope_axes_gfx950"}, {&b->rope_axes[1], "ctox_rope_axes_any_gfx950"},
+               {&b->plan, "ctox_paged_plan_gfx950"}, {&b->kv_append, "ctox_kv_append_q4_gfx950"}};
     for (auto &f : fns) {
         if (le != hipSuccess) break;
         le = hipModuleGetFunction(f.f, b->module, f.name);
@@ -2630,4 +2632,150 @@ extern "C" ctox_status ctox_hip_write_words_device(ctox_hip_backend *b, uint32_t
         if (st) return st;
     }
     return CTOX_OK;
+}
+
+// ======================================================================
+// a ragged batch's rows
+// ======================================================================
+namespace {
+// The backend's device made current for one call; the caller's is restored.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(const ctox_hip_backend *b) {
+        int d = 0;
+        if (hipGetDevice(&d) == hipSuccess && d != b->device && hipSetDevice(b->device) == hipSuccess) before = d;
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+bool aligned(const void *p, size_t n) { return (uintptr_t)p % n == 0; }
+
+// rows * stride + the last row, in values: within what 63 bits address.
+bool spans(uint64_t rows, uint64_t stride) { return stride < (1ull << 30) && rows < (1ull << 32); }
+}  // namespace
+
+extern "C" ctox_status ctox_hip_rope_axes_device(ctox_hip_backend *b, const ctox_rope_axes *op, void *stream) {
+    if (!op) return fail(CTOX_ERR_SHAPE, "null argument");
+    const uint32_t hd = op->head_dim, rd = op->rotary_dim;
+    // Q/src/reference.rs:115-155: the rotary dimension is even, non-zero and within the head.
+    if (rd == 0 || rd % 2 || rd > hd || rd > 2 * CTOX_ROPE_MAX_PAIRS || !std::isfinite(op->theta) || !(op->theta > 0.0f))
+        return fail(CTOX_ERR_SHAPE, "rotary dimension or theta is invalid");
+    if (hd > 1024 || op->axes == 0 || op->axes > 4 || op->q_heads > 32767 || op->k_heads > 32767 ||
+        op->q_heads + op->k_heads == 0)
+        return fail(CTOX_ERR_SHAPE, "rope heads or axes are empty or too large");
+    if ((op->q_norm || op->k_norm) && (!std::isfinite(op->eps) || !(op->eps > 0.0f)))
+        return fail(CTOX_ERR_SHAPE, "norm epsilon is invalid");
+    for (uint32_t i = 0; op->axis_of_pair && i < rd / 2; i++)
+        if (op->axis_of_pair[i] >= op->axes)
+            return fail(CTOX_ERR_SHAPE, "pair %u turns by axis %u of %u", i, op->axis_of_pair[i], op->axes);
+    const uint64_t rs[4] = {op->q_row_stride, op->k_row_stride, op->q_out_row_stride, op->k_out_row_stride};
+    const uint64_t hs[4] = {op->q_head_stride, op->k_head_stride, op->q_out_head_stride, op->k_out_head_stride};
+    const void *ptr[4] = {op->q, op->k, op->q_out, op->k_out};
+    bool vec = hd <= 256 && hd % 4 == 0 && rd % 8 == 0 && (!op->q_norm || aligned(op->q_norm, 16)) &&
+               (!op->k_norm || aligned(op->k_norm, 16));
+    for (int i = 0; i < 4; i++) {
+        const uint32_t heads = i % 2 ? op->k_heads : op->q_heads;
+        if (!heads) continue;
+        if (!ptr[i]) return fail(CTOX_ERR_SHAPE, "null argument");
+        if (!spans(op->rows, rs[i]) || !spans(heads, hs[i])) return fail(CTOX_ERR_SHAPE, "rope stride is too large");
+        // Outputs of two heads or rows must not meet: a row's heads lie within the row stride, or a head's
+        // rows within the head stride.
+        const uint64_t rows = std::max<uint64_t>(op->rows, 1);
+        const bool by_row = (heads == 1 || hs[i] >= hd) && (rows == 1 || rs[i] >= (heads - 1) * hs[i] + hd);
+        const bool by_head = (rows == 1 || rs[i] >= hd) && (heads == 1 || hs[i] >= (rows - 1) * rs[i] + hd);
+        if (i >= 2 && !by_row && !by_head) return fail(CTOX_ERR_SHAPE, "rope output rows or heads overlap");
+        if (i >= 2 && ptr[i] == ptr[i - 2] && (rs[i] != rs[i - 2] || hs[i] != hs[i - 2]))
+            return fail(CTOX_ERR_SHAPE, "rope in place needs equal strides");
+        vec = vec && aligned(ptr[i], 16) && rs[i] % 4 == 0 && hs[i] % 4 == 0;
+    }
+    if (!b || !op->positions) return fail(CTOX_ERR_SHAPE, "null argument");
+    if (op->rows == 0) return CTOX_OK;
+    RopeAxesArgs a{};
+    for (int i = 0; i < 2; i++) {
+        a.in[i] = (const float *)ptr[i];
+        a.out[i] = (float *)ptr[i + 2];
+        a.norm[i] = i ? op->k_norm : op->q_norm;
+        a.in_row[i] = rs[i];
+        a.in_head[i] = hs[i];
+        a.out_row[i] = rs[i + 2];
+        a.out_head[i] = hs[i + 2];
+        a.heads[i] = i ? op->k_heads : op->q_heads;
+    }
+    a.positions = op->positions;
+    a.row_count = op->row_count;
+    a.rows = op->rows;
+    a.hd = hd;
+    a.rd = rd;
+    a.axes = op->axes;
+    a.eps = op->eps;
+    for (uint32_t i = 0; i < rd / 2; i++) {
+        a.turns[i] = std::pow((double)op->theta, -2.0 * i / rd) / 6.283185307179586476925;
+        a.axis[i] = op->axis_of_pair ? op->axis_of_pair[i] : 0;
+    }
+    // A few rows are spread over the CUs by heads, four (one a wave) to a workgroup at least.
+    const uint32_t heads = op->q_heads + op->k_heads, want = std::max<uint32_t>(1, 512 / op->rows);
+    a.heads_per_wg = std::max<uint32_t>(4, (heads + want - 1) / want);
+    OnDevice on(b);
+    return launch(b->rope_axes[vec ? 0 : 1], dim3(op->rows, (heads + a.heads_per_wg - 1) / a.heads_per_wg), dim3(256),
+                  (hipStream_t)stream, a, "ctox_rope_axes_gfx950");
+}
+
+extern "C" ctox_status ctox_hip_paged_plan_device(ctox_hip_backend *b, const ctox_paged_plan *op, void *stream) {
+    if (!op) return fail(CTOX_ERR_SHAPE, "null argument");
+    if (op->requests == 0 || op->requests > CTOX_PLAN_REQUESTS)
+        return fail(CTOX_ERR_SHAPE, "plan of %u requests outside 1..%d", op->requests, CTOX_PLAN_REQUESTS);
+    if (op->page_tokens == 0 || op->max_pages == 0 || (uint64_t)op->max_pages * op->page_tokens > 0xffffffffull ||
+        (uint64_t)op->q4_slots * op->page_tokens > 0xffffffffull ||
+        (uint64_t)op->requests * op->max_pages > 0xffffffffull || op->max_rows > 0x7fffffffu)
+        return fail(CTOX_ERR_SHAPE, "plan geometry is empty or too large");
+    if (!b || !op->cached || !op->added || !op->descriptors || (op->free_count && !op->free_slots) || !op->row_starts ||
+        !op->tokens || !op->page_counts || !op->status || (op->max_rows && (!op->positions || !op->slots)))
+        return fail(CTOX_ERR_SHAPE, "null argument");
+    if (!aligned(op->descriptors, 16)) return fail(CTOX_ERR_SHAPE, "descriptors need 16-byte alignment");
+    PagedPlanArgs a{op->cached, op->added, (PagedKvDesc *)op->descriptors, op->free_slots, op->row_starts, op->tokens,
+                    op->page_counts, op->positions, op->slots, op->status, op->requests, op->page_tokens,
+                    op->max_pages, op->free_count, op->q4_slots, op->max_rows};
+    const uint32_t most = std::max(op->requests, op->max_rows);
+    const uint32_t wgs = std::min<uint32_t>((uint32_t)b->cus, (most + CTOX_PLAN_THREADS - 1) / CTOX_PLAN_THREADS);
+    OnDevice on(b);
+    return launch(b->plan, dim3(std::max<uint32_t>(1, wgs)), dim3(CTOX_PLAN_THREADS), (hipStream_t)stream, a,
+                  "ctox_paged_plan_gfx950");
+}
+
+extern "C" ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *b, uint8_t *d_q4_pages, const float *d_keys,
+                                                    size_t key_stride, const float *d_values, size_t value_stride,
+                                                    const uint32_t *d_slots, size_t rows, size_t component_values,
+                                                    uint32_t page_tokens, uint32_t q4_slots, uint32_t q4_page_bytes,
+                                                    void *stream) {
+    // Q/src/kv_cache.rs:238-252: a non-zero multiple of 64 values per component.
+    if (component_values == 0 || component_values % 64 || component_values > (1u << 24))
+        return fail(CTOX_ERR_SHAPE, "KV component width must be a non-zero multiple of 64");
+    const uint64_t token_bytes = component_values * 2 / 64 * 34;
+    if (page_tokens == 0 || page_tokens * token_bytes > q4_page_bytes || q4_page_bytes % 4 ||
+        (uint64_t)q4_slots * page_tokens > 0xffffffffull)
+        return fail(CTOX_ERR_SHAPE, "KV tokens do not fit the Q4 page");
+    if (rows > 0x7fffffffu || !spans(rows, key_stride) || !spans(rows, value_stride))
+        return fail(CTOX_ERR_SHAPE, "KV append is too large");
+    if (!b || !d_q4_pages || !d_keys || !d_values || !d_slots) return fail(CTOX_ERR_SHAPE, "null argument");
+    if (!aligned(d_q4_pages, 4)) return fail(CTOX_ERR_SHAPE, "the Q4 pool needs 4-byte alignment");
+    if (rows == 0) return CTOX_OK;
+    KvAppendArgs a{};
+    a.q4_pages = d_q4_pages;
+    a.keys = d_keys;
+    a.values = d_values;
+    a.slots = d_slots;
+    a.key_stride = key_stride;
+    a.value_stride = value_stride;
+    a.q4_page_bytes = q4_page_bytes;
+    a.rows = (uint32_t)rows;
+    a.component_values = (uint32_t)component_values;
+    a.page_tokens = page_tokens;
+    a.slot_limit = q4_slots * page_tokens;
+    a.rows_per_wg = std::max<uint32_t>(1, (uint32_t)(256 / (component_values / 4)));
+    a.vec = aligned(d_keys, 16) && aligned(d_values, 16) && key_stride % 4 == 0 && value_stride % 4 == 0;
+    OnDevice on(b);
+    return launch(b->kv_append, dim3((unsigned)((rows + a.rows_per_wg - 1) / a.rows_per_wg)), dim3(256),
+                  (hipStream_t)stream, a, "ctox_kv_append_q4_gfx950");
 }

@@ -199,6 +199,51 @@ class PagedGqaParams(ctypes.Structure):
         "q2_token_bytes", "q4_token_bytes", "q2_page_bytes", "q4_page_bytes")] + [("scale", ctypes.c_float)]
 
 
+
+class RopeAxes(ctypes.Structure):
+    """ctox_rope_axes. Strides are (row, head) in values; outputs are dense unless given,
+    axis_of_pair a sequence of rotary_dim / 2 axis numbers (None: all 0)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "q", "k", "q_out", "k_out", "q_norm", "k_norm", "positions", "row_count", "axis_of_pair")] + [
+        (f"{t}_{n}_stride", ctypes.c_uint64) for t in ("q", "k", "q_out", "k_out") for n in ("row", "head")] + [
+        (n, ctypes.c_uint32) for n in ("rows", "q_heads", "k_heads", "head_dim", "rotary_dim", "axes")] + [
+        ("theta", ctypes.c_float), ("eps", ctypes.c_float)]
+
+    def __init__(self, d_q, d_positions, rows, q_heads, head_dim, rotary_dim, theta, d_k=None, d_q_out=None,
+                 d_k_out=None, d_q_norm=None, d_k_norm=None, d_row_count=None, axis_of_pair=None, q_strides=None,
+                 k_strides=None, q_out_strides=None, k_out_strides=None, k_heads=0, axes=1, eps=1e-6):
+        self._axis = None
+        if axis_of_pair is not None:
+            if len(axis_of_pair) != rotary_dim // 2:
+                raise ShapeError("axis_of_pair needs one axis per rotary pair")
+            self._axis = (ctypes.c_uint8 * max(1, len(axis_of_pair)))(*axis_of_pair)
+        dense_q, dense_k = (q_heads * head_dim, head_dim), (k_heads * head_dim, head_dim)
+        q_strides, k_strides = q_strides or dense_q, k_strides or dense_k
+        # In place where no output is given.
+        q_out_strides = q_out_strides or (q_strides if d_q_out in (None, d_q) else dense_q)
+        k_out_strides = k_out_strides or (k_strides if d_k_out in (None, d_k) else dense_k)
+        super().__init__(d_q, d_k, d_q_out or d_q, d_k_out or d_k, d_q_norm, d_k_norm, d_positions, d_row_count,
+                         None if self._axis is None else ctypes.addressof(self._axis), *q_strides, *k_strides,
+                         *q_out_strides, *k_out_strides, rows, q_heads, k_heads, head_dim, rotary_dim, axes, theta, eps)
+
+
+NO_SLOT = 0xffffffff
+
+
+class PagedPlan(ctypes.Structure):
+    """ctox_paged_plan (all pointers are device addresses)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "cached", "added", "descriptors", "free_slots", "row_starts", "tokens", "page_counts", "positions", "slots",
+        "status")] + [(n, ctypes.c_uint32) for n in (
+            "requests", "page_tokens", "max_pages", "free_count", "q4_slots", "max_rows")]
+
+    def __init__(self, d_cached, d_added, d_descriptors, d_free_slots, d_row_starts, d_tokens, d_page_counts,
+                 d_positions, d_slots, d_status, requests, page_tokens, max_pages, free_count, q4_slots, max_rows):
+        super().__init__(d_cached, d_added, d_descriptors, d_free_slots, d_row_starts, d_tokens, d_page_counts,
+                         d_positions, d_slots, d_status, requests, page_tokens, max_pages, free_count, q4_slots,
+                         max_rows)
+
+
 # Every symbol include/ctox_hip.h declares: name -> (restype, argtypes).
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
@@ -261,6 +306,9 @@ SIGNATURES = {
                                          ctypes.c_float, _P, _U32, _P, _P, _P, _P, _P, _SZ, _P]),
     "ctox_hip_kv_demote_device": (_I32, [_P, _P, _P, _SZ, _SZ, _P]),
     "ctox_hip_paged_gqa_device": (_I32, [_P, _P, _P, _P, _P, ctypes.POINTER(PagedGqaParams), _SZ, _P, _P]),
+    "ctox_hip_rope_axes_device": (_I32, [_P, ctypes.POINTER(RopeAxes), _P]),
+    "ctox_hip_paged_plan_device": (_I32, [_P, ctypes.POINTER(PagedPlan), _P]),
+    "ctox_hip_kv_append_q4_device": (_I32, [_P, _P, _P, _SZ, _P, _SZ, _P, _SZ, _SZ, _U32, _U32, _U32, _P]),
     "ctox_hip_fill_random_device": (_I32, [_P, _P, ctypes.c_uint64, _U32, ctypes.c_uint64, ctypes.c_float,
                                            ctypes.c_float, _P]),
     "ctox_hip_embedding_rows_device": (_I32, [_P, _I32, _P, _P, _P, _P, _SZ, _SZ, _SZ, _P, _P]),
@@ -628,6 +676,25 @@ class HipBackend:
         """Q/src/reference.rs:420-499 over the paged cache."""
         _check(load_library().ctox_hip_paged_gqa_device(self.handle, d_query, d_q2_pages, d_q4_pages, d_descriptors,
                                                         ctypes.byref(params), rows, d_out, stream))
+
+    # ---- a ragged batch's rows (device pointers) ----
+    def rope_axes_device(self, op: RopeAxes, stream: Optional[int] = None) -> None:
+        """Optional per-head RMS norm, then rotary positions on several axes (Q/src/reference.rs:38-62, :115-155)."""
+        _check(load_library().ctox_hip_rope_axes_device(self.handle, ctypes.byref(op), stream))
+
+    def paged_plan_device(self, op: PagedPlan, stream: Optional[int] = None) -> None:
+        """Page descriptors and slot map of a batch's new tokens (Q/src/kv_cache.rs:394-429 for many requests)."""
+        _check(load_library().ctox_hip_paged_plan_device(self.handle, ctypes.byref(op), stream))
+
+    def kv_append_q4_device(self, d_q4_pages: int, d_keys: int, d_values: int, d_slots: int, rows: int,
+                            component_values: int, page_tokens: int, q4_slots: int, q4_page_bytes: int,
+                            key_stride: Optional[int] = None, value_stride: Optional[int] = None,
+                            stream: Optional[int] = None) -> None:
+        """K / V rows into the Q4 slots of a slot map (Q/src/kv_cache.rs:200-206 on the device)."""
+        _check(load_library().ctox_hip_kv_append_q4_device(
+            self.handle, d_q4_pages, d_keys, component_values if key_stride is None else key_stride, d_values,
+            component_values if value_stride is None else value_stride, d_slots, rows, component_values, page_tokens,
+            q4_slots, q4_page_bytes, stream))
 
     def synchronize(self) -> None:
         _check(load_library().ctox_hip_synchronize(self.handle))

@@ -585,6 +585,86 @@ ctox_status ctox_hip_paged_gqa_device(ctox_hip_backend *backend, const float *d_
                                       const ctox_paged_gqa_params *params, size_t query_tokens, float *d_out,
                                       void *stream);
 
+/* ---- a ragged batch's rows (device buffers) ----
+ * What a step of many requests with any number of new tokens each (prompt
+ * chunks, decoded tokens, draft rows) needs around its layers, where the
+ * entry points above take one sequence or at most eight rows. The rows of
+ * all requests lie one behind the other: request r has the rows
+ * row_starts[r] .. row_starts[r + 1] - 1. These calls allocate nothing, keep
+ * nothing between calls, never wait on the host and use no scratch of the
+ * backend (where one needs a workspace the caller gives it), so they may be
+ * captured into a graph and calls with different buffers may overlap. They
+ * run on the backend's device whichever device is current. */
+
+/* Per-head (1 + w) RMS norm (Q/src/reference.rs:38-62, where its weight is
+ * given) and rotary positions on up to 4 axes: for i < rotary_dim / 2 the
+ * pair (x[i], x[i + rotary_dim / 2]) turns by
+ * positions[t][axis_of_pair[i]] * theta^(-2 i / rotary_dim)
+ * (apply_partial_rope, Q/src/reference.rs:115-155, is the case of one axis;
+ * time / height / width sections, in blocks or interleaved, are tables of
+ * axis_of_pair). The angle is formed in 64 bits, so positions of any size
+ * keep a 32-bit result. Row t, head h starts at t * row_stride +
+ * h * head_stride values; an output may be its own input (same strides) and
+ * otherwise must not overlap an input. head_dim <= 1024, rotary_dim even and
+ * <= min(head_dim, 512). Rows from *row_count on (where it is given) are
+ * left as they are. */
+typedef struct {
+    const float *q, *k;            /* k may be NULL with k_heads = 0 */
+    float *q_out, *k_out;
+    const float *q_norm, *k_norm;  /* [head_dim] or NULL: no norm */
+    const uint32_t *positions;     /* [rows][axes] */
+    const uint32_t *row_count;     /* device word (e.g. a plan's row_starts[requests]) or NULL */
+    const uint8_t *axis_of_pair;   /* HOST [rotary_dim / 2], copied by the call; NULL: all axis 0 */
+    uint64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride;
+    uint64_t q_out_row_stride, q_out_head_stride, k_out_row_stride, k_out_head_stride;
+    uint32_t rows, q_heads, k_heads, head_dim, rotary_dim, axes;
+    float theta, eps;
+} ctox_rope_axes;
+ctox_status ctox_hip_rope_axes_device(ctox_hip_backend *backend, const ctox_rope_axes *op, void *stream);
+
+/* Page descriptors and slot map of a batch's new tokens, made on the device
+ * from the requests' lengths: PagedKvCache::push's bookkeeping
+ * (Q/src/kv_cache.rs:394-429) for many requests at once. Request r holds
+ * cached[r] tokens in the pages descriptors[r][0 ..] and gets added[r] more
+ * (0 is allowed): its last page is filled up, then free_slots are taken from
+ * the front, in the order of requests and pages. Written:
+ *   row_starts[requests + 1]  where each request's new rows start; the total
+ *   tokens[requests]          cached + added
+ *   page_counts[requests]     pages of tokens[r]
+ *   positions[max_rows]       a new row's position in its request (entries
+ *                             past the total are left as they are)
+ *   slots[max_rows]           a new row's Q4 slot * page_tokens + its token in
+ *                             the page; CTOX_NO_SLOT past the total
+ *   descriptors               tokens of a filled-up page, the new pages
+ *   status[4]                 code, slots taken, rows, pages of all requests
+ * A batch that cannot be placed leaves the descriptors as they are and has
+ * no rows (row_starts 0, slots CTOX_NO_SLOT, tokens = cached); status[0] says why:
+ * 1 a request exceeds max_pages, 2 more than max_rows rows, 3 too few free
+ * slots, 4 a page to be filled up is not a Q4 page of that request, 5 a free slot
+ * is past q4_slots. No output may overlap an input. requests <= 4096,
+ * max_pages * page_tokens and q4_slots * page_tokens below 2^32. Free slots
+ * must differ from each other and from those in use. */
+#define CTOX_NO_SLOT 0xffffffffu
+typedef struct {
+    const uint32_t *cached, *added;          /* [requests] */
+    ctox_paged_kv_descriptor *descriptors;   /* [requests][max_pages] */
+    const uint32_t *free_slots;              /* [free_count], may be NULL with free_count = 0 */
+    uint32_t *row_starts, *tokens, *page_counts, *positions, *slots, *status;
+    uint32_t requests, page_tokens, max_pages, free_count, q4_slots, max_rows;
+} ctox_paged_plan;
+ctox_status ctox_hip_paged_plan_device(ctox_hip_backend *backend, const ctox_paged_plan *op, void *stream);
+
+/* ctox_hip_kv_pack_q4_device through a slot map: row t of K and V (key_stride
+ * / value_stride values apart, component_values each) goes to token
+ * slots[t] % page_tokens of Q4 page slots[t] / page_tokens (the page of
+ * q4_page_bytes at that slot of the pool). Rows whose slot is not below
+ * q4_slots * page_tokens (CTOX_NO_SLOT) are skipped. Two rows must not share a
+ * slot. */
+ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *backend, uint8_t *d_q4_pages, const float *d_keys,
+                                         size_t key_stride, const float *d_values, size_t value_stride,
+                                         const uint32_t *d_slots, size_t rows, size_t component_values,
+                                         uint32_t page_tokens, uint32_t q4_slots, uint32_t q4_page_bytes, void *stream);
+
 /* ---- decode engine helpers (device buffers) ---- */
 /* Seeded synthetic tensors (counter-based, reproducible for any sub-range):
  * kind 0 Q4_B64 blocks and 1 Q2_B64 blocks (uniform codes, fp16 scale

@@ -1,0 +1,93 @@
+"""Refusals of the ragged-batch entry points. Every check of an argument runs
+before the backend handle is read, so all of them are reached without a GPU:
+the calls pass no backend, and a call that is in order ends at that."""
+import ctypes
+
+import pytest
+
+import ctox_hip
+from ctox_hip import PagedPlan, RopeAxes
+
+P = 0x10000  # an address that no check reads
+
+
+def call(name, *args):
+    lib = ctox_hip.load_library()
+    with pytest.raises(ctox_hip.ShapeError) as e:
+        ctox_hip._check(getattr(lib, name)(None, *args))
+    return str(e.value)
+
+
+def rope(**over):
+    kw = dict(d_q=P, d_positions=P, rows=3, q_heads=4, head_dim=256, rotary_dim=64, theta=1e7, d_k=P, k_heads=2,
+              d_q_norm=P, d_k_norm=P)
+    kw.update(over)
+    return call("ctox_hip_rope_axes_device", ctypes.byref(RopeAxes(**kw)), None)
+
+
+def test_rope_axes_in_order_without_a_backend():
+    assert rope() == "null argument"
+    assert rope(axis_of_pair=[0, 1] * 16, axes=2) == "null argument"
+    assert rope(d_k=None, k_heads=0, d_k_norm=None) == "null argument"
+    # heads outermost: [heads][rows][head_dim]
+    assert rope(q_out_strides=(256, 3 * 256), d_q_out=2 * P) == "null argument"
+
+
+@pytest.mark.parametrize("over,says", [
+    (dict(rotary_dim=0), "rotary"), (dict(rotary_dim=63), "rotary"), (dict(rotary_dim=258), "rotary"),
+    (dict(head_dim=1024, rotary_dim=514), "rotary"), (dict(theta=0.0), "theta"), (dict(theta=float("nan")), "theta"),
+    (dict(head_dim=1028), "heads or axes"), (dict(axes=0), "heads or axes"), (dict(axes=5), "heads or axes"),
+    (dict(q_heads=0, k_heads=0), "heads or axes"), (dict(eps=0.0), "epsilon"), (dict(eps=float("inf")), "epsilon"),
+    (dict(axis_of_pair=[0] * 31 + [1]), "axis 1 of 1"), (dict(d_q=None), "null"), (dict(d_k=None), "null"),
+    (dict(q_strides=(1 << 30, 256)), "stride"), (dict(d_q_out=2 * P, q_out_strides=(1024, 255)), "overlap"),
+    (dict(d_q_out=2 * P, q_out_strides=(256, 256)), "overlap"),
+    (dict(d_q_out=P, q_strides=(2048, 512), q_out_strides=(1024, 256)), "in place"),
+])
+def test_rope_axes_refuses(over, says):
+    assert says in rope(**over)
+
+
+def plan(**over):
+    kw = {f"d_{n}": P for n in ("cached", "added", "descriptors", "free_slots", "row_starts", "tokens", "page_counts",
+                                "positions", "slots", "status")}
+    kw.update(requests=3, page_tokens=16, max_pages=8, free_count=5, q4_slots=40, max_rows=64)
+    kw.update(over)
+    return call("ctox_hip_paged_plan_device", ctypes.byref(PagedPlan(**kw)), None)
+
+
+def test_plan_in_order_without_a_backend():
+    assert plan() == "null argument"
+
+
+@pytest.mark.parametrize("over,says", [
+    (dict(requests=0), "requests"), (dict(requests=4097), "requests"), (dict(page_tokens=0), "geometry"),
+    (dict(max_pages=0), "geometry"), (dict(max_pages=1 << 28), "geometry"), (dict(q4_slots=1 << 28), "geometry"),
+    (dict(requests=4096, max_pages=1 << 20, page_tokens=1), "geometry"), (dict(max_rows=1 << 31), "geometry"),
+])
+def test_plan_refuses(over, says):
+    assert says in plan(**over)
+
+
+def append(**over):
+    kw = dict(pages=P, keys=P, key_stride=1024, values=P, value_stride=1024, slots=P, rows=5, cv=1024, page=16,
+              q4_slots=9, page_bytes=16 * 1088)
+    kw.update(over)
+    return call("ctox_hip_kv_append_q4_device", *kw.values(), None)
+
+
+def test_append_in_order_without_a_backend():
+    assert append() == "null argument"
+
+
+@pytest.mark.parametrize("over,says", [
+    (dict(cv=0), "multiple of 64"), (dict(cv=96), "multiple of 64"), (dict(page=0), "fit"), (dict(page=17), "fit"),
+    (dict(page_bytes=16 * 1088 + 2), "fit"), (dict(q4_slots=1 << 28), "fit"), (dict(rows=1 << 31), "too large"),
+    (dict(key_stride=1 << 30), "too large"),
+])
+def test_append_refuses(over, says):
+    assert says in append(**over)
+
+
+def test_rope_axes_needs_one_axis_per_pair():
+    with pytest.raises(ctox_hip.ShapeError):
+        RopeAxes(d_q=P, d_positions=P, rows=1, q_heads=1, head_dim=64, rotary_dim=64, theta=1e4, axis_of_pair=[0] * 31)
