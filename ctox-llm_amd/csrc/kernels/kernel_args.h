@@ -605,6 +605,48 @@ struct KvAppendArgs {
     uint32_t vec;            // rows and strides allow 16-byte loads
 };
 
+// Activation rows staged for the row product (rows_matmul.hip).
+struct RowsStageArgs {
+    const void *x;           // f32 or f16 rows
+    const void *s_in;        // NULL, f32[columns] or f16[columns]
+    void *staged;            // [32-row tiles][blocks][parts][4 steps][64 lanes][8] f16
+    int32_t *exps;           // [rows]: |x s_in| < 2^exp over the row (parts == 2)
+    uint64_t x_stride;       // values between rows
+    uint32_t rows;
+    uint32_t columns;
+    uint32_t blocks;
+    uint32_t parts;          // 2: hi + lo of x s_in 2^(15 - exp); 1: f16 x as it is
+    uint32_t x_half;
+    uint32_t s_in_kind;
+    uint32_t q4;             // value order of Q4 (1) or Q2 (0) codes
+    uint32_t pad;
+};
+
+struct RowsMulArgs {
+    const uint8_t *weights;  // tiled units of one segment
+    const uint8_t *staged;
+    const int32_t *exps;
+    const void *s_out;       // the segment's
+    const float *bias;
+    const void *residual;    // NULL or rows of y's type
+    void *y;
+    float *partial;          // NULL, or [splits][rows][n] sums of a split K
+    uint64_t y_stride;
+    uint64_t residual_stride;
+    uint32_t rows;
+    uint32_t n;              // weight rows of the segment
+    uint32_t tiles;          // 16-row weight tiles
+    uint32_t x_tiles;        // 32-row tiles of x
+    uint32_t blocks;
+    uint32_t blocks_per_split;
+    uint32_t splits;
+    uint32_t col_groups;     // workgroups along the weight rows
+    uint32_t s_out_kind;
+    uint32_t activation;
+    uint32_t y_half;
+    uint32_t pad;
+};
+
 // Decode engine helpers (engine_ops.hip).
 struct FillArgs {
     void *ptr;

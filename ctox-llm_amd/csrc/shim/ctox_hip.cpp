@@ -125,6 +125,12 @@ bool block_scales_finite(const uint8_t *w, size_t rows, size_t blocks, size_t bb
     return true;
 }
 
+// Tile shapes of the row products: a workgroup's 32-row tiles of x, a wave's of the weights.
+struct RowShape {
+    uint32_t tt, rt;
+};
+constexpr RowShape kRowShapes[4] = {{1, 1}, {2, 1}, {4, 1}, {4, 2}};
+
 struct DevBuf {
     void *ptr = nullptr;
     size_t bytes = 0;
@@ -152,7 +158,10 @@ struct ctox_hip_backend {
                   gqa_combine = nullptr, fill = nullptr, embed = nullptr, norm_rows = nullptr, attn_gate = nullptr,
                   swiglu_rows = nullptr, copy_rows = nullptr, write_words = nullptr, norm_prep = nullptr,
                   prep_x = nullptr, finite = nullptr, gather = nullptr, topk_part = nullptr, topk_final = nullptr, stream_read = nullptr,
-                  write_segments = nullptr, rope_axes[2] = {}, plan = nullptr, kv_append = nullptr;
+                  write_segments = nullptr, rope_axes[2] = {}, plan = nullptr, kv_append = nullptr,
+                  rows_max = nullptr, rows_stage = nullptr, rows_reduce = nullptr;
+    // Row products: [q4][parts - 1][shape], shapes as kRowShapes.
+    hipFunction_t rows_mul[2][2][4] = {};
     // Batch-1 slice kernels per dtype [Q2, Q4]: [0] walks the slices, [n]
     // requests all n slices up front (n <= 3: more slices up front measured
     // slower than walking them).
@@ -940,7 +949,9 @@ extern "C" ctox_status ctox_hip_backend_create(int device, ctox_hip_backend **ou
                {&b->write_segments, "ctox_write_segments_gfx950"},
                {&b->topk_part, "ctox_topk_part_gfx950"}, {&b->topk_final, "ctox_topk_final_gfx950"},
                {&b->rope_axes[0], "ctox_rope_axes_gfx950"}, {&b->rope_axes[1], "ctox_rope_axes_any_gfx950"},
-               {&b->plan, "ctox_paged_plan_gfx950"}, {&b->kv_append, "ctox_kv_append_q4_gfx950"}};
+               {&b->plan, "ctox_paged_plan_gfx950"}, {&b->kv_append, "ctox_kv_append_q4_gfx950"},
+               {&b->rows_max, "ctox_rows_max_gfx950"}, {&b->rows_stage, "ctox_rows_stage_gfx950"},
+               {&b->rows_reduce, "ctox_rows_reduce_gfx950"}};
     for (auto &f : fns) {
         if (le != hipSuccess) break;
         le = hipModuleGetFunction(f.f, b->module, f.name);
@@ -977,6 +988,15 @@ extern "C" ctox_status ctox_hip_backend_create(int device, ctox_hip_backend **ou
                     return fail(CTOX_ERR_UNSUPPORTED_OPERATION, "kernel %s missing from code object: %s", name,
                                 hipGetErrorString(le));
                 }
+            }
+    // The row products, one per dtype, parts of an activation and tile shape.
+    for (int q = 0; q < 2 && le == hipSuccess; q++)
+        for (int p = 0; p < 2 && le == hipSuccess; p++)
+            for (int i = 0; i < 4 && le == hipSuccess; i++) {
+                char name[64];
+                std::snprintf(name, sizeof name, "ctox_rows_q%d_p%d_%ux%u_gfx950", q ? 4 : 2, p + 1, kRowShapes[i].tt,
+                              kRowShapes[i].rt);
+                le = hipModuleGetFunction(&b->rows_mul[q][p][i], b->module, name);
             }
     if (le != hipSuccess) {
         ctox_hip_backend_destroy(b);
@@ -2778,4 +2798,156 @@ extern "C" ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *b, uint8_t
     OnDevice on(b);
     return launch(b->kv_append, dim3((unsigned)((rows + a.rows_per_wg - 1) / a.rows_per_wg)), dim3(256),
                   (hipStream_t)stream, a, "ctox_kv_append_q4_gfx950");
+}
+
+namespace {
+// Shape and split of one segment's row product. A workgroup takes the most rows of x there are (up to
+// 128), and 256 weight rows rather than 128 where that still gives every CU two workgroups; where there are
+// fewer workgroups than CUs, the K range is split, into eight blocks at least.
+struct RowPlan {
+    uint32_t shape, col_groups, row_groups, per_split, splits;
+};
+RowPlan row_plan(uint32_t cus, uint32_t rows, uint32_t n, uint32_t blocks) {
+    RowPlan p{};
+    const uint32_t tiles = (rows + 31) / 32;
+    p.shape = tiles >= 3 ? 2 : tiles - 1;
+    if (p.shape == 2 && (uint64_t)((tiles + 3) / 4) * ((n + 255) / 256) >= 2 * cus) p.shape = 3;
+    const RowShape s = kRowShapes[p.shape];
+    p.row_groups = (tiles + s.tt - 1) / s.tt;
+    p.col_groups = (n + 128 * s.rt - 1) / (128 * s.rt);
+    const uint64_t wgs = (uint64_t)p.row_groups * p.col_groups;
+    uint32_t splits = 1;
+    if (wgs < cus) splits = std::min<uint32_t>((uint32_t)(2 * cus / wgs), std::max<uint32_t>(1, blocks / 8));
+    p.per_split = (blocks + splits - 1) / splits;
+    p.splits = (blocks + p.per_split - 1) / p.per_split;
+    return p;
+}
+
+// Where a row product's workspace holds what.
+struct RowSpace {
+    uint32_t parts;
+    uint64_t staged[2], exps, partial, total;  // byte offsets; staged per value order [Q2, Q4]
+};
+RowSpace row_space(const ctox_hip_matrix *m, uint64_t rows, int32_t x_dtype) {
+    RowSpace w{};
+    w.parts = x_dtype == CTOX_DTYPE_F16 && m->s_in_kind == CTOX_KSCALE_NONE ? 1 : 2;
+    uint64_t at = 0, partial = 0;
+    auto take = [&](uint64_t bytes) {
+        const uint64_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const uint64_t one = (rows + 31) / 32 * 32 * m->columns * 2 * w.parts;
+    for (int q4 = 0; q4 < 2; q4++) {
+        bool any = false;
+        for (const ctox_quant_segment &seg : m->segments) any = any || (seg.dtype == CTOX_DTYPE_Q4B64) == (q4 == 1);
+        w.staged[q4] = take(any ? one : 0);
+    }
+    for (const ctox_quant_segment &seg : m->segments) {
+        const uint32_t n = (uint32_t)(seg.row_end - seg.row_start);
+        const RowPlan p = row_plan((uint32_t)m->backend->cus, (uint32_t)rows, n, (uint32_t)(m->columns / kBlockLen));
+        if (p.splits > 1) partial = std::max<uint64_t>(partial, (uint64_t)p.splits * rows * n * sizeof(float));
+    }
+    w.exps = take(w.parts == 2 ? rows * sizeof(int32_t) : 0);
+    w.partial = take(partial);
+    w.total = at;
+    return w;
+}
+
+bool row_dtype(int32_t d) { return d == CTOX_DTYPE_F32 || d == CTOX_DTYPE_F16; }
+constexpr uint64_t kMostRows = 1u << 20;
+}  // namespace
+
+extern "C" ctox_status ctox_hip_matrix_rows_workspace(const ctox_hip_matrix *m, size_t rows, int32_t x_dtype,
+                                                      size_t *bytes) {
+    if (!bytes) return fail(CTOX_ERR_SHAPE, "null argument");
+    *bytes = 0;
+    if (!row_dtype(x_dtype)) return fail(CTOX_ERR_UNSUPPORTED_DTYPE, "activation dtype %d is not F32 or F16", x_dtype);
+    if (rows > kMostRows) return fail(CTOX_ERR_SHAPE, "%zu rows exceed 2^20", rows);
+    if (!m) return fail(CTOX_ERR_SHAPE, "null argument");
+    *bytes = rows ? (size_t)row_space(m, rows, x_dtype).total : 0;
+    return CTOX_OK;
+}
+
+extern "C" ctox_status ctox_hip_matrix_dispatch_rows(ctox_hip_backend *b, const ctox_hip_matrix *m,
+                                                     const ctox_matrix_rows *op, void *stream) {
+    if (!op) return fail(CTOX_ERR_SHAPE, "null argument");
+    if (!row_dtype(op->x_dtype) || !row_dtype(op->y_dtype))
+        return fail(CTOX_ERR_UNSUPPORTED_DTYPE, "activation dtypes %d and %d are not F32 or F16", op->x_dtype, op->y_dtype);
+    if (op->rows > kMostRows) return fail(CTOX_ERR_SHAPE, "%llu rows exceed 2^20", (unsigned long long)op->rows);
+    if (!spans(op->rows, op->x_stride) || !spans(op->rows, op->y_stride) || !spans(op->rows, op->residual_stride))
+        return fail(CTOX_ERR_SHAPE, "row stride is too large");
+    if (!b || !m) return fail(CTOX_ERR_SHAPE, "null argument");
+    if (m->backend != b) return fail(CTOX_ERR_INVALID_STATE, "the matrix belongs to another backend");
+    const uint64_t xs = op->x_stride ? op->x_stride : m->columns, ys = op->y_stride ? op->y_stride : m->rows;
+    const uint64_t rs = op->residual_stride ? op->residual_stride : m->rows;
+    if (xs < m->columns || ys < m->rows || rs < m->rows) return fail(CTOX_ERR_SHAPE, "row stride is smaller than a row");
+    if (op->residual == op->y && op->y && rs != ys) return fail(CTOX_ERR_SHAPE, "a residual in place needs y's stride");
+    if (op->rows == 0) return CTOX_OK;
+    if (!op->x || !op->y) return fail(CTOX_ERR_SHAPE, "null argument");
+    const size_t xb = op->x_dtype == CTOX_DTYPE_F16 ? 2 : 4, yb = op->y_dtype == CTOX_DTYPE_F16 ? 2 : 4;
+    if (!aligned(op->x, xb) || !aligned(op->y, yb) || !aligned(op->residual, yb))
+        return fail(CTOX_ERR_SHAPE, "an activation pointer is not aligned to its type");
+    const RowSpace w = row_space(m, op->rows, op->x_dtype);
+    if (op->workspace_bytes < w.total || !op->workspace || !aligned(op->workspace, 16))
+        return fail(CTOX_ERR_MEMORY_BUDGET, "workspace of %llu bytes, %llu needed, 16-byte aligned",
+                    (unsigned long long)op->workspace_bytes, (unsigned long long)w.total);
+    uint8_t *ws = (uint8_t *)op->workspace;
+    OnDevice on(b);
+    hipStream_t s = (hipStream_t)stream;
+    RowsStageArgs sa{};
+    sa.x = op->x;
+    sa.s_in = m->d_s_in;
+    sa.exps = (int32_t *)(ws + w.exps);
+    sa.x_stride = xs;
+    sa.rows = (uint32_t)op->rows;
+    sa.columns = (uint32_t)m->columns;
+    sa.blocks = (uint32_t)(m->columns / kBlockLen);
+    sa.parts = w.parts;
+    sa.x_half = op->x_dtype == CTOX_DTYPE_F16;
+    sa.s_in_kind = m->s_in_kind;
+    const uint32_t x_tiles = (sa.rows + 31) / 32;
+    ctox_status st = CTOX_OK;
+    if (w.parts == 2) st = launch(b->rows_max, dim3(sa.rows), dim3(256), s, sa, "ctox_rows_max_gfx950");
+    bool staged[2] = {false, false};
+    for (size_t i = 0; i < m->segments.size() && !st; i++) {
+        const ctox_quant_segment &seg = m->segments[i];
+        const TiledCopy &t = m->tiled[i];
+        const int q4 = seg.dtype == CTOX_DTYPE_Q4B64;
+        if (!staged[q4]) {
+            sa.staged = ws + w.staged[q4];
+            sa.q4 = (uint32_t)q4;
+            st = launch(b->rows_stage, dim3(sa.blocks, x_tiles), dim3(256), s, sa, "ctox_rows_stage_gfx950");
+            if (st) break;
+            staged[q4] = true;
+        }
+        const RowPlan p = row_plan((uint32_t)b->cus, sa.rows, t.rows, sa.blocks);
+        RowsMulArgs a{};
+        a.weights = (const uint8_t *)t.d;
+        a.staged = ws + w.staged[q4];
+        a.exps = sa.exps;
+        a.s_out_kind = m->s_out_kind;
+        if (m->d_s_out) a.s_out = (const uint8_t *)m->d_s_out + seg.row_start * (m->s_out_kind == CTOX_KSCALE_F32 ? 4 : 2);
+        a.bias = m->d_bias ? m->d_bias + seg.row_start : nullptr;
+        a.residual = op->residual ? (const uint8_t *)op->residual + seg.row_start * yb : nullptr;
+        a.y = (uint8_t *)op->y + seg.row_start * yb;
+        a.partial = p.splits > 1 ? (float *)(ws + w.partial) : nullptr;
+        a.y_stride = ys;
+        a.residual_stride = rs;
+        a.rows = sa.rows;
+        a.n = t.rows;
+        a.tiles = t.tiles;
+        a.x_tiles = x_tiles;
+        a.blocks = sa.blocks;
+        a.blocks_per_split = p.per_split;
+        a.splits = p.splits;
+        a.col_groups = p.col_groups;
+        a.activation = m->activation;
+        a.y_half = op->y_dtype == CTOX_DTYPE_F16;
+        st = launch(b->rows_mul[q4][w.parts - 1][p.shape], dim3(p.col_groups * p.row_groups, p.splits), dim3(256), s, a,
+                    "ctox_rows_gfx950");
+        if (!st && p.splits > 1)
+            st = launch(b->rows_reduce, dim3(a.rows, (a.n + 255) / 256), dim3(256), s, a, "ctox_rows_reduce_gfx950");
+    }
+    return st;
 }

@@ -200,6 +200,14 @@ class PagedGqaParams(ctypes.Structure):
 
 
 
+class _MatrixRows(ctypes.Structure):
+    """ctox_matrix_rows."""
+    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("residual", ctypes.c_void_p)] + [
+        (n, ctypes.c_uint64) for n in ("rows", "x_stride", "y_stride", "residual_stride")] + [
+        ("x_dtype", ctypes.c_int32), ("y_dtype", ctypes.c_int32), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64)]
+
+
 class RopeAxes(ctypes.Structure):
     """ctox_rope_axes. Strides are (row, head) in values; outputs are dense unless given,
     axis_of_pair a sequence of rotary_dim / 2 axis numbers (None: all 0)."""
@@ -306,6 +314,8 @@ SIGNATURES = {
                                          ctypes.c_float, _P, _U32, _P, _P, _P, _P, _P, _SZ, _P]),
     "ctox_hip_kv_demote_device": (_I32, [_P, _P, _P, _SZ, _SZ, _P]),
     "ctox_hip_paged_gqa_device": (_I32, [_P, _P, _P, _P, _P, ctypes.POINTER(PagedGqaParams), _SZ, _P, _P]),
+    "ctox_hip_matrix_rows_workspace": (_I32, [_P, _SZ, _I32, ctypes.POINTER(_SZ)]),
+    "ctox_hip_matrix_dispatch_rows": (_I32, [_P, _P, ctypes.POINTER(_MatrixRows), _P]),
     "ctox_hip_rope_axes_device": (_I32, [_P, ctypes.POINTER(RopeAxes), _P]),
     "ctox_hip_paged_plan_device": (_I32, [_P, ctypes.POINTER(PagedPlan), _P]),
     "ctox_hip_kv_append_q4_device": (_I32, [_P, _P, _P, _SZ, _P, _SZ, _P, _SZ, _SZ, _U32, _U32, _U32, _P]),
@@ -431,6 +441,22 @@ class HipMatrix:
         """Device pointers: d_input [batch, columns] f32, d_output [batch, rows] f32."""
         _check(load_library().ctox_hip_matrix_dispatch(self.backend.handle, self.handle, d_input, batch,
                                                        d_output, stream))
+
+    def rows_workspace(self, rows: int, x_dtype: TensorDType = TensorDType.F32) -> int:
+        """Workspace bytes of a dispatch_rows call of `rows` rows."""
+        n = ctypes.c_size_t()
+        _check(load_library().ctox_hip_matrix_rows_workspace(self.handle, rows, int(x_dtype), ctypes.byref(n)))
+        return n.value
+
+    def dispatch_rows(self, d_x: int, rows: int, d_y: int, d_workspace: int, workspace_bytes: int,
+                      d_residual: Optional[int] = None, x_dtype: TensorDType = TensorDType.F32,
+                      y_dtype: TensorDType = TensorDType.F32, x_stride: int = 0, y_stride: int = 0,
+                      residual_stride: int = 0, stream: Optional[int] = None) -> None:
+        """act((x * s_in . W^T + bias) * s_out) + residual for any number of rows; strides in
+        values (0: dense rows)."""
+        op = _MatrixRows(d_x, d_y, d_residual, rows, x_stride, y_stride, residual_stride, int(x_dtype), int(y_dtype),
+                         d_workspace, workspace_bytes)
+        _check(load_library().ctox_hip_matrix_dispatch_rows(self.backend.handle, self.handle, ctypes.byref(op), stream))
 
     def close(self) -> None:
         if self.handle:

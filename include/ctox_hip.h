@@ -596,6 +596,32 @@ ctox_status ctox_hip_paged_gqa_device(ctox_hip_backend *backend, const float *d_
  * captured into a graph and calls with different buffers may overlap. They
  * run on the backend's device whichever device is current. */
 
+/* ctox_hip_matrix_dispatch for any number of rows (a prompt's, or a batch of
+ * requests'), with a residual and f16 or f32 activations:
+ *   y[t] = act((x[t] * s_in . W^T + bias) * s_out) + residual[t],  t < rows.
+ * Row t of x starts at x_stride values times t (x_stride >= columns, or 0 for
+ * the dense row length; likewise y and residual). x_dtype and y_dtype are
+ * CTOX_DTYPE_F32 or CTOX_DTYPE_F16; residual (NULL = none) has y's type and may be
+ * y itself with y's stride. y must not overlap x. Products keep 22 bits of an
+ * f32 activation (of an f16 one times s_in likewise; without s_in all of it) and
+ * add up in 32 bits; an f16 result is rounded once. rows <= 2^20; rows = 0
+ * does nothing. Results of a row depend on the number of rows of the call in
+ * the last bits (the K range may be split). workspace holds
+ * ctox_hip_matrix_rows_workspace bytes, 16-byte aligned, and is free again when the
+ * call's work on the stream is done. */
+typedef struct {
+    const void *x;
+    void *y;
+    const void *residual;
+    uint64_t rows, x_stride, y_stride, residual_stride;
+    int32_t x_dtype, y_dtype;
+    void *workspace;
+    uint64_t workspace_bytes;
+} ctox_matrix_rows;
+ctox_status ctox_hip_matrix_rows_workspace(const ctox_hip_matrix *matrix, size_t rows, int32_t x_dtype, size_t *bytes);
+ctox_status ctox_hip_matrix_dispatch_rows(ctox_hip_backend *backend, const ctox_hip_matrix *matrix,
+                                          const ctox_matrix_rows *op, void *stream);
+
 /* Per-head (1 + w) RMS norm (Q/src/reference.rs:38-62, where its weight is
  * given) and rotary positions on up to 4 axes: for i < rotary_dim / 2 the
  * pair (x[i], x[i + rotary_dim / 2]) turns by

@@ -91,3 +91,29 @@ def test_append_refuses(over, says):
 def test_rope_axes_needs_one_axis_per_pair():
     with pytest.raises(ctox_hip.ShapeError):
         RopeAxes(d_q=P, d_positions=P, rows=1, q_heads=1, head_dim=64, rotary_dim=64, theta=1e4, axis_of_pair=[0] * 31)
+
+
+def rows_product(**over):
+    kw = dict(x=P, y=P, residual=None, rows=4, x_stride=0, y_stride=0, residual_stride=0, x_dtype=4, y_dtype=3,
+              workspace=P, workspace_bytes=1 << 20)
+    kw.update(over)
+    lib, op = ctox_hip.load_library(), ctox_hip._MatrixRows(*kw.values())
+    with pytest.raises(ctox_hip.EngineError) as e:
+        ctox_hip._check(lib.ctox_hip_matrix_dispatch_rows(None, None, ctypes.byref(op), None))
+    return str(e.value)
+
+
+@pytest.mark.parametrize("over,says", [
+    (dict(), "null argument"), (dict(x_dtype=1), "dtypes"), (dict(y_dtype=5), "dtypes"), (dict(rows=(1 << 20) + 1), "2^20"),
+    (dict(x_stride=1 << 30), "stride"), (dict(y_stride=1 << 31), "stride"), (dict(residual_stride=1 << 40), "stride"),
+])
+def test_rows_product_refuses(over, says):
+    assert says in rows_product(**over)
+
+
+def test_rows_workspace_refuses():
+    lib, n = ctox_hip.load_library(), ctypes.c_size_t()
+    for args, kind in (((None, 5, 4), ctox_hip.ShapeError), ((None, 5, 0), ctox_hip.UnsupportedDType),
+                       ((None, (1 << 20) + 1, 4), ctox_hip.ShapeError)):
+        with pytest.raises(kind):
+            ctox_hip._check(lib.ctox_hip_matrix_rows_workspace(*args, ctypes.byref(n)))
