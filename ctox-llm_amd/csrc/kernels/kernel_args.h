@@ -647,6 +647,39 @@ struct RowsMulArgs {
     uint32_t pad;
 };
 
+// Attention of a ragged batch's rows (paged_attention_rows.hip).
+struct GqaRowsArgs {
+    const float *query;      // [rows][query_heads][256]
+    float *out;              // [rows][query_heads][256]
+    const uint8_t *q2;
+    const uint8_t *q4;
+    const PagedKvDesc *desc; // [requests][max_pages]
+    const uint32_t *row_starts;  // [requests + 1]
+    const uint32_t *tokens;      // [requests]
+    float *part;             // [item]: [64][256] numerators, [64][2] (max base 2, denominator)
+    float *few_part;         // [item]: [16][256], [16][2] (max, denominator)
+    uint64_t q2_page_bytes;
+    uint64_t q4_page_bytes;
+    uint32_t requests;
+    uint32_t rows;           // rows of query and out
+    uint32_t max_pages;
+    uint32_t max_tokens;     // min(max_pages * page_tokens, 2^30)
+    uint32_t query_heads;
+    uint32_t kv_heads;
+    uint32_t group;
+    uint32_t page_tokens;
+    uint32_t q2_token_bytes;
+    uint32_t q4_token_bytes;
+    uint32_t v_off2;         // bytes from a token's K run of a head to its V run
+    uint32_t v_off4;
+    uint32_t split;          // token ranges are split and joined
+    uint32_t fill;           // workgroups that fill the chip, 64-query kernel
+    uint32_t few;            // requests of at most 16 queries go to the few-query kernel
+    uint32_t few_fill;
+    float scale;
+    uint32_t pad;
+};
+
 // Decode engine helpers (engine_ops.hip).
 struct FillArgs {
     void *ptr;

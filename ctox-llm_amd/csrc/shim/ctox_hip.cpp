@@ -159,7 +159,8 @@ struct ctox_hip_backend {
                   swiglu_rows = nullptr, copy_rows = nullptr, write_words = nullptr, norm_prep = nullptr,
                   prep_x = nullptr, finite = nullptr, gather = nullptr, topk_part = nullptr, topk_final = nullptr, stream_read = nullptr,
                   write_segments = nullptr, rope_axes[2] = {}, plan = nullptr, kv_append = nullptr,
-                  rows_max = nullptr, rows_stage = nullptr, rows_reduce = nullptr;
+                  rows_max = nullptr, rows_stage = nullptr, rows_reduce = nullptr,
+                  gqa_rows = nullptr, gqa_few[2] = {}, gqa_join = nullptr;
     // Row products: [q4][parts - 1][shape], shapes as kRowShapes.
     hipFunction_t rows_mul[2][2][4] = {};
     // Batch-1 slice kernels per dtype [Q2, Q4]: [0] walks the slices, [n]
@@ -951,7 +952,9 @@ extern "C" ctox_status ctox_hip_backend_create(int device, ctox_hip_backend **ou
                {&b->rope_axes[0], "ctox_rope_axes_gfx950"}, {&b->rope_axes[1], "ctox_rope_axes_any_gfx950"},
                {&b->plan, "ctox_paged_plan_gfx950"}, {&b->kv_append, "ctox_kv_append_q4_gfx950"},
                {&b->rows_max, "ctox_rows_max_gfx950"}, {&b->rows_stage, "ctox_rows_stage_gfx950"},
-               {&b->rows_reduce, "ctox_rows_reduce_gfx950"}};
+               {&b->rows_reduce, "ctox_rows_reduce_gfx950"},
+               {&b->gqa_rows, "ctox_gqa_rows_gfx950"}, {&b->gqa_few[0], "ctox_gqa_few_gfx950"},
+               {&b->gqa_few[1], "ctox_gqa_few_aligned_gfx950"}, {&b->gqa_join, "ctox_gqa_join_gfx950"}};
     for (auto &f : fns) {
         if (le != hipSuccess) break;
         le = hipModuleGetFunction(f.f, b->module, f.name);
@@ -2949,5 +2952,125 @@ extern "C" ctox_status ctox_hip_matrix_dispatch_rows(ctox_hip_backend *b, const 
         if (!st && p.splits > 1)
             st = launch(b->rows_reduce, dim3(a.rows, (a.n + 255) / 256), dim3(256), s, a, "ctox_rows_reduce_gfx950");
     }
+    return st;
+}
+
+namespace {
+ctox_status check_gqa_rows(const ctox_paged_gqa_rows *op) {
+    if (!op) return fail(CTOX_ERR_SHAPE, "null argument");
+    const ctox_paged_gqa_params &p = op->params;
+    if (p.head_dim != 256) return fail(CTOX_ERR_UNSUPPORTED_OPERATION, "paged attention needs head_dim 256");
+    if (p.key_value_heads == 0 || p.query_heads == 0 || p.query_heads % p.key_value_heads || p.query_heads > 65535 ||
+        p.page_tokens == 0 || p.page_count == 0 || !std::isfinite(p.scale))
+        return fail(CTOX_ERR_SHAPE, "invalid paged attention contract");
+    const uint64_t cv = (uint64_t)p.key_value_heads * 256;
+    if (p.combined_values != 2 * cv || p.q2_token_bytes != 2 * cv / 64 * 18 || p.q4_token_bytes != 2 * cv / 64 * 34 ||
+        (uint64_t)p.q2_page_bytes < (uint64_t)p.page_tokens * p.q2_token_bytes ||
+        (uint64_t)p.q4_page_bytes < (uint64_t)p.page_tokens * p.q4_token_bytes || p.q2_page_bytes % 4 ||
+        p.q4_page_bytes % 4)
+        return fail(CTOX_ERR_SHAPE, "paged KV geometry differs from the attention contract");
+    if (op->requests == 0 || op->requests > CTOX_PLAN_REQUESTS)
+        return fail(CTOX_ERR_SHAPE, "attention of %u requests outside 1..%d", op->requests, CTOX_PLAN_REQUESTS);
+    if (op->rows > kMostRows || op->rows * (p.query_heads / p.key_value_heads) > 0x3fffffffu)
+        return fail(CTOX_ERR_SHAPE, "attention rows are too many");
+    return CTOX_OK;
+}
+
+// Which kernels run and how many items each may have. Requests of at most 16 queries a KV head go to the
+// few-query kernel, unless the batch is one request that may have more. The 64-query kernel splits token
+// ranges where its query tiles alone would not give every CU two workgroups. An item bound is what the
+// device's ranges cannot exceed: the workgroups that fill the chip, plus one a tile for the rounding.
+struct GqaRowsPlan {
+    bool few, wide, split;
+    uint32_t few_fill, fill, few_items, items;
+    uint64_t few_bytes, bytes;
+};
+GqaRowsPlan gqa_rows_plan(uint32_t cus, const ctox_paged_gqa_rows *op) {
+    GqaRowsPlan g{};
+    const uint32_t kvh = op->params.key_value_heads, group = op->params.query_heads / kvh;
+    const uint64_t most = op->max_rows ? std::min<uint64_t>(op->max_rows, op->rows) : op->rows;
+    const uint64_t busy = std::min<uint64_t>(op->requests, op->rows);
+    g.wide = most * group > 16;
+    g.few = group <= 16 && !(g.wide && op->requests == 1);
+    g.few_fill = 2 * cus;
+    g.fill = cus;
+    if (g.few) {
+        g.few_items = (uint32_t)(g.few_fill + busy * kvh);
+        g.few_bytes = (uint64_t)g.few_items * 16 * 258 * sizeof(float);
+    }
+    if (g.wide) {
+        const uint64_t tiles = (op->rows * group + 63) / 64;
+        g.split = tiles * kvh < 2 * cus;
+        g.items = (uint32_t)((tiles + busy) * kvh + (g.split ? g.fill : 0));
+        g.bytes = g.split ? (uint64_t)g.items * 64 * 258 * sizeof(float) : 0;
+    }
+    return g;
+}
+}  // namespace
+
+extern "C" ctox_status ctox_hip_paged_gqa_rows_workspace(const ctox_hip_backend *b, const ctox_paged_gqa_rows *op,
+                                                         size_t *bytes) {
+    if (!bytes) return fail(CTOX_ERR_SHAPE, "null argument");
+    *bytes = 0;
+    if (ctox_status st = check_gqa_rows(op)) return st;
+    if (!b) return fail(CTOX_ERR_SHAPE, "null argument");
+    const GqaRowsPlan g = gqa_rows_plan((uint32_t)b->cus, op);
+    *bytes = (size_t)(g.few_bytes + g.bytes);
+    return CTOX_OK;
+}
+
+extern "C" ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *b, const ctox_paged_gqa_rows *op, void *stream) {
+    if (ctox_status st = check_gqa_rows(op)) return st;
+    if (!b || !op->q2_pages || !op->q4_pages || !op->descriptors || !op->row_starts || !op->tokens ||
+        (op->rows && (!op->query || !op->out)))
+        return fail(CTOX_ERR_SHAPE, "null argument");
+    if (!aligned(op->query, 16) || !aligned(op->out, 16) || !aligned(op->descriptors, 16) || !aligned(op->q2_pages, 4) ||
+        !aligned(op->q4_pages, 4))
+        return fail(CTOX_ERR_SHAPE, "an attention pointer is not aligned");
+    if (op->rows == 0) return CTOX_OK;
+    const GqaRowsPlan g = gqa_rows_plan((uint32_t)b->cus, op);
+    const uint64_t need = g.few_bytes + g.bytes;
+    if (need && (op->workspace_bytes < need || !op->workspace || !aligned(op->workspace, 16)))
+        return fail(CTOX_ERR_MEMORY_BUDGET, "workspace of %llu bytes, %llu needed, 16-byte aligned",
+                    (unsigned long long)op->workspace_bytes, (unsigned long long)need);
+    const ctox_paged_gqa_params &p = op->params;
+    const uint32_t cv = p.key_value_heads * 256;
+    GqaRowsArgs a{};
+    a.query = op->query;
+    a.out = op->out;
+    a.q2 = op->q2_pages;
+    a.q4 = op->q4_pages;
+    a.desc = (const PagedKvDesc *)op->descriptors;
+    a.row_starts = op->row_starts;
+    a.tokens = op->tokens;
+    a.few_part = (float *)op->workspace;
+    a.part = (float *)((uint8_t *)op->workspace + g.few_bytes);
+    a.q2_page_bytes = p.q2_page_bytes;
+    a.q4_page_bytes = p.q4_page_bytes;
+    a.requests = op->requests;
+    a.rows = (uint32_t)op->rows;
+    a.max_pages = p.page_count;
+    a.max_tokens = (uint32_t)std::min<uint64_t>((uint64_t)p.page_count * p.page_tokens, 1u << 30);
+    a.query_heads = p.query_heads;
+    a.kv_heads = p.key_value_heads;
+    a.group = p.query_heads / p.key_value_heads;
+    a.page_tokens = p.page_tokens;
+    a.q2_token_bytes = p.q2_token_bytes;
+    a.q4_token_bytes = p.q4_token_bytes;
+    a.v_off2 = cv / 64 * 18;
+    a.v_off4 = cv / 64 * 34;
+    a.split = g.split;
+    a.fill = g.fill;
+    a.few = g.few;
+    a.few_fill = g.few_fill;
+    a.scale = p.scale;
+    OnDevice on(b);
+    hipStream_t s = (hipStream_t)stream;
+    ctox_status st = CTOX_OK;
+    if (g.wide) st = launch(b->gqa_rows, dim3(g.items), dim3(512), s, a, "ctox_gqa_rows_gfx950");
+    if (!st && g.few)
+        st = launch(b->gqa_few[p.page_tokens % 16 == 0], dim3(g.few_items), dim3(256), s, a, "ctox_gqa_few_gfx950");
+    if (!st && (g.few || g.split))
+        st = launch(b->gqa_join, dim3(a.rows, p.query_heads), dim3(256), s, a, "ctox_gqa_join_gfx950");
     return st;
 }

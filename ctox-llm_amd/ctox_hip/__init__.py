@@ -252,6 +252,22 @@ class PagedPlan(ctypes.Structure):
                          max_rows)
 
 
+class PagedGqaRows(ctypes.Structure):
+    """ctox_paged_gqa_rows (device addresses; params.tokens is not read)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "query", "out", "q2_pages", "q4_pages", "descriptors", "row_starts", "tokens")] + [
+        ("rows", ctypes.c_uint64), ("requests", ctypes.c_uint32), ("max_rows", ctypes.c_uint32),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("params", PagedGqaParams)]
+
+    def __init__(self, d_query, d_out, d_q2_pages, d_q4_pages, d_descriptors, d_row_starts, d_tokens, rows, requests,
+                 params, max_rows=0, d_workspace=None, workspace_bytes=0):
+        super().__init__(d_query, d_out, d_q2_pages, d_q4_pages, d_descriptors, d_row_starts, d_tokens, rows, requests,
+                         max_rows, d_workspace, workspace_bytes, params)
+
+    def bind_workspace(self, d_workspace: int, workspace_bytes: int) -> None:
+        self.workspace, self.workspace_bytes = d_workspace, workspace_bytes
+
+
 # Every symbol include/ctox_hip.h declares: name -> (restype, argtypes).
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
@@ -318,6 +334,8 @@ SIGNATURES = {
     "ctox_hip_matrix_dispatch_rows": (_I32, [_P, _P, ctypes.POINTER(_MatrixRows), _P]),
     "ctox_hip_rope_axes_device": (_I32, [_P, ctypes.POINTER(RopeAxes), _P]),
     "ctox_hip_paged_plan_device": (_I32, [_P, ctypes.POINTER(PagedPlan), _P]),
+    "ctox_hip_paged_gqa_rows_workspace": (_I32, [_P, ctypes.POINTER(PagedGqaRows), ctypes.POINTER(_SZ)]),
+    "ctox_hip_paged_gqa_rows_device": (_I32, [_P, ctypes.POINTER(PagedGqaRows), _P]),
     "ctox_hip_kv_append_q4_device": (_I32, [_P, _P, _P, _SZ, _P, _SZ, _P, _SZ, _SZ, _U32, _U32, _U32, _P]),
     "ctox_hip_fill_random_device": (_I32, [_P, _P, ctypes.c_uint64, _U32, ctypes.c_uint64, ctypes.c_float,
                                            ctypes.c_float, _P]),
@@ -721,6 +739,16 @@ class HipBackend:
             self.handle, d_q4_pages, d_keys, component_values if key_stride is None else key_stride, d_values,
             component_values if value_stride is None else value_stride, d_slots, rows, component_values, page_tokens,
             q4_slots, q4_page_bytes, stream))
+
+    def paged_gqa_rows_workspace(self, op: PagedGqaRows) -> int:
+        """Workspace bytes of a paged_gqa_rows_device call (reads no device pointer of `op`)."""
+        n = ctypes.c_size_t()
+        _check(load_library().ctox_hip_paged_gqa_rows_workspace(self.handle, ctypes.byref(op), ctypes.byref(n)))
+        return n.value
+
+    def paged_gqa_rows_device(self, op: PagedGqaRows, stream: Optional[int] = None) -> None:
+        """Attention of a ragged batch's new rows over the paged cache (Q/src/reference.rs:420-499)."""
+        _check(load_library().ctox_hip_paged_gqa_rows_device(self.handle, ctypes.byref(op), stream))
 
     def synchronize(self) -> None:
         _check(load_library().ctox_hip_synchronize(self.handle))

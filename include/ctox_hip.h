@@ -691,6 +691,39 @@ ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *backend, uint8_t *d_q
                                          const uint32_t *d_slots, size_t rows, size_t component_values,
                                          uint32_t page_tokens, uint32_t q4_slots, uint32_t q4_page_bytes, void *stream);
 
+/* Causal grouped-query attention of a ragged batch's new rows over the paged
+ * cache (Q/src/reference.rs:420-499 for many requests, any number of rows):
+ * request r's rows row_starts[r] .. row_starts[r + 1] - 1 are its last cached
+ * tokens of tokens[r], the first of its n rows sees tokens 0 .. tokens[r] - n,
+ * each next one more. query and out are [rows][query_heads][256], dense,
+ * 16-byte aligned; rows before row_starts[0] or from row_starts[requests] on are left as
+ * they are. descriptors is [requests][params.page_count]; tokens outside
+ * every page's [first_token, first_token + tokens) are absent. A row that sees no token
+ * gets zeros. Lengths are read on the device: a plan's row_starts and
+ * tokens (row_starts not falling, at most `rows`; tokens[r] at most
+ * min(page_count * page_tokens, 2^30)). max_rows bounds the rows of any one request (0:
+ * rows); a request with more than 16 queries per KV head needs max_rows to
+ * say so. params.tokens is not read. f32 results: products keep 22 bits of each
+ * query value and probability (21 of a query value for requests of at most 16 queries
+ * per KV head), the cached codes are exact, sums are 32 bits. Limits: head_dim 256,
+ * requests <= 4096, rows <= 2^20. workspace holds ctox_hip_paged_gqa_rows_workspace bytes (of
+ * the same op; its device pointers are not read), 16-byte aligned. */
+typedef struct {
+    const float *query;
+    float *out;
+    const uint8_t *q2_pages, *q4_pages;
+    const ctox_paged_kv_descriptor *descriptors;
+    const uint32_t *row_starts, *tokens;
+    uint64_t rows;
+    uint32_t requests, max_rows;
+    void *workspace;
+    uint64_t workspace_bytes;
+    ctox_paged_gqa_params params;
+} ctox_paged_gqa_rows;
+ctox_status ctox_hip_paged_gqa_rows_workspace(const ctox_hip_backend *backend, const ctox_paged_gqa_rows *op,
+                                              size_t *bytes);
+ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *backend, const ctox_paged_gqa_rows *op, void *stream);
+
 /* ---- decode engine helpers (device buffers) ---- */
 /* Seeded synthetic tensors (counter-based, reproducible for any sub-range):
  * kind 0 Q4_B64 blocks and 1 Q2_B64 blocks (uniform codes, fp16 scale

@@ -1,0 +1,355 @@
+"""GPU parity of the ragged batch's attention over the paged cache.
+
+Against the formula in float64 over the values that the pages stand for.
+Tolerance, with e = 2^-24, S = max over visible tokens of scale sum |q k|, and
+Y = sum p |v|:
+  * a score: the query keeps 21 bits or more (8 e), a 64-dim block is at most 128
+    rounded sums, four blocks and the scale 8 more: |ds| <= 144 e S; the
+    exponent's argument and 2^x add 4 e max(1, 2 S);
+  * a probability is off by a factor within 1 +- 2 |ds| or so, in numerator and
+    denominator: 4 (144 e S + 4 e max(1, 2 S));
+  * P s_v keeps 21 bits (8 e), a sum over T tokens rounds at most 2 T times (two
+    parts), the denominator T times, joins and the end 64 times.
+So |out - exact| <= Y e (4 (144 S + 4 max(1, 2 S)) + 8 + 3 T + 64).
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged_kv as pk
+
+pytestmark = pytest.mark.gpu
+
+Q2, Q4 = 0, 1
+BB = {Q2: 18, Q4: 34}
+HD = 256
+
+
+def say(*a):
+    print(*a, flush=True)
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+class Batch:
+    """Requests (cached, new) with random pages; pages chosen by `q2` lie in the Q2 pool."""
+
+    def __init__(self, seed, requests, page, heads, kv_heads, q2=lambda r, p: False, max_pages=None, pad=0,
+                 k_scale=2.4, v_scale=1.5, edit=None):
+        rng = np.random.default_rng(seed)
+        self.requests, self.page, self.H, self.KV = requests, page, heads, kv_heads
+        self.n = [b for _, b in requests]
+        self.tokens = [a + b for a, b in requests]
+        cv = kv_heads * HD
+        self.blocks = 2 * cv // 64
+        pages = [-(-t // page) for t in self.tokens]
+        self.max_pages = max(1, max(pages)) if max_pages is None else max_pages
+        kinds = [[Q2 if q2(r, p) else Q4 for p in range(pages[r])] for r in range(len(requests))]
+        self.pool, self.slots = {}, {}
+        for kind in (Q2, Q4):
+            count = sum(k == kind for ks in kinds for k in ks) + 2
+            raw = rng.integers(0, 256, (count, page, self.blocks, BB[kind])).astype(np.uint8)
+            s = np.abs(rng.standard_normal(raw.shape[:3])) * 0.3 + 1.0
+            s[..., :self.blocks // 2] *= k_scale
+            s[..., self.blocks // 2:] *= v_scale
+            raw[..., :2] = s.astype(np.float16).view(np.uint8).reshape(*raw.shape[:3], 2)
+            self.pool[kind], self.slots[kind] = raw, iter(rng.permutation(count))
+        self.desc = np.zeros((len(requests), self.max_pages, 4), np.uint32)
+        for r, ks in enumerate(kinds):
+            for p, kind in enumerate(ks):
+                self.desc[r, p] = (kind, next(self.slots[kind]), min(page, self.tokens[r] - p * page), p * page)
+        M = sum(self.n)
+        self.M = M
+        self.q = rng.standard_normal((M + pad, heads, HD)).astype(np.float32)
+        self.starts = np.concatenate([[0], np.cumsum(self.n)]).astype(np.int32)
+        if edit:
+            edit(self)
+
+    def token_values(self, r):
+        """(K, V [tokens][KV][HD] float64, present [tokens]) of request r from its pages."""
+        T = self.tokens[r]
+        out, present = np.zeros((T, self.blocks * 64)), np.zeros(T, bool)
+        for p in range(min(self.max_pages, -(-T // self.page))):
+            kind, slot, count, first = (int(x) for x in self.desc[r, p])
+            for j in range(p * self.page, min((p + 1) * self.page, T)):
+                if first <= j < first + count:
+                    present[j] = True
+                    raw = self.pool[kind][slot, j - first]
+                    out[j] = pk.dequantize_bytes(raw.tobytes(), kind)
+        half = self.blocks * 32
+        return out[:, :half].reshape(T, self.KV, HD), out[:, half:].reshape(T, self.KV, HD), present
+
+    def expect(self):
+        want = np.zeros((self.M, self.H, HD))
+        tol = np.zeros((self.M, self.H, HD))
+        G, e = self.H // self.KV, 2.0 ** -24
+        for r, (cached, n) in enumerate(self.requests):
+            if n == 0:
+                continue
+            K, V, present = self.token_values(r)
+            j = np.arange(self.tokens[r])
+            for h in range(self.H):
+                k, v = K[:, h // G], V[:, h // G]
+                for t in range(n):
+                    at = self.starts[r] + t
+                    see = present & (j <= cached + t)
+                    if not see.any():
+                        continue
+                    q = self.q[at, h].astype(np.float64)
+                    s = k[see] @ q / 16.0
+                    S = (np.abs(k[see]) @ np.abs(q) / 16.0).max()
+                    p = np.exp(s - s.max())
+                    p /= p.sum()
+                    want[at, h] = p @ v[see]
+                    tol[at, h] = (p @ np.abs(v[see])) * e * (4 * (144 * S + 4 * max(1, 2 * S)) + 72 + 3 * see.sum())
+        return want, tol
+
+    def op(self, hip, rows=None, max_rows=0, share=None):
+        import ctox_hip as ch
+        b4, b2 = self.blocks * 34, self.blocks * 18
+        if not hasattr(self, "d"):
+            self.d = {n: dev(v) for n, v in dict(
+                q=self.q, q2=self.pool[Q2].reshape(-1), q4=self.pool[Q4].reshape(-1), desc=self.desc.view(np.int32),
+                starts=self.starts, tokens=np.array(self.tokens, np.int32)).items()}
+            self.d["out"] = torch.full(self.q.shape, 7.0, device="cuda")
+        d = self.d
+        params = ch.PagedGqaParams(self.H, self.KV, HD, 0, self.page, self.max_pages, self.blocks * 64, b2, b4,
+                                   self.page * b2, self.page * b4, 1.0 / math.sqrt(HD))
+        op = ch.PagedGqaRows(d["q"].data_ptr(), d["out"].data_ptr(), d["q2"].data_ptr(), d["q4"].data_ptr(),
+                             d["desc"].data_ptr(), d["starts"].data_ptr(), d["tokens"].data_ptr(),
+                             self.q.shape[0] if rows is None else rows, len(self.requests), params, max_rows)
+        n = hip.paged_gqa_rows_workspace(op)
+        self.ws = torch.full((n + 64,), 0xEE, dtype=torch.uint8, device="cuda")
+        op.bind_workspace(self.ws.data_ptr(), n)
+        return op
+
+    def run(self, hip, **kw):
+        op = self.op(hip, **kw)
+        hip.paged_gqa_rows_device(op, torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert bool((self.ws[-64:] == 0xEE).all())
+        return self.d["out"].cpu().numpy()
+
+    def check(self, got):
+        want, tol = self.expect()
+        assert (got[self.M:] == 7.0).all()
+        err = np.abs(got[:self.M].astype(np.float64) - want)
+        bad = ~(err <= tol)
+        assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:5].tolist(), float(np.nanmax(err / np.maximum(tol, 1e-30))))
+
+
+def old(r, p):
+    return p % 3 == 1
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(24, 4), (4, 4), (8, 1), (2, 2)])
+@pytest.mark.parametrize("page", [16, 24, 7, 128])
+def test_one_request_many_rows(hip, page, heads, kv_heads):
+    say(f"case rows attention page={page} heads={heads}/{kv_heads}")
+    b = Batch(page + heads, [(150, 43)], page, heads, kv_heads, q2=old)
+    b.check(b.run(hip))
+
+
+@pytest.mark.parametrize("cached,new", [(0, 17), (0, 1), (0, 64), (127, 20), (128, 20), (129, 20), (255, 3), (256, 1),
+                                        (0, 300), (1000, 18), (513, 129)])
+def test_lengths(hip, cached, new):
+    say(f"case rows attention cached={cached} new={new}")
+    b = Batch(cached + new, [(cached, new)], 16, 6, 1, q2=lambda r, p: p % 4 == 2 and 16 * p + 16 < cached)
+    b.check(b.run(hip))
+
+
+@pytest.mark.parametrize("page", [16, 24])
+def test_ragged_batch(hip, page):
+    say(f"case rows attention ragged page={page}")
+    b = Batch(5, [(40, 1), (0, 70), (300, 0), (513, 2), (7, 30), (0, 0), (260, 3), (90, 90)], page, 12, 2, q2=old, pad=6)
+    b.check(b.run(hip))
+
+
+@pytest.mark.parametrize("page", [16, 8, 20])
+@pytest.mark.parametrize("count", [1, 3, 40])
+def test_single_tokens(hip, page, count):
+    say(f"case rows attention decode page={page} requests={count}")
+    rng = np.random.default_rng(count)
+    b = Batch(count + page, [(int(x), 1) for x in rng.integers(0, 700, count)], page, 24, 4, q2=old, pad=2)
+    b.check(b.run(hip, max_rows=1))
+
+
+def test_long_decode_in_several_runs_per_wave(hip):
+    """A context whose ranges exceed 64 tiles a wave: descriptors are read again."""
+    say("case rows attention long decode")
+    b = Batch(3, [(24000, 1)] * 24, 16, 8, 8, q2=lambda r, p: p > 8)
+    # the same pages for every request: only the first needs the reference
+    b.desc[1:] = b.desc[0]
+    b.q[1:] = b.q[0]
+    got = b.run(hip, max_rows=1)
+    assert (got[1:] == got[0]).all()
+    b.requests, b.M, b.n = b.requests[:1], 1, [1]
+    b.check(got[:1])
+
+
+def test_a_join_of_many_parts(hip):
+    say("case rows attention split")
+    b = Batch(9, [(5000, 40)], 16, 6, 1, q2=lambda r, p: p < 250)
+    b.check(b.run(hip))
+
+
+def test_absent_tokens_and_rows_that_see_nothing(hip):
+    say("case rows attention holes")
+
+    def edit(b):
+        b.desc[0, 0, 2] = 0                # the first pages are gone: rows 0.. of request 0 see nothing
+        b.desc[0, 1, 2] = 0
+        b.desc[1, 3, 2] = 5                # a page that holds less than it should
+        b.desc[2, 0] = (Q4, 0, 16, 16)     # a page of other tokens
+        b.desc[3, :, 2] = 0                # nothing at all, one row
+        b.desc[4, :, 2] = 0
+    b = Batch(13, [(0, 60), (80, 40), (10, 1), (30, 1), (30, 30)], 16, 6, 1, edit=edit, pad=1)
+    got = b.run(hip)
+    b.check(got)
+    assert (got[:32] == 0).all() and (got[101] == 0).all() and (got[102:132] == 0).all()
+
+
+def test_what_is_masked_does_not_count(hip):
+    """Infinities and NaN in later tokens of the chunk, past the end of the last page and in no page."""
+    say("case rows attention non-finite masked")
+    for kind in (0x7c00, 0x7e00, 0xfc00):
+        def edit(b):
+            raw = np.array([kind & 255, kind >> 8], np.uint8)
+            last = int(b.desc[0, 6, 1])
+            b.pool[Q4][last, 2:, :, :2] = raw        # tokens 98 .. (the chunk's rows 18 ..) and past the end
+            b.pool[Q4][last, 2:, :, 2:] = 255
+            spare = set(range(b.pool[Q4].shape[0])) - {int(s) for s in b.desc[:, :, 1].reshape(-1)}
+            for s in spare:
+                b.pool[Q4][s, :, :, :2] = raw
+        b = Batch(17, [(80, 22), (37, 1)], 16, 6, 1, edit=edit)
+        got = b.run(hip)
+        clean = Batch(17, [(80, 22), (37, 1)], 16, 6, 1)
+        want, tol = clean.expect()
+        keep = np.r_[0:18, 22]
+        err = np.abs(got[keep].astype(np.float64) - want[keep])
+        assert (err <= tol[keep]).all(), kind
+
+
+def test_non_finite_queries_stay_in_their_rows(hip):
+    say("case rows attention non-finite queries")
+    b = Batch(19, [(60, 30), (20, 1)], 16, 4, 2)
+    want, tol = b.expect()
+    b.q[5, 1, 7], b.q[11, 2, 200], b.q[30, 0, 3] = np.nan, np.inf, np.nan
+    got = b.run(hip)
+    for r, h in ((5, 1), (11, 2), (30, 0)):
+        assert np.isnan(got[r, h]).all()
+        got[r, h], want[r, h] = 0, 0
+    assert (np.abs(got - want) <= tol).all()
+
+
+@pytest.mark.parametrize("k_scale,v_scale", [(30.0, 1.0), (1e-3, 1e-4), (2.0, 3000.0)])
+def test_peaked_flat_and_scaled(hip, k_scale, v_scale):
+    say(f"case rows attention scales {k_scale} {v_scale}")
+    b = Batch(23, [(200, 25), (333, 1)], 16, 6, 1, q2=old, k_scale=k_scale, v_scale=v_scale)
+    b.check(b.run(hip))
+
+
+def test_value_scales_that_grow_and_shrink(hip):
+    say("case rows attention value scales over six orders")
+
+    def edit(b):
+        for kind in (Q2, Q4):
+            raw = b.pool[kind]
+            rng = np.random.default_rng(kind)
+            mag = 10.0 ** rng.uniform(-3, 3, raw.shape[:3])
+            raw[..., b.blocks // 2:, :2] = mag[..., b.blocks // 2:].astype(np.float16).view(np.uint8).reshape(
+                *raw.shape[:2], b.blocks // 2, 2)
+    b = Batch(29, [(700, 25), (300, 2)], 16, 6, 1, q2=old, edit=edit)
+    b.check(b.run(hip))
+
+
+def test_growing_scores_move_the_maximum(hip):
+    say("case rows attention growing scores")
+
+    def edit(b):
+        s = np.zeros((b.tokens[0],))
+        for p in range(-(-b.tokens[0] // b.page)):
+            slot = int(b.desc[0, p, 1])
+            raw = b.pool[Q4]
+            v = np.float16(0.02 * 1.35 ** p)
+            raw[slot, :, :b.blocks // 2, :2] = np.array([v]).view(np.uint8)
+    b = Batch(31, [(360, 40)], 16, 6, 1, edit=edit)
+    b.check(b.run(hip))
+
+
+def test_agrees_with_the_attention_of_one_sequence(hip):
+    import ctox_hip as ch
+    say("case rows attention against paged_gqa")
+    b = Batch(37, [(500, 5)], 16, 24, 4, q2=old)
+    got = b.run(hip)
+    b4, b2 = b.blocks * 34, b.blocks * 18
+    out = torch.empty(5, 24, HD, device="cuda")
+    params = ch.PagedGqaParams(24, 4, HD, 505, 16, b.max_pages, b.blocks * 64, b2, b4, 16 * b2, 16 * b4, 1 / 16.0)
+    hip.paged_gqa_device(b.d["q"].data_ptr(), b.d["q2"].data_ptr(), b.d["q4"].data_ptr(), b.d["desc"].data_ptr(), params, 5,
+                         out.data_ptr())
+    torch.cuda.synchronize()
+    _, tol = b.expect()
+    assert (np.abs(out.cpu().numpy() - got) <= 2 * tol).all()
+
+
+def test_repeats_replays_and_other_lengths(hip):
+    """One captured call, replayed for batches of other lengths with eager work in between."""
+    say("case rows attention graph")
+    cases = [[(40, 1), (0, 50), (100, 9)], [(0, 0), (200, 3), (77, 57)], [(10, 20), (30, 20), (250, 20)]]
+    first = Batch(41, cases[0], 16, 6, 1, max_pages=20, q2=old)
+    hold = first.op(hip, max_rows=60)
+    big = {n: torch.zeros(max(v.numel(), 1 << 16), dtype=v.dtype, device="cuda") for n, v in first.d.items()}
+    big["q2"] = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    big["q4"] = torch.zeros(1 << 21, dtype=torch.uint8, device="cuda")
+    big["q"], big["out"] = (torch.zeros(64 * 6 * HD, device="cuda") for _ in range(2))
+    hold.query, hold.out = big["q"].data_ptr(), big["out"].data_ptr()
+    hold.q2_pages, hold.q4_pages = big["q2"].data_ptr(), big["q4"].data_ptr()
+    hold.descriptors, hold.row_starts, hold.tokens = (big[n].data_ptr() for n in ("desc", "starts", "tokens"))
+    hold.rows = 64
+    ws = torch.empty(hip.paged_gqa_rows_workspace(hold), dtype=torch.uint8, device="cuda")
+    hold.bind_workspace(ws.data_ptr(), ws.numel())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        hip.paged_gqa_rows_device(hold, torch.cuda.current_stream().cuda_stream)
+    for seed, c in enumerate(cases):
+        b = Batch(seed, c, 16, 6, 1, max_pages=20, q2=old)
+        b.op(hip)
+        for n in ("q", "q2", "q4", "desc", "starts", "tokens"):
+            big[n][:b.d[n].numel()] = b.d[n].reshape(-1)
+        outs = []
+        for how in ("eager", "replay", "replay"):
+            big["out"].fill_(7.0)
+            ws.fill_(0xFF)
+            torch.cuda.synchronize()
+            if how == "eager":
+                hip.paged_gqa_rows_device(hold, torch.cuda.current_stream().cuda_stream)
+            else:
+                graph.replay()
+            torch.cuda.synchronize()
+            outs.append(big["out"].clone())
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+        b.check(outs[0].cpu().numpy().reshape(64, 6, HD))
+
+
+def test_refusals_with_a_backend(hip):
+    import ctox_hip as ch
+    say("case rows attention refusals")
+    b = Batch(43, [(20, 20)], 16, 6, 1)
+    for kind, edit in ((ch.MemoryBudget, lambda o: o.bind_workspace(o.workspace, o.workspace_bytes - 1)),
+                       (ch.MemoryBudget, lambda o: o.bind_workspace(None, o.workspace_bytes)),
+                       (ch.MemoryBudget, lambda o: o.bind_workspace(o.workspace + 8, o.workspace_bytes)),
+                       (ch.ShapeError, lambda o: setattr(o, "query", o.query + 4)),
+                       (ch.ShapeError, lambda o: setattr(o, "out", o.out + 8)),
+                       (ch.ShapeError, lambda o: setattr(o, "tokens", None))):
+        op = b.op(hip)
+        edit(op)
+        with pytest.raises(kind):
+            hip.paged_gqa_rows_device(op)
+    op = b.op(hip, rows=0)
+    hip.paged_gqa_rows_device(op)
+    torch.cuda.synchronize()
+    assert bool((b.d["out"] == 7.0).all())

@@ -117,3 +117,32 @@ def test_rows_workspace_refuses():
                        ((None, (1 << 20) + 1, 4), ctox_hip.ShapeError)):
         with pytest.raises(kind):
             ctox_hip._check(lib.ctox_hip_matrix_rows_workspace(*args, ctypes.byref(n)))
+
+
+def attention(params=None, **over):
+    p = dict(query_heads=24, key_value_heads=4, head_dim=256, tokens=0, page_tokens=16, page_count=8,
+             combined_values=2048, q2_token_bytes=576, q4_token_bytes=1088, q2_page_bytes=16 * 576,
+             q4_page_bytes=16 * 1088, scale=0.0625)
+    p.update(params or {})
+    kw = dict(d_query=P, d_out=P, d_q2_pages=P, d_q4_pages=P, d_descriptors=P, d_row_starts=P, d_tokens=P, rows=9,
+              requests=3)
+    kw.update(over)
+    lib, op, n = ctox_hip.load_library(), ctox_hip.PagedGqaRows(params=ctox_hip.PagedGqaParams(*p.values()), **kw), ctypes.c_size_t()
+    said = []
+    for f, args in (("ctox_hip_paged_gqa_rows_workspace", (ctypes.byref(n),)), ("ctox_hip_paged_gqa_rows_device", (None,))):
+        with pytest.raises(ctox_hip.EngineError) as e:
+            ctox_hip._check(getattr(lib, f)(None, ctypes.byref(op), *args))
+        said.append(str(e.value))
+    assert said[0] == said[1]
+    return said[0]
+
+
+@pytest.mark.parametrize("params,over,says", [
+    ({}, {}, "null argument"), (dict(head_dim=128), {}, "head_dim 256"), (dict(key_value_heads=0), {}, "contract"),
+    (dict(query_heads=22), {}, "contract"), (dict(page_tokens=0), {}, "contract"), (dict(page_count=0), {}, "contract"),
+    (dict(scale=float("inf")), {}, "contract"), (dict(combined_values=1024), {}, "geometry"),
+    (dict(q4_page_bytes=16 * 1088 - 4), {}, "geometry"), (dict(q2_page_bytes=16 * 576 + 2), {}, "geometry"),
+    ({}, dict(requests=0), "requests"), ({}, dict(requests=4097), "requests"), ({}, dict(rows=(1 << 20) + 1), "rows"),
+])
+def test_attention_refuses(params, over, says):
+    assert says in attention(params, **over)
