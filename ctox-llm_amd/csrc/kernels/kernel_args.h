@@ -677,6 +677,8 @@ struct GqaRowsArgs {
     uint32_t few;            // requests of at most 16 queries go to the few-query kernel
     uint32_t few_fill;
     float scale;
+    uint32_t page_magic;     // token / page_tokens = token * page_magic >> page_shift, tokens < 2^30
+    uint32_t page_shift;
     uint32_t pad;
 };
 

@@ -173,7 +173,7 @@ struct GrLds {
     float mx[2][4][GR_QUERIES];
     float vmax[2][8];
     float lsum[4][GR_QUERIES];
-    uint64_t tok[4][GR_TOKENS];  // address of the token's K run | kind << 62 (0 absent, 1 Q2, 2 Q4)
+    uint64_t tok[4][GR_TOKENS];  // address of the token's K run | kind << 62 (0 absent: the query's, 1 Q2, 2 Q4)
     uint64_t present[4][2];
     uint32_t holes[4][2];      // [tile][half]: a visible token of it is absent
     uint32_t flag[4];
@@ -181,7 +181,13 @@ struct GrLds {
 };
 
 __device__ __forceinline__ uint32_t gr_kind(uint64_t t) { return (uint32_t)(t >> 62); }
-__device__ __forceinline__ const uint8_t *gr_at(uint64_t t) { return (const uint8_t *)(t & 0x3fffffffffffffffull); }
+// (in the global address space by type: a table's address would else be read as a flat one)
+typedef const __attribute__((address_space(1))) uint8_t *gr_bytes;
+__device__ __forceinline__ gr_bytes gr_at(uint64_t t) { return (gr_bytes)(t & 0x3fffffffffffffffull); }
+template <typename T>
+__device__ __forceinline__ T gr_load(gr_bytes p) {
+    return *(const __attribute__((address_space(1))) T *)p;
+}
 
 // Eight 2-bit codes (low 16 bits) as eight 4-bit codes of the same value: c -> 5 c.
 __device__ __forceinline__ uint32_t gr_widen(uint32_t x) {
@@ -222,7 +228,8 @@ __device__ __forceinline__ void gr_split(const float (&x)[8], rm_h8 &hi, rm_h8 &
     for (int i = 0; i < 8; i += 2) {
         const float u = x[at[i]], v = x[at[i + 1]];
         const rm_h2 h = __builtin_bit_cast(rm_h2, __builtin_amdgcn_cvt_pkrtz(u, v));
-        const rm_h2 l = __builtin_bit_cast(rm_h2, __builtin_amdgcn_cvt_pkrtz(u - (float)h[0], v - (float)h[1]));
+        const rm_h2 l = __builtin_bit_cast(
+            rm_h2, __builtin_amdgcn_cvt_pkrtz(fmaf((float)h[0], -1.0f, u), fmaf((float)h[1], -1.0f, v)));
         hi[i] = h[0], hi[i + 1] = h[1];
         lo[i] = l[0], lo[i + 1] = l[1];
     }
@@ -300,90 +307,82 @@ extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_rows_gfx950(GqaRow
         qs = ldexpf(1.0f, e - 15);
     }
 
-    // Token -> address. A token past what the tile's queries see, or in no page, is absent.
+    // Token -> address. A token past what the tile's queries see, or in no page, is absent: its loads
+    // go to the query rows (always there, and long enough), its scales count as 0.
     PagedKvDesc dsc{0, 0, 0, 0};
     auto desc_load = [&](uint32_t t) {
         const uint32_t j = t * GR_TOKENS + tid;
-        dsc.tokens = 0;
-        if (t < t1 && j < vis) dsc = a.desc[(size_t)it.request * a.max_pages + j / a.page_tokens];
+        const uint32_t p = (uint32_t)(((uint64_t)j * a.page_magic) >> a.page_shift);
+        dsc = a.desc[(size_t)it.request * a.max_pages + (t < t1 && j < vis ? p : 0)];
     };
     auto desc_write = [&](uint32_t t) {
         const uint32_t j = t * GR_TOKENS + tid, tip = j - dsc.first_token;
-        uint64_t at = 0;
         const bool want = t < t1 && j < vis;
-        if (want && j >= dsc.first_token && tip < min(dsc.tokens, a.page_tokens))
-            at = dsc.precision ? (uint64_t)(uintptr_t)(a.q4 + (size_t)dsc.physical_slot * a.q4_page_bytes +
-                                                       (size_t)tip * a.q4_token_bytes + kvh * 136) | (2ull << 62)
-                               : (uint64_t)(uintptr_t)(a.q2 + (size_t)dsc.physical_slot * a.q2_page_bytes +
-                                                       (size_t)tip * a.q2_token_bytes + kvh * 72) | (1ull << 62);
-        L.tok[t & 3][tid] = at;
-        const uint64_t here = __builtin_amdgcn_ballot_w64(at != 0);
-        const uint64_t gone = __builtin_amdgcn_ballot_w64(want && at == 0);
+        const bool in = want && j >= dsc.first_token && tip < min(dsc.tokens, a.page_tokens), q4 = dsc.precision != 0;
+        const uint8_t *pool = q4 ? a.q4 : a.q2;
+        const uint8_t *run = pool + (size_t)dsc.physical_slot * (q4 ? a.q4_page_bytes : a.q2_page_bytes) +
+                             (size_t)tip * (q4 ? a.q4_token_bytes : a.q2_token_bytes) + kvh * (q4 ? 136 : 72);
+        L.tok[t & 3][tid] = in ? (uint64_t)(uintptr_t)run | (q4 ? 2ull << 62 : 1ull << 62) : (uint64_t)(uintptr_t)a.query;
+        const uint64_t here = __builtin_amdgcn_ballot_w64(in);
+        const uint64_t gone = __builtin_amdgcn_ballot_w64(want && !in);
         if (lane == 0) {
             L.present[t & 3][wave] = here;
             L.holes[t & 3][wave] = gone != 0;
         }
     };
 
-    // Keys: this lane's half of four blocks of one token, and two of its scales.
+    // Keys: this lane's half of four blocks of one token, and two of its scales. A Q2 half is 8 of
+    // the 16 bytes read (what lies behind is the token's own).
     uint32_t kw[4][4];
     uint32_t kkind = 0, ksc[2];
     auto issue_k = [&](uint32_t t) {
-        const uint64_t at = t < t1 ? L.tok[t & 3][32 * tw + li] : 0;
-        const uint8_t *p = gr_at(at);
+        const uint64_t at = L.tok[t & 3][32 * tw + li];
         kkind = gr_kind(at);
-        ksc[0] = ksc[1] = 0;
-        if (kkind == 2) {
+        const uint32_t step = kkind == 1 ? 18 : 34;
+        const gr_bytes p = gr_at(at), c = p + 2 + (kkind == 1 ? 8 * h : 16 * h);
 #pragma unroll
-            for (int b = 0; b < 4; b++) {
-                const GrBytes16 x = *(const GrBytes16 *)(p + 34 * b + 2 + 16 * h);
+        for (int b = 0; b < 4; b++) {
+            const GrBytes16 x = gr_load<GrBytes16>(c + b * step);
 #pragma unroll
-                for (int i = 0; i < 4; i++) kw[b][i] = x.w[i];
-            }
-            ksc[0] = *(const uint16_t *)(p + 68 * h);
-            ksc[1] = *(const uint16_t *)(p + 68 * h + 34);
-        } else if (kkind == 1) {
-#pragma unroll
-            for (int b = 0; b < 4; b++) {
-                const GrBytes8 x = *(const GrBytes8 *)(p + 18 * b + 2 + 8 * h);
-                kw[b][0] = x.w[0], kw[b][1] = x.w[1];
-            }
-            ksc[0] = *(const uint16_t *)(p + 36 * h);
-            ksc[1] = *(const uint16_t *)(p + 36 * h + 18);
+            for (int i = 0; i < 4; i++) kw[b][i] = x.w[i];
         }
+        const gr_bytes sc = p + 2 * h * step;
+        ksc[0] = gr_load<uint16_t>(sc);
+        ksc[1] = gr_load<uint16_t>(sc + step);
     };
-    // Values: eight code bytes (Q4) of four tokens of one block; one scale.
+    // Values: eight code bytes (Q4) of four tokens of one block; one scale. The four bytes of a Q2 token
+    // are one half of an eight-byte piece of its block.
     const uint32_t vq = tid & 31, vb = (tid >> 5) & 3, vo = tid >> 7;  // token quad, block, octet of bytes
     const uint32_t sb = wave >> 1, st = tid & 127;                      // scale: block, token
-    uint32_t vw[4][2];
-    uint32_t vkind[4], vsc = 0;
+    const uint32_t vc4 = a.v_off4 + 34 * vb + 2 + 8 * vo, vc2 = a.v_off2 + 18 * vb + 2 + 8 * (vo >> 1);
+    const uint32_t vs4 = a.v_off4 + 34 * sb, vs2 = a.v_off2 + 18 * sb;
+    uint32_t vw[4][2], vtwo = 0, vsc = 0;  // vtwo: bit i where token i is Q2
+    bool vsk = false;
     auto issue_v = [&](uint32_t t) {
+        vtwo = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const uint64_t at = t < t1 ? L.tok[t & 3][4 * vq + i] : 0;
-            vkind[i] = gr_kind(at);
-            const uint8_t *p = gr_at(at);
-            vw[i][0] = vw[i][1] = 0;
-            if (vkind[i] == 2) {
-                const GrBytes8 x = *(const GrBytes8 *)(p + a.v_off4 + 34 * vb + 2 + 8 * vo);
-                vw[i][0] = x.w[0], vw[i][1] = x.w[1];
-            } else if (vkind[i] == 1) {
-                vw[i][0] = ((const GrBytes4 *)(p + a.v_off2 + 18 * vb + 2 + 4 * vo))->w;
-            }
+            const uint64_t at = L.tok[t & 3][4 * vq + i];
+            const bool two = gr_kind(at) == 1;
+            vtwo |= two ? 1u << i : 0u;
+            const GrBytes8 x = gr_load<GrBytes8>(gr_at(at) + (two ? vc2 : vc4));
+            vw[i][0] = x.w[0], vw[i][1] = x.w[1];
         }
-        const uint64_t at = t < t1 ? L.tok[t & 3][st] : 0;
-        const uint32_t k = gr_kind(at);
-        vsc = 0;
-        if (k) vsc = *(const uint16_t *)(gr_at(at) + (k == 2 ? a.v_off4 + 34 * sb : a.v_off2 + 18 * sb));
+        const uint64_t at = L.tok[t & 3][st];
+        vsk = gr_kind(at) != 0;
+        vsc = gr_load<uint16_t>(gr_at(at) + (gr_kind(at) == 1 ? vs2 : vs4));
     };
     auto write_v = [&](uint32_t t) {
         const uint32_t buf = t & 1;
+        if (__builtin_amdgcn_ballot_w64(vtwo != 0)) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (vkind[i] == 1) {
-                vw[i][1] = gr_widen(vw[i][0] >> 16);
-                vw[i][0] = gr_widen(vw[i][0]);
+            for (int i = 0; i < 4; i++) {
+                const uint32_t x = vo & 1 ? vw[i][1] : vw[i][0];
+                const bool two = vtwo >> i & 1;
+                vw[i][0] = two ? gr_widen(x) : vw[i][0];
+                vw[i][1] = two ? gr_widen(x >> 16) : vw[i][1];
             }
+        }
 #pragma unroll
         for (int w = 0; w < 2; w++) {
             // 4 x 4 bytes across: byte r of the four tokens into one dword.
@@ -397,7 +396,7 @@ extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_rows_gfx950(GqaRow
             L.v[buf][vb][r + 2][vq] = __builtin_amdgcn_perm(cd1, ab1, 0x05040100u);
             L.v[buf][vb][r + 3][vq] = __builtin_amdgcn_perm(cd1, ab1, 0x07060302u);
         }
-        const float s = (float)__builtin_bit_cast(_Float16, (uint16_t)vsc);
+        const float s = vsk ? (float)__builtin_bit_cast(_Float16, (uint16_t)vsc) : 0.0f;
         L.vs[buf][sb][st] = s;
         float m = fabsf(s) < INFINITY ? fabsf(s) : 0.0f;
 #pragma unroll
@@ -431,23 +430,21 @@ extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_rows_gfx950(GqaRow
         issue_v(t + 1);
         if (tid < GR_TOKENS) desc_load(t + 3);
         // ---- scores ----
-        if (kkind == 1) {
+        if (__builtin_amdgcn_ballot_w64(kkind == 1)) {
+            const bool two = kkind == 1;
 #pragma unroll
             for (int b = 0; b < 4; b++) {
-                kw[b][3] = gr_widen(kw[b][1] >> 16);
-                kw[b][2] = gr_widen(kw[b][1]);
-                kw[b][1] = gr_widen(kw[b][0] >> 16);
-                kw[b][0] = gr_widen(kw[b][0]);
+                const uint32_t x = kw[b][0], y = kw[b][1];
+                kw[b][0] = two ? gr_widen(x) : kw[b][0];
+                kw[b][1] = two ? gr_widen(x >> 16) : kw[b][1];
+                kw[b][2] = two ? gr_widen(y) : kw[b][2];
+                kw[b][3] = two ? gr_widen(y >> 16) : kw[b][3];
             }
-        } else if (kkind == 0) {
-#pragma unroll
-            for (int b = 0; b < 4; b++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) kw[b][i] = 0;
         }
 #pragma unroll
         for (int i = 0; i < 2; i++)
-            L.ks[wave][2 * h + i][li] = (float)__builtin_bit_cast(_Float16, (uint16_t)ksc[i]) * (1.0f / 15.0f);
+            L.ks[wave][2 * h + i][li] =
+                kkind ? (float)__builtin_bit_cast(_Float16, (uint16_t)ksc[i]) * (1.0f / 15.0f) : 0.0f;
         lds_wave_order();
         gr_v16 s;
 #pragma unroll

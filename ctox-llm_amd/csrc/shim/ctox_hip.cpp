@@ -3064,6 +3064,12 @@ extern "C" ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *b, const
     a.few = g.few;
     a.few_fill = g.few_fill;
     a.scale = p.scale;
+    // ceil(2^(30 + l) / d) with 2^l >= d: its error, below 1 / 2^(30 + l), times a token below 2^30 stays below
+    // the 1 / d that would reach the next quotient.
+    uint32_t l = 0;
+    while (l < 31 && (1u << l) < p.page_tokens) l++;
+    a.page_shift = 30 + l;
+    a.page_magic = (uint32_t)(((1ull << a.page_shift) + p.page_tokens - 1) / p.page_tokens);
     OnDevice on(b);
     hipStream_t s = (hipStream_t)stream;
     ctox_status st = CTOX_OK;
