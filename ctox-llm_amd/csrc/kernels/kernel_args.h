@@ -656,8 +656,8 @@ struct GqaRowsArgs {
     const PagedKvDesc *desc; // [requests][max_pages]
     const uint32_t *row_starts;  // [requests + 1]
     const uint32_t *tokens;      // [requests]
-    float *part;             // [item]: [64][256] numerators, [64][2] (max base 2, denominator)
-    float *few_part;         // [item]: [16][256], [16][2] (max, denominator)
+    float *part;             // [item]: [128][256] numerators, [128][2] (max base 2, denominator)
+    float *few_part;         // [item]: the same of 32 queries
     uint64_t q2_page_bytes;
     uint64_t q4_page_bytes;
     uint32_t requests;
@@ -672,10 +672,12 @@ struct GqaRowsArgs {
     uint32_t q4_token_bytes;
     uint32_t v_off2;         // bytes from a token's K run of a head to its V run
     uint32_t v_off4;
-    uint32_t split;          // token ranges are split and joined
-    uint32_t fill;           // workgroups that fill the chip, 64-query kernel
-    uint32_t few;            // requests of at most 16 queries go to the few-query kernel
-    uint32_t few_fill;
+    uint32_t split;          // the 128-query kernel's token ranges are split and joined
+    uint32_t slots;          // its workgroups that run at once
+    uint32_t items;          // most items it may be cut into
+    uint32_t few;            // requests of at most 32 queries a KV head go to the few-query kernel
+    uint32_t few_slots;
+    uint32_t few_items;
     float scale;
     uint32_t page_magic;     // token / page_tokens = token * page_magic >> page_shift, tokens < 2^30
     uint32_t page_shift;

@@ -939,19 +939,19 @@ struct PaLds16 {
 // grid (splits, kv heads), 256 threads; four waves take contiguous runs of
 // tiles_per_wave (<= 64) page-aligned tiles. Lane (li, lg) ends with O^T of
 // query 16 r + li at dims 64 b + 16 lg + 4 i + c in o[r][4 b + c][i].
-// LONG: a wave may take more than 64 tiles; their descriptors are then read 64 at a time.
-template <int R, bool LONG = false>
-__device__ __forceinline__ void paged_gqa_partial16(const GqaArgs &a, uint32_t h, uint32_t split, size_t base) {
+template <int R>
+__device__ __forceinline__ void paged_gqa_partial16(const GqaArgs &a) {
     __shared__ PaLds16<R> L;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t li = lane & 15, lg = lane >> 4;
+    const uint32_t h = blockIdx.y, split = blockIdx.x;
     const uint32_t gw = split * 4 + wave;
     const uint32_t t0 = gw * a.tiles_per_wave;
     const uint32_t t1 = min(t0 + a.tiles_per_wave, a.tiles);
     // The wave's page descriptors load together with the queries; the first
     // tile's loads go out (they need only the descriptors) before the query
     // limbs are computed.
-    uint4 dsc = pa_load_descs(a, t0, LONG ? min(t0 + 64, t1) : t1, lane);
+    const uint4 dsc = pa_load_descs(a, t0, t1, lane);
     float qv[R][16];
     pa_prep_load<R>(a, h, qv);
     PaStage sg;
@@ -991,14 +991,13 @@ __device__ __forceinline__ void paged_gqa_partial16(const GqaArgs &a, uint32_t h
         constexpr int Q4 = decltype(q4c)::value;
         for (uint32_t tile = t0; tile < t1; tile++) {
             pa_stage_write(stage, lane, Q4 >= 0 ? Q4 == 1 : PA.q4 != 0, sg);
-            if (LONG && (tile + 1 - t0) % 64 == 0) dsc = pa_load_descs(a, tile + 1, min(tile + 65, t1), lane);
-            const PaTile PN = pa_tile_of(a, dsc, LONG ? (tile + 1 - t0) % 64 : tile + 1 - t0);
+            const PaTile PN = pa_tile_of(a, dsc, tile + 1 - t0);
             pa_issue_stage(a, PN, (tile + 1) * 16, h, lane, sg);
             pa_tile16<R, Q4, SH>(a, L, L.u.run.limbs, wave, tile * 16, h, li, lg, PA, stage, qsl, st);
             PA = PN;
         }
     };
-    if ((!LONG || t1 <= t0 + 64) && __builtin_amdgcn_ballot_w64(lane < t1 - t0 && dsc.x != 0) == 0)
+    if (__builtin_amdgcn_ballot_w64(lane < t1 - t0 && dsc.x != 0) == 0)
         run(std::integral_constant<int, 0>{});
     else
         run(std::integral_constant<int, -1>{});
@@ -1043,6 +1042,7 @@ __device__ __forceinline__ void paged_gqa_partial16(const GqaArgs &a, uint32_t h
     __syncthreads();
     if (wave != 0) return;
     // Partial layout: [kv head][split][query][PA_HD]; stats [kv head][split][query][2].
+    const size_t base = ((size_t)h * a.splits + split) * a.queries;
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const uint32_t qi = 16 * r + li;
@@ -1085,10 +1085,11 @@ __device__ __forceinline__ void paged_gqa_partial16(const GqaArgs &a, uint32_t h
 
 
 template <int R>
-__device__ __forceinline__ void paged_gqa_partial(const GqaArgs &a, uint32_t h, uint32_t split, size_t base) {
+__device__ __forceinline__ void paged_gqa_partial(const GqaArgs &a) {
     __shared__ PaLds<R> L;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t li = lane & 15, lg = lane >> 4;
+    const uint32_t h = blockIdx.y, split = blockIdx.x;
     const uint32_t gw = split * 4 + wave;
     const uint32_t t0 = gw * a.tiles_per_wave;
     const uint32_t t1 = min(t0 + a.tiles_per_wave, a.tiles);
@@ -1194,6 +1195,7 @@ __device__ __forceinline__ void paged_gqa_partial(const GqaArgs &a, uint32_t h, 
     }
     if (wave != 0) return;
     // Partial layout: [kv head][split][query][PA_HD]; stats [kv head][split][query][2].
+    const size_t base = ((size_t)h * a.splits + split) * a.queries;
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const uint32_t qi = 16 * r + li;
@@ -1210,23 +1212,18 @@ __device__ __forceinline__ void paged_gqa_partial(const GqaArgs &a, uint32_t h, 
     }
 }
 
-// First partial row of this workgroup.
-__device__ __forceinline__ size_t pa_base(const GqaArgs &a) {
-    return ((size_t)blockIdx.y * a.splits + blockIdx.x) * a.queries;
-}
-
 extern "C" __global__ __launch_bounds__(256, 2) void ctox_paged_gqa_partial_r1_gfx950(GqaArgs a) {
-    paged_gqa_partial<1>(a, blockIdx.y, blockIdx.x, pa_base(a));
+    paged_gqa_partial<1>(a);
 }
 extern "C" __global__ __launch_bounds__(256, 1) void ctox_paged_gqa_partial_r2_gfx950(GqaArgs a) {
-    paged_gqa_partial<2>(a, blockIdx.y, blockIdx.x, pa_base(a));
+    paged_gqa_partial<2>(a);
 }
 // Page-aligned tiles (page_tokens % 16 == 0): P.V on f16 MFMA.
 extern "C" __global__ __launch_bounds__(256, 2) void ctox_paged_gqa_partial16_r1_gfx950(GqaArgs a) {
-    paged_gqa_partial16<1>(a, blockIdx.y, blockIdx.x, pa_base(a));
+    paged_gqa_partial16<1>(a);
 }
 extern "C" __global__ __launch_bounds__(256, 1) void ctox_paged_gqa_partial16_r2_gfx950(GqaArgs a) {
-    paged_gqa_partial16<2>(a, blockIdx.y, blockIdx.x, pa_base(a));
+    paged_gqa_partial16<2>(a);
 }
 
 #define PA_MAX_SPLITS 1024

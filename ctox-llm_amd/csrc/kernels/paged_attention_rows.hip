@@ -4,32 +4,32 @@
 //
 // A request's n new rows are its last n cached tokens; row t sees tokens 0 .. tokens - n + t.
 // Its queries are the pairs (row, head of the KV group), numbered row * group + head, so
-// that all heads that share a KV head share what is read of it. Three kernels:
+// that all heads that share a KV head share what is read of it.
 //
-//  * ctox_gqa_rows_gfx950: 64 queries of one KV head a workgroup (below).
-//  * ctox_gqa_few_gfx950: requests of at most 16 queries a KV head (decoded tokens), on the
-//    split-KV kernel of paged_attention.hip, which is bound by the cache's bytes.
+//  * ctox_gqa_rows_gfx950: 128 queries of one KV head a workgroup.
+//  * ctox_gqa_few_gfx950: the same for requests of at most 32 queries a KV head (decoded tokens,
+//    verified drafts), 32 queries a workgroup.
 //  * ctox_gqa_join_gfx950: joins the parts of a split token range.
 //
 // Which workgroup takes what is decided on the device from row_starts and tokens, so the
-// host needs no lengths and a captured launch stays right for other lengths. Every
-// workgroup adds up the batch's work for itself and finds its own item: a token range of one
-// query tile (or, few, of one request) and KV head. Ranges are made so long that the
-// items fill the chip about once.
+// host needs no lengths and a captured launch stays right for other lengths: every workgroup
+// works out for itself how the batch is cut (gr_range) and finds its own item, a token range
+// of one query tile and KV head.
 //
-// The 64-query kernel. Eight waves walk the tokens 128 at a time.
-//  Scores: wave (tw, qw) takes S^T = K Q^T of 32 tokens x 32 queries on f16 MFMA 32x32x16. K
-//    enters as the exact whole numbers 2c - 15 (a Q2 code c is the Q4 code 5c), a 64-dim block's
-//    sum is then multiplied by its f32 scale. A query is two f16 parts of q 2^-e (22 bits), held in
-//    LDS.
-//  Softmax: probabilities are 2^(s - m) with m the queries' maxima of earlier tiles; only when a
-//    score exceeds m by more than 2^6 is m moved and the tile's probabilities made again, so that
-//    no wave waits for the others' maxima. Sums are f32.
-//  Values: probabilities pass through LDS. Wave (blk, th) adds O^T += V^T (P s_v)^T for 64 dims, 64
-//    queries and 64 of the tokens, s_v the value block's scale: V is exact again, P s_v is two f16
-//    parts in units of 2^(E - 9) with 2^E above every scale so far. V's bytes are transposed on
-//    their way into LDS (a lane's operand is one byte column of eight tokens).
-// Loads of the next tile are under way during this one; page descriptors are read three ahead.
+// A wave takes 32 queries and walks tiles of 32 tokens; the waves of a workgroup are four (or
+// one) query subtiles times two (or four) shares of the tiles, and meet only at the end.
+//  Scores: S^T = K Q^T on f16 MFMA 32x32x16. K enters as the exact whole numbers 2c - 15 (a Q2
+//    code c is the Q4 code 5c), a 64-dim block's sum is then multiplied by its f32 scale. A query
+//    is two f16 parts of q 2^-e (22 bits), held in LDS.
+//  Softmax: a lane's sixteen scores belong to one query. Probabilities are 2^(s - m) with m the
+//    query's maximum at some earlier tile; only when a score exceeds m by more than GR_MOVE is m moved
+//    and the sums rescaled.
+//  Values: O^T += V^T (P s_v)^T. The scores' output layout is the probabilities' operand layout if the
+//    tokens are counted as gr_v_operands does, so they stay in registers. s_v is the value block's
+//    scale: V is exact again, P s_v is two f16 parts in units of 2^(E - 9) with 2^E above every scale
+//    of the dim block so far. V's bytes are transposed on their way through LDS, a lane's operand being
+//    one byte column of eight tokens.
+// Loads of the next tile are under way during this one, its page descriptors one tile before that.
 #include <hip/hip_runtime.h>
 
 #include "kernel_args.h"
@@ -37,18 +37,14 @@
 
 typedef float gr_v16 __attribute__((ext_vector_type(16)));
 
-#define GR_QUERIES 64
-#define GR_TOKENS 128
 #define GR_MOVE 6.0f  // base-2 slack before the running maximum moves
+#define GR_FEW 32     // queries of a request's KV head that the few-query kernel takes
 
 struct __attribute__((packed, aligned(2))) GrBytes16 {
     uint32_t w[4];
 };
 struct __attribute__((packed, aligned(2))) GrBytes8 {
     uint32_t w[2];
-};
-struct __attribute__((packed, aligned(2))) GrBytes4 {
-    uint32_t w;
 };
 
 // ---------------------------------------------------------------------------
@@ -60,57 +56,72 @@ struct GrRequest {
 
 __device__ __forceinline__ GrRequest gr_request(const GqaRowsArgs &a, uint32_t r) {
     const uint32_t s = min(a.row_starts[r], a.rows), e = min(a.row_starts[r + 1], a.rows);
-    GrRequest q{s, e > s ? e - s : 0u, a.tokens[r]};
-    q.tokens = min(q.tokens, a.max_tokens);
-    return q;
+    return {s, e > s ? e - s : 0u, min(a.tokens[r], a.max_tokens)};
 }
 
 __device__ __forceinline__ bool gr_few(const GqaRowsArgs &a, const GrRequest &q) {
-    return a.few && q.rows && q.rows * a.group <= 16;
+    return a.few && q.rows * a.group <= GR_FEW;
 }
 
-// Of one request: query tiles and units of the token axis (16 tokens for few queries, 128 else).
+// Of one request: query tiles, and units of the token axis (as many as a workgroup's waves take at once).
 struct GrShape {
     uint32_t qt, units;
 };
 __device__ __forceinline__ GrShape gr_shape(const GqaRowsArgs &a, const GrRequest &q, bool few) {
     GrShape s{0, 0};
     if (q.rows == 0 || gr_few(a, q) != few) return s;
-    s.qt = few ? 1u : (uint32_t)(((uint64_t)q.rows * a.group + GR_QUERIES - 1) / GR_QUERIES);
-    s.units = few ? max(1u, (q.tokens + 15) / 16) : max(1u, (q.tokens + GR_TOKENS - 1) / GR_TOKENS);
+    s.qt = few ? 1u : (q.rows * a.group + 127) / 128;
+    s.units = max(1u, few ? (q.tokens + 127) / 128 : (q.tokens + 63) / 64);
     return s;
 }
 
 struct GrScratch {
-    uint64_t sum[8];
+    uint32_t count[32], longest, range;
     uint32_t scan[8];
     uint32_t found[4];
 };
 
-__device__ __forceinline__ uint64_t gr_wave_sum(uint64_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-
-// Units a range may hold: few, a multiple of four (one run per wave).
+// Units of one item. Candidates: the longest request in n = 1 .. 16 and on to 256 ranges. A candidate
+// takes as many rounds of the chip as its items fill it, each as long as a range and the
+// GR_START units that a workgroup spends on starting and joining; the cheapest one is taken. n = 1
+// is always allowed, the others up to the items that the workspace holds.
+#define GR_START 3
 template <int NT>
 __device__ __forceinline__ uint32_t gr_range(const GqaRowsArgs &a, bool few, GrScratch &L) {
-    if (!few && !a.split) return 0xffffffffu;
-    uint64_t work = 0;
-    for (uint32_t r = threadIdx.x; r < a.requests; r += NT) {
-        const GrShape s = gr_shape(a, gr_request(a, r), few);
-        work += (uint64_t)s.qt * s.units;
-    }
-    work = gr_wave_sum(work);
-    if ((threadIdx.x & 63) == 0) L.sum[threadIdx.x >> 6] = work;
+    const uint32_t slots = few ? a.few_slots : a.slots, most = few ? a.few_items : a.items;
+    if ((!few && !a.split) || a.requests > 512) return 0x3fffffffu;
+    const uint32_t tid = threadIdx.x, c = tid & 31;
+    if (tid < 32) L.count[tid] = 0;
+    if (tid == 0) L.longest = 1;
     __syncthreads();
-    work = 0;
+    for (uint32_t r = tid; r < a.requests; r += NT) {
+        const GrShape s = gr_shape(a, gr_request(a, r), few);
+        if (s.qt) atomicMax(&L.longest, s.units);
+    }
+    __syncthreads();
+    const uint32_t n = c < 16 ? c + 1 : (uint32_t)(16.0f * __builtin_amdgcn_exp2f((float)(c - 15) * 0.25f));
+    const uint32_t range = (L.longest + n - 1) / n;
+    uint32_t items = 0;
+    for (uint32_t r = tid >> 5; r < a.requests; r += NT / 32) {
+        const GrShape s = gr_shape(a, gr_request(a, r), few);
+        items += s.qt * ((s.units + range - 1) / range);
+    }
+    atomicAdd(&L.count[c], items);  // whole numbers: their order does not matter
+    __syncthreads();
+    if (tid < 32) {
+        const uint32_t k = L.count[c] * a.kv_heads;
+        uint64_t cost = min((uint64_t)((k + slots - 1) / slots) * (range + GR_START), (uint64_t)0xfffffffe);
+        if (c && k > most) cost = 0xffffffff;
+        cost = cost << 32 | range;
 #pragma unroll
-    for (int w = 0; w < NT / 64; w++) work += L.sum[w];
-    const uint32_t fill = few ? 4 * a.few_fill : a.fill;
-    const uint32_t per = (uint32_t)min((work * a.kv_heads + fill - 1) / fill, (uint64_t)0x3fffffff);
-    return few ? 4 * max(1u, per) : max(1u, per);
+        for (int o = 16; o > 0; o >>= 1) {
+            const uint64_t x = __shfl_xor(cost, o);
+            cost = x < cost ? x : cost;
+        }
+        if (tid == 0) L.range = (uint32_t)cost;
+    }
+    __syncthreads();
+    return L.range;
 }
 
 struct GrItem {
@@ -130,7 +141,7 @@ __device__ __forceinline__ GrItem gr_find(const GqaRowsArgs &a, bool few, uint32
         uint32_t n = 0, ranges = 0;
         if (r < a.requests) {
             const GrShape s = gr_shape(a, gr_request(a, r), few);
-            ranges = (uint32_t)(((uint64_t)s.units + range - 1) / range);
+            ranges = (s.units + range - 1) / range;
             n = s.qt * ranges * a.kv_heads;
         }
         uint32_t in = n;
@@ -162,24 +173,8 @@ __device__ __forceinline__ GrItem gr_find(const GqaRowsArgs &a, bool few, uint32
 }
 
 // ---------------------------------------------------------------------------
-// the 64-query kernel
+// operands
 // ---------------------------------------------------------------------------
-struct GrLds {
-    float4 p[8][4][64];        // [tw + 4 qw][token octet j][lane]: tokens 8 j + 4 (lane / 32) ..
-    uint32_t v[2][4][32][33];  // [buffer][block][code byte][token / 4]: that byte of four tokens
-    rm_h8 q[2][2][16][64];     // [qw][lo, hi][k step][lane]
-    float vs[2][4][GR_TOKENS]; // [buffer][block][token]: value scale
-    float ks[8][4][32];        // [wave][block][token]: key scale / 15
-    float mx[2][4][GR_QUERIES];
-    float vmax[2][8];
-    float lsum[4][GR_QUERIES];
-    uint64_t tok[4][GR_TOKENS];  // address of the token's K run | kind << 62 (0 absent: the query's, 1 Q2, 2 Q4)
-    uint64_t present[4][2];
-    uint32_t holes[4][2];      // [tile][half]: a visible token of it is absent
-    uint32_t flag[4];
-    GrScratch scratch;
-};
-
 __device__ __forceinline__ uint32_t gr_kind(uint64_t t) { return (uint32_t)(t >> 62); }
 // (in the global address space by type: a table's address would else be read as a flat one)
 typedef const __attribute__((address_space(1))) uint8_t *gr_bytes;
@@ -198,75 +193,178 @@ __device__ __forceinline__ uint32_t gr_widen(uint32_t x) {
     return x | (x << 2);
 }
 
-__device__ __forceinline__ rm_h8 gr_k_operand(uint32_t x) {
-    const rm_h2 a = rm_pair<4, 15>(x << 4), b = rm_pair<4, 15>(x), c = rm_pair<4, 15>(x >> 4), d = rm_pair<4, 15>(x >> 8);
-    return rm_h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+__device__ __forceinline__ rm_h8 gr_k_operand(uint32_t x, const RmMagic &g) {
+    const uint32_t w[4] = {x, x, x, x};
+    return rm_unpack<true>(w, 0, g);
 }
 
 // Code byte of tokens 0..3 (x) and 4..7 (y) as operands: even dim (low nibble), odd dim; token
 // order 0 2 1 3 4 6 5 7.
-__device__ __forceinline__ void gr_v_operands(uint32_t x, uint32_t y, rm_h8 (&o)[2]) {
-    const rm_h2 a = rm_pair<4, 15>(x << 4), b = rm_pair<4, 15>(x >> 4), c = rm_pair<4, 15>(y << 4), d = rm_pair<4, 15>(y >> 4);
-    const rm_h2 e = rm_pair<4, 15>(x), f = rm_pair<4, 15>(x >> 8), g = rm_pair<4, 15>(y), h = rm_pair<4, 15>(y >> 8);
+__device__ __forceinline__ void gr_v_operands(uint32_t x, uint32_t y, const RmMagic &g, rm_h8 (&o)[2]) {
+    auto two = [&](uint32_t v) { return rm_pair<4, 15>(v, g.m[0], g.magic); };
+    const rm_h2 a = two(x << 4), b = two(x >> 4), c = two(y << 4), d = two(y >> 4);
+    const rm_h2 e = two(x), f = two(x >> 8), p = two(y), q = two(y >> 8);
     o[0] = rm_h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-    o[1] = rm_h8{e[0], e[1], f[0], f[1], g[0], g[1], h[0], h[1]};
-}
-
-// 0 times anything is 0 here: a probability of zero leaves a masked token's scale out, be it
-// infinite or no number.
-__device__ __forceinline__ float gr_mul(float p, float s) {
-    float x;
-    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(x) : "v"(p), "v"(s));
-    return x;
+    o[1] = rm_h8{e[0], e[1], f[0], f[1], p[0], p[1], q[0], q[1]};
 }
 
 // Two f16 parts of eight values in the value operand's token order. hi is rounded towards zero, so
 // what is left has hi's sign and at most 13 bits.
-__device__ __forceinline__ void gr_split(const float (&x)[8], rm_h8 &hi, rm_h8 &lo) {
+// (x - hi is one mixed-precision multiply-add by an opaque -1; a plain difference would convert first.)
+__device__ __forceinline__ void gr_split(const float (&x)[8], float minus_one, rm_h8 &hi, rm_h8 &lo) {
     constexpr int at[8] = {0, 2, 1, 3, 4, 6, 5, 7};
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         const float u = x[at[i]], v = x[at[i + 1]];
         const rm_h2 h = __builtin_bit_cast(rm_h2, __builtin_amdgcn_cvt_pkrtz(u, v));
-        const rm_h2 l = __builtin_bit_cast(
-            rm_h2, __builtin_amdgcn_cvt_pkrtz(fmaf((float)h[0], -1.0f, u), fmaf((float)h[1], -1.0f, v)));
+        const rm_h2 l = __builtin_bit_cast(rm_h2, __builtin_amdgcn_cvt_pkrtz(fmaf((float)h[0], minus_one, u), fmaf((float)h[1], minus_one, v)));
         hi[i] = h[0], hi[i + 1] = h[1];
         lo[i] = l[0], lo[i + 1] = l[1];
     }
 }
 
-extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_rows_gfx950(GqaRowsArgs a) {
-    __shared__ GrLds L;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t li = lane & 31, h = lane >> 5;
-    const uint32_t tw = wave & 3, qw = wave >> 2;   // scores: token subtile, query half
-    const uint32_t blk = wave & 3, th = wave >> 2;  // values: dim block, token half
-    const uint32_t range = gr_range<512>(a, false, L.scratch);
-    const GrItem it = gr_find<512>(a, false, range, blockIdx.x, true, L.scratch);
+// ---------------------------------------------------------------------------
+// attention of one item
+// ---------------------------------------------------------------------------
+// LDS of a workgroup of QS query subtiles x TS token shares: queries (while tiles run; the joined
+// sums afterwards), and what each wave keeps for itself.
+template <int QS, int TS>
+struct GrLds {
+    union {
+        rm_h8 q[QS][2][16][64];         // [subtile][lo, hi][k step][lane]
+        float4 sum[QS * TS / 2][32][64];  // [publishing wave][dim block, parity, register quad][lane]
+        GrScratch scratch;
+    } u;
+    uint32_t v[QS * TS][2][32][9];  // [wave][block of a pair][code byte][token / 4]: that byte of four tokens
+    float ks[QS * TS][4][32];       // [wave][block][token]: key scale / 15
+    float vs[QS * TS][4][32];       // value scale in units of 2^(E - 9)
+    uint64_t tok[QS * TS][32];      // address of the token's K run | kind << 62 (0 absent: the query's, 1 Q2, 2 Q4)
+    float stat[QS * TS][2][32];     // (maximum, denominator) of a publishing wave
+};
+
+template <int QS, int TS>
+__device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
+    constexpr int NT = 64 * QS * TS;
+    constexpr bool FEW = QS == 1;
+    constexpr uint32_t kQueries = 32 * QS;
+    __shared__ GrLds<QS, TS> L;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t li = lane & 31, h = lane >> 5, qsub = wave % QS, ts = wave / QS;
+    const uint32_t range = gr_range<NT>(a, FEW, L.u.scratch);
+    const GrItem it = gr_find<NT>(a, FEW, range, blockIdx.x, true, L.u.scratch);
     if (!it.ok) return;
     const GrRequest rq = gr_request(a, it.request);
     // Items of a request: query tiles from the last (the longest) to the first, in each the
     // ranges, in each the KV heads (neighbouring workgroups sit on different XCDs: an XCD's L2
     // then sees few of the KV heads).
-    const uint32_t nqt = (uint32_t)(((uint64_t)rq.rows * a.group + GR_QUERIES - 1) / GR_QUERIES);
+    const uint32_t nq = rq.rows * a.group, nqt = (nq + kQueries - 1) / kQueries;
     const uint32_t kvh = it.local % a.kv_heads, rest = it.local / a.kv_heads;
-    const uint32_t part = rest % it.ranges, qt = nqt - 1 - rest / it.ranges;
-    const uint32_t q0 = qt * GR_QUERIES, nq = rq.rows * a.group;
+    const uint32_t part = rest % it.ranges, q0 = (nqt - 1 - rest / it.ranges) * kQueries;
     const int32_t past = (int32_t)rq.tokens - (int32_t)rq.rows;  // tokens before the first row
-    const int32_t lim0 = past + (int32_t)(q0 / a.group);
-    const int32_t seen = past + (int32_t)(min(q0 + GR_QUERIES - 1, nq - 1) / a.group) + 1;
+    const int32_t seen = past + (int32_t)(min(q0 + kQueries - 1, nq - 1) / a.group) + 1;
     const uint32_t vis = (uint32_t)max(seen, 0);
-    const uint32_t vt = (vis + GR_TOKENS - 1) / GR_TOKENS, per = (vt + it.ranges - 1) / it.ranges;
-    const uint32_t t0 = min(part * per, vt), t1 = min(t0 + per, vt);
+    const uint32_t units = (vis + 32 * TS - 1) / (32 * TS), per = (units + it.ranges - 1) / it.ranges;
+    // Tiles of 32 tokens: this wave's are t0, t0 + TS, ... below t1.
+    const uint32_t t0 = min(part * per, units) * TS + ts, t1 = min(min(part * per + per, units) * TS, (vis + 31) / 32);
 
-    // This lane's query (the wave's half for the scores, both halves for the values).
-    const uint32_t qi = q0 + 32 * qw + li;
+    const uint32_t qi = q0 + 32 * qsub + li;  // this lane's query
     const bool valid = qi < nq;
     const int32_t lim = valid ? past + (int32_t)(qi / a.group) : -1;
+    const int32_t lim0 = past + (int32_t)(min(q0 + 32 * qsub, nq - 1) / a.group);  // the subtile's first query's
+    const uint32_t qrow = valid ? qi / a.group : 0, qg = valid ? qi - qrow * a.group : 0;
+    const size_t qat = ((size_t)(rq.row0 + qrow) * a.query_heads + kvh * a.group + qg) * 256;
+
+    // Token -> address. A token past what the tile's queries see, or in no page, is absent: its loads
+    // go to the query rows (always there, and long enough), its scales count as 0.
+    PagedKvDesc dsc{0, 0, 0, 0};
+    auto desc_load = [&](uint32_t t) {
+        const uint32_t j = t * 32 + li;
+        const uint32_t p = (uint32_t)(((uint64_t)j * a.page_magic) >> a.page_shift);
+        dsc = a.desc[(size_t)it.request * a.max_pages + (t < t1 && j < vis ? p : 0)];
+    };
+    uint64_t at = 0;
+    uint32_t present = 0, hole = 0;  // of the tile that `at` belongs to
+    auto resolve = [&](uint32_t t) {
+        const uint32_t j = t * 32 + li, tip = j - dsc.first_token;
+        const bool want = t < t1 && j < vis;
+        const bool in = want && j >= dsc.first_token && tip < min(dsc.tokens, a.page_tokens), q4 = dsc.precision != 0;
+        const uint8_t *pool = q4 ? a.q4 : a.q2;
+        const uint8_t *run = pool + (size_t)dsc.physical_slot * (q4 ? a.q4_page_bytes : a.q2_page_bytes) +
+                             (size_t)tip * (q4 ? a.q4_token_bytes : a.q2_token_bytes) + kvh * (q4 ? 136 : 72);
+        at = in ? (uint64_t)(uintptr_t)run | (q4 ? 2ull << 62 : 1ull << 62) : (uint64_t)(uintptr_t)a.query;
+        present = (uint32_t)__builtin_amdgcn_ballot_w64(in);
+        hole = __builtin_amdgcn_ballot_w64(want && !in) != 0;
+        if (h == 0) L.tok[wave][li] = at;
+        lds_wave_order();
+    };
+
+    // Keys: this lane's half of four blocks of its token; two scales of K and of V. A Q2 half is 8
+    // of the 16 bytes read (what lies behind is the token's own).
+    uint32_t kw[4][4], ksc[2], vsc[2], kkind = 0;
+    auto issue_k = [&]() {
+        kkind = gr_kind(at);
+        const uint32_t step = kkind == 1 ? 18 : 34;
+        const gr_bytes p = gr_at(at), c = p + 2 + (kkind == 1 ? 8 * h : 16 * h);
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            const GrBytes16 x = gr_load<GrBytes16>(c + b * step);
+#pragma unroll
+            for (int i = 0; i < 4; i++) kw[b][i] = x.w[i];
+        }
+        const gr_bytes sk = p + 2 * h * step, sv = sk + (kkind == 1 ? a.v_off2 : a.v_off4);
+        ksc[0] = gr_load<uint16_t>(sk);
+        ksc[1] = gr_load<uint16_t>(sk + step);
+        vsc[0] = gr_load<uint16_t>(sv);
+        vsc[1] = gr_load<uint16_t>(sv + step);
+    };
+    // Values of block pair p: eight code bytes (Q4) of four tokens of one block. The four bytes of a Q2
+    // token are one half of an eight-byte piece of its block.
+    const uint32_t vq = lane & 7, vo = (lane >> 3) & 3, vb = lane >> 5;  // token quad, octet of bytes, block of the pair
+    uint32_t vw[2][4][2], vtwo[2];                                         // vtwo: bit i where token i is Q2
+    auto issue_v = [&](int p) {
+        vtwo[p] = 0;
+        const uint32_t c4 = a.v_off4 + 34 * (2 * p + vb) + 2 + 8 * vo, c2 = a.v_off2 + 18 * (2 * p + vb) + 2 + 8 * (vo >> 1);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint64_t x = L.tok[wave][4 * vq + i];
+            const bool two = gr_kind(x) == 1;
+            vtwo[p] |= two ? 1u << i : 0u;
+            const GrBytes8 y = gr_load<GrBytes8>(gr_at(x) + (two ? c2 : c4));
+            vw[p][i][0] = y.w[0], vw[p][i][1] = y.w[1];
+        }
+    };
+    auto write_v = [&](int p) {
+        if (__builtin_amdgcn_ballot_w64(vtwo[p] != 0)) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t x = vo & 1 ? vw[p][i][1] : vw[p][i][0];
+                const bool two = vtwo[p] >> i & 1;
+                vw[p][i][0] = two ? gr_widen(x) : vw[p][i][0];
+                vw[p][i][1] = two ? gr_widen(x >> 16) : vw[p][i][1];
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            // 4 x 4 bytes across: byte r of the four tokens into one dword.
+            const uint32_t ab0 = __builtin_amdgcn_perm(vw[p][1][w], vw[p][0][w], 0x05010400u);
+            const uint32_t ab1 = __builtin_amdgcn_perm(vw[p][1][w], vw[p][0][w], 0x07030602u);
+            const uint32_t cd0 = __builtin_amdgcn_perm(vw[p][3][w], vw[p][2][w], 0x05010400u);
+            const uint32_t cd1 = __builtin_amdgcn_perm(vw[p][3][w], vw[p][2][w], 0x07030602u);
+            const uint32_t r = 8 * vo + 4 * w;
+            L.v[wave][vb][r][vq] = __builtin_amdgcn_perm(cd0, ab0, 0x05040100u);
+            L.v[wave][vb][r + 1][vq] = __builtin_amdgcn_perm(cd0, ab0, 0x07060302u);
+            L.v[wave][vb][r + 2][vq] = __builtin_amdgcn_perm(cd1, ab1, 0x05040100u);
+            L.v[wave][vb][r + 3][vq] = __builtin_amdgcn_perm(cd1, ab1, 0x07060302u);
+        }
+    };
+
+    const RmMagic magic = rm_magic<true>();
+    float minus_one = -1.0f;
+    asm("" : "+v"(minus_one));
+    desc_load(t0);
     float qs;
     {
-        const uint32_t row = valid ? qi / a.group : 0, g = valid ? qi - row * a.group : 0;
-        const float *q = a.query + ((size_t)(rq.row0 + row) * a.query_heads + kvh * a.group + g) * 256 + 32 * h;
+        const float *q = a.query + qat + 32 * h;
         const float pre = valid ? a.scale * 1.44269504088896341f : 0.0f;
         // Eight dims of k step s in the key operand's order (read twice rather than kept).
         auto load = [&](int s, float (&x)[8]) {
@@ -287,9 +385,11 @@ extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_rows_gfx950(GqaRow
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         int e = 0;
         frexpf(mx, &e);
-        asm volatile("" ::: "memory");
+        qs = ldexpf(1.0f, e - 15);
+        // The waves of a subtile write a share of it each.
 #pragma unroll
-        for (int s = 0; s < 16; s++) {
+        for (int k = 0; k < 16 / TS; k++) {
+            const int s = ts * (16 / TS) + k;
             float x[8];
             load(s, x);
             rm_h8 hi, lo;
@@ -299,137 +399,77 @@ extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_rows_gfx950(GqaRow
                 hi[i] = (_Float16)v;
                 lo[i] = fabsf(v) < INFINITY ? (_Float16)(v - (float)hi[i]) : (_Float16)0.0f;
             }
-            if ((uint32_t)(s >> 2) == tw) {  // the four waves of a half write a quarter each
-                L.q[qw][0][s][lane] = lo;
-                L.q[qw][1][s][lane] = hi;
-            }
+            L.u.q[qsub][0][s][lane] = lo;
+            L.u.q[qsub][1][s][lane] = hi;
         }
-        qs = ldexpf(1.0f, e - 15);
     }
+    __syncthreads();
 
-    // Token -> address. A token past what the tile's queries see, or in no page, is absent: its loads
-    // go to the query rows (always there, and long enough), its scales count as 0.
-    PagedKvDesc dsc{0, 0, 0, 0};
-    auto desc_load = [&](uint32_t t) {
-        const uint32_t j = t * GR_TOKENS + tid;
-        const uint32_t p = (uint32_t)(((uint64_t)j * a.page_magic) >> a.page_shift);
-        dsc = a.desc[(size_t)it.request * a.max_pages + (t < t1 && j < vis ? p : 0)];
-    };
-    auto desc_write = [&](uint32_t t) {
-        const uint32_t j = t * GR_TOKENS + tid, tip = j - dsc.first_token;
-        const bool want = t < t1 && j < vis;
-        const bool in = want && j >= dsc.first_token && tip < min(dsc.tokens, a.page_tokens), q4 = dsc.precision != 0;
-        const uint8_t *pool = q4 ? a.q4 : a.q2;
-        const uint8_t *run = pool + (size_t)dsc.physical_slot * (q4 ? a.q4_page_bytes : a.q2_page_bytes) +
-                             (size_t)tip * (q4 ? a.q4_token_bytes : a.q2_token_bytes) + kvh * (q4 ? 136 : 72);
-        L.tok[t & 3][tid] = in ? (uint64_t)(uintptr_t)run | (q4 ? 2ull << 62 : 1ull << 62) : (uint64_t)(uintptr_t)a.query;
-        const uint64_t here = __builtin_amdgcn_ballot_w64(in);
-        const uint64_t gone = __builtin_amdgcn_ballot_w64(want && !in);
-        if (lane == 0) {
-            L.present[t & 3][wave] = here;
-            L.holes[t & 3][wave] = gone != 0;
-        }
-    };
-
-    // Keys: this lane's half of four blocks of one token, and two of its scales. A Q2 half is 8 of
-    // the 16 bytes read (what lies behind is the token's own).
-    uint32_t kw[4][4];
-    uint32_t kkind = 0, ksc[2];
-    auto issue_k = [&](uint32_t t) {
-        const uint64_t at = L.tok[t & 3][32 * tw + li];
-        kkind = gr_kind(at);
-        const uint32_t step = kkind == 1 ? 18 : 34;
-        const gr_bytes p = gr_at(at), c = p + 2 + (kkind == 1 ? 8 * h : 16 * h);
+    gr_v16 o[4][2];  // [dim block][even, odd dims]
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
-            const GrBytes16 x = gr_load<GrBytes16>(c + b * step);
-#pragma unroll
-            for (int i = 0; i < 4; i++) kw[b][i] = x.w[i];
-        }
-        const gr_bytes sc = p + 2 * h * step;
-        ksc[0] = gr_load<uint16_t>(sc);
-        ksc[1] = gr_load<uint16_t>(sc + step);
-    };
-    // Values: eight code bytes (Q4) of four tokens of one block; one scale. The four bytes of a Q2 token
-    // are one half of an eight-byte piece of its block.
-    const uint32_t vq = tid & 31, vb = (tid >> 5) & 3, vo = tid >> 7;  // token quad, block, octet of bytes
-    const uint32_t sb = wave >> 1, st = tid & 127;                      // scale: block, token
-    const uint32_t vc4 = a.v_off4 + 34 * vb + 2 + 8 * vo, vc2 = a.v_off2 + 18 * vb + 2 + 8 * (vo >> 1);
-    const uint32_t vs4 = a.v_off4 + 34 * sb, vs2 = a.v_off2 + 18 * sb;
-    uint32_t vw[4][2], vtwo = 0, vsc = 0;  // vtwo: bit i where token i is Q2
-    bool vsk = false;
-    auto issue_v = [&](uint32_t t) {
-        vtwo = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint64_t at = L.tok[t & 3][4 * vq + i];
-            const bool two = gr_kind(at) == 1;
-            vtwo |= two ? 1u << i : 0u;
-            const GrBytes8 x = gr_load<GrBytes8>(gr_at(at) + (two ? vc2 : vc4));
-            vw[i][0] = x.w[0], vw[i][1] = x.w[1];
-        }
-        const uint64_t at = L.tok[t & 3][st];
-        vsk = gr_kind(at) != 0;
-        vsc = gr_load<uint16_t>(gr_at(at) + (gr_kind(at) == 1 ? vs2 : vs4));
-    };
-    auto write_v = [&](uint32_t t) {
-        const uint32_t buf = t & 1;
-        if (__builtin_amdgcn_ballot_w64(vtwo != 0)) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t x = vo & 1 ? vw[i][1] : vw[i][0];
-                const bool two = vtwo >> i & 1;
-                vw[i][0] = two ? gr_widen(x) : vw[i][0];
-                vw[i][1] = two ? gr_widen(x >> 16) : vw[i][1];
-            }
-        }
-#pragma unroll
-        for (int w = 0; w < 2; w++) {
-            // 4 x 4 bytes across: byte r of the four tokens into one dword.
-            const uint32_t ab0 = __builtin_amdgcn_perm(vw[1][w], vw[0][w], 0x05010400u);
-            const uint32_t ab1 = __builtin_amdgcn_perm(vw[1][w], vw[0][w], 0x07030602u);
-            const uint32_t cd0 = __builtin_amdgcn_perm(vw[3][w], vw[2][w], 0x05010400u);
-            const uint32_t cd1 = __builtin_amdgcn_perm(vw[3][w], vw[2][w], 0x07030602u);
-            const uint32_t r = 8 * vo + 4 * w;
-            L.v[buf][vb][r][vq] = __builtin_amdgcn_perm(cd0, ab0, 0x05040100u);
-            L.v[buf][vb][r + 1][vq] = __builtin_amdgcn_perm(cd0, ab0, 0x07060302u);
-            L.v[buf][vb][r + 2][vq] = __builtin_amdgcn_perm(cd1, ab1, 0x05040100u);
-            L.v[buf][vb][r + 3][vq] = __builtin_amdgcn_perm(cd1, ab1, 0x07060302u);
-        }
-        const float s = vsk ? (float)__builtin_bit_cast(_Float16, (uint16_t)vsc) : 0.0f;
-        L.vs[buf][sb][st] = s;
-        float m = fabsf(s) < INFINITY ? fabsf(s) : 0.0f;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-        if (lane == 0) L.vmax[buf][wave] = m;
-    };
-
-    gr_v16 o[2][2];  // [query half][even, odd dims]
-#pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int b = 0; b < 4; b++)
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) o[i][c][r] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, den = 0.0f;
-    int ev = -200;  // 2^ev above every value scale of the wave's block so far
+            for (int r = 0; r < 16; r++) o[b][c][r] = 0.0f;
+    float m = -INFINITY, den = 0.0f;
+    int ev[4] = {-100, -100, -100, -100};  // 2^ev above every value scale of the block so far
+    float bound[2], unit[2];               // 2^ev and 2^(9 - ev) of blocks 2 h, 2 h + 1
+#pragma unroll
+    for (int i = 0; i < 2; i++) bound[i] = ldexpf(1.0f, -100), unit[i] = ldexpf(1.0f, 109);
 
-    if (tid < 4) L.flag[tid] = 0;
-    __syncthreads();
-    if (tid < GR_TOKENS)
-        for (uint32_t t = t0; t < t0 + 3; t++) {
-            desc_load(t);
-            desc_write(t);
+    resolve(t0);
+    desc_load(t0 + TS);
+    issue_k();
+    issue_v(0);
+    issue_v(1);
+    // (nothing under way on entry: the loop's waits are then counted by the order of its own loads alone)
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    for (uint32_t t = t0; t < t1; t += TS) {
+        const uint32_t here = present, gone = hole;
+        // ---- this tile's scales; the next tile's addresses ----
+        float sv[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            L.ks[wave][2 * h + i][li] =
+                kkind ? (float)__builtin_bit_cast(_Float16, (uint16_t)ksc[i]) * (1.0f / 15.0f) : 0.0f;
+            sv[i] = kkind ? (float)__builtin_bit_cast(_Float16, (uint16_t)vsc[i]) : 0.0f;
         }
-    __syncthreads();
-    issue_v(t0);
-    issue_k(t0);
-    write_v(t0);
-    for (uint32_t t = t0; t < t1; t++) {
-        const uint32_t buf = t & 1;
-        issue_v(t + 1);
-        if (tid < GR_TOKENS) desc_load(t + 3);
-        // ---- scores ----
+        uint32_t odd = 0;  // bit i: this lane's token has no finite value scale in block 2 h + i
+        if (__builtin_amdgcn_ballot_w64(!(fabsf(sv[0]) < bound[0]) || !(fabsf(sv[1]) < bound[1]))) {
+            float z[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                if (!(fabsf(sv[i]) < INFINITY)) {
+                    sv[i] = 0.0f;
+                    odd |= 1u << i;
+                }
+                z[i] = fabsf(sv[i]);
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) z[i] = fmaxf(z[i], __shfl_xor(z[i], d));
+            }
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                int e = 0;
+                frexpf(z[b & 1], &e);
+                e = __builtin_amdgcn_readlane(e, 32 * (b >> 1));
+                const int d = max(ev[b] - e, -200);
+                if (d < 0) {
+#pragma unroll
+                    for (int c = 0; c < 2; c++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) o[b][c][r] = ldexpf(o[b][c][r], d);
+                    ev[b] = e;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int e = h ? ev[2 + i] : ev[i];
+                bound[i] = ldexpf(1.0f, e), unit[i] = ldexpf(1.0f, 9 - e);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) L.vs[wave][2 * h + i][li] = sv[i] * unit[i];
         if (__builtin_amdgcn_ballot_w64(kkind == 1)) {
             const bool two = kkind == 1;
 #pragma unroll
@@ -441,11 +481,9 @@ extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_rows_gfx950(GqaRow
                 kw[b][3] = two ? gr_widen(y >> 16) : kw[b][3];
             }
         }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            L.ks[wave][2 * h + i][li] =
-                kkind ? (float)__builtin_bit_cast(_Float16, (uint16_t)ksc[i]) * (1.0f / 15.0f) : 0.0f;
-        lds_wave_order();
+        resolve(t + TS);
+        desc_load(t + 2 * TS);
+        // ---- scores ----
         gr_v16 s;
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] = 0.0f;
@@ -459,9 +497,9 @@ extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_rows_gfx950(GqaRow
             for (int r = 0; r < 16; r++) x[r] = 0.0f;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const rm_h8 kf = gr_k_operand(kw[b][k]);
-                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, L.q[qw][0][4 * b + k][ql], x, 0, 0, 0);
-                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, L.q[qw][1][4 * b + k][ql], x, 0, 0, 0);
+                const rm_h8 kf = gr_k_operand(kw[b][k], magic);
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, L.u.q[qsub][0][4 * b + k][ql], x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, L.u.q[qsub][1][4 * b + k][ql], x, 0, 0, 0);
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -471,202 +509,167 @@ extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_rows_gfx950(GqaRow
                 s[4 * j + 2] = fmaf(f.z, x[4 * j + 2], s[4 * j + 2]);
                 s[4 * j + 3] = fmaf(f.w, x[4 * j + 3], s[4 * j + 3]);
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
+        issue_k();
         // ---- masks: a tile that ends past the first query's last token, or has absent tokens ----
-        if ((int32_t)((t + 1) * GR_TOKENS) - 1 > lim0 || (L.holes[t & 3][0] | L.holes[t & 3][1])) {
-            const uint32_t here = (uint32_t)(L.present[t & 3][tw >> 1] >> (32 * (tw & 1))) >> (4 * h);
-            const int32_t left = lim - (int32_t)(t * GR_TOKENS + 32 * tw + 4 * h);  // tokens up to this one
+        if ((int32_t)((t + 1) * 32) - 1 > lim0 || gone) {
+            const uint32_t on = here >> (4 * h);
+            const int32_t left = lim - (int32_t)(t * 32 + 4 * h);  // tokens up to this one
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int c = 8 * (r >> 2) + (r & 3);
-                if (c > left || !(here >> c & 1)) s[r] = -INFINITY;
+                if (c > left || !(on >> c & 1)) s[r] = -INFINITY;
             }
         }
+        // ---- softmax ----
         float top = s[0];
 #pragma unroll
         for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
         top = fmaxf(top, __shfl_xor(top, 32)) * qs;
-        if (h == 0) L.mx[buf][tw][32 * qw + li] = top;
-        float mq = qw ? m[1] : m[0];
-        if (__builtin_amdgcn_ballot_w64(top > mq + GR_MOVE) && lane == 0) L.flag[t & 3] = 1;
-        float sum = 0.0f;
-        auto probabilities = [&]() {
-            const float ms = mq == -INFINITY ? 0.0f : mq;
-            sum = 0.0f;
+        if (__builtin_amdgcn_ballot_w64(top > m + GR_MOVE)) {
+            const float mn = fmaxf(m, top), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float4 p;
-                p.x = __builtin_amdgcn_exp2f(fmaf(s[4 * j], qs, -ms));
-                p.y = __builtin_amdgcn_exp2f(fmaf(s[4 * j + 1], qs, -ms));
-                p.z = __builtin_amdgcn_exp2f(fmaf(s[4 * j + 2], qs, -ms));
-                p.w = __builtin_amdgcn_exp2f(fmaf(s[4 * j + 3], qs, -ms));
-                sum += (p.x + p.y) + (p.z + p.w);
-                L.p[wave][j][lane] = p;
-            }
-        };
-        issue_k(t + 1);
-        lds_barrier();  // every wave is done with the tile before's probabilities
-        probabilities();
-        lds_barrier();
-        if (L.flag[t & 3]) {  // the maxima move (the same for every wave)
-            float al[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                float mn = m[i];
-#pragma unroll
-                for (int w = 0; w < 4; w++) mn = fmaxf(mn, L.mx[buf][w][32 * i + li]);
-                al[i] = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[i] - mn);
-                m[i] = mn;
+            for (int b = 0; b < 4; b++)
 #pragma unroll
                 for (int c = 0; c < 2; c++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) o[i][c][r] *= al[i];
-            }
-            mq = qw ? m[1] : m[0];
-            den *= qw ? al[1] : al[0];
-            probabilities();
-            lds_barrier();
+                    for (int r = 0; r < 16; r++) o[b][c][r] *= al;
+            den *= al;
+            m = mn;
         }
-        den += sum;
-        if (tid == 0) L.flag[(t + 2) & 3] = 0;
-        write_v(t + 1);
-        // ---- values ----
         {
-            const float vm = fmaxf(L.vmax[buf][2 * blk], L.vmax[buf][2 * blk + 1]);
-            int e = 0;
-            frexpf(vm, &e);
-            e = __builtin_amdgcn_readfirstlane(vm > 0.0f ? e : -200);
-            if (e > ev) {
-                const int d = max(ev - e, -300);
+            const float ms = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-                for (int i = 0; i < 2; i++)
+            for (int r = 0; r < 16; r++) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], qs, -ms));
+            float d = 0.0f;
 #pragma unroll
-                    for (int c = 0; c < 2; c++)
+            for (int r = 0; r < 16; r += 4) d += (s[r] + s[r + 1]) + (s[r + 2] + s[r + 3]);
+            den += d;
+        }
+        // ---- values ----
+        // A value block without a finite scale makes its dims no numbers for every query that sees the token, and
+        // does not count for the others (its scale is 0 from here on).
+        if (__builtin_amdgcn_ballot_w64(odd != 0)) {
 #pragma unroll
-                        for (int r = 0; r < 16; r++) o[i][c][r] = ldexpf(o[i][c][r], d);
-                ev = e;
+            for (int b = 0; b < 4; b++) {
+                const uint64_t who = __builtin_amdgcn_ballot_w64(odd >> (b & 1) & 1);
+                const uint32_t bad = (uint32_t)(who >> (32 * (b >> 1))) >> (4 * h);
+                bool any = false;
+#pragma unroll
+                for (int r = 0; r < 16; r++) any |= (bad >> (8 * (r >> 2) + (r & 3)) & 1) && s[r] != 0.0f;
+                any |= __shfl_xor((int)any, 32) != 0;
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) o[b][c][r] = any ? __builtin_nanf("") : o[b][c][r];
             }
         }
-        const float unit = ldexpf(1.0f, 9 - max(ev, -100));
 #pragma unroll
-        for (int kk = 0; kk < 4; kk++) {
-            const uint32_t w = 2 * th + (kk >> 1), k = kk & 1, tq = 8 * w + 4 * k + h;
-            const uint32_t *vr = L.v[buf][blk][li];
-            rm_h8 vf[2];
-            gr_v_operands(vr[tq], vr[tq + 2], vf);
-            const float4 f0 = *(const float4 *)&L.vs[buf][blk][4 * tq], f1 = *(const float4 *)&L.vs[buf][blk][4 * tq + 8];
-            const float f[8] = {f0.x * unit, f0.y * unit, f0.z * unit, f0.w * unit,
-                                f1.x * unit, f1.y * unit, f1.z * unit, f1.w * unit};
+        for (int p = 0; p < 2; p++) {
+            write_v(p);
+            lds_wave_order();
+            issue_v(p);
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float4 p0 = L.p[w + 4 * i][2 * k][lane], p1 = L.p[w + 4 * i][2 * k + 1][lane];
-                const float p[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
-                float x[8];
-    #pragma unroll
-                for (int r = 0; r < 8; r++) x[r] = gr_mul(p[r], f[r]);
-                rm_h8 hi, lo;
-                gr_split(x, hi, lo);
+            for (int b = 0; b < 2; b++)
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    o[i][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c], lo, o[i][c], 0, 0, 0);
-                    o[i][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c], hi, o[i][c], 0, 0, 0);
-                }
-            }
-            __builtin_amdgcn_sched_barrier(0);
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t tq = 4 * k + h;
+                    rm_h8 vf[2];
+                    gr_v_operands(L.v[wave][b][li][tq], L.v[wave][b][li][tq + 2], magic, vf);
+                    const float4 f0 = *(const float4 *)&L.vs[wave][2 * p + b][4 * tq];
+                    const float4 f1 = *(const float4 *)&L.vs[wave][2 * p + b][4 * tq + 8];
+                    const float x[8] = {s[8 * k] * f0.x,     s[8 * k + 1] * f0.y,
+                                        s[8 * k + 2] * f0.z, s[8 * k + 3] * f0.w,
+                                        s[8 * k + 4] * f1.x, s[8 * k + 5] * f1.y,
+                                        s[8 * k + 6] * f1.z, s[8 * k + 7] * f1.w};
+                    rm_h8 hi, lo;
+                    gr_split(x, minus_one, hi, lo);
+                    gr_v16 *y = o[2 * p + b];
+#pragma unroll
+                    for (int c = 0; c < 2; c++) y[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c], lo, y[c], 0, 0, 0);
+#pragma unroll
+                    for (int c = 0; c < 2; c++) y[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c], hi, y[c], 0, 0, 0);
+                        }
+            lds_wave_order();
         }
-        // The table of tile t + 3 takes the place of tile t - 1's, which no wave reads after this tile's barrier.
-        if (tid < GR_TOKENS) desc_write(t + 3);
     }
-    // ---- join the two token halves; every wave writes one query half of its dim block ----
+    // ---- join the token shares, half of the waves publishing to the other half, and write ----
     den += __shfl_xor(den, 32);
-    if (h == 0) L.lsum[tw][32 * qw + li] = den;
-    __syncthreads();
-    float4 *xo = (float4 *)L.q;  // (the queries are dead)
-    const uint32_t mine = th, other = 1 - th;
 #pragma unroll
-    for (int c = 0; c < 2; c++)
+    for (int b = 0; b < 4; b++) {
+        const float f = ldexpf(1.0f / 15.0f, ev[b] - 9);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const gr_v16 &x = other ? o[1][c] : o[0][c];
-            xo[((wave * 2 + c) * 4 + j) * 64 + lane] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[b][c][r] *= f;
+    }
+#pragma unroll
+    for (int n = TS / 2; n > 0; n >>= 1) {
+        __syncthreads();  // the queries (and the last round's sums) are dead
+        if ((int)ts >= n && (int)ts < 2 * n) {
+            const uint32_t slot = (ts - n) * QS + qsub;
+            if (h == 0) {
+                L.stat[slot][0][li] = m;
+                L.stat[slot][1][li] = den;
+            }
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        L.u.sum[slot][(b * 2 + c) * 4 + j][lane] =
+                            make_float4(o[b][c][4 * j], o[b][c][4 * j + 1], o[b][c][4 * j + 2], o[b][c][4 * j + 3]);
         }
-    __syncthreads();
-    const uint32_t src = blk + 4 * other, qo = q0 + 32 * mine + li;
-    const float total = (L.lsum[0][32 * mine + li] + L.lsum[1][32 * mine + li]) +
-                        (L.lsum[2][32 * mine + li] + L.lsum[3][32 * mine + li]);
-    float f = ldexpf(1.0f / 15.0f, max(ev, -100) - 9);
-    float *dst;
-    if (a.split) {
-        float *slot = a.part + (size_t)blockIdx.x * (GR_QUERIES * 258);
-        dst = slot + (size_t)(32 * mine + li) * 256;
-        if (blk == 0 && h == 0) {
-            const float mo = mine ? m[1] : m[0];
+        __syncthreads();
+        if ((int)ts < n) {
+            const uint32_t slot = ts * QS + qsub;
+            const float m2 = L.stat[slot][0][li], mn = fmaxf(m, m2);
+            const float f1 = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float f2 = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m2 - mn);
+            den = den * f1 + L.stat[slot][1][li] * f2;
+            m = mn;
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float4 x = L.u.sum[slot][(b * 2 + c) * 4 + j][lane];
+                        o[b][c][4 * j] = fmaf(x.x, f2, o[b][c][4 * j] * f1);
+                        o[b][c][4 * j + 1] = fmaf(x.y, f2, o[b][c][4 * j + 1] * f1);
+                        o[b][c][4 * j + 2] = fmaf(x.z, f2, o[b][c][4 * j + 2] * f1);
+                        o[b][c][4 * j + 3] = fmaf(x.w, f2, o[b][c][4 * j + 3] * f1);
+                    }
+        }
+    }
+    if (ts || !valid) return;
+    float *dst, f = 1.0f;
+    if (FEW || a.split) {
+        float *slot = (FEW ? a.few_part : a.part) + (size_t)blockIdx.x * (kQueries * 258);
+        const uint32_t in = 32 * qsub + li;
+        dst = slot + (size_t)in * 256;
+        if (h == 0) {
             // (scores that are no numbers move no maximum; the part is not an empty one)
-            slot[GR_QUERIES * 256 + 2 * (32 * mine + li)] = total != total && mo == -INFINITY ? 0.0f : mo;
-            slot[GR_QUERIES * 256 + 2 * (32 * mine + li) + 1] = total;
+            slot[kQueries * 256 + 2 * in] = den != den && m == -INFINITY ? 0.0f : m;
+            slot[kQueries * 256 + 2 * in + 1] = den;
         }
     } else {
-        const uint32_t row = qo / a.group, g = qo - row * a.group;
-        if (qo >= nq) return;
-        dst = a.out + ((size_t)(rq.row0 + row) * a.query_heads + kvh * a.group + g) * 256;
-        f = total != 0.0f ? f / total : 0.0f;
+        dst = a.out + qat;
+        f = den != 0.0f ? 1.0f / den : 0.0f;
     }
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        float4 x[2];
+    for (int b = 0; b < 4; b++)
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const float4 y = xo[((src * 2 + c) * 4 + j) * 64 + lane];
-            const gr_v16 &z = mine ? o[1][c] : o[0][c];
-            x[c] = make_float4((z[4 * j] + y.x) * f, (z[4 * j + 1] + y.y) * f, (z[4 * j + 2] + y.z) * f,
-                               (z[4 * j + 3] + y.w) * f);
+        for (int j = 0; j < 4; j++) {
+            float4 *d = (float4 *)(dst + 64 * b + 16 * j + 8 * h);
+            const gr_v16 &x = o[b][0], &y = o[b][1];
+            d[0] = make_float4(x[4 * j] * f, y[4 * j] * f, x[4 * j + 1] * f, y[4 * j + 1] * f);
+            d[1] = make_float4(x[4 * j + 2] * f, y[4 * j + 2] * f, x[4 * j + 3] * f, y[4 * j + 3] * f);
         }
-        float4 *d = (float4 *)(dst + 64 * blk + 16 * j + 8 * h);
-        d[0] = make_float4(x[0].x, x[1].x, x[0].y, x[1].y);
-        d[1] = make_float4(x[0].z, x[1].z, x[0].w, x[1].w);
-    }
 }
-
-// ---------------------------------------------------------------------------
-// few queries: the split-KV kernel of one sequence, a workgroup for each item
-// ---------------------------------------------------------------------------
-template <bool ALIGNED>
-__device__ __forceinline__ void gqa_few(const GqaRowsArgs &a) {
-    __shared__ GrScratch L;
-    const uint32_t range = gr_range<256>(a, true, L);
-    const GrItem it = gr_find<256>(a, true, range, blockIdx.x, true, L);
-    if (!it.ok) return;
-    const GrRequest rq = gr_request(a, it.request);
-    GqaArgs g{};
-    g.query = a.query + (size_t)rq.row0 * a.query_heads * 256;
-    g.q2 = a.q2;
-    g.q4 = a.q4;
-    g.desc = a.desc + (size_t)it.request * a.max_pages;
-    g.part_out = a.few_part + (size_t)blockIdx.x * (16 * 258);
-    g.part_stats = g.part_out + 16 * 256;
-    g.q2_page_bytes = a.q2_page_bytes;
-    g.q4_page_bytes = a.q4_page_bytes;
-    g.query_heads = a.query_heads;
-    g.group = a.group;
-    g.tokens = rq.tokens;
-    g.rows = rq.rows;
-    g.queries = rq.rows * a.group;
-    g.page_tokens = a.page_tokens;
-    g.page_count = a.max_pages;
-    g.component_values = a.kv_heads * 256;
-    g.q2_token_bytes = a.q2_token_bytes;
-    g.q4_token_bytes = a.q4_token_bytes;
-    g.tiles = (rq.tokens + 15) / 16;
-    g.tiles_per_wave = range / 4;
-    g.scale = a.scale;
-    g.tile_pages = ALIGNED;
-    const uint32_t kvh = it.local % a.kv_heads, part = it.local / a.kv_heads;
-    if constexpr (ALIGNED) paged_gqa_partial16<1, true>(g, kvh, part, 0);
-    else paged_gqa_partial<1>(g, kvh, part, 0);
-}
-extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few_aligned_gfx950(GqaRowsArgs a) { gqa_few<true>(a); }
-extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few_gfx950(GqaRowsArgs a) { gqa_few<false>(a); }
+extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_rows_gfx950(GqaRowsArgs a) { gqa_rows<4, 2>(a); }
+extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few_gfx950(GqaRowsArgs a) { gqa_rows<1, 4>(a); }
 
 // ---------------------------------------------------------------------------
 // join: grid (rows, query heads), four waves take every fourth part, 64 lanes x 4 dims
@@ -690,12 +693,9 @@ extern "C" __global__ __launch_bounds__(256) void ctox_gqa_join_gfx950(GqaRowsAr
     const GrItem it = gr_find<256>(a, few, range, lo, false, L);
     if (!it.ok) return;
     const uint32_t kvh = head / a.group, q = (row - rq.row0) * a.group + head % a.group;
-    const uint32_t nqt = (uint32_t)(((uint64_t)rq.rows * a.group + GR_QUERIES - 1) / GR_QUERIES);
-    const uint32_t tile = few ? 0 : nqt - 1 - q / GR_QUERIES, size = few ? 16 : GR_QUERIES;
-    const uint32_t slot0 = it.base + tile * it.ranges * a.kv_heads + kvh;
+    const uint32_t size = few ? 32 : 128, nqt = (rq.rows * a.group + size - 1) / size, in = q % size;
+    const uint32_t slot0 = it.base + (nqt - 1 - q / size) * it.ranges * a.kv_heads + kvh;
     const float *base = few ? a.few_part : a.part;
-    const uint32_t in = few ? q : q % GR_QUERIES;
-    const float unit = few ? 1.44269504088896341f : 1.0f;  // few: maxima in natural units
     float m = -INFINITY, den = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (uint32_t s0 = wave; s0 < it.ranges; s0 += 16) {
@@ -706,7 +706,7 @@ extern "C" __global__ __launch_bounds__(256) void ctox_gqa_join_gfx950(GqaRowsAr
             const uint32_t s = min(s0 + 4 * k, it.ranges - 1);
             const float *p = base + (size_t)(slot0 + s * a.kv_heads) * (size * 258);
             v[k] = ((const float4 *)(p + (size_t)in * 256))[lane];
-            ms[k] = s0 + 4 * k < it.ranges ? p[size * 256 + 2 * in] * unit : -INFINITY;
+            ms[k] = s0 + 4 * k < it.ranges ? p[size * 256 + 2 * in] : -INFINITY;
             ds[k] = p[size * 256 + 2 * in + 1];
         }
         float mn = m;
@@ -743,13 +743,7 @@ extern "C" __global__ __launch_bounds__(256) void ctox_gqa_join_gfx950(GqaRowsAr
         out = make_float4(fmaf(x.x, f, out.x), fmaf(x.y, f, out.y), fmaf(x.z, f, out.z), fmaf(x.w, f, out.w));
         total = fmaf(st[w][1], f, total);
     }
-    float inv = total != 0.0f ? 1.0f / total : 0.0f;
-    if (few) {  // the few-query kernel's fixed point has no infinities: such a query's scores are no numbers
-        const float4 x = ((const float4 *)(a.query + ((size_t)row * a.query_heads + head) * 256))[lane];
-        const float big = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-        const bool bad = !(big < INFINITY) || x.x != x.x || x.y != x.y || x.z != x.z || x.w != x.w;
-        if (__builtin_amdgcn_ballot_w64(bad) && total != 0.0f) inv = __builtin_nanf("");
-    }
+    const float inv = total != 0.0f ? 1.0f / total : 0.0f;
     ((float4 *)(a.out + ((size_t)row * a.query_heads + head) * 256))[lane] =
         make_float4(out.x * inv, out.y * inv, out.z * inv, out.w * inv);
 }

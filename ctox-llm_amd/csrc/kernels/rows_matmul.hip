@@ -94,29 +94,44 @@ __device__ __forceinline__ rm_h2 rm_h(uint32_t x) { return __builtin_bit_cast(rm
 
 // Eight codes of a lane (k step s) as odd whole numbers. An f16 with the bits 0x6400 | c << p is
 // 1024 + c 2^p; one packed multiply-add makes it 2c - L exactly where 2^(11-p) + L is an f16, so
-// p is never 0.
+// p is never 0. The constants are opaque so that they stay in registers and mask and magic go into
+// one v_and_or_b32.
+struct RmMagic {
+    uint32_t magic, m[3];
+    __device__ __forceinline__ explicit RmMagic(uint32_t m0, uint32_t m1 = 0, uint32_t m2 = 0)
+        : magic(0x64006400u), m{m0, m1, m2} {
+        asm("" : "+v"(magic));
+        asm("" : "+s"(m[0]));
+        asm("" : "+s"(m[1]));
+        asm("" : "+s"(m[2]));
+    }
+};
 template <int P, int L>
-__device__ __forceinline__ rm_h2 rm_pair(uint32_t x) {
-    constexpr uint32_t m = (L == 15 ? 0x000F000Fu : 0x00030003u) << P;
+__device__ __forceinline__ rm_h2 rm_pair(uint32_t x, uint32_t mask, uint32_t magic) {
     constexpr _Float16 f = (_Float16)(2.0f / (1 << P)), g = (_Float16)-(2048.0f / (1 << P) + L);
-    return __builtin_elementwise_fma(rm_h((x & m) | 0x64006400u), rm_h2{f, f}, rm_h2{g, g});
+    return __builtin_elementwise_fma(rm_h((x & mask) | magic), rm_h2{f, f}, rm_h2{g, g});
 }
 
 template <bool Q4>
-__device__ __forceinline__ rm_h8 rm_unpack(const uint32_t (&w)[4], int s) {
+__device__ __forceinline__ RmMagic rm_magic() {
+    return Q4 ? RmMagic(0x00F000F0u) : RmMagic(0x000C000Cu, 0x00300030u, 0x00C000C0u);
+}
+
+template <bool Q4>
+__device__ __forceinline__ rm_h8 rm_unpack(const uint32_t (&w)[4], int s, const RmMagic &g) {
     rm_h2 o[4];
     if constexpr (Q4) {
         const uint32_t x = w[s];
-        o[0] = rm_pair<4, 15>(x << 4);
-        o[1] = rm_pair<4, 15>(x);
-        o[2] = rm_pair<4, 15>(x >> 4);
-        o[3] = rm_pair<4, 15>(x >> 8);
+        o[0] = rm_pair<4, 15>(x << 4, g.m[0], g.magic);
+        o[1] = rm_pair<4, 15>(x, g.m[0], g.magic);
+        o[2] = rm_pair<4, 15>(x >> 4, g.m[0], g.magic);
+        o[3] = rm_pair<4, 15>(x >> 8, g.m[0], g.magic);
     } else {
         const uint32_t x = s & 1 ? w[s >> 1] >> 8 : w[s >> 1];
-        o[0] = rm_pair<2, 3>(s & 1 ? w[s >> 1] >> 6 : w[s >> 1] << 2);
-        o[1] = rm_pair<2, 3>(x);
-        o[2] = rm_pair<4, 3>(x);
-        o[3] = rm_pair<6, 3>(x);
+        o[0] = rm_pair<2, 3>(s & 1 ? w[s >> 1] >> 6 : w[s >> 1] << 2, g.m[0], g.magic);
+        o[1] = rm_pair<2, 3>(x, g.m[0], g.magic);
+        o[2] = rm_pair<4, 3>(x, g.m[1], g.magic);
+        o[3] = rm_pair<6, 3>(x, g.m[2], g.magic);
     }
     return rm_h8{o[0][0], o[0][1], o[1][0], o[1][1], o[2][0], o[2][1], o[3][0], o[3][1]};
 }
@@ -173,6 +188,7 @@ __device__ __forceinline__ void rows_product(const RowsMulArgs &a) {
     const uint32_t n0 = (col * 4 + wave) * RT * 32;       // first weight row of the wave
     const uint32_t h = lane >> 5, j = lane & 15;
     constexpr uint32_t kUnit = Q4 ? 8704 : 4608, kCodes = Q4 ? 8192 : 4096;
+    const RmMagic magic = rm_magic<Q4>();
 
     // This lane's weight tile (16 rows) of each RT tile; tiles past the matrix read the last one.
     const uint8_t *wp[RT];
@@ -223,7 +239,7 @@ __device__ __forceinline__ void rows_product(const RowsMulArgs &a) {
         for (int r = 0; r < RT; r++) {
             sc[r] = (float)__builtin_bit_cast(_Float16, (uint16_t)s[r]);
 #pragma unroll
-            for (int k = 0; k < 4; k++) w[r][k] = rm_unpack<Q4>(c[r], k);
+            for (int k = 0; k < 4; k++) w[r][k] = rm_unpack<Q4>(c[r], k, magic);
         }
 #pragma unroll
         for (int t = 0; t < TT; t++) {

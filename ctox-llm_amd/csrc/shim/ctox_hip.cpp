@@ -160,7 +160,7 @@ struct ctox_hip_backend {
                   prep_x = nullptr, finite = nullptr, gather = nullptr, topk_part = nullptr, topk_final = nullptr, stream_read = nullptr,
                   write_segments = nullptr, rope_axes[2] = {}, plan = nullptr, kv_append = nullptr,
                   rows_max = nullptr, rows_stage = nullptr, rows_reduce = nullptr,
-                  gqa_rows = nullptr, gqa_few[2] = {}, gqa_join = nullptr;
+                  gqa_rows = nullptr, gqa_few = nullptr, gqa_join = nullptr;
     // Row products: [q4][parts - 1][shape], shapes as kRowShapes.
     hipFunction_t rows_mul[2][2][4] = {};
     // Batch-1 slice kernels per dtype [Q2, Q4]: [0] walks the slices, [n]
@@ -953,8 +953,7 @@ extern "C" ctox_status ctox_hip_backend_create(int device, ctox_hip_backend **ou
                {&b->plan, "ctox_paged_plan_gfx950"}, {&b->kv_append, "ctox_kv_append_q4_gfx950"},
                {&b->rows_max, "ctox_rows_max_gfx950"}, {&b->rows_stage, "ctox_rows_stage_gfx950"},
                {&b->rows_reduce, "ctox_rows_reduce_gfx950"},
-               {&b->gqa_rows, "ctox_gqa_rows_gfx950"}, {&b->gqa_few[0], "ctox_gqa_few_gfx950"},
-               {&b->gqa_few[1], "ctox_gqa_few_aligned_gfx950"}, {&b->gqa_join, "ctox_gqa_join_gfx950"}};
+               {&b->gqa_rows, "ctox_gqa_rows_gfx950"}, {&b->gqa_few, "ctox_gqa_few_gfx950"}, {&b->gqa_join, "ctox_gqa_join_gfx950"}};
     for (auto &f : fns) {
         if (le != hipSuccess) break;
         le = hipModuleGetFunction(f.f, b->module, f.name);
@@ -2976,13 +2975,13 @@ ctox_status check_gqa_rows(const ctox_paged_gqa_rows *op) {
     return CTOX_OK;
 }
 
-// Which kernels run and how many items each may have. Requests of at most 16 queries a KV head go to the
-// few-query kernel, unless the batch is one request that may have more. The 64-query kernel splits token
-// ranges where its query tiles alone would not give every CU two workgroups. An item bound is what the
-// device's ranges cannot exceed: the workgroups that fill the chip, plus one a tile for the rounding.
+// Which kernels run and how many items each may have. Requests of at most 32 queries a KV head go to the
+// few-query kernel, unless the batch is one request that may have more. The 128-query kernel splits token
+// ranges where its query tiles alone would not give every CU two workgroups. Items: one a query tile and
+// KV head at least; the device cuts ranges into more up to the bound given here, two rounds of the chip.
 struct GqaRowsPlan {
     bool few, wide, split;
-    uint32_t few_fill, fill, few_items, items;
+    uint32_t few_slots, slots, few_items, items;
     uint64_t few_bytes, bytes;
 };
 GqaRowsPlan gqa_rows_plan(uint32_t cus, const ctox_paged_gqa_rows *op) {
@@ -2990,19 +2989,19 @@ GqaRowsPlan gqa_rows_plan(uint32_t cus, const ctox_paged_gqa_rows *op) {
     const uint32_t kvh = op->params.key_value_heads, group = op->params.query_heads / kvh;
     const uint64_t most = op->max_rows ? std::min<uint64_t>(op->max_rows, op->rows) : op->rows;
     const uint64_t busy = std::min<uint64_t>(op->requests, op->rows);
-    g.wide = most * group > 16;
-    g.few = group <= 16 && !(g.wide && op->requests == 1);
-    g.few_fill = 2 * cus;
-    g.fill = cus;
+    g.wide = most * group > 32;
+    g.few = group <= 32 && !(g.wide && op->requests == 1);
+    g.few_slots = 2 * cus;
+    g.slots = cus;
     if (g.few) {
-        g.few_items = (uint32_t)(g.few_fill + busy * kvh);
-        g.few_bytes = (uint64_t)g.few_items * 16 * 258 * sizeof(float);
+        g.few_items = (uint32_t)(busy * kvh + 2 * g.few_slots);
+        g.few_bytes = (uint64_t)g.few_items * 32 * 258 * sizeof(float);
     }
     if (g.wide) {
-        const uint64_t tiles = (op->rows * group + 63) / 64;
+        const uint64_t tiles = (op->rows * group + 127) / 128;
         g.split = tiles * kvh < 2 * cus;
-        g.items = (uint32_t)((tiles + busy) * kvh + (g.split ? g.fill : 0));
-        g.bytes = g.split ? (uint64_t)g.items * 64 * 258 * sizeof(float) : 0;
+        g.items = (uint32_t)((tiles + busy) * kvh + (g.split ? 2 * g.slots : 0));
+        g.bytes = g.split ? (uint64_t)g.items * 128 * 258 * sizeof(float) : 0;
     }
     return g;
 }
@@ -3060,9 +3059,11 @@ extern "C" ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *b, const
     a.v_off2 = cv / 64 * 18;
     a.v_off4 = cv / 64 * 34;
     a.split = g.split;
-    a.fill = g.fill;
+    a.slots = g.slots;
+    a.items = g.items;
     a.few = g.few;
-    a.few_fill = g.few_fill;
+    a.few_slots = g.few_slots;
+    a.few_items = g.few_items;
     a.scale = p.scale;
     // ceil(2^(30 + l) / d) with 2^l >= d: its error, below 1 / 2^(30 + l), times a token below 2^30 stays below
     // the 1 / d that would reach the next quotient.
@@ -3075,7 +3076,7 @@ extern "C" ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *b, const
     ctox_status st = CTOX_OK;
     if (g.wide) st = launch(b->gqa_rows, dim3(g.items), dim3(512), s, a, "ctox_gqa_rows_gfx950");
     if (!st && g.few)
-        st = launch(b->gqa_few[p.page_tokens % 16 == 0], dim3(g.few_items), dim3(256), s, a, "ctox_gqa_few_gfx950");
+        st = launch(b->gqa_few, dim3(g.few_items), dim3(256), s, a, "ctox_gqa_few_gfx950");
     if (!st && (g.few || g.split))
         st = launch(b->gqa_join, dim3(a.rows, p.query_heads), dim3(256), s, a, "ctox_gqa_join_gfx950");
     return st;

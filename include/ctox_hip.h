@@ -702,11 +702,9 @@ ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *backend, uint8_t *d_q
  * gets zeros. Lengths are read on the device: a plan's row_starts and
  * tokens (row_starts not falling, at most `rows`; tokens[r] at most
  * min(page_count * page_tokens, 2^30)). max_rows bounds the rows of any one request (0:
- * rows); a request with more than 16 queries per KV head needs max_rows to
- * say so. params.tokens is not read. f32 results: products keep 22 bits of each
- * query value and probability (21 of a query value for requests of at most 16 queries
- * per KV head), the cached codes are exact, sums are 32 bits. Limits: head_dim 256,
- * requests <= 4096, rows <= 2^20. workspace holds ctox_hip_paged_gqa_rows_workspace bytes (of
+ * rows); no request may have more. params.tokens is not read. f32 results: products
+ * keep 22 bits of each query value and probability, the cached codes are
+ * exact, sums are 32 bits. Limits: head_dim 256, requests <= 4096, rows <= 2^20. workspace holds ctox_hip_paged_gqa_rows_workspace bytes (of
  * the same op; its device pointers are not read), 16-byte aligned. */
 typedef struct {
     const float *query;
