@@ -11,8 +11,8 @@
 // within 2^-17 of the row's largest, an absolute 2^-40 of it below that), an
 // f16 activation without s_in as itself. Sums are f32 throughout.
 //
-//  * ctox_rows_max_gfx950: a row's exponent e.
-//  * ctox_rows_stage_gfx950: x into MFMA operand order, [32-row tile][block]
+//  * ctox_rows_max_*: a row's exponent e.
+//  * ctox_rows_stage_*: x into MFMA operand order, [32-row tile][block]
 //    [part][k step][lane][8 f16]: a fragment is 1 KiB that one wave reads at once.
 //  * ctox_rows_q{2,4}_*: the product. A workgroup's four waves share TT 32-row
 //    tiles of x in LDS (two buffers, loaded straight from memory while the other is
@@ -31,61 +31,124 @@ typedef _Float16 rm_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 rm_h2 __attribute__((ext_vector_type(2)));
 typedef uint32_t rm_u4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ float rm_x(const RowsStageArgs &a, uint32_t t, uint32_t k) {
+// Eight values of row t from column k on (four and four `gap` columns apart), times s_in. VEC: rows,
+// strides and s_in allow 16-byte (f16: 8-byte) loads.
+template <bool VEC>
+__device__ __forceinline__ void rm_eight(const RowsStageArgs &a, uint32_t t, uint32_t k, uint32_t gap, float (&v)[8]) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
     const size_t at = (size_t)t * a.x_stride + k;
-    return a.x_half ? (float)((const _Float16 *)a.x)[at] : ((const float *)a.x)[at];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const size_t p = at + i * gap;
+        if constexpr (VEC) {
+            if (a.x_half) {
+                const h4 x = *(const h4 *)((const _Float16 *)a.x + p);
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[4 * i + j] = (float)x[j];
+            } else {
+                const float4 x = *(const float4 *)((const float *)a.x + p);
+                v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                v[4 * i + j] = a.x_half ? (float)((const _Float16 *)a.x)[p + j] : ((const float *)a.x)[p + j];
+        }
+        const uint32_t c = k + i * gap;
+        if (a.s_in_kind == CTOX_KSCALE_F16) {
+            const h4 s = *(const h4 *)((const _Float16 *)a.s_in + c);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[4 * i + j] *= (float)s[j];
+        } else if (a.s_in_kind == CTOX_KSCALE_F32) {
+            const float4 s = *(const float4 *)((const float *)a.s_in + c);
+            v[4 * i] *= s.x, v[4 * i + 1] *= s.y, v[4 * i + 2] *= s.z, v[4 * i + 3] *= s.w;
+        }
+    }
 }
 
-__device__ __forceinline__ float rm_s_in(const RowsStageArgs &a, uint32_t k) {
-    if (a.s_in_kind == CTOX_KSCALE_NONE) return 1.0f;
-    return a.s_in_kind == CTOX_KSCALE_F32 ? ((const float *)a.s_in)[k] : (float)((const _Float16 *)a.s_in)[k];
-}
-
-// grid (rows): exponent with |x| < 2^e over the row's finite values (0 for a row of zeros).
-extern "C" __global__ __launch_bounds__(256) void ctox_rows_max_gfx950(RowsStageArgs a) {
-    __shared__ float red[4];
-    const uint32_t t = blockIdx.x;
+// Exponent e with |x s_in| < 2^e over row t's finite values (0 for a row of zeros), to all threads.
+template <bool VEC, int NT>
+__device__ __forceinline__ int rm_exponent(const RowsStageArgs &a, uint32_t t, float *red) {
     float m = 0.0f;
-    for (uint32_t k = threadIdx.x; k < a.columns; k += 256) {
-        const float v = fabsf(rm_x(a, t, k) * rm_s_in(a, k));
-        if (v < INFINITY) m = fmaxf(m, v);
+#pragma unroll 4
+    for (uint32_t k = 8 * threadIdx.x; k < a.columns; k += 8 * NT) {
+        float v[8];
+        rm_eight<VEC>(a, t, k, 4, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]) < INFINITY ? fabsf(v[i]) : 0.0f);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     lds_barrier();
-    if (threadIdx.x == 0) {
-        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        int e = 0;
-        frexpf(m, &e);
-        a.exps[t] = e;
-    }
-}
-
-// Column of value i of the fragment (block, step s, lane half h): the order in which the
-// codes of a lane's words unpack (rm_unpack below).
-__device__ __forceinline__ uint32_t rm_column(bool q4, uint32_t h, uint32_t s, uint32_t i) {
-    return q4 ? 32 * h + 8 * s + (i >> 1) + 4 * (i & 1) : 32 * h + 16 * (s >> 1) + 4 * (s & 1) + (i >> 1) + 8 * (i & 1);
-}
-
-// grid (blocks, 32-row tiles), one wave per k step.
-extern "C" __global__ __launch_bounds__(256) void ctox_rows_stage_gfx950(RowsStageArgs a) {
-    const uint32_t b = blockIdx.x, tile = blockIdx.y, lane = threadIdx.x & 63, s = threadIdx.x >> 6;
-    const uint32_t t = tile * 32 + (lane & 31), h = lane >> 5;
-    rm_h8 hi, lo;
-    const int e = a.parts == 2 && t < a.rows ? 15 - a.exps[t] : 0;
+    m = red[0];
 #pragma unroll
-    for (uint32_t i = 0; i < 8; i++) {
-        const uint32_t k = 64 * b + rm_column(a.q4, h, s, i);
-        float v = t < a.rows ? rm_x(a, t, k) : 0.0f;
-        if (a.parts == 2) v = ldexpf(v * rm_s_in(a, k), e);
-        hi[i] = (_Float16)v;
-        lo[i] = fabsf(v) < INFINITY ? (_Float16)(v - (float)hi[i]) : (_Float16)0.0f;
+    for (int w = 1; w < NT / 64; w++) m = fmaxf(m, red[w]);
+    int e = 0;
+    frexpf(m, &e);
+    return e;
+}
+
+// First column and gap of the eight values of fragment (k step s, lane half h), in the order in which the
+// codes of a lane's words unpack (rm_unpack): value i is column first + i / 2 + gap * (i % 2).
+__device__ __forceinline__ uint32_t rm_first(bool q4, uint32_t h, uint32_t s) {
+    return q4 ? 32 * h + 8 * s : 32 * h + 16 * (s >> 1) + 4 * (s & 1);
+}
+
+// The fragment piece (block b, k step s, lane half h) of row t, its parts 4 KiB apart.
+template <bool VEC>
+__device__ __forceinline__ void rm_piece(const RowsStageArgs &a, uint32_t t, uint32_t b, uint32_t s, uint32_t h, int e) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = 0.0f;
+    if (t < a.rows) rm_eight<VEC>(a, t, 64 * b + rm_first(a.q4, h, s), a.q4 ? 4 : 8, v);
+    rm_h8 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        float x = v[(i >> 1) + 4 * (i & 1)];
+        if (a.parts == 2) x = ldexpf(x, 15 - e);
+        hi[i] = (_Float16)x;
+        lo[i] = fabsf(x) < INFINITY ? (_Float16)(x - (float)hi[i]) : (_Float16)0.0f;
     }
-    rm_h8 *dst = (rm_h8 *)a.staged + ((size_t)tile * a.blocks + b) * a.parts * 256 + threadIdx.x;
+    rm_h8 *dst = (rm_h8 *)a.staged + ((size_t)(t >> 5) * a.blocks + b) * a.parts * 256 + 64 * s + 32 * h + (t & 31);
     dst[0] = hi;
     if (a.parts == 2) dst[256] = lo;
 }
+
+// grid (rows): the rows' exponents.
+template <bool VEC>
+__device__ __forceinline__ void rows_max(const RowsStageArgs &a) {
+    __shared__ float red[4];
+    const int e = rm_exponent<VEC, 256>(a, blockIdx.x, red);
+    if (threadIdx.x == 0) a.exps[blockIdx.x] = e;
+}
+extern "C" __global__ __launch_bounds__(256) void ctox_rows_max_vec_gfx950(RowsStageArgs a) { rows_max<true>(a); }
+extern "C" __global__ __launch_bounds__(256) void ctox_rows_max_gfx950(RowsStageArgs a) { rows_max<false>(a); }
+
+// grid (blocks, 32-row tiles), one wave per k step: fragments leave as whole KiB.
+template <bool VEC>
+__device__ __forceinline__ void rows_stage(const RowsStageArgs &a) {
+    const uint32_t lane = threadIdx.x & 63, t = blockIdx.y * 32 + (lane & 31);
+    rm_piece<VEC>(a, t, blockIdx.x, threadIdx.x >> 6, lane >> 5, a.parts == 2 && t < a.rows ? a.exps[t] : 0);
+}
+extern "C" __global__ __launch_bounds__(256) void ctox_rows_stage_vec_gfx950(RowsStageArgs a) { rows_stage<true>(a); }
+extern "C" __global__ __launch_bounds__(256) void ctox_rows_stage_gfx950(RowsStageArgs a) { rows_stage<false>(a); }
+
+// grid (rows of whole tiles): exponent and pieces of one row in one launch, for few rows (its 16-byte
+// pieces of many rows would reach memory as parts of lines).
+template <bool VEC>
+__device__ __forceinline__ void rows_stage_few(const RowsStageArgs &a) {
+    __shared__ float red[8];
+    const uint32_t t = blockIdx.x;
+    int e = 0;
+    if (a.parts == 2 && t < a.rows) {
+        e = rm_exponent<VEC, 512>(a, t, red);
+        if (threadIdx.x == 0) a.exps[t] = e;
+    }
+    for (uint32_t p = threadIdx.x; p < 8 * a.blocks; p += 512) rm_piece<VEC>(a, t, p >> 3, (p >> 1) & 3, p & 1, e);
+}
+extern "C" __global__ __launch_bounds__(512) void ctox_rows_stage_few_vec_gfx950(RowsStageArgs a) { rows_stage_few<true>(a); }
+extern "C" __global__ __launch_bounds__(512) void ctox_rows_stage_few_gfx950(RowsStageArgs a) { rows_stage_few<false>(a); }
 
 // ---------------------------------------------------------------------------
 // product

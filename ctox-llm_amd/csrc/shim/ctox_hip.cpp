@@ -159,7 +159,7 @@ struct ctox_hip_backend {
                   swiglu_rows = nullptr, copy_rows = nullptr, write_words = nullptr, norm_prep = nullptr,
                   prep_x = nullptr, finite = nullptr, gather = nullptr, topk_part = nullptr, topk_final = nullptr, stream_read = nullptr,
                   write_segments = nullptr, rope_axes[2] = {}, plan = nullptr, kv_append = nullptr,
-                  rows_max = nullptr, rows_stage = nullptr, rows_reduce = nullptr,
+                  rows_max[2] = {}, rows_stage[2] = {}, rows_stage_few[2] = {}, rows_reduce = nullptr,
                   gqa_rows = nullptr, gqa_few = nullptr, gqa_join = nullptr;
     // Row products: [q4][parts - 1][shape], shapes as kRowShapes.
     hipFunction_t rows_mul[2][2][4] = {};
@@ -951,7 +951,10 @@ extern "C" ctox_status ctox_hip_backend_create(int device, ctox_hip_backend **ou
                {&b->topk_part, "ctox_topk_part_gfx950"}, {&b->topk_final, "ctox_topk_final_gfx950"},
                {&b->rope_axes[0], "ctox_rope_axes_gfx950"}, {&b->rope_axes[1], "ctox_rope_axes_any_gfx950"},
                {&b->plan, "ctox_paged_plan_gfx950"}, {&b->kv_append, "ctox_kv_append_q4_gfx950"},
-               {&b->rows_max, "ctox_rows_max_gfx950"}, {&b->rows_stage, "ctox_rows_stage_gfx950"},
+               {&b->rows_max[0], "ctox_rows_max_gfx950"}, {&b->rows_max[1], "ctox_rows_max_vec_gfx950"},
+               {&b->rows_stage[0], "ctox_rows_stage_gfx950"}, {&b->rows_stage[1], "ctox_rows_stage_vec_gfx950"},
+               {&b->rows_stage_few[0], "ctox_rows_stage_few_gfx950"},
+               {&b->rows_stage_few[1], "ctox_rows_stage_few_vec_gfx950"},
                {&b->rows_reduce, "ctox_rows_reduce_gfx950"},
                {&b->gqa_rows, "ctox_gqa_rows_gfx950"}, {&b->gqa_few, "ctox_gqa_few_gfx950"}, {&b->gqa_join, "ctox_gqa_join_gfx950"}};
     for (auto &f : fns) {
@@ -2910,7 +2913,10 @@ extern "C" ctox_status ctox_hip_matrix_dispatch_rows(ctox_hip_backend *b, const 
     sa.s_in_kind = m->s_in_kind;
     const uint32_t x_tiles = (sa.rows + 31) / 32;
     ctox_status st = CTOX_OK;
-    if (w.parts == 2) st = launch(b->rows_max, dim3(sa.rows), dim3(256), s, sa, "ctox_rows_max_gfx950");
+    const bool vec = aligned(op->x, 4 * xb) && xs % 4 == 0;
+    // Up to 64 rows are staged in one launch, a workgroup to a row.
+    const bool few = sa.rows <= 64;
+    if (w.parts == 2 && !few) st = launch(b->rows_max[vec], dim3(sa.rows), dim3(256), s, sa, "ctox_rows_max_gfx950");
     bool staged[2] = {false, false};
     for (size_t i = 0; i < m->segments.size() && !st; i++) {
         const ctox_quant_segment &seg = m->segments[i];
@@ -2919,7 +2925,8 @@ extern "C" ctox_status ctox_hip_matrix_dispatch_rows(ctox_hip_backend *b, const 
         if (!staged[q4]) {
             sa.staged = ws + w.staged[q4];
             sa.q4 = (uint32_t)q4;
-            st = launch(b->rows_stage, dim3(sa.blocks, x_tiles), dim3(256), s, sa, "ctox_rows_stage_gfx950");
+            st = few ? launch(b->rows_stage_few[vec], dim3(32 * x_tiles), dim3(512), s, sa, "ctox_rows_stage_few_gfx950")
+                     : launch(b->rows_stage[vec], dim3(sa.blocks, x_tiles), dim3(256), s, sa, "ctox_rows_stage_gfx950");
             if (st) break;
             staged[q4] = true;
         }
