@@ -2806,26 +2806,39 @@ extern "C" ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *b, uint8_t
 }
 
 namespace {
-// Shape and split of one segment's row product. A workgroup takes the most rows of x there are (up to
-// 128), and 256 weight rows rather than 128 where that still gives every CU two workgroups; where there are
-// fewer workgroups than CUs, the K range is split, into eight blocks at least.
+// Shape and K split of one segment's row product, the cheapest by this count: workgroups a CU (between their
+// mean and the whole number that the fullest CU has: idle CUs leave the others a higher clock), times the
+// 32 x 128 tiles and blocks of one, times how much longer a shape takes for the same tile area; a CU
+// with a single workgroup hides less; a split adds a launch and writes and reads its parts.
+// Measured us, 17408 x 5120 Q4 (shapes 32x128, 64x128, 128x128, 128x256): 200 rows 113, 126, 157, -; 777
+// rows 330, 325, 334, 312; 4096 rows 1714, 1519, 1449, 1379; 200 rows of 5120 x 17408 in 1, 4, 8 parts 150, 121, 118.
 struct RowPlan {
     uint32_t shape, col_groups, row_groups, per_split, splits;
 };
-RowPlan row_plan(uint32_t cus, uint32_t rows, uint32_t n, uint32_t blocks) {
-    RowPlan p{};
+RowPlan row_plan(uint32_t cus, uint32_t rows, uint32_t n, uint32_t blocks, uint32_t parts) {
+    const double longer[4] = {1.2, 1.1, 1.05, 1.0}, block_us = parts == 2 ? 0.28 : 0.17;
     const uint32_t tiles = (rows + 31) / 32;
-    p.shape = tiles >= 3 ? 2 : tiles - 1;
-    if (p.shape == 2 && (uint64_t)((tiles + 3) / 4) * ((n + 255) / 256) >= 2 * cus) p.shape = 3;
-    const RowShape s = kRowShapes[p.shape];
-    p.row_groups = (tiles + s.tt - 1) / s.tt;
-    p.col_groups = (n + 128 * s.rt - 1) / (128 * s.rt);
-    const uint64_t wgs = (uint64_t)p.row_groups * p.col_groups;
-    uint32_t splits = 1;
-    if (wgs < cus) splits = std::min<uint32_t>((uint32_t)(2 * cus / wgs), std::max<uint32_t>(1, blocks / 8));
-    p.per_split = (blocks + splits - 1) / splits;
-    p.splits = (blocks + p.per_split - 1) / p.per_split;
-    return p;
+    RowPlan best{};
+    double least = 0.0;
+    for (uint32_t shape = 0; shape < 4; shape++) {
+        const RowShape s = kRowShapes[shape];
+        if (s.tt > 1 && tiles <= s.tt / 2) continue;
+        RowPlan p{shape, (n + 128 * s.rt - 1) / (128 * s.rt), (tiles + s.tt - 1) / s.tt, 0, 0};
+        const double wgs = (double)p.row_groups * p.col_groups;
+        for (uint32_t splits : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u}) {
+            if (splits > 1 && (blocks < 4 * splits || wgs * splits > 8.0 * cus)) break;
+            p.per_split = (blocks + splits - 1) / splits;
+            p.splits = (blocks + p.per_split - 1) / p.per_split;
+            const double x = wgs * p.splits / cus, a_cu = x < 1.0 ? 1.0 : 0.5 * (x + std::ceil(x));
+            double us = a_cu * s.tt * s.rt * p.per_split * longer[shape] * block_us * (1.0 + 0.4 / std::max(x, 1.0));
+            if (p.splits > 1) us += 4.0 + (double)p.splits * rows * n * 8.0 / 4e6;
+            if (least == 0.0 || us < least) {
+                least = us;
+                best = p;
+            }
+        }
+    }
+    return best;
 }
 
 // Where a row product's workspace holds what.
@@ -2842,6 +2855,7 @@ RowSpace row_space(const ctox_hip_matrix *m, uint64_t rows, int32_t x_dtype) {
         at += (bytes + 255) / 256 * 256;
         return here;
     };
+    const uint32_t blocks = (uint32_t)(m->columns / kBlockLen);
     const uint64_t one = (rows + 31) / 32 * 32 * m->columns * 2 * w.parts;
     for (int q4 = 0; q4 < 2; q4++) {
         bool any = false;
@@ -2850,8 +2864,8 @@ RowSpace row_space(const ctox_hip_matrix *m, uint64_t rows, int32_t x_dtype) {
     }
     for (const ctox_quant_segment &seg : m->segments) {
         const uint32_t n = (uint32_t)(seg.row_end - seg.row_start);
-        const RowPlan p = row_plan((uint32_t)m->backend->cus, (uint32_t)rows, n, (uint32_t)(m->columns / kBlockLen));
-        if (p.splits > 1) partial = std::max<uint64_t>(partial, (uint64_t)p.splits * rows * n * sizeof(float));
+        const uint32_t parts = row_plan((uint32_t)m->backend->cus, (uint32_t)rows, n, blocks, w.parts).splits;
+        if (parts > 1) partial = std::max<uint64_t>(partial, (uint64_t)parts * rows * n * sizeof(float));
     }
     w.exps = take(w.parts == 2 ? rows * sizeof(int32_t) : 0);
     w.partial = take(partial);
@@ -2930,7 +2944,7 @@ extern "C" ctox_status ctox_hip_matrix_dispatch_rows(ctox_hip_backend *b, const 
             if (st) break;
             staged[q4] = true;
         }
-        const RowPlan p = row_plan((uint32_t)b->cus, sa.rows, t.rows, sa.blocks);
+        const RowPlan p = row_plan((uint32_t)b->cus, sa.rows, t.rows, sa.blocks, w.parts);
         RowsMulArgs a{};
         a.weights = (const uint8_t *)t.d;
         a.staged = ws + w.staged[q4];
