@@ -658,6 +658,7 @@ struct GqaRowsArgs {
     const uint32_t *tokens;      // [requests]
     float *part;             // [item]: [128][256] numerators, [128][2] (max base 2, denominator)
     float *few_part;         // [item]: the same of 32 queries
+    uint32_t *cuts;          // [requests][2]: a request's first item, and its token ranges
     uint64_t q2_page_bytes;
     uint64_t q4_page_bytes;
     uint32_t requests;

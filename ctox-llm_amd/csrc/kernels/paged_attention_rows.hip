@@ -14,10 +14,12 @@
 // Which workgroup takes what is decided on the device from row_starts and tokens, so the
 // host needs no lengths and a captured launch stays right for other lengths: every workgroup
 // works out for itself how the batch is cut (gr_range) and finds its own item, a token range
-// of one query tile and KV head.
+// of one query tile and KV head. What is in one range is written at once, the rest is joined, from
+// the cuts that a request's first item leaves in the workspace.
 //
 // A wave takes 32 queries and walks tiles of 32 tokens; the waves of a workgroup are four (or
-// one) query subtiles times two (or four) shares of the tiles, and meet only at the end.
+// one) query subtiles times two (or four) shares of the tiles. The four subtiles of a share load and
+// store a quarter of each tile for all four; the shares meet at the end.
 //  Scores: S^T = K Q^T on f16 MFMA 32x32x16. K enters as the exact whole numbers 2c - 15 (a Q2
 //    code c is the Q4 code 5c), a 64-dim block's sum is then multiplied by its f32 scale. A query
 //    is two f16 parts of q 2^-e (22 bits), held in LDS.
@@ -27,9 +29,11 @@
 //  Values: O^T += V^T (P s_v)^T. The scores' output layout is the probabilities' operand layout if the
 //    tokens are counted as gr_v_operands does, so they stay in registers. s_v is the value block's
 //    scale: V is exact again, P s_v is two f16 parts in units of 2^(E - 9) with 2^E above every scale
-//    of the dim block so far. V's bytes are transposed on their way through LDS, a lane's operand being
+//    of the dim block so far. V's bytes are transposed on their way into LDS, a lane's operand being
 //    one byte column of eight tokens.
 // Loads of the next tile are under way during this one, its page descriptors one tile before that.
+// With four subtiles K is stored while V is in use and V while K is, so that one buffer each is
+// enough beside the 128 KiB of queries, and LDS operands are read one step ahead of the products.
 #include <hip/hip_runtime.h>
 
 #include "kernel_args.h"
@@ -42,9 +46,6 @@ typedef float gr_v16 __attribute__((ext_vector_type(16)));
 
 struct __attribute__((packed, aligned(2))) GrBytes16 {
     uint32_t w[4];
-};
-struct __attribute__((packed, aligned(2))) GrBytes8 {
-    uint32_t w[2];
 };
 
 // ---------------------------------------------------------------------------
@@ -175,10 +176,7 @@ __device__ __forceinline__ GrItem gr_find(const GqaRowsArgs &a, bool few, uint32
 // ---------------------------------------------------------------------------
 // operands
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t gr_kind(uint64_t t) { return (uint32_t)(t >> 62); }
-// (in the global address space by type: a table's address would else be read as a flat one)
 typedef const __attribute__((address_space(1))) uint8_t *gr_bytes;
-__device__ __forceinline__ gr_bytes gr_at(uint64_t t) { return (gr_bytes)(t & 0x3fffffffffffffffull); }
 template <typename T>
 __device__ __forceinline__ T gr_load(gr_bytes p) {
     return *(const __attribute__((address_space(1))) T *)p;
@@ -208,6 +206,23 @@ __device__ __forceinline__ void gr_v_operands(uint32_t x, uint32_t y, const RmMa
     o[1] = rm_h8{e[0], e[1], f[0], f[1], p[0], p[1], q[0], q[1]};
 }
 
+// Four lanes' dwords across: lane i of four gets byte i of each.
+__device__ __forceinline__ uint32_t gr_across(uint32_t x, uint32_t lane) {
+    const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true);  // of lane ^ 2
+    const uint32_t a = lane & 2 ? __builtin_amdgcn_perm(x, y, 0x07060302u) : __builtin_amdgcn_perm(y, x, 0x05040100u);
+    const uint32_t b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0xB1, 0xF, 0xF, true);  // of lane ^ 1
+    return lane & 1 ? __builtin_amdgcn_perm(a, b, 0x07030501u) : __builtin_amdgcn_perm(b, a, 0x06020400u);
+}
+
+// A loading lane's token (of 32) and block (of a pair), and the tokens' bits out of a ballot of the first block's.
+__device__ __forceinline__ uint32_t gr_token(uint32_t lane) { return (lane & 3) | (lane >> 3) << 2; }
+__device__ __forceinline__ uint32_t gr_tokens(uint64_t x) {
+    x &= 0x0F0F0F0F0F0F0F0Full;
+    x = (x | x >> 4) & 0x00FF00FF00FF00FFull;
+    x = (x | x >> 8) & 0x0000FFFF0000FFFFull;
+    return (uint32_t)(x | x >> 16);
+}
+
 // Two f16 parts of eight values in the value operand's token order. hi is rounded towards zero, so
 // what is left has hi's sign and at most 13 bits.
 // (x - hi is one mixed-precision multiply-add by an opaque -1; a plain difference would convert first.)
@@ -226,20 +241,24 @@ __device__ __forceinline__ void gr_split(const float (&x)[8], float minus_one, r
 // ---------------------------------------------------------------------------
 // attention of one item
 // ---------------------------------------------------------------------------
-// LDS of a workgroup of QS query subtiles x TS token shares: queries (while tiles run; the joined
-// sums afterwards), and what each wave keeps for itself.
+// LDS of a workgroup of QS query subtiles x TS token shares: queries and the shares' tiles (while
+// tiles run; the joined sums afterwards).
 template <int QS, int TS>
 struct GrLds {
     union {
-        rm_h8 q[QS][2][16][64];         // [subtile][lo, hi][k step][lane]
+        struct {
+            rm_h8 q[QS][2][16][64];     // [subtile][lo, hi][k step][lane]
+            uint4 k[TS][4][2][34];      // [share][block][half][token]: that half's code bytes
+            uint32_t v[TS][4][32][9];   // [share][block][code byte][token / 4]: that byte of four tokens
+            float ks[TS][4][32];        // [share][block][token]: key scale / 15
+            float vs[TS][4][32];        // value scale in units of 2^(9 - E)
+            int ev[TS][4];              // E of a block
+            uint32_t bad[TS][4];        // its tokens without a finite value scale
+        } t;
         float4 sum[QS * TS / 2][32][64];  // [publishing wave][dim block, parity, register quad][lane]
         GrScratch scratch;
     } u;
-    uint32_t v[QS * TS][2][32][9];  // [wave][block of a pair][code byte][token / 4]: that byte of four tokens
-    float ks[QS * TS][4][32];       // [wave][block][token]: key scale / 15
-    float vs[QS * TS][4][32];       // value scale in units of 2^(E - 9)
-    uint64_t tok[QS * TS][32];      // address of the token's K run | kind << 62 (0 absent: the query's, 1 Q2, 2 Q4)
-    float stat[QS * TS][2][32];     // (maximum, denominator) of a publishing wave
+    float stat[QS * TS][2][32];  // (maximum, denominator) of a publishing wave
 };
 
 template <int QS, int TS>
@@ -253,6 +272,10 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     const uint32_t range = gr_range<NT>(a, FEW, L.u.scratch);
     const GrItem it = gr_find<NT>(a, FEW, range, blockIdx.x, true, L.u.scratch);
     if (!it.ok) return;
+    if (it.local == 0 && threadIdx.x == 0) {
+        a.cuts[2 * it.request] = it.base;
+        a.cuts[2 * it.request + 1] = it.ranges;
+    }
     const GrRequest rq = gr_request(a, it.request);
     // Items of a request: query tiles from the last (the longest) to the first, in each the
     // ranges, in each the KV heads (neighbouring workgroups sit on different XCDs: an XCD's L2
@@ -264,8 +287,8 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     const int32_t seen = past + (int32_t)(min(q0 + kQueries - 1, nq - 1) / a.group) + 1;
     const uint32_t vis = (uint32_t)max(seen, 0);
     const uint32_t units = (vis + 32 * TS - 1) / (32 * TS), per = (units + it.ranges - 1) / it.ranges;
-    // Tiles of 32 tokens: this wave's are t0, t0 + TS, ... below t1.
-    const uint32_t t0 = min(part * per, units) * TS + ts, t1 = min(min(part * per + per, units) * TS, (vis + 31) / 32);
+    // Tiles of 32 tokens: this wave's are t0, t0 + TS, ... below t1 (a last one may have no tokens).
+    const uint32_t t0 = min(part * per, units) * TS + ts, t1 = min(part * per + per, units) * TS;
 
     const uint32_t qi = q0 + 32 * qsub + li;  // this lane's query
     const bool valid = qi < nq;
@@ -274,88 +297,86 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     const uint32_t qrow = valid ? qi / a.group : 0, qg = valid ? qi - qrow * a.group : 0;
     const size_t qat = ((size_t)(rq.row0 + qrow) * a.query_heads + kvh * a.group + qg) * 256;
 
-    // Token -> address. A token past what the tile's queries see, or in no page, is absent: its loads
-    // go to the query rows (always there, and long enough), its scales count as 0.
+    // Tiles come in four pieces: two of K, two of V, of two dim blocks each. A lane loads one block of one token: 32
+    // code bytes (Q2: 16, both loads the same) and a scale. With four subtiles each wave loads one piece of its
+    // share's tile for all four, else the one wave all of them. A token past what the tile's queries
+    // see, or in no page, is absent: its loads go to the query rows, its scales count as 0.
+    constexpr int R = QS == 4 ? 1 : 4;
+    constexpr int AHEAD = QS == 4 ? 1 : 0;  // steps that LDS operands are read ahead (no registers for it in the other)
+    const uint32_t token = gr_token(lane), pb = lane >> 2 & 1;
+    const uint32_t piece = QS == 4 ? qsub : 0;
     PagedKvDesc dsc{0, 0, 0, 0};
     auto desc_load = [&](uint32_t t) {
-        const uint32_t j = t * 32 + li;
+        const uint32_t j = t * 32 + token;
         const uint32_t p = (uint32_t)(((uint64_t)j * a.page_magic) >> a.page_shift);
         dsc = a.desc[(size_t)it.request * a.max_pages + (t < t1 && j < vis ? p : 0)];
     };
-    uint64_t at = 0;
-    uint32_t present = 0, hole = 0;  // of the tile that `at` belongs to
-    auto resolve = [&](uint32_t t) {
-        const uint32_t j = t * 32 + li, tip = j - dsc.first_token;
+    uint32_t raw[R][8], rsc[R], rkind = 0;  // rkind: 0 absent, 1 Q2, 2 Q4
+    uint32_t here = 0, next = 0;            // tokens that are there: of the tile before, and of the one in `raw`
+    auto issue = [&](uint32_t t) {
+        const uint32_t j = t * 32 + token, tip = j - dsc.first_token;
         const bool want = t < t1 && j < vis;
         const bool in = want && j >= dsc.first_token && tip < min(dsc.tokens, a.page_tokens), q4 = dsc.precision != 0;
         const uint8_t *pool = q4 ? a.q4 : a.q2;
+        const uint32_t bytes = q4 ? 34 : 18;
         const uint8_t *run = pool + (size_t)dsc.physical_slot * (q4 ? a.q4_page_bytes : a.q2_page_bytes) +
-                             (size_t)tip * (q4 ? a.q4_token_bytes : a.q2_token_bytes) + kvh * (q4 ? 136 : 72);
-        at = in ? (uint64_t)(uintptr_t)run | (q4 ? 2ull << 62 : 1ull << 62) : (uint64_t)(uintptr_t)a.query;
-        present = (uint32_t)__builtin_amdgcn_ballot_w64(in);
-        hole = __builtin_amdgcn_ballot_w64(want && !in) != 0;
-        if (h == 0) L.tok[wave][li] = at;
-        lds_wave_order();
-    };
-
-    // Keys: this lane's half of four blocks of its token; two scales of K and of V. A Q2 half is 8
-    // of the 16 bytes read (what lies behind is the token's own).
-    uint32_t kw[4][4], ksc[2], vsc[2], kkind = 0;
-    auto issue_k = [&]() {
-        kkind = gr_kind(at);
-        const uint32_t step = kkind == 1 ? 18 : 34;
-        const gr_bytes p = gr_at(at), c = p + 2 + (kkind == 1 ? 8 * h : 16 * h);
+                             (size_t)tip * (q4 ? a.q4_token_bytes : a.q2_token_bytes) + (4 * kvh + pb) * bytes;
+        rkind = in ? (q4 ? 2u : 1u) : 0u;
+        here = next;
+        next = gr_tokens(__builtin_amdgcn_ballot_w64(in));
+        const gr_bytes p = in ? (gr_bytes)(uintptr_t)run : (gr_bytes)(uintptr_t)a.query;
+        const uint32_t second = rkind == 1 ? 2 : 18, pair = in ? 2 * bytes : 0, v = in ? (q4 ? a.v_off4 : a.v_off2) : 0;
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
-            const GrBytes16 x = gr_load<GrBytes16>(c + b * step);
+        for (int i = 0; i < R; i++) {
+            const uint32_t n = piece + i;
+            const gr_bytes c = p + (n & 1 ? pair : 0) + (n >> 1 ? v : 0);
+            const GrBytes16 x = gr_load<GrBytes16>(c + 2), y = gr_load<GrBytes16>(c + second);
 #pragma unroll
-            for (int i = 0; i < 4; i++) kw[b][i] = x.w[i];
-        }
-        const gr_bytes sk = p + 2 * h * step, sv = sk + (kkind == 1 ? a.v_off2 : a.v_off4);
-        ksc[0] = gr_load<uint16_t>(sk);
-        ksc[1] = gr_load<uint16_t>(sk + step);
-        vsc[0] = gr_load<uint16_t>(sv);
-        vsc[1] = gr_load<uint16_t>(sv + step);
-    };
-    // Values of block pair p: eight code bytes (Q4) of four tokens of one block. The four bytes of a Q2
-    // token are one half of an eight-byte piece of its block.
-    const uint32_t vq = lane & 7, vo = (lane >> 3) & 3, vb = lane >> 5;  // token quad, octet of bytes, block of the pair
-    uint32_t vw[2][4][2], vtwo[2];                                         // vtwo: bit i where token i is Q2
-    auto issue_v = [&](int p) {
-        vtwo[p] = 0;
-        const uint32_t c4 = a.v_off4 + 34 * (2 * p + vb) + 2 + 8 * vo, c2 = a.v_off2 + 18 * (2 * p + vb) + 2 + 8 * (vo >> 1);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint64_t x = L.tok[wave][4 * vq + i];
-            const bool two = gr_kind(x) == 1;
-            vtwo[p] |= two ? 1u << i : 0u;
-            const GrBytes8 y = gr_load<GrBytes8>(gr_at(x) + (two ? c2 : c4));
-            vw[p][i][0] = y.w[0], vw[p][i][1] = y.w[1];
+            for (int w = 0; w < 4; w++) raw[i][w] = x.w[w], raw[i][4 + w] = y.w[w];
+            rsc[i] = gr_load<uint16_t>(c);
         }
     };
-    auto write_v = [&](int p) {
-        if (__builtin_amdgcn_ballot_w64(vtwo[p] != 0)) {
+    auto widen = [&](uint32_t (&x)[8]) {
+        if (__builtin_amdgcn_ballot_w64(rkind == 1)) {
+            const uint32_t y[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t x = vo & 1 ? vw[p][i][1] : vw[p][i][0];
-                const bool two = vtwo[p] >> i & 1;
-                vw[p][i][0] = two ? gr_widen(x) : vw[p][i][0];
-                vw[p][i][1] = two ? gr_widen(x >> 16) : vw[p][i][1];
-            }
+            for (int w = 0; w < 8; w++) x[w] = rkind == 1 ? gr_widen(w & 1 ? y[w >> 1] >> 16 : y[w >> 1]) : x[w];
+        }
+    };
+    auto store_k = [&](int i) {
+        const uint32_t b = 2 * ((piece + i) & 1) + pb;
+        widen(raw[i]);
+        L.u.t.ks[ts][b][token] = rkind ? (float)__builtin_bit_cast(_Float16, (uint16_t)rsc[i]) * (1.0f / 15.0f) : 0.0f;
+        L.u.t.k[ts][b][0][token] = make_uint4(raw[i][0], raw[i][1], raw[i][2], raw[i][3]);
+        L.u.t.k[ts][b][1][token] = make_uint4(raw[i][4], raw[i][5], raw[i][6], raw[i][7]);
+    };
+    int ve[R];  // 2^ve above every value scale of the lane's block so far
+#pragma unroll
+    for (int i = 0; i < R; i++) ve[i] = -100;
+    auto store_v = [&](int i) {
+        const uint32_t b = 2 * ((piece + i) & 1) + pb;
+        widen(raw[i]);
+        float sv = rkind ? (float)__builtin_bit_cast(_Float16, (uint16_t)rsc[i]) : 0.0f;
+        uint32_t bad = 0;
+        if (__builtin_amdgcn_ballot_w64(!(fabsf(ldexpf(sv, -ve[i])) < 1.0f))) {
+            const bool odd = !(fabsf(sv) < INFINITY);
+            bad = gr_tokens(__builtin_amdgcn_ballot_w64(odd) >> (4 * pb));
+            if (odd) sv = 0.0f;
+            float z = fabsf(sv);
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1)
+                if (d != 4) z = fmaxf(z, __shfl_xor(z, d));
+            int e = 0;
+            frexpf(z, &e);
+            ve[i] = max(ve[i], e);
+        }
+        L.u.t.vs[ts][b][token] = ldexpf(sv, 9 - ve[i]);
+        if ((lane & 59) == 0) {
+            L.u.t.ev[ts][b] = ve[i];
+            L.u.t.bad[ts][b] = bad;
         }
 #pragma unroll
-        for (int w = 0; w < 2; w++) {
-            // 4 x 4 bytes across: byte r of the four tokens into one dword.
-            const uint32_t ab0 = __builtin_amdgcn_perm(vw[p][1][w], vw[p][0][w], 0x05010400u);
-            const uint32_t ab1 = __builtin_amdgcn_perm(vw[p][1][w], vw[p][0][w], 0x07030602u);
-            const uint32_t cd0 = __builtin_amdgcn_perm(vw[p][3][w], vw[p][2][w], 0x05010400u);
-            const uint32_t cd1 = __builtin_amdgcn_perm(vw[p][3][w], vw[p][2][w], 0x07030602u);
-            const uint32_t r = 8 * vo + 4 * w;
-            L.v[wave][vb][r][vq] = __builtin_amdgcn_perm(cd0, ab0, 0x05040100u);
-            L.v[wave][vb][r + 1][vq] = __builtin_amdgcn_perm(cd0, ab0, 0x07060302u);
-            L.v[wave][vb][r + 2][vq] = __builtin_amdgcn_perm(cd1, ab1, 0x05040100u);
-            L.v[wave][vb][r + 3][vq] = __builtin_amdgcn_perm(cd1, ab1, 0x07060302u);
-        }
+        for (int w = 0; w < 8; w++) L.u.t.v[ts][b][4 * w + (lane & 3)][lane >> 3] = gr_across(raw[i][w], lane);
     };
 
     const RmMagic magic = rm_magic<true>();
@@ -399,11 +420,11 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
                 hi[i] = (_Float16)v;
                 lo[i] = fabsf(v) < INFINITY ? (_Float16)(v - (float)hi[i]) : (_Float16)0.0f;
             }
-            L.u.q[qsub][0][s][lane] = lo;
-            L.u.q[qsub][1][s][lane] = hi;
+            L.u.t.q[qsub][0][s][lane] = lo;
+            L.u.t.q[qsub][1][s][lane] = hi;
         }
     }
-    __syncthreads();
+    if (QS == 1) __syncthreads();
 
     gr_v16 o[4][2];  // [dim block][even, odd dims]
 #pragma unroll
@@ -413,76 +434,35 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
 #pragma unroll
             for (int r = 0; r < 16; r++) o[b][c][r] = 0.0f;
     float m = -INFINITY, den = 0.0f;
-    int ev[4] = {-100, -100, -100, -100};  // 2^ev above every value scale of the block so far
-    float bound[2], unit[2];               // 2^ev and 2^(9 - ev) of blocks 2 h, 2 h + 1
-#pragma unroll
-    for (int i = 0; i < 2; i++) bound[i] = ldexpf(1.0f, -100), unit[i] = ldexpf(1.0f, 109);
+    int ev[4] = {-100, -100, -100, -100};  // E of the blocks' sums
 
-    resolve(t0);
+    issue(t0);
     desc_load(t0 + TS);
-    issue_k();
-    issue_v(0);
-    issue_v(1);
+    if (QS == 4 && piece < 2) {
+        store_k(0);
+        issue(t0 + TS);
+        desc_load(t0 + 2 * TS);
+    }
     // (nothing under way on entry: the loop's waits are then counted by the order of its own loads alone)
     __builtin_amdgcn_s_waitcnt(0x0F70);
     for (uint32_t t = t0; t < t1; t += TS) {
-        const uint32_t here = present, gone = hole;
-        // ---- this tile's scales; the next tile's addresses ----
-        float sv[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            L.ks[wave][2 * h + i][li] =
-                kkind ? (float)__builtin_bit_cast(_Float16, (uint16_t)ksc[i]) * (1.0f / 15.0f) : 0.0f;
-            sv[i] = kkind ? (float)__builtin_bit_cast(_Float16, (uint16_t)vsc[i]) : 0.0f;
+        // ---- this tile's bytes and scales into LDS; the next tile's loads ----
+        // With four subtiles K is written during the values before it, V during the scores before it:
+        // `raw` holds K of the next tile, or V of this one.
+        if (QS == 4) {
+            lds_barrier();  // K is written, the last tile's V is no longer read
+            if (piece >= 2) store_v(0);
+        } else {
+            store_k(0);
+            store_k(1);
+            store_v(2);
+            store_v(3);
+            lds_wave_order();
         }
-        uint32_t odd = 0;  // bit i: this lane's token has no finite value scale in block 2 h + i
-        if (__builtin_amdgcn_ballot_w64(!(fabsf(sv[0]) < bound[0]) || !(fabsf(sv[1]) < bound[1]))) {
-            float z[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                if (!(fabsf(sv[i]) < INFINITY)) {
-                    sv[i] = 0.0f;
-                    odd |= 1u << i;
-                }
-                z[i] = fabsf(sv[i]);
-#pragma unroll
-                for (int d = 16; d > 0; d >>= 1) z[i] = fmaxf(z[i], __shfl_xor(z[i], d));
-            }
-#pragma unroll
-            for (int b = 0; b < 4; b++) {
-                int e = 0;
-                frexpf(z[b & 1], &e);
-                e = __builtin_amdgcn_readlane(e, 32 * (b >> 1));
-                const int d = max(ev[b] - e, -200);
-                if (d < 0) {
-#pragma unroll
-                    for (int c = 0; c < 2; c++)
-#pragma unroll
-                        for (int r = 0; r < 16; r++) o[b][c][r] = ldexpf(o[b][c][r], d);
-                    ev[b] = e;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int e = h ? ev[2 + i] : ev[i];
-                bound[i] = ldexpf(1.0f, e), unit[i] = ldexpf(1.0f, 9 - e);
-            }
+        if (QS != 4 || piece >= 2) {
+            issue(t + TS);
+            desc_load(t + 2 * TS);
         }
-#pragma unroll
-        for (int i = 0; i < 2; i++) L.vs[wave][2 * h + i][li] = sv[i] * unit[i];
-        if (__builtin_amdgcn_ballot_w64(kkind == 1)) {
-            const bool two = kkind == 1;
-#pragma unroll
-            for (int b = 0; b < 4; b++) {
-                const uint32_t x = kw[b][0], y = kw[b][1];
-                kw[b][0] = two ? gr_widen(x) : kw[b][0];
-                kw[b][1] = two ? gr_widen(x >> 16) : kw[b][1];
-                kw[b][2] = two ? gr_widen(y) : kw[b][2];
-                kw[b][3] = two ? gr_widen(y >> 16) : kw[b][3];
-            }
-        }
-        resolve(t + TS);
-        desc_load(t + 2 * TS);
         // ---- scores ----
         gr_v16 s;
 #pragma unroll
@@ -490,29 +470,48 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
         // (opaque: the queries do not change from tile to tile, but are not to be kept in registers)
         uint32_t ql = lane;
         asm volatile("" : "+v"(ql));
+        // Operands are read a step (two products) ahead; without the fences the reads would sink to their uses.
+        rm_h8 qf[2][2];
+        float4 kf4[4];
+        uint4 kq, kn;
+        if (AHEAD) kq = L.u.t.k[ts][0][h][li];
+        if (AHEAD) qf[0][0] = L.u.t.q[qsub][0][0][ql], qf[0][1] = L.u.t.q[qsub][1][0][ql];
+        gr_v16 x;
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
-            gr_v16 x;
-#pragma unroll
-            for (int r = 0; r < 16; r++) x[r] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const rm_h8 kf = gr_k_operand(kw[b][k], magic);
-                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, L.u.q[qsub][0][4 * b + k][ql], x, 0, 0, 0);
-                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, L.u.q[qsub][1][4 * b + k][ql], x, 0, 0, 0);
+        for (int n = 0; n < 16; n++) {
+            const int b = n >> 2, k = n & 3;
+            if (n + AHEAD < 16) {
+                qf[(n + AHEAD) & 1][0] = L.u.t.q[qsub][0][n + AHEAD][ql];
+                qf[(n + AHEAD) & 1][1] = L.u.t.q[qsub][1][n + AHEAD][ql];
             }
+            if (AHEAD && k == 3)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float4 f = *(const float4 *)&L.ks[wave][b][8 * j + 4 * h];
-                s[4 * j] = fmaf(f.x, x[4 * j], s[4 * j]);
-                s[4 * j + 1] = fmaf(f.y, x[4 * j + 1], s[4 * j + 1]);
-                s[4 * j + 2] = fmaf(f.z, x[4 * j + 2], s[4 * j + 2]);
-                s[4 * j + 3] = fmaf(f.w, x[4 * j + 3], s[4 * j + 3]);
+                for (int j = 0; j < 4; j++) kf4[j] = *(const float4 *)&L.u.t.ks[ts][b][8 * j + 4 * h];
+            if (AHEAD && k == 2) kn = L.u.t.k[ts][min(b + 1, 3)][h][li];
+            if (k == 0) {
+                if (!AHEAD) kq = L.u.t.k[ts][b][h][li];
+#pragma unroll
+                for (int r = 0; r < 16; r++) x[r] = 0.0f;
+            }
+            if (AHEAD) __builtin_amdgcn_sched_barrier(0x76);
+            const rm_h8 kf = gr_k_operand(k == 0 ? kq.x : k == 1 ? kq.y : k == 2 ? kq.z : kq.w, magic);
+            x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[n & 1][0], x, 0, 0, 0);
+            x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[n & 1][1], x, 0, 0, 0);
+            if (AHEAD) __builtin_amdgcn_sched_barrier(0x76);
+            if (k == 3) {
+                if (AHEAD) kq = kn;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float4 f = AHEAD ? kf4[j] : *(const float4 *)&L.u.t.ks[ts][b][8 * j + 4 * h];
+                    s[4 * j] = fmaf(f.x, x[4 * j], s[4 * j]);
+                    s[4 * j + 1] = fmaf(f.y, x[4 * j + 1], s[4 * j + 1]);
+                    s[4 * j + 2] = fmaf(f.z, x[4 * j + 2], s[4 * j + 2]);
+                    s[4 * j + 3] = fmaf(f.w, x[4 * j + 3], s[4 * j + 3]);
+                }
             }
         }
-        issue_k();
         // ---- masks: a tile that ends past the first query's last token, or has absent tokens ----
-        if ((int32_t)((t + 1) * 32) - 1 > lim0 || gone) {
+        if ((int32_t)((t + 1) * 32) - 1 > lim0 || here != ~0u) {
             const uint32_t on = here >> (4 * h);
             const int32_t left = lim - (int32_t)(t * 32 + 4 * h);  // tokens up to this one
 #pragma unroll
@@ -547,13 +546,35 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
             den += d;
         }
         // ---- values ----
-        // A value block without a finite scale makes its dims no numbers for every query that sees the token, and
-        // does not count for the others (its scale is 0 from here on).
-        if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+        if (QS == 4) {
+            lds_barrier();  // V is written, K is no longer read
+            if (piece < 2) {
+                store_k(0);
+                issue(t + 2 * TS);
+                desc_load(t + 3 * TS);
+            }
+        }
+        const int4 e4 = *(const int4 *)L.u.t.ev[ts];
+        const uint4 bad4 = *(const uint4 *)L.u.t.bad[ts];
+        const int e[4] = {e4.x, e4.y, e4.z, e4.w};
+        if (__builtin_amdgcn_ballot_w64(e[0] != ev[0] || e[1] != ev[1] || e[2] != ev[2] || e[3] != ev[3])) {
 #pragma unroll
             for (int b = 0; b < 4; b++) {
-                const uint64_t who = __builtin_amdgcn_ballot_w64(odd >> (b & 1) & 1);
-                const uint32_t bad = (uint32_t)(who >> (32 * (b >> 1))) >> (4 * h);
+                const int d = max(ev[b] - e[b], -200);
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) o[b][c][r] = ldexpf(o[b][c][r], d);
+                ev[b] = __builtin_amdgcn_readfirstlane(e[b]);
+            }
+        }
+        // A value block without a finite scale makes its dims no numbers for every query that sees the token, and
+        // does not count for the others (its scale is 0).
+        if (__builtin_amdgcn_ballot_w64((bad4.x | bad4.y | bad4.z | bad4.w) != 0)) {
+            const uint32_t bads[4] = {bad4.x, bad4.y, bad4.z, bad4.w};
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const uint32_t bad = bads[b] >> (4 * h);
                 bool any = false;
 #pragma unroll
                 for (int r = 0; r < 16; r++) any |= (bad >> (8 * (r >> 2) + (r & 3)) & 1) && s[r] != 0.0f;
@@ -564,34 +585,34 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
                     for (int r = 0; r < 16; r++) o[b][c][r] = any ? __builtin_nanf("") : o[b][c][r];
             }
         }
+        uint32_t vx[2][2];
+        float4 fx[2][2];
+        auto read_v = [&](int n) {
+            const uint32_t b = n >> 1, tq = 4 * (n & 1) + h;
+            vx[n & 1][0] = L.u.t.v[ts][b][li][tq], vx[n & 1][1] = L.u.t.v[ts][b][li][tq + 2];
+            fx[n & 1][0] = *(const float4 *)&L.u.t.vs[ts][b][4 * tq];
+            fx[n & 1][1] = *(const float4 *)&L.u.t.vs[ts][b][4 * tq + 8];
+        };
+        if (AHEAD) read_v(0);
 #pragma unroll
-        for (int p = 0; p < 2; p++) {
-            write_v(p);
-            lds_wave_order();
-            issue_v(p);
+        for (int n = 0; n < 8; n++) {
+            const int b = n >> 1, k = n & 1;
+            if (n + AHEAD < 8) read_v(n + AHEAD);
+            if (AHEAD) __builtin_amdgcn_sched_barrier(0x76);
+            rm_h8 vf[2];
+            gr_v_operands(vx[k][0], vx[k][1], magic, vf);
+            const float4 f0 = fx[k][0], f1 = fx[k][1];
+            const float x[8] = {s[8 * k] * f0.x,     s[8 * k + 1] * f0.y, s[8 * k + 2] * f0.z, s[8 * k + 3] * f0.w,
+                                s[8 * k + 4] * f1.x, s[8 * k + 5] * f1.y, s[8 * k + 6] * f1.z, s[8 * k + 7] * f1.w};
+            rm_h8 hi, lo;
+            gr_split(x, minus_one, hi, lo);
 #pragma unroll
-            for (int b = 0; b < 2; b++)
+            for (int c = 0; c < 2; c++) o[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c], lo, o[b][c], 0, 0, 0);
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const uint32_t tq = 4 * k + h;
-                    rm_h8 vf[2];
-                    gr_v_operands(L.v[wave][b][li][tq], L.v[wave][b][li][tq + 2], magic, vf);
-                    const float4 f0 = *(const float4 *)&L.vs[wave][2 * p + b][4 * tq];
-                    const float4 f1 = *(const float4 *)&L.vs[wave][2 * p + b][4 * tq + 8];
-                    const float x[8] = {s[8 * k] * f0.x,     s[8 * k + 1] * f0.y,
-                                        s[8 * k + 2] * f0.z, s[8 * k + 3] * f0.w,
-                                        s[8 * k + 4] * f1.x, s[8 * k + 5] * f1.y,
-                                        s[8 * k + 6] * f1.z, s[8 * k + 7] * f1.w};
-                    rm_h8 hi, lo;
-                    gr_split(x, minus_one, hi, lo);
-                    gr_v16 *y = o[2 * p + b];
-#pragma unroll
-                    for (int c = 0; c < 2; c++) y[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c], lo, y[c], 0, 0, 0);
-#pragma unroll
-                    for (int c = 0; c < 2; c++) y[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c], hi, y[c], 0, 0, 0);
-                        }
-            lds_wave_order();
+            for (int c = 0; c < 2; c++) o[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c], hi, o[b][c], 0, 0, 0);
+            if (AHEAD) __builtin_amdgcn_sched_barrier(0x76);
         }
+        lds_wave_order();
     }
     // ---- join the token shares, half of the waves publishing to the other half, and write ----
     den += __shfl_xor(den, 32);
@@ -645,7 +666,7 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     }
     if (ts || !valid) return;
     float *dst, f = 1.0f;
-    if (FEW || a.split) {
+    if (it.ranges > 1) {
         float *slot = (FEW ? a.few_part : a.part) + (size_t)blockIdx.x * (kQueries * 258);
         const uint32_t in = 32 * qsub + li;
         dst = slot + (size_t)in * 256;
@@ -675,38 +696,37 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few_gfx950(GqaRows
 // join: grid (rows, query heads), four waves take every fourth part, 64 lanes x 4 dims
 // ---------------------------------------------------------------------------
 extern "C" __global__ __launch_bounds__(256) void ctox_gqa_join_gfx950(GqaRowsArgs a) {
-    __shared__ GrScratch L;
     __shared__ float4 acc4[4][64];
     __shared__ float st[4][2];
     const uint32_t row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (row >= min(a.row_starts[a.requests], a.rows)) return;
     uint32_t lo = 0, hi = a.requests;  // the request of this row: the last that starts at or before it
     while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (a.row_starts[mid] <= row) lo = mid;
-        else hi = mid;
+        const uint32_t step = (hi - lo + 63) / 64, at = lo + lane * step;
+        const uint32_t n = __popcll(__builtin_amdgcn_ballot_w64(at < hi && a.row_starts[min(at, hi - 1)] <= row));
+        lo += max(n, 1u) * step - step;
+        hi = min(lo + step, hi);
     }
     const GrRequest rq = gr_request(a, lo);
+    if (row < rq.row0 || row - rq.row0 >= rq.rows) return;
     const bool few = gr_few(a, rq);
-    if ((!few && !a.split) || row < rq.row0 || row - rq.row0 >= rq.rows) return;
-    const uint32_t range = gr_range<256>(a, few, L);
-    const GrItem it = gr_find<256>(a, few, range, lo, false, L);
-    if (!it.ok) return;
+    const uint32_t first = a.cuts[2 * lo], ranges = a.cuts[2 * lo + 1];
+    if (ranges < 2) return;
     const uint32_t kvh = head / a.group, q = (row - rq.row0) * a.group + head % a.group;
     const uint32_t size = few ? 32 : 128, nqt = (rq.rows * a.group + size - 1) / size, in = q % size;
-    const uint32_t slot0 = it.base + (nqt - 1 - q / size) * it.ranges * a.kv_heads + kvh;
+    const uint32_t slot0 = first + (nqt - 1 - q / size) * ranges * a.kv_heads + kvh;
     const float *base = few ? a.few_part : a.part;
     float m = -INFINITY, den = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (uint32_t s0 = wave; s0 < it.ranges; s0 += 16) {
+    for (uint32_t s0 = wave; s0 < ranges; s0 += 16) {
         float4 v[4];
         float ms[4], ds[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const uint32_t s = min(s0 + 4 * k, it.ranges - 1);
+            const uint32_t s = min(s0 + 4 * k, ranges - 1);
             const float *p = base + (size_t)(slot0 + s * a.kv_heads) * (size * 258);
             v[k] = ((const float4 *)(p + (size_t)in * 256))[lane];
-            ms[k] = s0 + 4 * k < it.ranges ? p[size * 256 + 2 * in] : -INFINITY;
+            ms[k] = s0 + 4 * k < ranges ? p[size * 256 + 2 * in] : -INFINITY;
             ds[k] = p[size * 256 + 2 * in + 1];
         }
         float mn = m;

@@ -3003,7 +3003,7 @@ ctox_status check_gqa_rows(const ctox_paged_gqa_rows *op) {
 struct GqaRowsPlan {
     bool few, wide, split;
     uint32_t few_slots, slots, few_items, items;
-    uint64_t few_bytes, bytes;
+    uint64_t cut_bytes, few_bytes, bytes;
 };
 GqaRowsPlan gqa_rows_plan(uint32_t cus, const ctox_paged_gqa_rows *op) {
     GqaRowsPlan g{};
@@ -3014,6 +3014,7 @@ GqaRowsPlan gqa_rows_plan(uint32_t cus, const ctox_paged_gqa_rows *op) {
     g.few = group <= 32 && !(g.wide && op->requests == 1);
     g.few_slots = 2 * cus;
     g.slots = cus;
+    g.cut_bytes = ((uint64_t)op->requests * 8 + 15) / 16 * 16;
     if (g.few) {
         g.few_items = (uint32_t)(busy * kvh + 2 * g.few_slots);
         g.few_bytes = (uint64_t)g.few_items * 32 * 258 * sizeof(float);
@@ -3035,7 +3036,7 @@ extern "C" ctox_status ctox_hip_paged_gqa_rows_workspace(const ctox_hip_backend 
     if (ctox_status st = check_gqa_rows(op)) return st;
     if (!b) return fail(CTOX_ERR_SHAPE, "null argument");
     const GqaRowsPlan g = gqa_rows_plan((uint32_t)b->cus, op);
-    *bytes = (size_t)(g.few_bytes + g.bytes);
+    *bytes = (size_t)(g.cut_bytes + g.few_bytes + g.bytes);
     return CTOX_OK;
 }
 
@@ -3049,8 +3050,8 @@ extern "C" ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *b, const
         return fail(CTOX_ERR_SHAPE, "an attention pointer is not aligned");
     if (op->rows == 0) return CTOX_OK;
     const GqaRowsPlan g = gqa_rows_plan((uint32_t)b->cus, op);
-    const uint64_t need = g.few_bytes + g.bytes;
-    if (need && (op->workspace_bytes < need || !op->workspace || !aligned(op->workspace, 16)))
+    const uint64_t need = g.cut_bytes + g.few_bytes + g.bytes;
+    if ((op->workspace_bytes < need || !op->workspace || !aligned(op->workspace, 16)))
         return fail(CTOX_ERR_MEMORY_BUDGET, "workspace of %llu bytes, %llu needed, 16-byte aligned",
                     (unsigned long long)op->workspace_bytes, (unsigned long long)need);
     const ctox_paged_gqa_params &p = op->params;
@@ -3063,8 +3064,9 @@ extern "C" ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *b, const
     a.desc = (const PagedKvDesc *)op->descriptors;
     a.row_starts = op->row_starts;
     a.tokens = op->tokens;
-    a.few_part = (float *)op->workspace;
-    a.part = (float *)((uint8_t *)op->workspace + g.few_bytes);
+    a.cuts = (uint32_t *)op->workspace;
+    a.few_part = (float *)((uint8_t *)op->workspace + g.cut_bytes);
+    a.part = (float *)((uint8_t *)op->workspace + g.cut_bytes + g.few_bytes);
     a.q2_page_bytes = p.q2_page_bytes;
     a.q4_page_bytes = p.q4_page_bytes;
     a.requests = op->requests;
