@@ -304,7 +304,8 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     constexpr int R = QS == 4 ? 1 : 4;
     constexpr int AHEAD = QS == 4 ? 1 : 0;  // steps that LDS operands are read ahead (no registers for it in the other)
     const uint32_t token = gr_token(lane), pb = lane >> 2 & 1;
-    const uint32_t piece = QS == 4 ? qsub : 0;
+    // (a SIMD has one wave of each share: one of them stores K, the other V, so that SIMDs stay level)
+    const uint32_t piece = QS == 4 ? qsub ^ (2 * ts) : 0;
     PagedKvDesc dsc{0, 0, 0, 0};
     auto desc_load = [&](uint32_t t) {
         const uint32_t j = t * 32 + token;
