@@ -3101,6 +3101,6 @@ extern "C" ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *b, const
     if (!st && g.few)
         st = launch(b->gqa_few, dim3(g.few_items), dim3(256), s, a, "ctox_gqa_few_gfx950");
     if (!st && (g.few || g.split))
-        st = launch(b->gqa_join, dim3(a.rows, p.query_heads), dim3(256), s, a, "ctox_gqa_join_gfx950");
+        st = launch(b->gqa_join, dim3(a.rows, (p.query_heads + 3) / 4), dim3(256), s, a, "ctox_gqa_join_gfx950");
     return st;
 }
