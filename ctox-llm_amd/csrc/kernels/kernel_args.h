@@ -657,7 +657,7 @@ struct GqaRowsArgs {
     const uint32_t *row_starts;  // [requests + 1]
     const uint32_t *tokens;      // [requests]
     float *part;             // [item]: [128][256] numerators, [128][2] (max base 2, denominator)
-    float *few_part;         // [item]: the same of 32 queries
+    float *few_part;         // [item]: the same of `few` queries
     uint32_t *cuts;          // [requests][2]: a request's first item, and its token ranges
     uint64_t q2_page_bytes;
     uint64_t q4_page_bytes;
@@ -676,7 +676,7 @@ struct GqaRowsArgs {
     uint32_t split;          // the 128-query kernel's token ranges are split and joined
     uint32_t slots;          // its workgroups that run at once
     uint32_t items;          // most items it may be cut into
-    uint32_t few;            // requests of at most 32 queries a KV head go to the few-query kernel
+    uint32_t few;            // requests of at most this many queries a KV head (0, 16, 32) go to a few-query kernel
     uint32_t few_slots;
     uint32_t few_items;
     float scale;

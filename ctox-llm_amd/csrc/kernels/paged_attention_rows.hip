@@ -7,8 +7,9 @@
 // that all heads that share a KV head share what is read of it.
 //
 //  * ctox_gqa_rows_gfx950: 128 queries of one KV head a workgroup.
-//  * ctox_gqa_few_gfx950: the same for requests of at most 32 queries a KV head (decoded tokens,
-//    verified drafts), 32 queries a workgroup.
+//  * ctox_gqa_few_gfx950: the same for requests of at most 32 queries a KV head (verified drafts),
+//    32 queries a workgroup.
+//  * ctox_gqa_few16_gfx950: the same for batches in which no request has more than 16 (decoded tokens).
 //  * ctox_gqa_join_gfx950: joins the parts of a split token range.
 //
 // Which workgroup takes what is decided on the device from row_starts and tokens, so the
@@ -42,7 +43,6 @@
 typedef float gr_v16 __attribute__((ext_vector_type(16)));
 
 #define GR_MOVE 6.0f  // base-2 slack before the running maximum moves
-#define GR_FEW 32     // queries of a request's KV head that the few-query kernel takes
 
 struct __attribute__((packed, aligned(2))) GrBytes16 {
     uint32_t w[4];
@@ -61,7 +61,7 @@ __device__ __forceinline__ GrRequest gr_request(const GqaRowsArgs &a, uint32_t r
 }
 
 __device__ __forceinline__ bool gr_few(const GqaRowsArgs &a, const GrRequest &q) {
-    return a.few && q.rows * a.group <= GR_FEW;
+    return q.rows * a.group <= a.few;
 }
 
 // Of one request: query tiles, and units of the token axis (as many as a workgroup's waves take at once).
@@ -239,6 +239,96 @@ __device__ __forceinline__ void gr_split(const float (&x)[8], float minus_one, r
 }
 
 // ---------------------------------------------------------------------------
+// tiles from the pages
+// ---------------------------------------------------------------------------
+// A tile of 32 tokens comes in four pieces, two of K and two of V, of two dim blocks each. A lane loads one block of one
+// token: 32 code bytes (Q2: 16, both loads the same) and a scale. A token past what the item's queries see, or
+// in no page, is absent: its loads go to the query rows (always there), its scales count as 0. R: pieces
+// of one wave, from `piece` on.
+template <int R>
+struct GrLoad {
+    const GqaRowsArgs &a;
+    const uint32_t request, kvh, vis, t1, token, pb, piece;
+    PagedKvDesc dsc{0, 0, 0, 0};
+    uint32_t raw[R][8], rsc[R], rkind = 0;  // rkind: 0 absent, 1 Q2, 2 Q4
+    uint32_t here = 0, next = 0;            // tokens that are there: of the tile before, and of the one in `raw`
+    int ve[R];                              // 2^ve above every value scale of the lane's block so far
+
+    __device__ __forceinline__ GrLoad(const GqaRowsArgs &a, uint32_t request, uint32_t kvh, uint32_t vis, uint32_t t1,
+                                      uint32_t lane, uint32_t piece)
+        : a(a), request(request), kvh(kvh), vis(vis), t1(t1), token(gr_token(lane)), pb(lane >> 2 & 1), piece(piece) {
+#pragma unroll
+        for (int i = 0; i < R; i++) ve[i] = -100;
+    }
+    __device__ __forceinline__ uint32_t block(int i) const { return 2 * ((piece + i) & 1) + pb; }
+    __device__ __forceinline__ void desc_load(uint32_t t) {
+        const uint32_t j = t * 32 + token;
+        const uint32_t p = (uint32_t)(((uint64_t)j * a.page_magic) >> a.page_shift);
+        dsc = a.desc[(size_t)request * a.max_pages + (t < t1 && j < vis ? p : 0)];
+    }
+    __device__ __forceinline__ void issue(uint32_t t) {
+        const uint32_t j = t * 32 + token, tip = j - dsc.first_token;
+        const bool want = t < t1 && j < vis;
+        const bool in = want && j >= dsc.first_token && tip < min(dsc.tokens, a.page_tokens), q4 = dsc.precision != 0;
+        const uint8_t *pool = q4 ? a.q4 : a.q2;
+        const uint32_t bytes = q4 ? 34 : 18;
+        const uint8_t *run = pool + (size_t)dsc.physical_slot * (q4 ? a.q4_page_bytes : a.q2_page_bytes) +
+                             (size_t)tip * (q4 ? a.q4_token_bytes : a.q2_token_bytes) + (4 * kvh + pb) * bytes;
+        rkind = in ? (q4 ? 2u : 1u) : 0u;
+        here = next;
+        next = gr_tokens(__builtin_amdgcn_ballot_w64(in));
+        const gr_bytes p = in ? (gr_bytes)(uintptr_t)run : (gr_bytes)(uintptr_t)a.query;
+        const uint32_t second = rkind == 1 ? 2 : 18, pair = in ? 2 * bytes : 0, v = in ? (q4 ? a.v_off4 : a.v_off2) : 0;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const uint32_t n = piece + i;
+            const gr_bytes c = p + (n & 1 ? pair : 0) + (n >> 1 ? v : 0);
+            const GrBytes16 x = gr_load<GrBytes16>(c + 2), y = gr_load<GrBytes16>(c + second);
+#pragma unroll
+            for (int w = 0; w < 4; w++) raw[i][w] = x.w[w], raw[i][4 + w] = y.w[w];
+            rsc[i] = gr_load<uint16_t>(c);
+        }
+    }
+    __device__ __forceinline__ void widen(int i) {
+        if (__builtin_amdgcn_ballot_w64(rkind == 1)) {
+            const uint32_t y[4] = {raw[i][0], raw[i][1], raw[i][2], raw[i][3]};
+#pragma unroll
+            for (int w = 0; w < 8; w++) raw[i][w] = rkind == 1 ? gr_widen(w & 1 ? y[w >> 1] >> 16 : y[w >> 1]) : raw[i][w];
+        }
+    }
+    __device__ __forceinline__ float scale(int i) const {
+        return rkind ? (float)__builtin_bit_cast(_Float16, (uint16_t)rsc[i]) : 0.0f;
+    }
+    __device__ __forceinline__ float key_scale(int i) const { return scale(i) * (1.0f / 15.0f); }
+    // Piece i, of V: code bytes across, scales in units of 2^(9 - E), E, and the tokens without a finite scale.
+    __device__ __forceinline__ void store_v(int i, uint32_t lane, uint32_t (&v)[32][9], float (&vs)[32], int &ev,
+                                            uint32_t &bads) {
+        widen(i);
+        float sv = scale(i);
+        uint32_t bad = 0;
+        if (__builtin_amdgcn_ballot_w64(!(fabsf(ldexpf(sv, -ve[i])) < 1.0f))) {
+            const bool odd = !(fabsf(sv) < INFINITY);
+            bad = gr_tokens(__builtin_amdgcn_ballot_w64(odd) >> (4 * pb));
+            if (odd) sv = 0.0f;
+            float z = fabsf(sv);
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1)
+                if (d != 4) z = fmaxf(z, __shfl_xor(z, d));
+            int e = 0;
+            frexpf(z, &e);
+            ve[i] = max(ve[i], e);
+        }
+        vs[token] = ldexpf(sv, 9 - ve[i]);
+        if ((lane & 59) == 0) {
+            ev = ve[i];
+            bads = bad;
+        }
+#pragma unroll
+        for (int w = 0; w < 8; w++) v[4 * w + (lane & 3)][lane >> 3] = gr_across(raw[i][w], lane);
+    }
+};
+
+// ---------------------------------------------------------------------------
 // attention of one item
 // ---------------------------------------------------------------------------
 // LDS of a workgroup of QS query subtiles x TS token shares: queries and the shares' tiles (while
@@ -297,93 +387,28 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     const uint32_t qrow = valid ? qi / a.group : 0, qg = valid ? qi - qrow * a.group : 0;
     const size_t qat = ((size_t)(rq.row0 + qrow) * a.query_heads + kvh * a.group + qg) * 256;
 
-    // Tiles come in four pieces: two of K, two of V, of two dim blocks each. A lane loads one block of one token: 32
-    // code bytes (Q2: 16, both loads the same) and a scale. With four subtiles each wave loads one piece of its
-    // share's tile for all four, else the one wave all of them. A token past what the tile's queries
-    // see, or in no page, is absent: its loads go to the query rows, its scales count as 0.
+    // With four subtiles each wave loads one piece of its share's tile for all four, else the one wave all of them.
+    // (A SIMD has one wave of each share: one of them stores K, the other V, so that SIMDs stay level.)
     constexpr int R = QS == 4 ? 1 : 4;
     constexpr int AHEAD = QS == 4 ? 1 : 0;  // steps that LDS operands are read ahead (no registers for it in the other)
-    const uint32_t token = gr_token(lane), pb = lane >> 2 & 1;
-    // (a SIMD has one wave of each share: one of them stores K, the other V, so that SIMDs stay level)
-    const uint32_t piece = QS == 4 ? qsub ^ (2 * ts) : 0;
-    PagedKvDesc dsc{0, 0, 0, 0};
-    auto desc_load = [&](uint32_t t) {
-        const uint32_t j = t * 32 + token;
-        const uint32_t p = (uint32_t)(((uint64_t)j * a.page_magic) >> a.page_shift);
-        dsc = a.desc[(size_t)it.request * a.max_pages + (t < t1 && j < vis ? p : 0)];
-    };
-    uint32_t raw[R][8], rsc[R], rkind = 0;  // rkind: 0 absent, 1 Q2, 2 Q4
-    uint32_t here = 0, next = 0;            // tokens that are there: of the tile before, and of the one in `raw`
-    auto issue = [&](uint32_t t) {
-        const uint32_t j = t * 32 + token, tip = j - dsc.first_token;
-        const bool want = t < t1 && j < vis;
-        const bool in = want && j >= dsc.first_token && tip < min(dsc.tokens, a.page_tokens), q4 = dsc.precision != 0;
-        const uint8_t *pool = q4 ? a.q4 : a.q2;
-        const uint32_t bytes = q4 ? 34 : 18;
-        const uint8_t *run = pool + (size_t)dsc.physical_slot * (q4 ? a.q4_page_bytes : a.q2_page_bytes) +
-                             (size_t)tip * (q4 ? a.q4_token_bytes : a.q2_token_bytes) + (4 * kvh + pb) * bytes;
-        rkind = in ? (q4 ? 2u : 1u) : 0u;
-        here = next;
-        next = gr_tokens(__builtin_amdgcn_ballot_w64(in));
-        const gr_bytes p = in ? (gr_bytes)(uintptr_t)run : (gr_bytes)(uintptr_t)a.query;
-        const uint32_t second = rkind == 1 ? 2 : 18, pair = in ? 2 * bytes : 0, v = in ? (q4 ? a.v_off4 : a.v_off2) : 0;
-#pragma unroll
-        for (int i = 0; i < R; i++) {
-            const uint32_t n = piece + i;
-            const gr_bytes c = p + (n & 1 ? pair : 0) + (n >> 1 ? v : 0);
-            const GrBytes16 x = gr_load<GrBytes16>(c + 2), y = gr_load<GrBytes16>(c + second);
-#pragma unroll
-            for (int w = 0; w < 4; w++) raw[i][w] = x.w[w], raw[i][4 + w] = y.w[w];
-            rsc[i] = gr_load<uint16_t>(c);
-        }
-    };
-    auto widen = [&](uint32_t (&x)[8]) {
-        if (__builtin_amdgcn_ballot_w64(rkind == 1)) {
-            const uint32_t y[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-            for (int w = 0; w < 8; w++) x[w] = rkind == 1 ? gr_widen(w & 1 ? y[w >> 1] >> 16 : y[w >> 1]) : x[w];
-        }
-    };
+    GrLoad<R> ld{a, it.request, kvh, vis, t1, lane, QS == 4 ? qsub ^ (2 * ts) : 0};
     auto store_k = [&](int i) {
-        const uint32_t b = 2 * ((piece + i) & 1) + pb;
-        widen(raw[i]);
-        L.u.t.ks[ts][b][token] = rkind ? (float)__builtin_bit_cast(_Float16, (uint16_t)rsc[i]) * (1.0f / 15.0f) : 0.0f;
-        L.u.t.k[ts][b][0][token] = make_uint4(raw[i][0], raw[i][1], raw[i][2], raw[i][3]);
-        L.u.t.k[ts][b][1][token] = make_uint4(raw[i][4], raw[i][5], raw[i][6], raw[i][7]);
+        const uint32_t b = ld.block(i);
+        ld.widen(i);
+        L.u.t.ks[ts][b][ld.token] = ld.key_scale(i);
+        const uint32_t(&x)[8] = ld.raw[i];
+        L.u.t.k[ts][b][0][ld.token] = make_uint4(x[0], x[1], x[2], x[3]);
+        L.u.t.k[ts][b][1][ld.token] = make_uint4(x[4], x[5], x[6], x[7]);
     };
-    int ve[R];  // 2^ve above every value scale of the lane's block so far
-#pragma unroll
-    for (int i = 0; i < R; i++) ve[i] = -100;
     auto store_v = [&](int i) {
-        const uint32_t b = 2 * ((piece + i) & 1) + pb;
-        widen(raw[i]);
-        float sv = rkind ? (float)__builtin_bit_cast(_Float16, (uint16_t)rsc[i]) : 0.0f;
-        uint32_t bad = 0;
-        if (__builtin_amdgcn_ballot_w64(!(fabsf(ldexpf(sv, -ve[i])) < 1.0f))) {
-            const bool odd = !(fabsf(sv) < INFINITY);
-            bad = gr_tokens(__builtin_amdgcn_ballot_w64(odd) >> (4 * pb));
-            if (odd) sv = 0.0f;
-            float z = fabsf(sv);
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1)
-                if (d != 4) z = fmaxf(z, __shfl_xor(z, d));
-            int e = 0;
-            frexpf(z, &e);
-            ve[i] = max(ve[i], e);
-        }
-        L.u.t.vs[ts][b][token] = ldexpf(sv, 9 - ve[i]);
-        if ((lane & 59) == 0) {
-            L.u.t.ev[ts][b] = ve[i];
-            L.u.t.bad[ts][b] = bad;
-        }
-#pragma unroll
-        for (int w = 0; w < 8; w++) L.u.t.v[ts][b][4 * w + (lane & 3)][lane >> 3] = gr_across(raw[i][w], lane);
+        const uint32_t b = ld.block(i);
+        ld.store_v(i, lane, L.u.t.v[ts][b], L.u.t.vs[ts][b], L.u.t.ev[ts][b], L.u.t.bad[ts][b]);
     };
 
     const RmMagic magic = rm_magic<true>();
     float minus_one = -1.0f;
     asm("" : "+v"(minus_one));
-    desc_load(t0);
+    ld.desc_load(t0);
     float qs;
     {
         const float *q = a.query + qat + 32 * h;
@@ -437,12 +462,12 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     float m = -INFINITY, den = 0.0f;
     int ev[4] = {-100, -100, -100, -100};  // E of the blocks' sums
 
-    issue(t0);
-    desc_load(t0 + TS);
-    if (QS == 4 && piece < 2) {
+    ld.issue(t0);
+    ld.desc_load(t0 + TS);
+    if (QS == 4 && ld.piece < 2) {
         store_k(0);
-        issue(t0 + TS);
-        desc_load(t0 + 2 * TS);
+        ld.issue(t0 + TS);
+        ld.desc_load(t0 + 2 * TS);
     }
     // (nothing under way on entry: the loop's waits are then counted by the order of its own loads alone)
     __builtin_amdgcn_s_waitcnt(0x0F70);
@@ -452,7 +477,7 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
         // `raw` holds K of the next tile, or V of this one.
         if (QS == 4) {
             lds_barrier();  // K is written, the last tile's V is no longer read
-            if (piece >= 2) store_v(0);
+            if (ld.piece >= 2) store_v(0);
         } else {
             store_k(0);
             store_k(1);
@@ -460,9 +485,9 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
             store_v(3);
             lds_wave_order();
         }
-        if (QS != 4 || piece >= 2) {
-            issue(t + TS);
-            desc_load(t + 2 * TS);
+        if (QS != 4 || ld.piece >= 2) {
+            ld.issue(t + TS);
+            ld.desc_load(t + 2 * TS);
         }
         // ---- scores ----
         gr_v16 s;
@@ -512,8 +537,8 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
             }
         }
         // ---- masks: a tile that ends past the first query's last token, or has absent tokens ----
-        if ((int32_t)((t + 1) * 32) - 1 > lim0 || here != ~0u) {
-            const uint32_t on = here >> (4 * h);
+        if ((int32_t)((t + 1) * 32) - 1 > lim0 || ld.here != ~0u) {
+            const uint32_t on = ld.here >> (4 * h);
             const int32_t left = lim - (int32_t)(t * 32 + 4 * h);  // tokens up to this one
 #pragma unroll
             for (int r = 0; r < 16; r++) {
@@ -549,10 +574,10 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
         // ---- values ----
         if (QS == 4) {
             lds_barrier();  // V is written, K is no longer read
-            if (piece < 2) {
+            if (ld.piece < 2) {
                 store_k(0);
-                issue(t + 2 * TS);
-                desc_load(t + 3 * TS);
+                ld.issue(t + 2 * TS);
+                ld.desc_load(t + 3 * TS);
             }
         }
         const int4 e4 = *(const int4 *)L.u.t.ev[ts];
@@ -694,6 +719,300 @@ extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_rows_gfx950(GqaRow
 extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few_gfx950(GqaRowsArgs a) { gqa_rows<1, 4>(a); }
 
 // ---------------------------------------------------------------------------
+// at most 16 queries a KV head
+// ---------------------------------------------------------------------------
+// Four waves, each with all queries and every fourth tile, on f16 MFMA 16x16x32: half the products, softmax and splits
+// of the 32-query kernel, and sums in 64 registers, so that the queries stay in registers too.
+typedef float gr_v4 __attribute__((ext_vector_type(4)));
+struct GrLds16 {
+    union {
+        struct {
+            uint2 k[4][4][4][36];   // [wave][block][quarter][token]: that quarter's code bytes
+            uint32_t v[4][4][32][9];  // [wave][block][code byte][token / 4]: that byte of four tokens
+            float ks[4][4][32];
+            float vs[4][4][32];
+            int ev[4][4];
+            uint32_t bad[4][4];
+        } t;
+        float4 sum[2][16][64];  // [publishing wave][dim block, half, parity][lane]
+        GrScratch scratch;
+    } u;
+    float stat[2][2][16];
+};
+
+extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRowsArgs a) {
+    __shared__ GrLds16 L;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t li = lane & 15, g = lane >> 4;
+    const uint32_t range = gr_range<256>(a, true, L.u.scratch);
+    const GrItem it = gr_find<256>(a, true, range, blockIdx.x, true, L.u.scratch);
+    if (!it.ok) return;
+    if (it.local == 0 && threadIdx.x == 0) {
+        a.cuts[2 * it.request] = it.base;
+        a.cuts[2 * it.request + 1] = it.ranges;
+    }
+    const GrRequest rq = gr_request(a, it.request);
+    const uint32_t nq = rq.rows * a.group, kvh = it.local % a.kv_heads, part = it.local / a.kv_heads;
+    const int32_t past = (int32_t)rq.tokens - (int32_t)rq.rows;  // tokens before the first row
+    const uint32_t vis = rq.tokens;
+    const uint32_t units = (vis + 127) / 128, per = (units + it.ranges - 1) / it.ranges;
+    const uint32_t t0 = min(part * per, units) * 4 + wave, t1 = min(part * per + per, units) * 4;
+    const bool valid = li < nq;
+    const int32_t lim = valid ? past + (int32_t)(li / a.group) : -1;
+    const uint32_t qrow = valid ? li / a.group : 0, qg = valid ? li - qrow * a.group : 0;
+    const size_t qat = ((size_t)(rq.row0 + qrow) * a.query_heads + kvh * a.group + qg) * 256;
+
+    GrLoad<4> ld{a, it.request, kvh, vis, t1, lane, 0};
+    ld.desc_load(t0);
+    rm_h8 qf[2][8];  // [lo, hi][k step]: 8 dims of each quarter of a block
+    float qs;
+    {
+        const float *q = a.query + qat + 16 * g;
+        const float pre = valid ? a.scale * 1.44269504088896341f : 0.0f;
+        auto load = [&](int s, float (&x)[8]) {
+            const float4 u = *(const float4 *)(q + 64 * (s >> 1) + 8 * (s & 1));
+            const float4 v = *(const float4 *)(q + 64 * (s >> 1) + 8 * (s & 1) + 4);
+            const float y[8] = {u.x, v.x, u.y, v.y, u.z, v.z, u.w, v.w};
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = y[i] * pre;
+        };
+        float mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            float x[8];
+            load(s, x);
+#pragma unroll
+            for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[i]) < INFINITY ? fabsf(x[i]) : 0.0f);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        int e = 0;
+        frexpf(mx, &e);
+        qs = ldexpf(1.0f, e - 15);
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            float x[8];
+            load(s, x);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float v = ldexpf(x[i], 15 - e);
+                qf[1][s][i] = (_Float16)v;
+                qf[0][s][i] = fabsf(v) < INFINITY ? (_Float16)(v - (float)qf[1][s][i]) : (_Float16)0.0f;
+            }
+        }
+    }
+    const RmMagic magic = rm_magic<true>();
+    float minus_one = -1.0f;
+    asm("" : "+v"(minus_one));
+    gr_v4 o[4][2][2];  // [dim block][half of its code bytes][even, odd dims]
+#pragma unroll
+    for (int b = 0; b < 4; b++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) o[b][c >> 1][c & 1] = gr_v4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, den = 0.0f;
+    int ev[4] = {-100, -100, -100, -100};  // E of the blocks' sums
+
+    ld.issue(t0);
+    ld.desc_load(t0 + 4);
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    for (uint32_t t = t0; t < t1; t += 4) {
+        // ---- this tile's bytes and scales into LDS; the next tile's loads ----
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t b = ld.block(i);
+            ld.widen(i);
+            L.u.t.ks[wave][b][ld.token] = ld.key_scale(i);
+#pragma unroll
+            for (int w = 0; w < 4; w++) L.u.t.k[wave][b][w][ld.token] = make_uint2(ld.raw[i][2 * w], ld.raw[i][2 * w + 1]);
+        }
+#pragma unroll
+        for (int i = 2; i < 4; i++) {
+            const uint32_t b = ld.block(i);
+            ld.store_v(i, lane, L.u.t.v[wave][b], L.u.t.vs[wave][b], L.u.t.ev[wave][b], L.u.t.bad[wave][b]);
+        }
+        lds_wave_order();
+        ld.issue(t + 4);
+        ld.desc_load(t + 8);
+        // ---- scores: tokens 16 n + 4 g + r ----
+        gr_v4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            uint2 kw[2];
+            gr_v4 x[2];
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                kw[n] = L.u.t.k[wave][b][g][16 * n + li];
+                x[n] = gr_v4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const rm_h8 kf = gr_k_operand(k ? kw[n].y : kw[n].x, magic);
+                    x[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[0][2 * b + k], x[n], 0, 0, 0);
+                    x[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[1][2 * b + k], x[n], 0, 0, 0);
+                }
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const float4 f = *(const float4 *)&L.u.t.ks[wave][b][16 * n + 4 * g];
+                s[n][0] = fmaf(f.x, x[n][0], s[n][0]);
+                s[n][1] = fmaf(f.y, x[n][1], s[n][1]);
+                s[n][2] = fmaf(f.z, x[n][2], s[n][2]);
+                s[n][3] = fmaf(f.w, x[n][3], s[n][3]);
+            }
+        }
+        // ---- masks ----
+        if ((int32_t)((t + 1) * 32) - 1 > past || ld.here != ~0u) {
+            const uint32_t on = ld.here >> (4 * g);
+            const int32_t left = lim - (int32_t)(t * 32 + 4 * g);  // tokens up to this one
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int c = 16 * n + r;
+                    if (c > left || !(on >> c & 1)) s[n][r] = -INFINITY;
+                }
+        }
+        // ---- softmax ----
+        float top = s[0][0];
+#pragma unroll
+        for (int r = 1; r < 8; r++) top = fmaxf(top, s[r >> 2][r & 3]);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32)) * qs;
+        if (__builtin_amdgcn_ballot_w64(top > m + GR_MOVE)) {
+            const float mn = fmaxf(m, top), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) o[b][c >> 1][c & 1] *= al;
+            den *= al;
+            m = mn;
+        }
+        float p[8];
+        {
+            const float ms = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int r = 0; r < 8; r++) p[r] = __builtin_amdgcn_exp2f(fmaf(s[r >> 2][r & 3], qs, -ms));
+            den += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        }
+        // ---- values ----
+        const int4 e4 = *(const int4 *)L.u.t.ev[wave];
+        const uint4 bad4 = *(const uint4 *)L.u.t.bad[wave];
+        const int e[4] = {e4.x, e4.y, e4.z, e4.w};
+        if (__builtin_amdgcn_ballot_w64(e[0] != ev[0] || e[1] != ev[1] || e[2] != ev[2] || e[3] != ev[3])) {
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const int d = max(ev[b] - e[b], -200);
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) o[b][c >> 1][c & 1][r] = ldexpf(o[b][c >> 1][c & 1][r], d);
+                ev[b] = __builtin_amdgcn_readfirstlane(e[b]);
+            }
+        }
+        // (as above: no numbers for every query that sees the token, nothing for the others)
+        if (__builtin_amdgcn_ballot_w64((bad4.x | bad4.y | bad4.z | bad4.w) != 0)) {
+            const uint32_t bads[4] = {bad4.x, bad4.y, bad4.z, bad4.w};
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const uint32_t bad = bads[b] >> (4 * g);
+                bool any = false;
+#pragma unroll
+                for (int r = 0; r < 8; r++) any |= (bad >> (16 * (r >> 2) + (r & 3)) & 1) && p[r] != 0.0f;
+                any |= __shfl_xor((int)any, 16) != 0;
+                any |= __shfl_xor((int)any, 32) != 0;
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) o[b][c >> 1][c & 1][r] = any ? __builtin_nanf("") : o[b][c >> 1][c & 1][r];
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            const float4 f0 = *(const float4 *)&L.u.t.vs[wave][b][4 * g];
+            const float4 f1 = *(const float4 *)&L.u.t.vs[wave][b][16 + 4 * g];
+            const float x[8] = {p[0] * f0.x, p[1] * f0.y, p[2] * f0.z, p[3] * f0.w,
+                                p[4] * f1.x, p[5] * f1.y, p[6] * f1.z, p[7] * f1.w};
+            rm_h8 hi, lo;
+            gr_split(x, minus_one, hi, lo);
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                rm_h8 vf[2];
+                gr_v_operands(L.u.t.v[wave][b][16 * c + li][g], L.u.t.v[wave][b][16 * c + li][4 + g], magic, vf);
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    o[b][c][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[n], lo, o[b][c][n], 0, 0, 0);
+                    o[b][c][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[n], hi, o[b][c][n], 0, 0, 0);
+                }
+            }
+        }
+        lds_wave_order();
+    }
+    // ---- join the waves, half of them publishing to the other half, and write ----
+    den += __shfl_xor(den, 16);
+    den += __shfl_xor(den, 32);
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        const float f = ldexpf(1.0f / 15.0f, ev[b] - 9);
+#pragma unroll
+        for (int c = 0; c < 4; c++) o[b][c >> 1][c & 1] *= f;
+    }
+#pragma unroll
+    for (uint32_t n = 2; n > 0; n >>= 1) {
+        __syncthreads();  // the tiles (and the last round's sums) are dead
+        if (wave >= n && wave < 2 * n) {
+            const uint32_t slot = wave - n;
+            if (g == 0) {
+                L.stat[slot][0][li] = m;
+                L.stat[slot][1][li] = den;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const gr_v4 x = o[i >> 2][i >> 1 & 1][i & 1];
+                L.u.sum[slot][i][lane] = make_float4(x[0], x[1], x[2], x[3]);
+            }
+        }
+        __syncthreads();
+        if (wave < n) {
+            const float m2 = L.stat[wave][0][li], mn = fmaxf(m, m2);
+            const float f1 = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float f2 = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m2 - mn);
+            den = den * f1 + L.stat[wave][1][li] * f2;
+            m = mn;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                gr_v4 &y = o[i >> 2][i >> 1 & 1][i & 1];
+                const float4 x = L.u.sum[wave][i][lane];
+                y = gr_v4{fmaf(x.x, f2, y[0] * f1), fmaf(x.y, f2, y[1] * f1), fmaf(x.z, f2, y[2] * f1),
+                          fmaf(x.w, f2, y[3] * f1)};
+            }
+        }
+    }
+    if (wave || !valid) return;
+    float *dst, f = 1.0f;
+    if (it.ranges > 1) {
+        float *slot = a.few_part + (size_t)blockIdx.x * (16 * 258);
+        dst = slot + (size_t)li * 256;
+        if (g == 0) {
+            slot[16 * 256 + 2 * li] = den != den && m == -INFINITY ? 0.0f : m;
+            slot[16 * 256 + 2 * li + 1] = den;
+        }
+    } else {
+        dst = a.out + qat;
+        f = den != 0.0f ? 1.0f / den : 0.0f;
+    }
+#pragma unroll
+    for (int b = 0; b < 4; b++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            float4 *d = (float4 *)(dst + 64 * b + 32 * c + 8 * g);
+            const gr_v4 &x = o[b][c][0], &y = o[b][c][1];
+            d[0] = make_float4(x[0] * f, y[0] * f, x[1] * f, y[1] * f);
+            d[1] = make_float4(x[2] * f, y[2] * f, x[3] * f, y[3] * f);
+        }
+}
+
+// ---------------------------------------------------------------------------
 // join: grid (rows, quarters of the query heads), 64 lanes x 4 dims
 // ---------------------------------------------------------------------------
 // A wave takes a head of its own, or, where there are more than GR_ALONE parts, every fourth part of one head after the
@@ -716,7 +1035,7 @@ extern "C" __global__ __launch_bounds__(256) void ctox_gqa_join_gfx950(GqaRowsAr
     const bool few = gr_few(a, rq);
     const uint32_t first = a.cuts[2 * lo], ranges = a.cuts[2 * lo + 1];
     if (ranges < 2) return;
-    const uint32_t size = few ? 32 : 128, nqt = (rq.rows * a.group + size - 1) / size;
+    const uint32_t size = few ? a.few : 128, nqt = (rq.rows * a.group + size - 1) / size;
     const float *base = few ? a.few_part : a.part;
     const bool alone = ranges <= GR_ALONE;
     float m, den;

@@ -160,7 +160,7 @@ struct ctox_hip_backend {
                   prep_x = nullptr, finite = nullptr, gather = nullptr, topk_part = nullptr, topk_final = nullptr, stream_read = nullptr,
                   write_segments = nullptr, rope_axes[2] = {}, plan = nullptr, kv_append = nullptr,
                   rows_max[2] = {}, rows_stage[2] = {}, rows_stage_few[2] = {}, rows_reduce = nullptr,
-                  gqa_rows = nullptr, gqa_few = nullptr, gqa_join = nullptr;
+                  gqa_rows = nullptr, gqa_few = nullptr, gqa_few16 = nullptr, gqa_join = nullptr;
     // Row products: [q4][parts - 1][shape], shapes as kRowShapes.
     hipFunction_t rows_mul[2][2][4] = {};
     // Batch-1 slice kernels per dtype [Q2, Q4]: [0] walks the slices, [n]
@@ -956,7 +956,8 @@ extern "C" ctox_status ctox_hip_backend_create(int device, ctox_hip_backend **ou
                {&b->rows_stage_few[0], "ctox_rows_stage_few_gfx950"},
                {&b->rows_stage_few[1], "ctox_rows_stage_few_vec_gfx950"},
                {&b->rows_reduce, "ctox_rows_reduce_gfx950"},
-               {&b->gqa_rows, "ctox_gqa_rows_gfx950"}, {&b->gqa_few, "ctox_gqa_few_gfx950"}, {&b->gqa_join, "ctox_gqa_join_gfx950"}};
+               {&b->gqa_rows, "ctox_gqa_rows_gfx950"}, {&b->gqa_few, "ctox_gqa_few_gfx950"},
+               {&b->gqa_few16, "ctox_gqa_few16_gfx950"}, {&b->gqa_join, "ctox_gqa_join_gfx950"}};
     for (auto &f : fns) {
         if (le != hipSuccess) break;
         le = hipModuleGetFunction(f.f, b->module, f.name);
@@ -2997,12 +2998,13 @@ ctox_status check_gqa_rows(const ctox_paged_gqa_rows *op) {
 }
 
 // Which kernels run and how many items each may have. Requests of at most 32 queries a KV head go to the
-// few-query kernel, unless the batch is one request that may have more. The 128-query kernel splits token
+// few-query kernel, unless the batch is one request that may have more; where none has more than 16, to the
+// one of 16 queries. The 128-query kernel splits token
 // ranges where its query tiles alone would not give every CU two workgroups. Items: one a query tile and
 // KV head at least; the device cuts ranges into more up to the bound given here, two rounds of the chip.
 struct GqaRowsPlan {
-    bool few, wide, split;
-    uint32_t few_slots, slots, few_items, items;
+    bool wide, split;
+    uint32_t few, few_slots, slots, few_items, items;
     uint64_t cut_bytes, few_bytes, bytes;
 };
 GqaRowsPlan gqa_rows_plan(uint32_t cus, const ctox_paged_gqa_rows *op) {
@@ -3011,13 +3013,13 @@ GqaRowsPlan gqa_rows_plan(uint32_t cus, const ctox_paged_gqa_rows *op) {
     const uint64_t most = op->max_rows ? std::min<uint64_t>(op->max_rows, op->rows) : op->rows;
     const uint64_t busy = std::min<uint64_t>(op->requests, op->rows);
     g.wide = most * group > 32;
-    g.few = group <= 32 && !(g.wide && op->requests == 1);
+    g.few = group > 32 || (g.wide && op->requests == 1) ? 0 : most * group <= 16 ? 16 : 32;
     g.few_slots = 2 * cus;
     g.slots = cus;
     g.cut_bytes = ((uint64_t)op->requests * 8 + 15) / 16 * 16;
     if (g.few) {
         g.few_items = (uint32_t)(busy * kvh + 2 * g.few_slots);
-        g.few_bytes = (uint64_t)g.few_items * 32 * 258 * sizeof(float);
+        g.few_bytes = (uint64_t)g.few_items * g.few * 258 * sizeof(float);
     }
     if (g.wide) {
         const uint64_t tiles = (op->rows * group + 127) / 128;
@@ -3099,7 +3101,7 @@ extern "C" ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *b, const
     ctox_status st = CTOX_OK;
     if (g.wide) st = launch(b->gqa_rows, dim3(g.items), dim3(512), s, a, "ctox_gqa_rows_gfx950");
     if (!st && g.few)
-        st = launch(b->gqa_few, dim3(g.few_items), dim3(256), s, a, "ctox_gqa_few_gfx950");
+        st = launch(g.few == 16 ? b->gqa_few16 : b->gqa_few, dim3(g.few_items), dim3(256), s, a, "ctox_gqa_few_gfx950");
     if (!st && (g.few || g.split))
         st = launch(b->gqa_join, dim3(a.rows, (p.query_heads + 3) / 4), dim3(256), s, a, "ctox_gqa_join_gfx950");
     return st;
