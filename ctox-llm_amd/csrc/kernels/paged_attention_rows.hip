@@ -182,10 +182,9 @@ __device__ __forceinline__ T gr_load(gr_bytes p) {
     return *(const __attribute__((address_space(1))) T *)p;
 }
 
-// Eight 2-bit codes (low 16 bits) as eight 4-bit codes of the same value: c -> 5 c.
-__device__ __forceinline__ uint32_t gr_widen(uint32_t x) {
-    x &= 0xffffu;
-    x = (x | (x << 8)) & 0x00FF00FFu;
+// Eight 2-bit codes (16 bits of x: the upper ones if `upper`) as eight 4-bit codes of the same value: c -> 5 c.
+__device__ __forceinline__ uint32_t gr_widen(uint32_t x, bool upper) {
+    x = __builtin_amdgcn_perm(0u, x, upper ? 0x0C030C02u : 0x0C010C00u);  // (0x0C: a byte of zeros)
     x = (x | (x << 4)) & 0x0F0F0F0Fu;
     x = (x | (x << 2)) & 0x33333333u;
     return x | (x << 2);
@@ -208,10 +207,12 @@ __device__ __forceinline__ void gr_v_operands(uint32_t x, uint32_t y, const RmMa
 
 // Four lanes' dwords across: lane i of four gets byte i of each.
 __device__ __forceinline__ uint32_t gr_across(uint32_t x, uint32_t lane) {
+    // selectors out of (own, other): halves with lane ^ 2, then bytes with lane ^ 1
+    const uint32_t two = lane & 2 ? 0x07060302u : 0x01000504u, one = lane & 1 ? 0x07030501u : 0x02060004u;
     const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, true);  // of lane ^ 2
-    const uint32_t a = lane & 2 ? __builtin_amdgcn_perm(x, y, 0x07060302u) : __builtin_amdgcn_perm(y, x, 0x05040100u);
+    const uint32_t a = __builtin_amdgcn_perm(x, y, two);
     const uint32_t b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0xB1, 0xF, 0xF, true);  // of lane ^ 1
-    return lane & 1 ? __builtin_amdgcn_perm(a, b, 0x07030501u) : __builtin_amdgcn_perm(b, a, 0x06020400u);
+    return __builtin_amdgcn_perm(a, b, one);
 }
 
 // A loading lane's token (of 32) and block (of a pair), and the tokens' bits out of a ballot of the first block's.
@@ -291,9 +292,10 @@ struct GrLoad {
     }
     __device__ __forceinline__ void widen(int i) {
         if (__builtin_amdgcn_ballot_w64(rkind == 1)) {
+            const uint32_t two = rkind == 1 ? ~0u : 0u;  // (a mask: a choice would become a branch for every word)
             const uint32_t y[4] = {raw[i][0], raw[i][1], raw[i][2], raw[i][3]};
 #pragma unroll
-            for (int w = 0; w < 8; w++) raw[i][w] = rkind == 1 ? gr_widen(w & 1 ? y[w >> 1] >> 16 : y[w >> 1]) : raw[i][w];
+            for (int w = 0; w < 8; w++) raw[i][w] = (gr_widen(y[w >> 1], w & 1) & two) | (raw[i][w] & ~two);
         }
     }
     __device__ __forceinline__ float scale(int i) const {
@@ -303,6 +305,8 @@ struct GrLoad {
     // Piece i, of V: code bytes across, scales in units of 2^(9 - E), E, and the tokens without a finite scale.
     __device__ __forceinline__ void store_v(int i, uint32_t lane, uint32_t (&v)[32][9], float (&vs)[32], int &ev,
                                             uint32_t &bads) {
+        // (opaque with one piece: what follows from the lane alone is not to be kept in registers from tile to tile)
+        if (R == 1) asm volatile("" : "+v"(lane));
         widen(i);
         float sv = scale(i);
         uint32_t bad = 0;
@@ -318,7 +322,7 @@ struct GrLoad {
             frexpf(z, &e);
             ve[i] = max(ve[i], e);
         }
-        vs[token] = ldexpf(sv, 9 - ve[i]);
+        vs[R == 1 ? gr_token(lane) : token] = ldexpf(sv, 9 - ve[i]);
         if ((lane & 59) == 0) {
             ev = ve[i];
             bads = bad;
