@@ -1038,8 +1038,9 @@ extern "C" __global__ __launch_bounds__(256) void ctox_gqa_join_gfx950(GqaRowsAr
     if (row < rq.row0 || row - rq.row0 >= rq.rows) return;
     const bool few = gr_few(a, rq);
     const uint32_t first = a.cuts[2 * lo], ranges = a.cuts[2 * lo + 1];
-    if (ranges < 2) return;
     const uint32_t size = few ? a.few : 128, nqt = (rq.rows * a.group + size - 1) / size;
+    // (Lengths that break the contract can leave a request without items, and its cut unwritten.)
+    if (ranges < 2 || first + (uint64_t)nqt * ranges * a.kv_heads > (few ? a.few_items : a.items)) return;
     const float *base = few ? a.few_part : a.part;
     const bool alone = ranges <= GR_ALONE;
     float m, den;

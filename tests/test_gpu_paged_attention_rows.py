@@ -353,3 +353,37 @@ def test_refusals_with_a_backend(hip):
     hip.paged_gqa_rows_device(op)
     torch.cuda.synchronize()
     assert bool((b.d["out"] == 7.0).all())
+
+
+@pytest.mark.parametrize("heads,kv_heads,most", [(16, 1, 1), (32, 2, 1), (34, 2, 1), (33, 1, 1), (80, 2, 1), (24, 4, 2),
+                                                 (24, 4, 3), (2, 1, 8), (2, 1, 9), (6, 6, 16), (6, 6, 17), (5, 1, 6)])
+def test_few_queries_at_the_limits(hip, heads, kv_heads, most):
+    """Requests of up to `most` rows around 16 and 32 queries a KV head, and groups that reach them alone."""
+    say(f"case rows attention few heads={heads}/{kv_heads} most={most}")
+    rows = [most, 1, 0, max(1, most - 1), most, 1]
+    b = Batch(heads + most, list(zip([0, 31, 40, 333, 1000, 0], rows)), 16, heads, kv_heads, q2=old, pad=3)
+    b.check(b.run(hip, max_rows=most))
+
+
+@pytest.mark.parametrize("most", [1, 5, 40])
+def test_pages_past_four_gibibytes(hip, most):
+    """Pages at the far end of pools of more than 2^32 bytes."""
+    say(f"case rows attention far pages most={most}")
+    b = Batch(most, [(200, most), (31, 1)], 16, 12, 2, q2=old)
+    op = b.op(hip, max_rows=most)
+    pools = {}
+    for kind, name in ((Q2, "q2"), (Q4, "q4")):
+        near = b.d[name]
+        page = 16 * b.blocks * BB[kind]
+        skip = (2 ** 32 + 5 * page) // page + 1
+        pools[name] = torch.empty(skip * page + near.numel(), dtype=torch.uint8, device="cuda")
+        pools[name][skip * page:] = near
+        b.desc[..., 1] += np.where((b.desc[..., 0] == kind) & (b.desc[..., 2] > 0), skip, 0).astype(np.uint32)
+    b.d["desc"].copy_(dev(b.desc.view(np.int32)))
+    op.q2_pages, op.q4_pages = pools["q2"].data_ptr(), pools["q4"].data_ptr()
+    hip.paged_gqa_rows_device(op, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    for kind, name in ((Q2, "q2"), (Q4, "q4")):  # (the reference reads the near copies)
+        skip = (2 ** 32 + 5 * 16 * b.blocks * BB[kind]) // (16 * b.blocks * BB[kind]) + 1
+        b.desc[..., 1] -= np.where((b.desc[..., 0] == kind) & (b.desc[..., 2] > 0), skip, 0).astype(np.uint32)
+    b.check(b.d["out"].cpu().numpy())

@@ -378,3 +378,26 @@ def test_plan_append_and_rope_replay_in_a_graph(hip):
         assert int(out[0][3][-1]) == int(added.sum()) and bool(out[0][0].any())
         n = int(added.sum())
         assert torch.equal(out[0][1][n:], dev(kk)[n:])  # rows behind the last request
+
+
+def test_append_past_four_gibibytes(hip):
+    """A slot at the far end of a pool of more than 2^32 bytes."""
+    say("case append far slot")
+    rng = np.random.default_rng(12)
+    cv, page = 256, 16
+    tb = 2 * cv // 64 * 34
+    slots = 2 ** 32 // (page * tb) + 4
+    k, v = rng.standard_normal((2, 2, cv)).astype(np.float32)
+    dk, dv = dev(k), dev(v)
+    pool = torch.empty(slots * page * tb, dtype=torch.uint8, device="cuda")
+    pool[:2 * page * tb] = 9
+    pool[-2 * page * tb:] = 9
+    ds = dev(np.array([slots * page - 1, slots * page - page], np.uint32).view(np.int32))
+    hip.kv_append_q4_device(pool.data_ptr(), dk.data_ptr(), dv.data_ptr(), ds.data_ptr(), 2, cv, page, slots, page * tb,
+                            stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert bool((pool[:2 * page * tb] == 9).all())
+    want = np.full((2 * page, tb), 9, np.uint8)
+    for t, at in ((0, 2 * page - 1), (1, page)):
+        want[at] = np.frombuffer(pk.quantize_values(np.concatenate([k[t], v[t]]), pk.Q4), np.uint8)
+    assert np.array_equal(pool[-2 * page * tb:].cpu().numpy().reshape(2 * page, tb), want)
