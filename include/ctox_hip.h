@@ -704,8 +704,10 @@ ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *backend, uint8_t *d_q
  * min(page_count * page_tokens, 2^30)). max_rows bounds the rows of any one request (0:
  * rows); no request may have more. params.tokens is not read. f32 results: products
  * keep 22 bits of each query value and probability, the cached codes are
- * exact, sums are 32 bits. Limits: head_dim 256, requests <= 4096, rows <= 2^20. workspace holds ctox_hip_paged_gqa_rows_workspace bytes (of
- * the same op; its device pointers are not read), 16-byte aligned. */
+ * exact, sums are 32 bits. Limits: head_dim 256, requests <= 4096, rows <= 2^20.
+ * workspace holds ctox_hip_paged_gqa_rows_workspace bytes (of the same op; its device
+ * pointers are not read), 16-byte aligned, and is free again when the call's work on
+ * the stream is done. */
 typedef struct {
     const float *query;
     float *out;
