@@ -267,7 +267,8 @@ struct GrLoad {
         const uint32_t p = (uint32_t)(((uint64_t)j * a.page_magic) >> a.page_shift);
         dsc = a.desc[(size_t)request * a.max_pages + (t < t1 && j < vis ? p : 0)];
     }
-    __device__ __forceinline__ void issue(uint32_t t) {
+    // The loads of tile t, after those of tile `after`'s descriptors, which are waited for first.
+    __device__ __forceinline__ void issue(uint32_t t, uint32_t after) {
         const uint32_t j = t * 32 + token, tip = j - dsc.first_token;
         const bool want = t < t1 && j < vis;
         const bool in = want && j >= dsc.first_token && tip < min(dsc.tokens, a.page_tokens), q4 = dsc.precision != 0;
@@ -278,6 +279,7 @@ struct GrLoad {
         rkind = in ? (q4 ? 2u : 1u) : 0u;
         here = next;
         next = gr_tokens(__builtin_amdgcn_ballot_w64(in));
+        desc_load(after);
         const gr_bytes p = in ? (gr_bytes)(uintptr_t)run : (gr_bytes)(uintptr_t)a.query;
         const uint32_t second = rkind == 1 ? 2 : 18, pair = in ? 2 * bytes : 0, v = in ? (q4 ? a.v_off4 : a.v_off2) : 0;
 #pragma unroll
@@ -466,12 +468,10 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     float m = -INFINITY, den = 0.0f;
     int ev[4] = {-100, -100, -100, -100};  // E of the blocks' sums
 
-    ld.issue(t0);
-    ld.desc_load(t0 + TS);
+    ld.issue(t0, t0 + TS);
     if (QS == 4 && ld.piece < 2) {
         store_k(0);
-        ld.issue(t0 + TS);
-        ld.desc_load(t0 + 2 * TS);
+        ld.issue(t0 + TS, t0 + 2 * TS);
     }
     // (nothing under way on entry: the loop's waits are then counted by the order of its own loads alone)
     __builtin_amdgcn_s_waitcnt(0x0F70);
@@ -490,8 +490,7 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
             lds_wave_order();
         }
         if (QS != 4 || ld.piece >= 2) {
-            ld.issue(t + TS);
-            ld.desc_load(t + 2 * TS);
+            ld.issue(t + TS, t + 2 * TS);
         }
         // ---- scores ----
         gr_v16 s;
@@ -580,8 +579,7 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
             lds_barrier();  // V is written, K is no longer read
             if (ld.piece < 2) {
                 store_k(0);
-                ld.issue(t + 2 * TS);
-                ld.desc_load(t + 3 * TS);
+                ld.issue(t + 2 * TS, t + 3 * TS);
             }
         }
         const int4 e4 = *(const int4 *)L.u.t.ev[ts];
@@ -816,8 +814,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
     float m = -INFINITY, den = 0.0f;
     int ev[4] = {-100, -100, -100, -100};  // E of the blocks' sums
 
-    ld.issue(t0);
-    ld.desc_load(t0 + 4);
+    ld.issue(t0, t0 + 4);
     __builtin_amdgcn_s_waitcnt(0x0F70);
     for (uint32_t t = t0; t < t1; t += 4) {
         // ---- this tile's bytes and scales into LDS; the next tile's loads ----
@@ -835,8 +832,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
             ld.store_v(i, lane, L.u.t.v[wave][b], L.u.t.vs[wave][b], L.u.t.ev[wave][b], L.u.t.bad[wave][b]);
         }
         lds_wave_order();
-        ld.issue(t + 4);
-        ld.desc_load(t + 8);
+        ld.issue(t + 4, t + 8);
         // ---- scores: tokens 16 n + 4 g + r ----
         gr_v4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
