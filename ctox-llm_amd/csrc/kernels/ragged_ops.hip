@@ -6,15 +6,17 @@
 //    Bound by HBM bytes. The angle is formed in turns in 64 bits (position * frequency, less
 //    its nearest integer), where 32 would leave an error of position * 2^-24 turns; only the
 //    remainder, at most half a turn, goes to the 32-bit sine and cosine. A workgroup makes one
-//    row's table once and its four waves take the heads in turn, one head a wave.
+//    row's table once and its four waves take the heads in turn, one head a wave. 4096 rows of
+//    28 heads of 256, three axes: 69 us, 3.4 TB/s; 16 rows: 7 us, the launch.
 //  * ctox_paged_plan_gfx950: page descriptors, slot map and row offsets of a batch from the
 //    requests' cached and added lengths (PagedKvCache::push's page bookkeeping,
 //    Q/src/kv_cache.rs:394-429, for many requests at once). One launch: every workgroup makes
 //    both prefix sums (rows, pages) in LDS for itself, then writes its share of the rows and
-//    pages; nothing passes between workgroups.
+//    pages; nothing passes between workgroups. 8 requests 6.8 us, 512 requests 8.6 us.
 //  * ctox_kv_append_q4_gfx950: token rows of K and V into the Q4 slots of the slot map,
 //    bit-exact with Q4Block64::quantize (Q/src/quant.rs:144-168). Eight lanes hold a 64-value
-//    block; a token's bytes are assembled in LDS and leave as whole dwords.
+//    block; a token's bytes are assembled in LDS and leave as whole dwords. 32 rows of 2 x 1024
+//    values 4.9 us, 4096 rows 12 us (3.1 TB/s read and written).
 #include <hip/hip_runtime.h>
 
 #include "kernel_args.h"
