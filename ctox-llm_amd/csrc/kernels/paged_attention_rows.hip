@@ -82,7 +82,10 @@ __device__ __forceinline__ GrShape gr_shape(const GqaRowsArgs &a, const GrReques
     return s;
 }
 
+#define GR_MOST 512            // requests of a batch whose token axes may be cut
+#define GR_UNCUT 0x3fffffffu  // a range that holds any request
 struct GrScratch {
+    GrShape shape[GR_MOST];
     uint32_t count[32], longest, range;
     uint32_t scan[8];
     uint32_t found[4];
@@ -97,13 +100,14 @@ struct GrScratch {
 template <int NT>
 __device__ __forceinline__ uint32_t gr_range(const GqaRowsArgs &a, bool few, GrScratch &L) {
     const uint32_t slots = few ? a.few_slots : a.slots, most = few ? a.few_items : a.items;
-    if ((!few && !a.split) || a.requests > 512) return 0x3fffffffu;
+    if ((!few && !a.split) || a.requests > GR_MOST) return GR_UNCUT;
     const uint32_t tid = threadIdx.x, c = tid & 31;
     if (tid < 32) L.count[tid] = 0;
     if (tid == 0) L.longest = 1;
     __syncthreads();
     for (uint32_t r = tid; r < a.requests; r += NT) {
         const GrShape s = gr_shape(a, gr_request(a, r), few);
+        L.shape[r] = s;
         if (s.qt) atomicMax(&L.longest, s.units);
     }
     __syncthreads();
@@ -111,7 +115,7 @@ __device__ __forceinline__ uint32_t gr_range(const GqaRowsArgs &a, bool few, GrS
     const uint32_t range = (L.longest + n - 1) / n;
     uint32_t items = 0;
     for (uint32_t r = tid >> 5; r < a.requests; r += NT / 32) {
-        const GrShape s = gr_shape(a, gr_request(a, r), few);
+        const GrShape s = L.shape[r];
         items += s.qt * ((s.units + range - 1) / range);
     }
     atomicAdd(&L.count[c], items);  // whole numbers: their order does not matter
@@ -148,7 +152,7 @@ __device__ __forceinline__ GrItem gr_find(const GqaRowsArgs &a, bool few, uint32
         const uint32_t r = r0 + threadIdx.x;
         uint32_t n = 0, ranges = 0;
         if (r < a.requests) {
-            const GrShape s = gr_shape(a, gr_request(a, r), few);
+            const GrShape s = range == GR_UNCUT ? gr_shape(a, gr_request(a, r), few) : L.shape[r];
             ranges = (s.units + range - 1) / range;
             n = s.qt * ranges * a.kv_heads;
         }
