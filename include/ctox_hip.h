@@ -702,7 +702,8 @@ ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *backend, uint8_t *d_q
  * gets zeros. Lengths are read on the device: a plan's row_starts and
  * tokens (row_starts not falling, at most `rows`; tokens[r] at most
  * min(page_count * page_tokens, 2^30)). max_rows bounds the rows of any one request (0:
- * rows); no request may have more. params.tokens is not read. f32 results: products
+ * rows); no request may have more (rows of one that has may be left as they are).
+ * params.tokens is not read. f32 results: products
  * keep 22 bits of each query value and probability, the cached codes are
  * exact, sums are 32 bits. Limits: head_dim 256, requests <= 4096, rows <= 2^20.
  * workspace holds ctox_hip_paged_gqa_rows_workspace bytes (of the same op; its device
