@@ -235,6 +235,15 @@ __device__ __forceinline__ uint32_t gr_tokens(uint64_t x) {
     return (uint32_t)(x | x >> 16);
 }
 
+// Exponent of a query whose largest |q * scale * log2 e| is mx: mx < 2^e. Not below -64, so that the scores' unit
+// 2^(e - 15) stays a normal number (0 times a masked score's -inf would be no number). What a smaller
+// query loses there, 2^-24 units of each value, moves a score by less than 2^(-24 - 79 + 16 + 8).
+__device__ __forceinline__ int gr_query_exponent(float mx) {
+    int e = 0;
+    frexpf(mx, &e);
+    return max(e, -64);
+}
+
 // Two f16 parts of eight values in the value operand's token order. hi is rounded towards zero, so
 // what is left has hi's sign and at most 13 bits.
 // (x - hi is one mixed-precision multiply-add by an opaque -1; a plain difference would convert first.)
@@ -447,8 +456,7 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
             for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[i]) < INFINITY ? fabsf(x[i]) : 0.0f);
         }
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        int e = 0;
-        frexpf(mx, &e);
+        const int e = gr_query_exponent(mx);
         qs = ldexpf(1.0f, e - 15);
         // The waves of a subtile write a share of it each.
 #pragma unroll
@@ -799,8 +807,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
         }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        int e = 0;
-        frexpf(mx, &e);
+        const int e = gr_query_exponent(mx);
         qs = ldexpf(1.0f, e - 15);
 #pragma unroll
         for (int s = 0; s < 8; s++) {

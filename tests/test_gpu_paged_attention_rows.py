@@ -387,3 +387,25 @@ def test_pages_past_four_gibibytes(hip, most):
         skip = (2 ** 32 + 5 * 16 * b.blocks * BB[kind]) // (16 * b.blocks * BB[kind]) + 1
         b.desc[..., 1] -= np.where((b.desc[..., 0] == kind) & (b.desc[..., 2] > 0), skip, 0).astype(np.uint32)
     b.check(b.d["out"].cpu().numpy())
+
+
+# (name, heads, KV heads, requests, max_rows): one batch for each of the three kernels
+KERNELS = [("128 queries", 6, 1, [(80, 40), (21, 30)], 0), ("32 queries", 6, 1, [(80, 5), (21, 3)], 5),
+           ("16 queries", 6, 1, [(80, 2), (21, 1)], 2)]
+
+
+@pytest.mark.parametrize("name,heads,kv_heads,requests,most", KERNELS)
+@pytest.mark.parametrize("holes", [False, True])
+def test_queries_below_the_normal_range(hip, name, heads, kv_heads, requests, most, holes):
+    """Rows whose largest value is an f32 subnormal, beside ordinary ones, over masked and absent tokens: all
+    scores are 0 to within any step, so they get the mean of what they see."""
+    say(f"case rows attention subnormal queries {name} holes={holes}")
+
+    def edit(b):
+        for i, size in enumerate((1e-42, 1e-39, 3e-45, 1e-37)):
+            b.q[i::5] *= np.float32(size)
+        if holes:
+            b.desc[0, 1, 2] = 0
+            b.desc[1, 0, 2] = 5
+    b = Batch(47, requests, 16, heads, kv_heads, q2=old, edit=edit, pad=2)
+    b.check(b.run(hip, max_rows=most))
