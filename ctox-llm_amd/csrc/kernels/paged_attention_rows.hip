@@ -30,8 +30,8 @@
 //  Values: O^T += V^T (P s_v)^T. The scores' output layout is the probabilities' operand layout if the
 //    tokens are counted as gr_v_operands does, so they stay in registers. s_v is the value block's
 //    scale: V is exact again, P s_v is two f16 parts in units of 2^(E - 9) with 2^E above every scale
-//    of the dim block so far. V's bytes are transposed on their way into LDS, a lane's operand being
-//    one byte column of eight tokens.
+//    of the dim block so far; where those scales differ by more than 2^5 every query has its own unit (GrUnit). V's bytes
+//    are transposed on their way into LDS, a lane's operand being one byte column of eight tokens.
 // Loads of the next tile are under way during this one, its page descriptors one tile before that.
 //
 // Measured, 24 query heads over 4 KV heads, pages of 16 tokens, old ones of 2-bit codes: a prompt of 4096 tokens
@@ -259,6 +259,25 @@ __device__ __forceinline__ void gr_split(const float (&x)[8], float minus_one, r
     }
 }
 
+// Value scales of a wide range. P s_v in units of 2^(E - 9) ends at f16's last bit, 2^-24 of them. That is far below
+// any result as long as all scales so far lie within 2^-6 .. 1 of 2^E: a query's largest probability is 1 or
+// more, so its sum of p |v| is at least 2^(E - 6) / 15, and T tokens lose at most T 2^(E - 33), less than the
+// roundings of a sum of T in 32 bits. Otherwise (a token that the query does not see, or hardly counts, may have set E; a
+// scale may be 0) every query takes a unit of its own for the tile: its largest |P s_v| goes to 2^14 .. 2^15, the sums
+// with it and back, by powers of two. (Measured where every third page has a token of scales 64 times smaller: 32 decoded
+// tokens 82 us instead of 73, 512 rows behind 32768 1350 us instead of 1038. The choice costs all others 2 %.)
+struct GrUnit {
+    float up, down;
+    // (60 at most: sums of 2^30 tokens stay below 2^(30 + 19 + 60))
+    __device__ __forceinline__ explicit GrUnit(float z) {
+        int e = 0;
+        frexpf(z, &e);
+        const int d = z > 0.0f ? max(0, min(15 - e, 60)) : 0;
+        up = ldexpf(1.0f, d);
+        down = ldexpf(1.0f, -d);
+    }
+};
+
 // ---------------------------------------------------------------------------
 // tiles from the pages
 // ---------------------------------------------------------------------------
@@ -324,15 +343,16 @@ struct GrLoad {
         return rkind ? (float)__builtin_bit_cast(_Float16, (uint16_t)rsc[i]) : 0.0f;
     }
     __device__ __forceinline__ float key_scale(int i) const { return scale(i) * (1.0f / 15.0f); }
-    // Piece i, of V: code bytes across, scales in units of 2^(9 - E), E, and the tokens without a finite scale.
+    // Piece i, of V: code bytes across, scales in units of 2^(9 - E), E, the tokens without a finite scale, and marks:
+    // 1 there are such tokens, 2 there are scales below 2^(E - 5).
     __device__ __forceinline__ void store_v(int i, uint32_t lane, uint32_t (&v)[32][9], float (&vs)[32], int &ev,
-                                            uint32_t &bads) {
+                                            uint32_t &bads, uint32_t &marks) {
         // (opaque with one piece: what follows from the lane alone is not to be kept in registers from tile to tile)
         if (R == 1) asm volatile("" : "+v"(lane));
         widen(i);
-        float sv = scale(i);
-        uint32_t bad = 0;
-        if (__builtin_amdgcn_ballot_w64(!(fabsf(ldexpf(sv, -ve[i])) < 1.0f))) {
+        float sv = scale(i), u = ldexpf(sv, 9 - ve[i]);
+        uint32_t bad = 0, mark = 0;
+        if (__builtin_amdgcn_ballot_w64(rkind && !(fabsf(u) >= 16.0f && fabsf(u) < 512.0f))) {
             const bool odd = !(fabsf(sv) < INFINITY);
             bad = gr_tokens(__builtin_amdgcn_ballot_w64(odd) >> (4 * pb));
             if (odd) sv = 0.0f;
@@ -342,12 +362,15 @@ struct GrLoad {
                 if (d != 4) z = fmaxf(z, __shfl_xor(z, d));
             int e = 0;
             frexpf(z, &e);
-            ve[i] = max(ve[i], e);
+            if (z != 0.0f) ve[i] = max(ve[i], e);
+            u = ldexpf(sv, 9 - ve[i]);
+            mark = (bad ? 1u : 0u) | (__builtin_amdgcn_ballot_w64(rkind && fabsf(u) < 16.0f) ? 2u : 0u);
         }
-        vs[R == 1 ? gr_token(lane) : token] = ldexpf(sv, 9 - ve[i]);
+        vs[R == 1 ? gr_token(lane) : token] = u;
         if ((lane & 59) == 0) {
             ev = ve[i];
             bads = bad;
+            marks = mark;
         }
 #pragma unroll
         for (int w = 0; w < 8; w++) v[4 * w + (lane & 3)][lane >> 3] = gr_across(raw[i][w], lane);
@@ -370,6 +393,7 @@ struct GrLds {
             float vs[TS][4][32];        // value scale in units of 2^(9 - E)
             int ev[TS][4];              // E of a block
             uint32_t bad[TS][4];        // its tokens without a finite value scale
+            uint32_t marks[TS][4];      // as store_v leaves them
         } t;
         float4 sum[QS * TS / 2][32][64];  // [publishing wave][dim block, parity, register quad][lane]
         GrScratch scratch;
@@ -428,7 +452,7 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     };
     auto store_v = [&](int i) {
         const uint32_t b = ld.block(i);
-        ld.store_v(i, lane, L.u.t.v[ts][b], L.u.t.vs[ts][b], L.u.t.ev[ts][b], L.u.t.bad[ts][b]);
+        ld.store_v(i, lane, L.u.t.v[ts][b], L.u.t.vs[ts][b], L.u.t.ev[ts][b], L.u.t.bad[ts][b], L.u.t.marks[ts][b]);
     };
 
     const RmMagic magic = rm_magic<true>();
@@ -486,6 +510,8 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
             for (int r = 0; r < 16; r++) o[b][c][r] = 0.0f;
     float m = -INFINITY, den = 0.0f;
     int ev[4] = {-100, -100, -100, -100};  // E of the blocks' sums
+    int first[4] = {0, 0, 0, 0};           // the first of them
+    bool wide = false;                     // value scales that GrUnit is for have been seen
 
     ld.issue(t0, t0 + TS);
     if (QS == 4 && ld.piece < 2) {
@@ -602,7 +628,7 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
             }
         }
         const int4 e4 = *(const int4 *)L.u.t.ev[ts];
-        const uint4 bad4 = *(const uint4 *)L.u.t.bad[ts];
+        const uint4 marks = *(const uint4 *)L.u.t.marks[ts];
         const int e[4] = {e4.x, e4.y, e4.z, e4.w};
         if (__builtin_amdgcn_ballot_w64(e[0] != ev[0] || e[1] != ev[1] || e[2] != ev[2] || e[3] != ev[3])) {
 #pragma unroll
@@ -612,12 +638,18 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
                 for (int c = 0; c < 2; c++)
 #pragma unroll
                     for (int r = 0; r < 16; r++) o[b][c][r] = ldexpf(o[b][c][r], d);
-                ev[b] = __builtin_amdgcn_readfirstlane(e[b]);
+                const int now = __builtin_amdgcn_readfirstlane(e[b]);
+                if (ev[b] == -100) first[b] = now;
+                if (now > first[b] + 1) wide = true;
+                ev[b] = now;
             }
         }
         // A value block without a finite scale makes its dims no numbers for every query that sees the token, and
         // does not count for the others (its scale is 0).
-        if (__builtin_amdgcn_ballot_w64((bad4.x | bad4.y | bad4.z | bad4.w) != 0)) {
+        const uint32_t mark = __builtin_amdgcn_readfirstlane(marks.x | marks.y | marks.z | marks.w);
+        wide |= mark >> 1;
+        if (mark & 1) {
+            const uint4 bad4 = *(const uint4 *)L.u.t.bad[ts];
             const uint32_t bads[4] = {bad4.x, bad4.y, bad4.z, bad4.w};
 #pragma unroll
             for (int b = 0; b < 4; b++) {
@@ -632,6 +664,25 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
                     for (int r = 0; r < 16; r++) o[b][c][r] = any ? __builtin_nanf("") : o[b][c][r];
             }
         }
+        // Into the block's units of a wide range and back: probabilities and sums.
+        float down;
+        auto into = [&](int b) {
+            float z = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float4 f = *(const float4 *)&L.u.t.vs[ts][b][8 * j + 4 * h];
+                z = fmaxf(fmaxf(z, fabsf(s[4 * j] * f.x)), fabsf(s[4 * j + 1] * f.y));
+                z = fmaxf(fmaxf(z, fabsf(s[4 * j + 2] * f.z)), fabsf(s[4 * j + 3] * f.w));
+            }
+            const GrUnit u(fmaxf(z, __shfl_xor(z, 32)));
+            down = u.down;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] *= u.up, o[b][0][r] *= u.up, o[b][1][r] *= u.up;
+        };
+        auto back = [&](int b) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] *= down, o[b][0][r] *= down, o[b][1][r] *= down;
+        };
         uint32_t vx[2][2];
         float4 fx[2][2];
         auto read_v = [&](int n) {
@@ -644,6 +695,10 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
 #pragma unroll
         for (int n = 0; n < 8; n++) {
             const int b = n >> 1, k = n & 1;
+            if (k == 0 && wide) {
+                if (b) back(b - 1);
+                into(b);
+            }
             if (n + AHEAD < 8) read_v(n + AHEAD);
             if (AHEAD) __builtin_amdgcn_sched_barrier(0x76);
             rm_h8 vf[2];
@@ -659,6 +714,7 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
             for (int c = 0; c < 2; c++) o[b][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c], hi, o[b][c], 0, 0, 0);
             if (AHEAD) __builtin_amdgcn_sched_barrier(0x76);
         }
+        if (wide) back(3);
         lds_wave_order();
     }
     // ---- join the token shares, half of the waves publishing to the other half, and write ----
@@ -753,7 +809,7 @@ struct GrLds16 {
             float ks[4][4][32];
             float vs[4][4][32];
             int ev[4][4];
-            uint32_t bad[4][4];
+            uint32_t bad[4][4], marks[4][4];
         } t;
         float4 sum[2][16][64];  // [publishing wave][dim block, half, parity][lane]
         GrScratch scratch;
@@ -831,6 +887,8 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
         for (int c = 0; c < 4; c++) o[b][c >> 1][c & 1] = gr_v4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, den = 0.0f;
     int ev[4] = {-100, -100, -100, -100};  // E of the blocks' sums
+    int first[4] = {0, 0, 0, 0};           // the first of them
+    bool wide = false;                     // value scales that GrUnit is for have been seen
 
     ld.issue(t0, t0 + 4);
     __builtin_amdgcn_s_waitcnt(0x0F70);
@@ -847,7 +905,8 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
 #pragma unroll
         for (int i = 2; i < 4; i++) {
             const uint32_t b = ld.block(i);
-            ld.store_v(i, lane, L.u.t.v[wave][b], L.u.t.vs[wave][b], L.u.t.ev[wave][b], L.u.t.bad[wave][b]);
+            ld.store_v(i, lane, L.u.t.v[wave][b], L.u.t.vs[wave][b], L.u.t.ev[wave][b], L.u.t.bad[wave][b],
+                       L.u.t.marks[wave][b]);
         }
         lds_wave_order();
         ld.issue(t + 4, t + 8);
@@ -915,7 +974,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
         }
         // ---- values ----
         const int4 e4 = *(const int4 *)L.u.t.ev[wave];
-        const uint4 bad4 = *(const uint4 *)L.u.t.bad[wave];
+        const uint4 marks = *(const uint4 *)L.u.t.marks[wave];
         const int e[4] = {e4.x, e4.y, e4.z, e4.w};
         if (__builtin_amdgcn_ballot_w64(e[0] != ev[0] || e[1] != ev[1] || e[2] != ev[2] || e[3] != ev[3])) {
 #pragma unroll
@@ -925,11 +984,17 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
                 for (int c = 0; c < 4; c++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) o[b][c >> 1][c & 1][r] = ldexpf(o[b][c >> 1][c & 1][r], d);
-                ev[b] = __builtin_amdgcn_readfirstlane(e[b]);
+                const int now = __builtin_amdgcn_readfirstlane(e[b]);
+                if (ev[b] == -100) first[b] = now;
+                if (now > first[b] + 1) wide = true;
+                ev[b] = now;
             }
         }
         // (as above: no numbers for every query that sees the token, nothing for the others)
-        if (__builtin_amdgcn_ballot_w64((bad4.x | bad4.y | bad4.z | bad4.w) != 0)) {
+        const uint32_t mark = __builtin_amdgcn_readfirstlane(marks.x | marks.y | marks.z | marks.w);
+        wide |= mark >> 1;
+        if (mark & 1) {
+            const uint4 bad4 = *(const uint4 *)L.u.t.bad[wave];
             const uint32_t bads[4] = {bad4.x, bad4.y, bad4.z, bad4.w};
 #pragma unroll
             for (int b = 0; b < 4; b++) {
@@ -949,8 +1014,21 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
         for (int b = 0; b < 4; b++) {
             const float4 f0 = *(const float4 *)&L.u.t.vs[wave][b][4 * g];
             const float4 f1 = *(const float4 *)&L.u.t.vs[wave][b][16 + 4 * g];
-            const float x[8] = {p[0] * f0.x, p[1] * f0.y, p[2] * f0.z, p[3] * f0.w,
-                                p[4] * f1.x, p[5] * f1.y, p[6] * f1.z, p[7] * f1.w};
+            float x[8] = {p[0] * f0.x, p[1] * f0.y, p[2] * f0.z, p[3] * f0.w,
+                          p[4] * f1.x, p[5] * f1.y, p[6] * f1.z, p[7] * f1.w};
+            float down = 1.0f;
+            if (wide) {
+                float z = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 8; r++) z = fmaxf(z, fabsf(x[r]));
+                z = fmaxf(z, __shfl_xor(z, 16));
+                const GrUnit u(fmaxf(z, __shfl_xor(z, 32)));
+#pragma unroll
+                for (int r = 0; r < 8; r++) x[r] *= u.up;
+#pragma unroll
+                for (int c = 0; c < 4; c++) o[b][c >> 1][c & 1] *= u.up;
+                down = u.down;
+            }
             rm_h8 hi, lo;
             gr_split(x, minus_one, hi, lo);
 #pragma unroll
@@ -963,6 +1041,9 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
                     o[b][c][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[n], hi, o[b][c][n], 0, 0, 0);
                 }
             }
+            if (wide)
+#pragma unroll
+                for (int c = 0; c < 4; c++) o[b][c >> 1][c & 1] *= down;
         }
         lds_wave_order();
     }

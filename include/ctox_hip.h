@@ -704,7 +704,10 @@ ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *backend, uint8_t *d_q
  * min(page_count * page_tokens, 2^30)). max_rows bounds the rows of any one request (0:
  * rows); no request may have more (rows of one that has may be left as they are).
  * params.tokens is not read. f32 results: products
- * keep 22 bits of each query value and probability, the cached codes are
+ * keep 22 bits of each query value (of one below 2^-17 of its head's largest an
+ * absolute 2^-40 of that) and 21 bits of each probability times value scale (of a small
+ * one an absolute step that adds up to less than the roundings of a 32-bit sum over the
+ * row's tokens, whatever the value scales of other tokens), the cached codes are
  * exact, sums are 32 bits. Limits: head_dim 256, requests <= 4096, rows <= 2^20.
  * workspace holds ctox_hip_paged_gqa_rows_workspace bytes (of the same op; its device
  * pointers are not read), 16-byte aligned, and is free again when the call's work on

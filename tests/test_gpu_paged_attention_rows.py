@@ -409,3 +409,67 @@ def test_queries_below_the_normal_range(hip, name, heads, kv_heads, requests, mo
             b.desc[1, 0, 2] = 5
     b = Batch(47, requests, 16, heads, kv_heads, q2=old, edit=edit, pad=2)
     b.check(b.run(hip, max_rows=most))
+
+
+def value_scales(b, r, at, scale):
+    """V scales of the tokens `at` of request r."""
+    for j in at:
+        kind, slot, _, first = (int(x) for x in b.desc[r, j // b.page])
+        b.pool[kind][slot, j - first, b.blocks // 2:, :2] = np.array([scale], np.float16).view(np.uint8)
+
+
+def look_at(b, r, token, rows, score):
+    """Queries of request r's rows that give `token` about that score (natural units) and others a small one."""
+    G = b.H // b.KV
+    k, _, _ = b.token_values(r)
+    for t in rows:
+        for h in range(b.H):
+            x = k[token, h // G]
+            b.q[b.starts[r] + t, h] = (x * (score * 16.0 / (x @ x))).astype(np.float32)
+
+
+@pytest.mark.parametrize("name,heads,kv_heads,requests,most", KERNELS)
+@pytest.mark.parametrize("large", [1e3, 6e4])
+@pytest.mark.parametrize("small", [1e-3, 6e-5])
+def test_large_values_out_of_sight(hip, name, heads, kv_heads, requests, most, large, small):
+    """The chunk's last token is of a large value scale: rows before it do not see it, and keep their bits."""
+    say(f"case rows attention large value masked {name} {large} {small}")
+
+    def edit(b):
+        for r, (cached, n) in enumerate(requests):
+            value_scales(b, r, range(cached + n), small)
+            value_scales(b, r, [cached + n - 1], large)
+    b = Batch(53, requests, 16, heads, kv_heads, q2=old, edit=edit)
+    b.check(b.run(hip, max_rows=most))
+
+
+@pytest.mark.parametrize("name,heads,kv_heads,requests,most", KERNELS)
+@pytest.mark.parametrize("token,others", [(3, range(4, 120)), (70, range(0, 64)), (3, range(40, 120)), (70, range(64, 70))])
+@pytest.mark.parametrize("small,large,score", [(1e-3, 1e3, 16.0), (1e-3, 6e4, 20.0), (6e-5, 6e4, 25.0), (0.0, 1.0, 16.0),
+                                               (0.0, 6e-8, 10.0), (3e-7, 6e4, 40.0)])
+def test_small_values_of_a_peak(hip, name, heads, kv_heads, requests, most, token, others, small, large, score):
+    """Probability 1 - tiny on a token of small (or no) values, tiny ones on tokens of large values: before, behind
+    and beside it in its tile, and in later tiles alone."""
+    say(f"case rows attention peak {name} {token} {others} {small} {large} {score}")
+
+    def edit(b):
+        n = sum(requests[0])
+        value_scales(b, 0, range(n), small)
+        value_scales(b, 0, [j for j in others if j < n], large)
+        look_at(b, 0, token, range(requests[0][1]), score)
+    b = Batch(59, requests, 16, heads, kv_heads, q2=old, edit=edit)
+    b.check(b.run(hip, max_rows=most))
+
+
+@pytest.mark.parametrize("name,heads,kv_heads,requests,most", KERNELS)
+def test_a_peak_that_comes_late(hip, name, heads, kv_heads, requests, most):
+    """Large values first, then a token of small ones whose score is far above: what was summed shrinks to nothing."""
+    say(f"case rows attention late peak {name}")
+
+    def edit(b):
+        n = sum(requests[0])
+        value_scales(b, 0, range(n), 1e-3)
+        value_scales(b, 0, range(48), 6e4)
+        look_at(b, 0, 66, range(requests[0][1]), 60.0)
+    b = Batch(61, requests, 16, heads, kv_heads, q2=old, edit=edit)
+    b.check(b.run(hip, max_rows=most))
