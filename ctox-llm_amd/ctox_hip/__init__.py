@@ -199,6 +199,25 @@ class PagedGqaParams(ctypes.Structure):
         "q2_token_bytes", "q4_token_bytes", "q2_page_bytes", "q4_page_bytes")] + [("scale", ctypes.c_float)]
 
 
+def _fit(bits: int, *values: int) -> None:
+    """Refuses what ctypes would take modulo 2^bits."""
+    if min(values) < 0 or max(values) >= 1 << bits:
+        raise ShapeError(f"one of {values} does not fit {bits} bits")
+
+
+class _Op(ctypes.Structure):
+    """A kept call's description whose numbers are refused, not wrapped, where they do not fit."""
+
+    def __setattr__(self, name, value):
+        bits = self._bits.get(name)
+        if bits:
+            _fit(bits, value)
+        super().__setattr__(name, value)
+
+
+def _bits(fields):
+    return {n: 8 * ctypes.sizeof(t) for n, t in fields if t in (ctypes.c_uint32, ctypes.c_uint64)}
+
 
 class _MatrixRows(ctypes.Structure):
     """ctox_matrix_rows."""
@@ -208,7 +227,7 @@ class _MatrixRows(ctypes.Structure):
         ("workspace_bytes", ctypes.c_uint64)]
 
 
-class RopeAxes(ctypes.Structure):
+class RopeAxes(_Op):
     """ctox_rope_axes. Strides are (row, head) in values; outputs are dense unless given,
     axis_of_pair a sequence of rotary_dim / 2 axis numbers (None: all 0)."""
     _fields_ = [(n, ctypes.c_void_p) for n in (
@@ -216,6 +235,7 @@ class RopeAxes(ctypes.Structure):
         (f"{t}_{n}_stride", ctypes.c_uint64) for t in ("q", "k", "q_out", "k_out") for n in ("row", "head")] + [
         (n, ctypes.c_uint32) for n in ("rows", "q_heads", "k_heads", "head_dim", "rotary_dim", "axes")] + [
         ("theta", ctypes.c_float), ("eps", ctypes.c_float)]
+    _bits = _bits(_fields_)
 
     def __init__(self, d_q, d_positions, rows, q_heads, head_dim, rotary_dim, theta, d_k=None, d_q_out=None,
                  d_k_out=None, d_q_norm=None, d_k_norm=None, d_row_count=None, axis_of_pair=None, q_strides=None,
@@ -224,6 +244,7 @@ class RopeAxes(ctypes.Structure):
         if axis_of_pair is not None:
             if len(axis_of_pair) != rotary_dim // 2:
                 raise ShapeError("axis_of_pair needs one axis per rotary pair")
+            _fit(8, 0, *axis_of_pair)
             self._axis = (ctypes.c_uint8 * max(1, len(axis_of_pair)))(*axis_of_pair)
         dense_q, dense_k = (q_heads * head_dim, head_dim), (k_heads * head_dim, head_dim)
         q_strides, k_strides = q_strides or dense_q, k_strides or dense_k
@@ -238,12 +259,13 @@ class RopeAxes(ctypes.Structure):
 NO_SLOT = 0xffffffff
 
 
-class PagedPlan(ctypes.Structure):
+class PagedPlan(_Op):
     """ctox_paged_plan (all pointers are device addresses)."""
     _fields_ = [(n, ctypes.c_void_p) for n in (
         "cached", "added", "descriptors", "free_slots", "row_starts", "tokens", "page_counts", "positions", "slots",
         "status")] + [(n, ctypes.c_uint32) for n in (
             "requests", "page_tokens", "max_pages", "free_count", "q4_slots", "max_rows")]
+    _bits = _bits(_fields_)
 
     def __init__(self, d_cached, d_added, d_descriptors, d_free_slots, d_row_starts, d_tokens, d_page_counts,
                  d_positions, d_slots, d_status, requests, page_tokens, max_pages, free_count, q4_slots, max_rows):
@@ -252,12 +274,13 @@ class PagedPlan(ctypes.Structure):
                          max_rows)
 
 
-class PagedGqaRows(ctypes.Structure):
+class PagedGqaRows(_Op):
     """ctox_paged_gqa_rows (device addresses; params.tokens is not read)."""
     _fields_ = [(n, ctypes.c_void_p) for n in (
         "query", "out", "q2_pages", "q4_pages", "descriptors", "row_starts", "tokens")] + [
         ("rows", ctypes.c_uint64), ("requests", ctypes.c_uint32), ("max_rows", ctypes.c_uint32),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("params", PagedGqaParams)]
+    _bits = _bits(_fields_)
 
     def __init__(self, d_query, d_out, d_q2_pages, d_q4_pages, d_descriptors, d_row_starts, d_tokens, rows, requests,
                  params, max_rows=0, d_workspace=None, workspace_bytes=0):
@@ -463,6 +486,7 @@ class HipMatrix:
     def rows_workspace(self, rows: int, x_dtype: TensorDType = TensorDType.F32) -> int:
         """Workspace bytes of a dispatch_rows call of `rows` rows."""
         n = ctypes.c_size_t()
+        _fit(64, rows)
         _check(load_library().ctox_hip_matrix_rows_workspace(self.handle, rows, int(x_dtype), ctypes.byref(n)))
         return n.value
 
@@ -472,6 +496,7 @@ class HipMatrix:
                       residual_stride: int = 0, stream: Optional[int] = None) -> None:
         """act((x * s_in . W^T + bias) * s_out) + residual for any number of rows; strides in
         values (0: dense rows)."""
+        _fit(64, rows, x_stride, y_stride, residual_stride, workspace_bytes)
         op = _MatrixRows(d_x, d_y, d_residual, rows, x_stride, y_stride, residual_stride, int(x_dtype), int(y_dtype),
                          d_workspace, workspace_bytes)
         _check(load_library().ctox_hip_matrix_dispatch_rows(self.backend.handle, self.handle, ctypes.byref(op), stream))
@@ -735,10 +760,13 @@ class HipBackend:
                             key_stride: Optional[int] = None, value_stride: Optional[int] = None,
                             stream: Optional[int] = None) -> None:
         """K / V rows into the Q4 slots of a slot map (Q/src/kv_cache.rs:200-206 on the device)."""
+        key_stride = component_values if key_stride is None else key_stride
+        value_stride = component_values if value_stride is None else value_stride
+        _fit(64, rows, component_values, key_stride, value_stride)
+        _fit(32, page_tokens, q4_slots, q4_page_bytes)
         _check(load_library().ctox_hip_kv_append_q4_device(
-            self.handle, d_q4_pages, d_keys, component_values if key_stride is None else key_stride, d_values,
-            component_values if value_stride is None else value_stride, d_slots, rows, component_values, page_tokens,
-            q4_slots, q4_page_bytes, stream))
+            self.handle, d_q4_pages, d_keys, key_stride, d_values, value_stride, d_slots, rows, component_values,
+            page_tokens, q4_slots, q4_page_bytes, stream))
 
     def paged_gqa_rows_workspace(self, op: PagedGqaRows) -> int:
         """Workspace bytes of a paged_gqa_rows_device call (reads no device pointer of `op`)."""

@@ -146,3 +146,62 @@ def attention(params=None, **over):
 ])
 def test_attention_refuses(params, over, says):
     assert says in attention(params, **over)
+
+
+@pytest.mark.parametrize("make", [
+    lambda: RopeAxes(d_q=P, d_positions=P, rows=1, q_heads=1, head_dim=64, rotary_dim=64, theta=1e4,
+                     axis_of_pair=[0] * 31 + [256]),
+    lambda: RopeAxes(d_q=P, d_positions=P, rows=1, q_heads=1, head_dim=64, rotary_dim=64, theta=1e4,
+                     axis_of_pair=[0] * 31 + [-1]),
+    lambda: RopeAxes(d_q=P, d_positions=P, rows=2 ** 32 + 1, q_heads=1, head_dim=64, rotary_dim=64, theta=1e4),
+    lambda: RopeAxes(d_q=P, d_positions=P, rows=1, q_heads=1, head_dim=64, rotary_dim=64, theta=1e4, q_strides=(-64, 64)),
+    lambda: PagedPlan(*[P] * 10, requests=2 ** 32 + 3, page_tokens=16, max_pages=8, free_count=5, q4_slots=40, max_rows=64),
+    lambda: PagedPlan(*[P] * 10, requests=3, page_tokens=16, max_pages=8, free_count=-1, q4_slots=40, max_rows=64),
+    lambda: ctox_hip.PagedGqaRows(*[P] * 7, rows=-1, requests=3, params=ctox_hip.PagedGqaParams()),
+    lambda: ctox_hip.PagedGqaRows(*[P] * 7, rows=9, requests=2 ** 32 + 3, params=ctox_hip.PagedGqaParams()),
+    lambda: ctox_hip.PagedGqaRows(*[P] * 7, rows=9, requests=3, params=ctox_hip.PagedGqaParams(), max_rows=2 ** 32),
+])
+def test_numbers_that_do_not_fit_are_refused(make):
+    """A field takes its value or refuses it; none is taken modulo the field's size."""
+    with pytest.raises(ctox_hip.ShapeError):
+        make()
+
+
+def test_a_field_set_later_is_checked_too():
+    op = ctox_hip.PagedGqaRows(*[P] * 7, rows=9, requests=3, params=ctox_hip.PagedGqaParams())
+    with pytest.raises(ctox_hip.ShapeError):
+        op.requests = 2 ** 32 + 3
+    op.requests = 2 ** 32 - 1
+    assert op.requests == 2 ** 32 - 1 and op.query == P
+
+
+def unbound(cls):
+    """A handle without a device: every check of these calls comes before it is read."""
+    x = object.__new__(cls)
+    x.handle = x.backend = None
+    return x
+
+
+@pytest.mark.parametrize("over", [dict(rows=2 ** 64 + 1), dict(component_values=-64), dict(page_tokens=2 ** 32 + 16),
+                                  dict(q4_slots=2 ** 32 + 9), dict(q4_page_bytes=-4), dict(key_stride=-1024),
+                                  dict(value_stride=2 ** 64 + 1024)])
+def test_append_numbers_that_do_not_fit_are_refused(over):
+    kw = dict(d_q4_pages=P, d_keys=P, d_values=P, d_slots=P, rows=5, component_values=1024, page_tokens=16, q4_slots=9,
+              q4_page_bytes=16 * 1088)
+    kw.update(over)
+    with pytest.raises(ctox_hip.ShapeError, match="does not fit"):
+        unbound(ctox_hip.HipBackend).kv_append_q4_device(**kw)
+
+
+@pytest.mark.parametrize("over", [dict(rows=2 ** 64 + 4), dict(x_stride=-1), dict(y_stride=2 ** 64), dict(residual_stride=-5),
+                                  dict(workspace_bytes=-1)])
+def test_rows_product_numbers_that_do_not_fit_are_refused(over):
+    kw = dict(d_x=P, rows=4, d_y=P, d_workspace=P, workspace_bytes=1 << 20)
+    kw.update(over)
+    m = unbound(ctox_hip.HipMatrix)
+    m.backend = unbound(ctox_hip.HipBackend)
+    with pytest.raises(ctox_hip.ShapeError, match="does not fit"):
+        m.dispatch_rows(**kw)
+    if "rows" in over:
+        with pytest.raises(ctox_hip.ShapeError, match="does not fit"):
+            m.rows_workspace(over["rows"])
