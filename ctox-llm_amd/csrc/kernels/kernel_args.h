@@ -648,6 +648,7 @@ struct RowsMulArgs {
 };
 
 // Attention of a ragged batch's rows (paged_attention_rows.hip).
+#define CTOX_GQA_CUT_REQUESTS 512  // requests of a batch whose token axes may be cut
 struct GqaRowsArgs {
     const float *query;      // [rows][query_heads][256]
     float *out;              // [rows][query_heads][256]

@@ -82,10 +82,9 @@ __device__ __forceinline__ GrShape gr_shape(const GqaRowsArgs &a, const GrReques
     return s;
 }
 
-#define GR_MOST 512            // requests of a batch whose token axes may be cut
 #define GR_UNCUT 0x3fffffffu  // a range that holds any request
 struct GrScratch {
-    GrShape shape[GR_MOST];
+    GrShape shape[CTOX_GQA_CUT_REQUESTS];
     uint32_t count[32], longest, range;
     uint32_t scan[8];
     uint32_t found[4];
@@ -100,7 +99,7 @@ struct GrScratch {
 template <int NT>
 __device__ __forceinline__ uint32_t gr_range(const GqaRowsArgs &a, bool few, GrScratch &L) {
     const uint32_t slots = few ? a.few_slots : a.slots, most = few ? a.few_items : a.items;
-    if ((!few && !a.split) || a.requests > GR_MOST) return GR_UNCUT;
+    if ((!few && !a.split) || a.requests > CTOX_GQA_CUT_REQUESTS) return GR_UNCUT;
     const uint32_t tid = threadIdx.x, c = tid & 31;
     if (tid < 32) L.count[tid] = 0;
     if (tid == 0) L.longest = 1;

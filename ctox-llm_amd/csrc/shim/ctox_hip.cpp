@@ -236,6 +236,9 @@ struct ctox_hip_matrix {
     // Per segment: the same rows rewritten into the tiled layout (kernel_args.h).
     using Tiled = TiledCopy;
     std::vector<Tiled> tiled;
+    // Row products: [parts - 1][32-row tiles of x - 1]: partial sums' bytes that any call of up to so many
+    // whole tiles may need; the last entry holds for more.
+    std::vector<uint64_t> row_partials[2];
 };
 
 namespace {
@@ -1112,6 +1115,8 @@ ctox_status tile_segments(ctox_hip_backend *b, ctox_hip_matrix *m) {
     return CTOX_OK;
 }
 
+void note_row_partials(ctox_hip_matrix *m);
+
 ctox_status prepare_impl(ctox_hip_backend *b, const ctox_fused_matvec *op, ctox_hip_matrix **out) {
     size_t blocks;
     ctox_status st = validate_matvec(op, false, &blocks);
@@ -1148,6 +1153,7 @@ ctox_status prepare_impl(ctox_hip_backend *b, const ctox_fused_matvec *op, ctox_
         return st;
     }
     m->activation = (uint32_t)op->activation;
+    note_row_partials(m);
     *out = m;
     return CTOX_OK;
 }
@@ -2842,7 +2848,39 @@ RowPlan row_plan(uint32_t cus, uint32_t rows, uint32_t n, uint32_t blocks, uint3
     return best;
 }
 
-// Where a row product's workspace holds what.
+// Partial sums' bytes of a call of `rows` rows, at least. Within a 32-row tile of rows a plan's cost is a line in
+// rows, steeper with more splits, so the cheapest plan never splits more than at the tile's first row: with that
+// many splits the bytes do not fall from row to row.
+uint64_t row_partial_bytes(const ctox_hip_matrix *m, uint32_t rows, uint32_t parts) {
+    const uint32_t cus = (uint32_t)m->backend->cus, blocks = (uint32_t)(m->columns / kBlockLen);
+    const uint32_t first = (rows - 1) / 32 * 32 + 1;
+    uint64_t most = 0;
+    for (const ctox_quant_segment &seg : m->segments) {
+        const uint32_t n = (uint32_t)(seg.row_end - seg.row_start);
+        const uint32_t splits = std::max(row_plan(cus, first, n, blocks, parts).splits, row_plan(cus, rows, n, blocks, parts).splits);
+        if (splits > 1) most = std::max<uint64_t>(most, (uint64_t)splits * rows * n * sizeof(float));
+    }
+    return most;
+}
+
+// From one tile to the next a plan may go from many splits to few, so the matrix keeps the most up to each count of
+// tiles (up to where no segment's K can be split any more: row_plan's bound on workgroups).
+void note_row_partials(ctox_hip_matrix *m) {
+    size_t least = m->rows;
+    for (const ctox_quant_segment &seg : m->segments) least = std::min(least, seg.row_end - seg.row_start);
+    const RowShape wide = kRowShapes[3];
+    const uint64_t groups = std::max<uint64_t>(1, (least + 128 * wide.rt - 1) / (128 * wide.rt));
+    const uint64_t tiles = m->columns / kBlockLen < 8 ? 0 : (4 * (uint64_t)m->backend->cus / groups + 1) * wide.tt;
+    for (uint32_t parts = 1; parts <= 2; parts++) {
+        uint64_t most = 0;
+        for (uint64_t t = 1; t <= std::min<uint64_t>(tiles, (1u << 20) / 32); t++) {
+            most = std::max(most, row_partial_bytes(m, (uint32_t)(32 * t), parts));
+            m->row_partials[parts - 1].push_back(most);
+        }
+    }
+}
+
+// Where a row product's workspace holds what. No call of fewer rows needs more.
 struct RowSpace {
     uint32_t parts;
     uint64_t staged[2], exps, partial, total;  // byte offsets; staged per value order [Q2, Q4]
@@ -2850,24 +2888,22 @@ struct RowSpace {
 RowSpace row_space(const ctox_hip_matrix *m, uint64_t rows, int32_t x_dtype) {
     RowSpace w{};
     w.parts = x_dtype == CTOX_DTYPE_F16 && m->s_in_kind == CTOX_KSCALE_NONE ? 1 : 2;
-    uint64_t at = 0, partial = 0;
+    uint64_t at = 0;
     auto take = [&](uint64_t bytes) {
         const uint64_t here = at;
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    const uint32_t blocks = (uint32_t)(m->columns / kBlockLen);
     const uint64_t one = (rows + 31) / 32 * 32 * m->columns * 2 * w.parts;
     for (int q4 = 0; q4 < 2; q4++) {
         bool any = false;
         for (const ctox_quant_segment &seg : m->segments) any = any || (seg.dtype == CTOX_DTYPE_Q4B64) == (q4 == 1);
         w.staged[q4] = take(any ? one : 0);
     }
-    for (const ctox_quant_segment &seg : m->segments) {
-        const uint32_t n = (uint32_t)(seg.row_end - seg.row_start);
-        const uint32_t parts = row_plan((uint32_t)m->backend->cus, (uint32_t)rows, n, blocks, w.parts).splits;
-        if (parts > 1) partial = std::max<uint64_t>(partial, (uint64_t)parts * rows * n * sizeof(float));
-    }
+    const std::vector<uint64_t> &before = m->row_partials[w.parts - 1];
+    const size_t whole = std::min<size_t>((rows - 1) / 32, before.size());
+    uint64_t partial = row_partial_bytes(m, (uint32_t)rows, w.parts);
+    if (whole) partial = std::max(partial, before[whole - 1]);
     w.exps = take(w.parts == 2 ? rows * sizeof(int32_t) : 0);
     w.partial = take(partial);
     w.total = at;
@@ -3003,9 +3039,10 @@ ctox_status check_gqa_rows(const ctox_paged_gqa_rows *op) {
 // ranges where its query tiles alone would not give every CU two workgroups. Items: one a query tile and
 // KV head at least; the device cuts ranges into more up to the bound given here, two rounds of the chip.
 struct GqaRowsPlan {
-    bool wide, split;
+    bool wide, split, cut;  // cut: token ranges may be
     uint32_t few, few_slots, slots, few_items, items;
-    uint64_t cut_bytes, few_bytes, bytes;
+    uint64_t cut_bytes, few_bytes;
+    uint64_t need;  // the workspace: enough for every call of at most so many rows, requests and max_rows
 };
 GqaRowsPlan gqa_rows_plan(uint32_t cus, const ctox_paged_gqa_rows *op) {
     GqaRowsPlan g{};
@@ -3016,17 +3053,24 @@ GqaRowsPlan gqa_rows_plan(uint32_t cus, const ctox_paged_gqa_rows *op) {
     g.few = group > 32 || (g.wide && op->requests == 1) ? 0 : most * group <= 16 ? 16 : 32;
     g.few_slots = 2 * cus;
     g.slots = cus;
+    g.cut = op->requests <= CTOX_GQA_CUT_REQUESTS;
     g.cut_bytes = ((uint64_t)op->requests * 8 + 15) / 16 * 16;
+    const uint64_t part = 258 * sizeof(float), tiles = (op->rows * group + 127) / 128;
     if (g.few) {
-        g.few_items = (uint32_t)(busy * kvh + 2 * g.few_slots);
-        g.few_bytes = (uint64_t)g.few_items * g.few * 258 * sizeof(float);
+        g.few_items = (uint32_t)(busy * kvh + (g.cut ? 2 * g.few_slots : 0));
+        g.few_bytes = g.cut ? g.few_items * g.few * part : 0;
     }
     if (g.wide) {
-        const uint64_t tiles = (op->rows * group + 127) / 128;
-        g.split = tiles * kvh < 2 * cus;
+        g.split = g.cut && tiles * kvh < 2 * cus;
         g.items = (uint32_t)((tiles + busy) * kvh + (g.split ? 2 * g.slots : 0));
-        g.bytes = g.split ? (uint64_t)g.items * 128 * 258 * sizeof(float) : 0;
     }
+    // Fewer rows may go to another kernel, or be split where more are not. The few-query kernels need most with the
+    // most requests that are cut and have rows; the 128-query kernel with the most tiles that still miss two
+    // workgroups a CU. One request goes to one of the two, several may go to both.
+    const uint64_t cut = std::min<uint64_t>(busy, CTOX_GQA_CUT_REQUESTS), most_tiles = std::min<uint64_t>(tiles, (2 * cus - 1) / kvh);
+    const uint64_t few = group > 32 ? 0 : (cut * kvh + 2 * g.few_slots) * (most * group <= 16 ? 16 : 32) * part;
+    const uint64_t wide = g.wide && most_tiles ? ((most_tiles + cut) * kvh + 2 * g.slots) * 128 * part : 0;
+    g.need = g.cut_bytes + (op->requests == 1 ? std::max(few, wide) : few + wide);
     return g;
 }
 }  // namespace
@@ -3038,7 +3082,7 @@ extern "C" ctox_status ctox_hip_paged_gqa_rows_workspace(const ctox_hip_backend 
     if (ctox_status st = check_gqa_rows(op)) return st;
     if (!b) return fail(CTOX_ERR_SHAPE, "null argument");
     const GqaRowsPlan g = gqa_rows_plan((uint32_t)b->cus, op);
-    *bytes = (size_t)(g.cut_bytes + g.few_bytes + g.bytes);
+    *bytes = (size_t)g.need;
     return CTOX_OK;
 }
 
@@ -3052,10 +3096,9 @@ extern "C" ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *b, const
         return fail(CTOX_ERR_SHAPE, "an attention pointer is not aligned");
     if (op->rows == 0) return CTOX_OK;
     const GqaRowsPlan g = gqa_rows_plan((uint32_t)b->cus, op);
-    const uint64_t need = g.cut_bytes + g.few_bytes + g.bytes;
-    if ((op->workspace_bytes < need || !op->workspace || !aligned(op->workspace, 16)))
+    if ((op->workspace_bytes < g.need || !op->workspace || !aligned(op->workspace, 16)))
         return fail(CTOX_ERR_MEMORY_BUDGET, "workspace of %llu bytes, %llu needed, 16-byte aligned",
-                    (unsigned long long)op->workspace_bytes, (unsigned long long)need);
+                    (unsigned long long)op->workspace_bytes, (unsigned long long)g.need);
     const ctox_paged_gqa_params &p = op->params;
     const uint32_t cv = p.key_value_heads * 256;
     GqaRowsArgs a{};
@@ -3102,7 +3145,7 @@ extern "C" ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *b, const
     if (g.wide) st = launch(b->gqa_rows, dim3(g.items), dim3(512), s, a, "ctox_gqa_rows_gfx950");
     if (!st && g.few)
         st = launch(g.few == 16 ? b->gqa_few16 : b->gqa_few, dim3(g.few_items), dim3(256), s, a, "ctox_gqa_few_gfx950");
-    if (!st && (g.few || g.split))
+    if (!st && g.cut && (g.few || g.split))
         st = launch(b->gqa_join, dim3(a.rows, (p.query_heads + 3) / 4), dim3(256), s, a, "ctox_gqa_join_gfx950");
     return st;
 }

@@ -608,7 +608,7 @@ ctox_status ctox_hip_paged_gqa_device(ctox_hip_backend *backend, const float *d_
  * does nothing. Results of a row depend on the number of rows of the call in
  * the last bits (the K range may be split). workspace holds
  * ctox_hip_matrix_rows_workspace bytes, 16-byte aligned, and is free again when the
- * call's work on the stream is done. */
+ * call's work on the stream is done; one for the most rows serves calls of fewer. */
 typedef struct {
     const void *x;
     void *y;
@@ -711,7 +711,8 @@ ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *backend, uint8_t *d_q
  * exact, sums are 32 bits. Limits: head_dim 256, requests <= 4096, rows <= 2^20.
  * workspace holds ctox_hip_paged_gqa_rows_workspace bytes (of the same op; its device
  * pointers are not read), 16-byte aligned, and is free again when the call's work on
- * the stream is done. */
+ * the stream is done; one for the most rows, requests and max_rows (0 counts as rows)
+ * serves calls of fewer over the same heads. */
 typedef struct {
     const float *query;
     float *out;

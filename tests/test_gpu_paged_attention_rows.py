@@ -473,3 +473,37 @@ def test_a_peak_that_comes_late(hip, name, heads, kv_heads, requests, most):
         look_at(b, 0, 66, range(requests[0][1]), 60.0)
     b = Batch(61, requests, 16, heads, kv_heads, q2=old, edit=edit)
     b.check(b.run(hip, max_rows=most))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(24, 4), (6, 1), (4, 4), (34, 1), (1024, 512)])
+def test_a_workspace_for_many_rows_serves_fewer(hip, heads, kv_heads):
+    """Its size does not fall with rows, requests or max_rows."""
+    import ctox_hip as ch
+    say(f"case rows attention workspace {heads}/{kv_heads}")
+    b4, b2 = 2 * kv_heads * 4 * 34, 2 * kv_heads * 4 * 18
+    params = ch.PagedGqaParams(heads, kv_heads, HD, 0, 16, 8, 2 * kv_heads * HD, b2, b4, 16 * b2, 16 * b4, 1 / 16.0)
+
+    def size(rows, requests, most):
+        return hip.paged_gqa_rows_workspace(ch.PagedGqaRows(*[1 << 16] * 7, rows=rows, requests=requests, params=params,
+                                                            max_rows=most))
+    rows = [0, 1, 2, 3, 5, 6, 16, 17, 32, 33, 100, 500, 511, 512, 513, 2000, 2700, 2731, 4096, 10923, 100000]
+    requests = [1, 2, 3, 32, 511, 512, 513, 4096]
+    most = [1, 2, 3, 5, 6, 16, 17, 32, 33, 500, 0]
+    got = np.array([[[size(r, q, x) for x in most] for q in requests] for r in rows])
+    for axis in range(3):
+        assert (np.diff(got, axis=axis) >= 0).all(), axis
+
+
+def test_one_workspace_for_a_prompt_and_its_chunks(hip):
+    say("case rows attention workspace reuse")
+    big = Batch(67, [(0, 700)], 16, 4, 4)
+    hold = big.op(hip)
+    need, ws = hold.workspace_bytes, big.ws
+    for requests, most in (([(0, 700)], 0), ([(300, 40)], 0), ([(700, 1)], 1), ([(100, 9)], 9), ([(90, 600)], 0)):
+        b = Batch(71, requests, 16, 4, 4, q2=old)
+        op = b.op(hip, max_rows=most)
+        op.bind_workspace(ws.data_ptr(), need)
+        hip.paged_gqa_rows_device(op, torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert bool((ws[-64:] == 0xEE).all())
+        b.check(b.d["out"].cpu().numpy())

@@ -312,3 +312,26 @@ def test_refusals_with_a_matrix(hip):
         m.dispatch_rows(p, 8, p + 4096, w, ws.numel())
     m.backend = hip
     other.close()
+
+
+@pytest.mark.parametrize("dtypes,n,cols", [([Q4], [16], 5120), ([Q2], [96], 17408), ([Q4], [1500], 4096), ([Q2, Q4], [64, 700], 2048),
+                                           ([Q4], [40], 448)])
+def test_a_workspace_for_many_rows_serves_fewer(hip, dtypes, n, cols):
+    import ctox_hip as ch
+    say(f"case rows product workspace {dtypes} {n} {cols}")
+    rng = np.random.default_rng(59)
+    m, d = build(hip, rng, dtypes, n, cols, s_in=False)
+    for xt in (ch.TensorDType.F32, ch.TensorDType.F16):
+        sizes = [m.rows_workspace(r, xt) for r in [*range(0, 1100), *range(1100, 20000, 37), *range(20000, 2 ** 20, 9973)]]
+        assert all(a <= b for a, b in zip(sizes, sizes[1:]))
+    most = 700
+    ws = torch.full((m.rows_workspace(most) + 64,), 0xAA, dtype=torch.uint8, device="cuda")
+    x = rng.standard_normal((most, cols)).astype(np.float32)
+    dx, y = torch.from_numpy(x).cuda(), torch.empty(most, sum(n), device="cuda")
+    for rows in (most, 1, 17, 64, 200, 333):
+        y.fill_(7.0)
+        m.dispatch_rows(dx.data_ptr(), rows, y.data_ptr(), ws.data_ptr(), ws.numel() - 64,
+                        stream=torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        check(y[:rows].cpu().numpy(), *expect(d, x[:rows], None), False)
+        assert bool((y[rows:] == 7.0).all()) and bool((ws[-64:] == 0xAA).all())
