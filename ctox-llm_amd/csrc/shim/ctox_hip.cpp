@@ -2925,6 +2925,21 @@ extern "C" ctox_status ctox_hip_matrix_rows_workspace(const ctox_hip_matrix *m, 
     return CTOX_OK;
 }
 
+extern "C" ctox_status ctox_hip_matrix_rows_tiling(const ctox_hip_matrix *m, size_t rows, int32_t x_dtype, size_t segment,
+                                                   uint32_t tiling[3]) {
+    if (!tiling) return fail(CTOX_ERR_SHAPE, "null argument");
+    if (!row_dtype(x_dtype)) return fail(CTOX_ERR_UNSUPPORTED_DTYPE, "activation dtype %d is not F32 or F16", x_dtype);
+    if (rows == 0 || rows > kMostRows) return fail(CTOX_ERR_SHAPE, "%zu rows outside 1..2^20", rows);
+    if (!m) return fail(CTOX_ERR_SHAPE, "null argument");
+    if (segment >= m->segments.size()) return fail(CTOX_ERR_SHAPE, "segment %zu of %zu", segment, m->segments.size());
+    const RowPlan p = row_plan((uint32_t)m->backend->cus, (uint32_t)rows, m->tiled[segment].rows,
+                               (uint32_t)(m->columns / kBlockLen), row_space(m, rows, x_dtype).parts);
+    tiling[0] = 32 * kRowShapes[p.shape].tt;
+    tiling[1] = 128 * kRowShapes[p.shape].rt;
+    tiling[2] = p.splits;
+    return CTOX_OK;
+}
+
 extern "C" ctox_status ctox_hip_matrix_dispatch_rows(ctox_hip_backend *b, const ctox_hip_matrix *m,
                                                      const ctox_matrix_rows *op, void *stream) {
     if (!op) return fail(CTOX_ERR_SHAPE, "null argument");

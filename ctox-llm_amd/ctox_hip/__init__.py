@@ -354,6 +354,7 @@ SIGNATURES = {
     "ctox_hip_kv_demote_device": (_I32, [_P, _P, _P, _SZ, _SZ, _P]),
     "ctox_hip_paged_gqa_device": (_I32, [_P, _P, _P, _P, _P, ctypes.POINTER(PagedGqaParams), _SZ, _P, _P]),
     "ctox_hip_matrix_rows_workspace": (_I32, [_P, _SZ, _I32, ctypes.POINTER(_SZ)]),
+    "ctox_hip_matrix_rows_tiling": (_I32, [_P, _SZ, _I32, _SZ, ctypes.POINTER(_U32)]),
     "ctox_hip_matrix_dispatch_rows": (_I32, [_P, _P, ctypes.POINTER(_MatrixRows), _P]),
     "ctox_hip_rope_axes_device": (_I32, [_P, ctypes.POINTER(RopeAxes), _P]),
     "ctox_hip_paged_plan_device": (_I32, [_P, ctypes.POINTER(PagedPlan), _P]),
@@ -489,6 +490,13 @@ class HipMatrix:
         _fit(64, rows)
         _check(load_library().ctox_hip_matrix_rows_workspace(self.handle, rows, int(x_dtype), ctypes.byref(n)))
         return n.value
+
+    def rows_tiling(self, rows: int, x_dtype: TensorDType = TensorDType.F32, segment: int = 0):
+        """(rows of x, outputs) of a workgroup's tile and parts of K of a dispatch_rows call of `rows` rows."""
+        t = (ctypes.c_uint32 * 3)()
+        _fit(64, rows, segment)
+        _check(load_library().ctox_hip_matrix_rows_tiling(self.handle, rows, int(x_dtype), segment, t))
+        return tuple(t)
 
     def dispatch_rows(self, d_x: int, rows: int, d_y: int, d_workspace: int, workspace_bytes: int,
                       d_residual: Optional[int] = None, x_dtype: TensorDType = TensorDType.F32,

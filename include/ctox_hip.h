@@ -621,6 +621,11 @@ typedef struct {
 ctox_status ctox_hip_matrix_rows_workspace(const ctox_hip_matrix *matrix, size_t rows, int32_t x_dtype, size_t *bytes);
 ctox_status ctox_hip_matrix_dispatch_rows(ctox_hip_backend *backend, const ctox_hip_matrix *matrix,
                                           const ctox_matrix_rows *op, void *stream);
+/* How such a call of `rows` (>= 1) rows takes segment `segment` of the matrix (0 of a
+ * pure one), for profiles and tests: tiling[0] rows of x and tiling[1] outputs a
+ * workgroup, tiling[2] parts of K. */
+ctox_status ctox_hip_matrix_rows_tiling(const ctox_hip_matrix *matrix, size_t rows, int32_t x_dtype, size_t segment,
+                                        uint32_t tiling[3]);
 
 /* Per-head (1 + w) RMS norm (Q/src/reference.rs:38-62, where its weight is
  * given) and rotary positions on up to 4 axes: for i < rotary_dim / 2 the

@@ -335,3 +335,33 @@ def test_a_workspace_for_many_rows_serves_fewer(hip, dtypes, n, cols):
         torch.cuda.synchronize()
         check(y[:rows].cpu().numpy(), *expect(d, x[:rows], None), False)
         assert bool((y[rows:] == 7.0).all()) and bool((ws[-64:] == 0xAA).all())
+
+
+# (rows of x, outputs) of a workgroup's tile, split K or not, parts of an activation -> a call that gets them:
+# rows and outputs that leave the last tiles part-filled.
+TILED = [((32, 128), False, 1, (33, 72, 128)), ((32, 128), False, 2, (33, 72, 128)), ((32, 128), True, 1, (33, 72, 2112)),
+         ((32, 128), True, 2, (33, 72, 2112)), ((64, 128), False, 1, (300, 17000, 128)),
+         ((64, 128), False, 2, (300, 17000, 128)), ((64, 128), True, 1, (6000, 72, 17408)),
+         ((64, 128), True, 2, (33, 10250, 17408)), ((128, 128), False, 1, (1500, 12300, 192)),
+         ((128, 128), False, 2, (1500, 12300, 192)), ((128, 128), True, 1, (4100, 1500, 17408)),
+         ((128, 128), True, 2, (9000, 520, 17408)), ((128, 256), False, 1, (4100, 17000, 128)),
+         ((128, 256), False, 2, (4100, 17000, 128)), ((128, 256), True, 1, (2050, 5000, 17408)),
+         ((128, 256), True, 2, (2050, 5000, 17408))]
+
+
+@pytest.mark.parametrize("dtype", [Q2, Q4])
+@pytest.mark.parametrize("tile,split,parts,size", TILED)
+def test_every_tile_shape(hip, dtype, tile, split, parts, size):
+    import ctox_hip as ch
+    say(f"case rows product tile={tile} split={split} parts={parts} dtype={dtype} {size}")
+    rows, n, cols = size
+    rng = np.random.default_rng(rows + n + cols + dtype)
+    m, d = build(hip, rng, [dtype], [n], cols, s_in=parts == 2, bias=True)
+    half = parts == 1
+    got = m.rows_tiling(rows, ch.TensorDType.F16 if half else ch.TensorDType.F32)
+    assert got[:2] == tile and (got[2] > 1) == split
+    x = rng.standard_normal((rows, cols), dtype=np.float32).astype(np.float16 if half else np.float32)
+    pick = np.unique(np.r_[0, 31, rows - 1 - np.arange(5), rng.integers(0, rows, 40)] % rows)
+    y = run(m, x)
+    check(y[pick], *expect(d, x[pick], None), False)
+    m.close()

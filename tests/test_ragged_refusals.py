@@ -205,3 +205,12 @@ def test_rows_product_numbers_that_do_not_fit_are_refused(over):
     if "rows" in over:
         with pytest.raises(ctox_hip.ShapeError, match="does not fit"):
             m.rows_workspace(over["rows"])
+
+
+def test_rows_tiling_refuses():
+    lib, t = ctox_hip.load_library(), (ctypes.c_uint32 * 3)()
+    for args, kind in (((5, 4, 0, None), ctox_hip.ShapeError), ((5, 1, 0, t), ctox_hip.UnsupportedDType),
+                       ((0, 4, 0, t), ctox_hip.ShapeError), (((1 << 20) + 1, 4, 0, t), ctox_hip.ShapeError),
+                       ((5, 4, 0, t), ctox_hip.ShapeError)):
+        with pytest.raises(kind):
+            ctox_hip._check(lib.ctox_hip_matrix_rows_tiling(None, *args))
