@@ -507,3 +507,59 @@ def test_one_workspace_for_a_prompt_and_its_chunks(hip):
         torch.cuda.synchronize()
         assert bool((ws[-64:] == 0xEE).all())
         b.check(b.d["out"].cpu().numpy())
+
+
+def check_some(b, got, picks):
+    """The rows (request, row, head) of `picks` against float64, all others finite, rows past the end untouched."""
+    G, e, last = b.H // b.KV, 2.0 ** -24, None
+    assert (got[b.M:] == 7.0).all() and np.isfinite(got[:b.M]).all()
+    for r, t, h in sorted(picks):
+        if r != last:
+            last, (K, V, present) = r, b.token_values(r)
+        see = present & (np.arange(b.tokens[r]) <= b.requests[r][0] + t)
+        k, v, q = K[see, h // G], V[see, h // G], b.q[b.starts[r] + t, h].astype(np.float64)
+        s, S = k @ q / 16.0, (np.abs(k) @ np.abs(q) / 16.0).max()
+        p = np.exp(s - s.max())
+        p /= p.sum()
+        tol = (p @ np.abs(v)) * e * (4 * (144 * S + 4 * max(1, 2 * S)) + 72 + 3 * see.sum())
+        assert (np.abs(got[b.starts[r] + t, h] - p @ v) <= tol).all(), (r, t, h)
+
+
+@pytest.mark.parametrize("count", [65, 257, 300, 512, 513, 1025, 4096])
+@pytest.mark.parametrize("kind", ["one row", "few rows", "mixed"])
+def test_many_requests(hip, count, kind):
+    """More requests than a workgroup's lanes (256 or 512) and than are cut (512), a third of them without rows, one of a
+    long context: its token axis is cut up to 512 requests."""
+    say(f"case rows attention requests={count} {kind}")
+    rng = np.random.default_rng(count)
+    most = {"one row": 1, "few rows": 4, "mixed": 40}[kind]
+    rows = rng.integers(1, most + 1, count) if kind != "mixed" else np.where(np.arange(count) % 37 == 5, 40, 1)
+    rows[rng.permutation(count)[:count // 3]] = 0
+    cached = rng.integers(0, 30, count)
+    for r in (count - 3, count // 2):
+        rows[r], cached[r] = max(1, most), 2500
+    b = Batch(count, list(zip(cached.tolist(), rows.tolist())), 16, 6, 1, q2=old, pad=2)
+    got = b.run(hip, max_rows=most)
+    picks = [(r, t, h) for r in (*rng.permutation(count)[:60].tolist(), 0, count - 3, count // 2, count - 1)
+             for t in range(b.n[r]) for h in (0, 5)]
+    check_some(b, got, picks)
+
+
+def test_a_prompt_whose_tiles_fill_the_chip(hip):
+    """Two workgroups a CU or more from query tiles alone: token ranges are not cut and nothing is joined."""
+    say("case rows attention uncut prompt")
+    b = Batch(73, [(30, 2075), (5, 1), (0, 33)], 16, 32, 16, q2=lambda r, p: p % 4 == 1, pad=3)
+    got = b.run(hip)
+    rng = np.random.default_rng(5)
+    picks = [(0, int(t), int(h)) for t in (*range(3), *range(2070, 2075), *rng.integers(0, 2075, 40))
+             for h in rng.permutation(32)[:8]]
+    check_some(b, got, picks + [(1, 0, h) for h in range(32)] + [(2, t, h) for t in (0, 31, 32) for h in range(32)])
+
+
+def test_one_prompt_alone_whose_tiles_fill_the_chip(hip):
+    say("case rows attention uncut prompt of one request")
+    b = Batch(79, [(0, 1100)], 24, 120, 60, q2=lambda r, p: p % 4 == 1)
+    got = b.run(hip)
+    rng = np.random.default_rng(7)
+    check_some(b, got, [(0, int(t), int(h)) for t in (0, 1, 62, 63, 64, 1098, 1099, *rng.integers(0, 1100, 20))
+                        for h in rng.permutation(120)[:6]])
