@@ -140,9 +140,9 @@ struct GrItem {
     bool ok;
 };
 
-// The item `want` (by_item), or the items of request `want`. All threads get the answer.
+// The request of item `want`. All threads get the answer.
 template <int NT>
-__device__ __forceinline__ GrItem gr_find(const GqaRowsArgs &a, bool few, uint32_t range, uint32_t want, bool by_item,
+__device__ __forceinline__ GrItem gr_find(const GqaRowsArgs &a, bool few, uint32_t range, uint32_t want,
                                           GrScratch &L) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (threadIdx.x == 0) L.found[0] = 0xffffffffu;
@@ -170,12 +170,12 @@ __device__ __forceinline__ GrItem gr_find(const GqaRowsArgs &a, bool few, uint32
             if (w < (int)wave) at += L.scan[w];
             before += L.scan[w];
         }
-        if (n && (by_item ? want >= at && want - at < n : want == r)) {
+        if (n && want >= at && want - at < n) {
             L.found[0] = r;
             L.found[1] = at;
             L.found[2] = ranges;
         }
-        if (by_item && want < before) break;
+        if (want < before) break;
     }
     __syncthreads();
     GrItem it{L.found[0], want - L.found[1], L.found[1], L.found[2], L.found[0] != 0xffffffffu};
@@ -409,7 +409,7 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t li = lane & 31, h = lane >> 5, qsub = wave % QS, ts = wave / QS;
     const uint32_t range = gr_range<NT>(a, FEW, L.u.scratch);
-    const GrItem it = gr_find<NT>(a, FEW, range, blockIdx.x, true, L.u.scratch);
+    const GrItem it = gr_find<NT>(a, FEW, range, blockIdx.x, L.u.scratch);
     if (!it.ok) return;
     if (it.local == 0 && threadIdx.x == 0) {
         a.cuts[2 * it.request] = it.base;
@@ -821,7 +821,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t li = lane & 15, g = lane >> 4;
     const uint32_t range = gr_range<256>(a, true, L.u.scratch);
-    const GrItem it = gr_find<256>(a, true, range, blockIdx.x, true, L.u.scratch);
+    const GrItem it = gr_find<256>(a, true, range, blockIdx.x, L.u.scratch);
     if (!it.ok) return;
     if (it.local == 0 && threadIdx.x == 0) {
         a.cuts[2 * it.request] = it.base;
