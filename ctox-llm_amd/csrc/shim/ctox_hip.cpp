@@ -2686,6 +2686,9 @@ bool aligned(const void *p, size_t n) { return (uintptr_t)p % n == 0; }
 
 // rows * stride + the last row, in values: within what 63 bits address.
 bool spans(uint64_t rows, uint64_t stride) { return stride < (1ull << 30) && rows < (1ull << 32); }
+
+// A launch's first axis holds less than 2^32 threads.
+constexpr uint64_t kMostGroups256 = (1ull << 24) - 1, kMostGroups512 = (1ull << 23) - 1;
 }  // namespace
 
 extern "C" ctox_status ctox_hip_rope_axes_device(ctox_hip_backend *b, const ctox_rope_axes *op, void *stream) {
@@ -2697,6 +2700,7 @@ extern "C" ctox_status ctox_hip_rope_axes_device(ctox_hip_backend *b, const ctox
     if (hd > 1024 || op->axes == 0 || op->axes > 4 || op->q_heads > 32767 || op->k_heads > 32767 ||
         op->q_heads + op->k_heads == 0)
         return fail(CTOX_ERR_SHAPE, "rope heads or axes are empty or too large");
+    if (op->rows > kMostGroups256) return fail(CTOX_ERR_SHAPE, "%u rope rows reach 2^24", op->rows);
     if ((op->q_norm || op->k_norm) && (!std::isfinite(op->eps) || !(op->eps > 0.0f)))
         return fail(CTOX_ERR_SHAPE, "norm epsilon is invalid");
     for (uint32_t i = 0; op->axis_of_pair && i < rd / 2; i++)
@@ -2788,7 +2792,7 @@ extern "C" ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *b, uint8_t
     if (page_tokens == 0 || page_tokens * token_bytes > q4_page_bytes || q4_page_bytes % 4 ||
         (uint64_t)q4_slots * page_tokens > 0xffffffffull)
         return fail(CTOX_ERR_SHAPE, "KV tokens do not fit the Q4 page");
-    if (rows > 0x7fffffffu || !spans(rows, key_stride) || !spans(rows, value_stride))
+    if (rows > kMostGroups256 || !spans(rows, key_stride) || !spans(rows, value_stride))
         return fail(CTOX_ERR_SHAPE, "KV append is too large");
     if (!b || !d_q4_pages || !d_keys || !d_values || !d_slots) return fail(CTOX_ERR_SHAPE, "null argument");
     if (!aligned(d_q4_pages, 4)) return fail(CTOX_ERR_SHAPE, "the Q4 pool needs 4-byte alignment");
@@ -3045,6 +3049,10 @@ ctox_status check_gqa_rows(const ctox_paged_gqa_rows *op) {
         return fail(CTOX_ERR_SHAPE, "attention of %u requests outside 1..%d", op->requests, CTOX_PLAN_REQUESTS);
     if (op->rows > kMostRows || op->rows * (p.query_heads / p.key_value_heads) > 0x3fffffffu)
         return fail(CTOX_ERR_SHAPE, "attention rows are too many");
+    // (an item a query tile of 128, request and KV head, and as many again as the chip holds twice)
+    const uint64_t tiles = (op->rows * (p.query_heads / p.key_value_heads) + 127) / 128;
+    if ((tiles + std::min<uint64_t>(op->requests, op->rows)) * p.key_value_heads > kMostGroups512 - 4096)
+        return fail(CTOX_ERR_SHAPE, "attention rows of so many heads exceed a launch");
     return CTOX_OK;
 }
 

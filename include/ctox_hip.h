@@ -636,8 +636,8 @@ ctox_status ctox_hip_matrix_rows_tiling(const ctox_hip_matrix *matrix, size_t ro
  * axis_of_pair). The angle is formed in 64 bits, so positions of any size
  * keep a 32-bit result. Row t, head h starts at t * row_stride +
  * h * head_stride values; an output may be its own input (same strides) and
- * otherwise must not overlap an input. head_dim <= 1024, rotary_dim even and
- * <= min(head_dim, 512). Rows from *row_count on (where it is given) are
+ * otherwise must not overlap an input. rows < 2^24, head_dim <= 1024, rotary_dim even
+ * and <= min(head_dim, 512). Rows from *row_count on (where it is given) are
  * left as they are. */
 typedef struct {
     const float *q, *k;            /* k may be NULL with k_heads = 0 */
@@ -690,7 +690,7 @@ ctox_status ctox_hip_paged_plan_device(ctox_hip_backend *backend, const ctox_pag
  * slots[t] % page_tokens of Q4 page slots[t] / page_tokens (the page of
  * q4_page_bytes at that slot of the pool). Rows whose slot is not below
  * q4_slots * page_tokens (CTOX_NO_SLOT) are skipped. Two rows must not share a
- * slot. */
+ * slot. rows < 2^24. */
 ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *backend, uint8_t *d_q4_pages, const float *d_keys,
                                          size_t key_stride, const float *d_values, size_t value_stride,
                                          const uint32_t *d_slots, size_t rows, size_t component_values,
@@ -713,7 +713,9 @@ ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *backend, uint8_t *d_q
  * absolute 2^-40 of that) and 21 bits of each probability times value scale (of a small
  * one an absolute step that adds up to less than the roundings of a 32-bit sum over the
  * row's tokens, whatever the value scales of other tokens), the cached codes are
- * exact, sums are 32 bits. Limits: head_dim 256, requests <= 4096, rows <= 2^20.
+ * exact, sums are 32 bits. Limits: head_dim 256, requests <= 4096, rows <= 2^20,
+ * (ceil(rows * query_heads / key_value_heads / 128) + requests) * key_value_heads
+ * below 2^23 - 4096.
  * workspace holds ctox_hip_paged_gqa_rows_workspace bytes (of the same op; its device
  * pointers are not read), 16-byte aligned, and is free again when the call's work on
  * the stream is done; one for the most rows, requests and max_rows (0 counts as rows)

@@ -214,3 +214,15 @@ def test_rows_tiling_refuses():
                        ((5, 4, 0, t), ctox_hip.ShapeError)):
         with pytest.raises(kind):
             ctox_hip._check(lib.ctox_hip_matrix_rows_tiling(None, *args))
+
+
+def test_more_rows_than_a_launch_holds_are_refused():
+    """A grid holds less than 2^32 threads along its first axis; the calls' workgroups of 256 or 512 reach it."""
+    assert rope(rows=(1 << 24) - 1) == "null argument"
+    assert "rows" in rope(rows=1 << 24)
+    assert append(rows=(1 << 24) - 1) == "null argument"
+    assert "too large" in append(rows=1 << 24)
+    wide = dict(query_heads=8192, key_value_heads=8192, combined_values=8192 * 512, q2_token_bytes=8192 * 144,
+                q4_token_bytes=8192 * 272, q2_page_bytes=16 * 8192 * 144, q4_page_bytes=16 * 8192 * 272)
+    assert attention(wide, rows=100000) == "null argument"
+    assert "rows" in attention(wide, rows=1 << 17)
