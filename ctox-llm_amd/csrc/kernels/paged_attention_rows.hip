@@ -643,8 +643,8 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
                 ev[b] = now;
             }
         }
-        // A value block without a finite scale makes its dims no numbers for every query that sees the token, and
-        // does not count for the others (its scale is 0).
+        // A value block without a finite scale makes its dims no numbers for every query that sees the token, however
+        // small its probability, and does not count for the others (its scale is 0).
         const uint32_t mark = __builtin_amdgcn_readfirstlane(marks.x | marks.y | marks.z | marks.w);
         wide |= mark >> 1;
         if (mark & 1) {
@@ -655,7 +655,10 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
                 const uint32_t bad = bads[b] >> (4 * h);
                 bool any = false;
 #pragma unroll
-                for (int r = 0; r < 16; r++) any |= (bad >> (8 * (r >> 2) + (r & 3)) & 1) && s[r] != 0.0f;
+                for (int r = 0; r < 16; r++) {
+                    const int c = 8 * (r >> 2) + (r & 3);
+                    any |= (bad >> c & 1) && c <= lim - (int32_t)(t * 32 + 4 * h);
+                }
                 any |= __shfl_xor((int)any, 32) != 0;
 #pragma unroll
                 for (int c = 0; c < 2; c++)
@@ -1000,7 +1003,10 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
                 const uint32_t bad = bads[b] >> (4 * g);
                 bool any = false;
 #pragma unroll
-                for (int r = 0; r < 8; r++) any |= (bad >> (16 * (r >> 2) + (r & 3)) & 1) && p[r] != 0.0f;
+                for (int r = 0; r < 8; r++) {
+                    const int c = 16 * (r >> 2) + (r & 3);
+                    any |= (bad >> c & 1) && c <= lim - (int32_t)(t * 32 + 4 * g);
+                }
                 any |= __shfl_xor((int)any, 16) != 0;
                 any |= __shfl_xor((int)any, 32) != 0;
 #pragma unroll

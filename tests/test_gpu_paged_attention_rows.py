@@ -563,3 +563,25 @@ def test_one_prompt_alone_whose_tiles_fill_the_chip(hip):
     rng = np.random.default_rng(7)
     check_some(b, got, [(0, int(t), int(h)) for t in (0, 1, 62, 63, 64, 1098, 1099, *rng.integers(0, 1100, 20))
                         for h in rng.permutation(120)[:6]])
+
+
+@pytest.mark.parametrize("name,heads,kv_heads,requests,most", KERNELS)
+@pytest.mark.parametrize("kind", [0x7c00, 0x7e00])
+def test_non_finite_values_of_a_hardly_weighted_token(hip, name, heads, kv_heads, requests, most, kind):
+    """A probability below f32's range is not 0: the rows that see a token of infinite values get no numbers, the rows
+    before it keep theirs."""
+    say(f"case rows attention non-finite value {name} {kind:x}")
+    n = sum(requests[0])
+
+    def edit(b):
+        look_at(b, 0, 3, range(requests[0][1]), 400.0)
+        value_scales(b, 0, [n - 1], 0.5)
+    clean = Batch(83, requests, 16, heads, kv_heads, q2=old, edit=edit)
+    want, tol = clean.expect()
+    b = Batch(83, requests, 16, heads, kv_heads, q2=old, edit=edit)
+    value_scales(b, 0, [n - 1], np.uint16(kind).view(np.float16))
+    got = b.run(hip, max_rows=most)
+    last = requests[0][1] - 1
+    assert not np.isfinite(got[last]).any()
+    keep = [i for i in range(b.M) if i != last]
+    assert (np.abs(got[keep] - want[keep]) <= tol[keep]).all()
