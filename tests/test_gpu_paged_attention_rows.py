@@ -585,3 +585,34 @@ def test_non_finite_values_of_a_hardly_weighted_token(hip, name, heads, kv_heads
     assert not np.isfinite(got[last]).any()
     keep = [i for i in range(b.M) if i != last]
     assert (np.abs(got[keep] - want[keep]) <= tol[keep]).all()
+
+
+@pytest.mark.parametrize("name,heads,kv_heads,requests,most", KERNELS)
+def test_more_rows_than_tokens_and_rows_in_front(hip, name, heads, kv_heads, requests, most):
+    """Requests whose lengths say fewer tokens than rows (the first rows see nothing), or none; rows that lie before the
+    first request's are left alone."""
+    say(f"case rows attention short {name}")
+    n = [r[1] for r in requests]
+    b = Batch(89, [(0, n[0]), (0, n[1]), (40, n[1])], 16, heads, kv_heads, q2=old, pad=5)
+    op = b.op(hip, max_rows=most)
+    short = n[0] // 2
+    b.d["tokens"].copy_(dev(np.array([short, 0, b.tokens[2]], np.int32)))
+    b.d["starts"].add_(3)
+    hip.paged_gqa_rows_device(op, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    got = b.d["out"].cpu().numpy()
+    assert (got[:3] == 7.0).all() and (got[b.M + 3:] == 7.0).all()
+    got, q = got[3:b.M + 3], b.q[3:b.M + 3].astype(np.float64)
+    assert (got[:n[0] - short] == 0).all() and (got[n[0]:n[0] + n[1]] == 0).all()
+    G, e = heads // kv_heads, 2.0 ** -24
+    for r, first, tokens in ((0, 0, short), (2, n[0] + n[1], b.tokens[2])):
+        K, V, _ = b.token_values(r)
+        for t in range(max(0, n[r if r == 0 else 1] - tokens), n[r if r == 0 else 1]):
+            seen = tokens - n[r if r == 0 else 1] + t + 1
+            for h in range(heads):
+                k, v, x = K[:seen, h // G], V[:seen, h // G], q[first + t, h]
+                s, S = k @ x / 16.0, (np.abs(k) @ np.abs(x) / 16.0).max()
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                tol = (p @ np.abs(v)) * e * (4 * (144 * S + 4 * max(1, 2 * S)) + 72 + 3 * seen)
+                assert (np.abs(got[first + t, h] - p @ v) <= tol).all(), (r, t, h)

@@ -401,3 +401,19 @@ def test_append_past_four_gibibytes(hip):
     for t, at in ((0, 2 * page - 1), (1, page)):
         want[at] = np.frombuffer(pk.quantize_values(np.concatenate([k[t], v[t]]), pk.Q4), np.uint8)
     assert np.array_equal(pool[-2 * page * tb:].cpu().numpy().reshape(2 * page, tb), want)
+
+
+@pytest.mark.parametrize("hd,rd", [(256, 64), (96, 30)])
+def test_rope_axes_of_keys_alone(hip, hd, rd):
+    import ctox_hip
+    say(f"case rope keys alone hd={hd}")
+    rng = np.random.default_rng(hd)
+    x = rng.standard_normal((11, 3, hd)).astype(np.float32)
+    pos = rng.integers(0, 5000, (11, 1)).astype(np.uint32)
+    dx, dp = dev(x), dev(pos.view(np.int32))
+    hip.rope_axes_device(ctox_hip.RopeAxes(d_q=None, d_k=dx.data_ptr(), d_positions=dp.data_ptr(), rows=11, q_heads=0,
+                                           k_heads=3, head_dim=hd, rotary_dim=rd, theta=1e4),
+                         torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    want, mag = rope64(x.astype(np.float64), None, pos.astype(np.float64), np.zeros(rd // 2, int), rd, 1e4, 1e-6)
+    assert (np.abs(dx.cpu().numpy() - want) <= 26 * 2.0 ** -24 * mag).all()

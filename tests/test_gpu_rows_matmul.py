@@ -365,3 +365,13 @@ def test_every_tile_shape(hip, dtype, tile, split, parts, size):
     y = run(m, x)
     check(y[pick], *expect(d, x[pick], None), False)
     m.close()
+
+
+@pytest.mark.parametrize("dtype", [Q2, Q4])
+def test_f16_activations_below_the_normal_range(hip, dtype):
+    say(f"case rows product f16 subnormals dtype={dtype}")
+    rng = np.random.default_rng(61)
+    m, d = build(hip, rng, [dtype], [70], 256, s_in=False, bias=False)
+    x = (rng.standard_normal((40, 256)) * 10.0 ** rng.uniform(-7.5, -4, (40, 1))).astype(np.float16)
+    x[7] = np.uint16(1).view(np.float16)
+    check(run(m, x), *expect(d, x, None), False)
