@@ -35,10 +35,11 @@
 // Loads of the next tile are under way during this one, its page descriptors one tile before that.
 //
 // Measured, 24 query heads over 4 KV heads, pages of 16 tokens, old ones of 2-bit codes: a prompt of 4096 tokens
-// 575 us (206 G score and value operations, each twice for the two parts: 717 TFLOP/s of products, where a large
-// f16 matrix product of the card reaches 1108), 512 rows behind 32768 tokens 1034 us, 32 decoded tokens over up to 8192
-// cached ones 68 us (1.26 TB/s). Bound by vector operations (about 830 a tile and wave, 57 % of all issue,
-// beside 31 % of the matrix units' time): 352 of them turn codes into f16 operands, 192 split P s_v.
+// 584 us (206 G score and value operations, each twice for the two parts: 706 TFLOP/s of products, where a large
+// f16 matrix product of the card reaches 1108), 512 rows behind 32768 tokens 1038 us, 32 decoded tokens over up to 8192
+// cached ones 70 us (1.23 TB/s). Bound by vector operations (about 840 a tile and wave, 56 % of all issue,
+// beside 30 % of the matrix units' time): 352 of them turn codes into f16 operands, 192 split P s_v. All 256 registers
+// are taken; the 7 (128 queries) and 8 (32) spilled ones are read outside the tile loop and in its rare branches.
 // With four subtiles K is stored while V is in use and V while K is, so that one buffer each is
 // enough beside the 128 KiB of queries, and LDS operands are read one step ahead of the products.
 #include <hip/hip_runtime.h>

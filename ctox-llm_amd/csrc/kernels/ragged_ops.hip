@@ -7,7 +7,8 @@
 //    its nearest integer), where 32 would leave an error of position * 2^-24 turns; only the
 //    remainder, at most half a turn, goes to the 32-bit sine and cosine. A workgroup makes one
 //    row's table once and its four waves take the heads in turn, one head a wave. 4096 rows of
-//    28 heads of 256, three axes: 69 us, 3.4 TB/s; 16 rows: 7 us, the launch.
+//    28 heads of 256, three axes: 69 us, 3.4 TB/s (51 us where the same rows come from the Infinity
+//    Cache); 16 rows: 7 us, the launch.
 //  * ctox_paged_plan_gfx950: page descriptors, slot map and row offsets of a batch from the
 //    requests' cached and added lengths (PagedKvCache::push's page bookkeeping,
 //    Q/src/kv_cache.rs:394-429, for many requests at once). One launch: every workgroup makes

@@ -19,9 +19,9 @@
 //    in use) and take RT 32-row weight tiles each; weights come from the
 //    tiled copy (kernel_args.h) into registers, one block ahead, and are unpacked
 //    there once for all TT tiles.
-//    Measured: 4096 rows, 5120 x 17408 Q2, f32 (two parts) 1.55 ms with 0.2 ms of it staging: 944
-//    TFLOP/s of f16 products, against 1108 of the card's large product; 777 rows, 17408 x 5120 Q4 321 us;
-//    2048 rows, 5120 x 6144 Q4, f16 194 us (664 TFLOP/s); 16 rows, 14336 x 5120 Q4 24 us (1.6 TB/s).
+//    Measured, from card to card: 4096 rows, 5120 x 17408 Q2, f32 (two parts) 1.55-1.64 ms with 0.2 ms of it staging:
+//    890-944 TFLOP/s of f16 products, against 1108 of the card's large product; 777 rows, 17408 x 5120 Q4 321-327 us;
+//    2048 rows, 5120 x 6144 Q4, f16 194-201 us (641-664 TFLOP/s); 16 rows, 14336 x 5120 Q4 24-25 us (1.6 TB/s).
 //  * ctox_rows_reduce_gfx950: adds the partial sums of a split K in order and
 //    applies the epilogue.
 #include <hip/hip_runtime.h>

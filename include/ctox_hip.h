@@ -603,9 +603,9 @@ ctox_status ctox_hip_paged_gqa_device(ctox_hip_backend *backend, const float *d_
  * the dense row length; likewise y and residual). x_dtype and y_dtype are
  * CTOX_DTYPE_F32 or CTOX_DTYPE_F16; residual (NULL = none) has y's type and may be
  * y itself with y's stride. y must not overlap x. Products keep 22 bits of an
- * f32 activation (of an f16 one times s_in likewise; without s_in all of it) and
- * add up in 32 bits; an f16 result is rounded once. rows <= 2^20; rows = 0
- * does nothing. Results of a row depend on the number of rows of the call in
+ * f32 activation (of one below 2^-17 of its row's largest an absolute 2^-40 of that;
+ * of an f16 one times s_in likewise; without s_in all of it) and add up in 32 bits;
+ * an f16 result is rounded once. rows <= 2^20; rows = 0 does nothing. Results of a row depend on the number of rows of the call in
  * the last bits (the K range may be split). workspace holds
  * ctox_hip_matrix_rows_workspace bytes, 16-byte aligned, and is free again when the
  * call's work on the stream is done; one for the most rows serves calls of fewer. */
@@ -633,8 +633,9 @@ ctox_status ctox_hip_matrix_rows_tiling(const ctox_hip_matrix *matrix, size_t ro
  * positions[t][axis_of_pair[i]] * theta^(-2 i / rotary_dim)
  * (apply_partial_rope, Q/src/reference.rs:115-155, is the case of one axis;
  * time / height / width sections, in blocks or interleaved, are tables of
- * axis_of_pair). The angle is formed in 64 bits, so positions of any size
- * keep a 32-bit result. Row t, head h starts at t * row_stride +
+ * axis_of_pair). The angle is formed in 64 bits: positions up to 2^26
+ * keep a 32-bit result, larger ones an angle within position * 2^-51 (beside its
+ * rounding to 32 bits). Row t, head h starts at t * row_stride +
  * h * head_stride values; an output may be its own input (same strides) and
  * otherwise must not overlap an input. rows < 2^24, head_dim <= 1024, rotary_dim even
  * and <= min(head_dim, 512). Rows from *row_count on (where it is given) are
@@ -701,7 +702,7 @@ ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *backend, uint8_t *d_q
  * request r's rows row_starts[r] .. row_starts[r + 1] - 1 are its last cached
  * tokens of tokens[r], the first of its n rows sees tokens 0 .. tokens[r] - n,
  * each next one more. query and out are [rows][query_heads][256], dense,
- * 16-byte aligned; rows before row_starts[0] or from row_starts[requests] on are left as
+ * 16-byte aligned (out must not overlap an input); rows before row_starts[0] or from row_starts[requests] on are left as
  * they are. descriptors is [requests][params.page_count]; tokens outside
  * every page's [first_token, first_token + tokens) are absent. A row that sees no token
  * gets zeros. Lengths are read on the device: a plan's row_starts and
