@@ -23,6 +23,9 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <memory>
+#include <mutex>
+#include <new>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -236,9 +239,9 @@ struct ctox_hip_matrix {
     // Per segment: the same rows rewritten into the tiled layout (kernel_args.h).
     using Tiled = TiledCopy;
     std::vector<Tiled> tiled;
-    // Row products: [parts - 1][32-row tiles of x - 1]: partial sums' bytes that any call of up to so many
-    // whole tiles may need; the last entry holds for more.
-    std::vector<uint64_t> row_partials[2];
+    // Row products: [parts - 1][32-row tiles of x - 1]: as row_partials_up_to keeps them.
+    mutable std::once_flag row_once[2];
+    mutable std::unique_ptr<uint64_t[]> row_partials[2];
 };
 
 namespace {
@@ -1115,8 +1118,6 @@ ctox_status tile_segments(ctox_hip_backend *b, ctox_hip_matrix *m) {
     return CTOX_OK;
 }
 
-void note_row_partials(ctox_hip_matrix *m);
-
 ctox_status prepare_impl(ctox_hip_backend *b, const ctox_fused_matvec *op, ctox_hip_matrix **out) {
     size_t blocks;
     ctox_status st = validate_matvec(op, false, &blocks);
@@ -1153,7 +1154,6 @@ ctox_status prepare_impl(ctox_hip_backend *b, const ctox_fused_matvec *op, ctox_
         return st;
     }
     m->activation = (uint32_t)op->activation;
-    note_row_partials(m);
     *out = m;
     return CTOX_OK;
 }
@@ -2817,6 +2817,8 @@ extern "C" ctox_status ctox_hip_kv_append_q4_device(ctox_hip_backend *b, uint8_t
 }
 
 namespace {
+constexpr uint64_t kMostRows = 1u << 20;
+
 // Shape and K split of one segment's row product, the cheapest by this count: workgroups a CU (between their
 // mean and the whole number that the fullest CU has: idle CUs leave the others a higher clock), times the
 // 32 x 128 tiles and blocks of one, times how much longer a shape takes for the same tile area; a CU
@@ -2856,33 +2858,46 @@ RowPlan row_plan(uint32_t cus, uint32_t rows, uint32_t n, uint32_t blocks, uint3
 // Partial sums' bytes of a call of `rows` rows, at least. Within a 32-row tile of rows a plan's cost is a line in
 // rows, steeper with more splits, so the cheapest plan never splits more than at the tile's first row: with that
 // many splits the bytes do not fall from row to row.
-uint64_t row_partial_bytes(const ctox_hip_matrix *m, uint32_t rows, uint32_t parts) {
+uint64_t row_partial_bytes(const ctox_hip_matrix *m, uint32_t rows, uint32_t parts, bool exact) {
     const uint32_t cus = (uint32_t)m->backend->cus, blocks = (uint32_t)(m->columns / kBlockLen);
     const uint32_t first = (rows - 1) / 32 * 32 + 1;
     uint64_t most = 0;
     for (const ctox_quant_segment &seg : m->segments) {
         const uint32_t n = (uint32_t)(seg.row_end - seg.row_start);
-        const uint32_t splits = std::max(row_plan(cus, first, n, blocks, parts).splits, row_plan(cus, rows, n, blocks, parts).splits);
+        uint32_t splits = row_plan(cus, first, n, blocks, parts).splits;
+        // (the plan that runs, in case two plans' costs are equal but for a rounding)
+        if (exact) splits = std::max(splits, row_plan(cus, rows, n, blocks, parts).splits);
         if (splits > 1) most = std::max<uint64_t>(most, (uint64_t)splits * rows * n * sizeof(float));
     }
     return most;
 }
 
-// From one tile to the next a plan may go from many splits to few, so the matrix keeps the most up to each count of
-// tiles (up to where no segment's K can be split any more: row_plan's bound on workgroups).
-void note_row_partials(ctox_hip_matrix *m) {
+// The same of any call of up to `tiles` whole 32-row tiles of x: from one tile to the next a plan may go from many
+// splits to few. The matrix keeps the most up to each count from its first such call on, up to where no segment's K
+// can be split any more (row_plan's bound on workgroups): 0.02 ms once for 17408 rows, 0.3 for 1024, 1.6 for 128 or fewer.
+uint64_t row_partials_up_to(const ctox_hip_matrix *m, uint64_t tiles, uint32_t parts) {
     size_t least = m->rows;
     for (const ctox_quant_segment &seg : m->segments) least = std::min(least, seg.row_end - seg.row_start);
     const RowShape wide = kRowShapes[3];
     const uint64_t groups = std::max<uint64_t>(1, (least + 128 * wide.rt - 1) / (128 * wide.rt));
-    const uint64_t tiles = m->columns / kBlockLen < 8 ? 0 : (4 * (uint64_t)m->backend->cus / groups + 1) * wide.tt;
-    for (uint32_t parts = 1; parts <= 2; parts++) {
+    const uint64_t all = m->columns / kBlockLen < 8
+                             ? 0 : std::min<uint64_t>((4 * (uint64_t)m->backend->cus / groups + 1) * wide.tt, kMostRows / 32);
+    tiles = std::min(tiles, all);
+    if (!tiles) return 0;
+    auto fill = [&](uint64_t count, uint64_t *kept) {
         uint64_t most = 0;
-        for (uint64_t t = 1; t <= std::min<uint64_t>(tiles, (1u << 20) / 32); t++) {
-            most = std::max(most, row_partial_bytes(m, (uint32_t)(32 * t), parts));
-            m->row_partials[parts - 1].push_back(most);
+        for (uint64_t t = 1; t <= count; t++) {
+            most = std::max(most, row_partial_bytes(m, (uint32_t)(32 * t), parts, false));
+            if (kept) kept[t - 1] = most;
         }
-    }
+        return most;
+    };
+    std::unique_ptr<uint64_t[]> &kept = m->row_partials[parts - 1];
+    std::call_once(m->row_once[parts - 1], [&] {
+        kept.reset(new (std::nothrow) uint64_t[all]);
+        if (kept) fill(all, kept.get());
+    });
+    return kept ? kept[tiles - 1] : fill(tiles, nullptr);
 }
 
 // Where a row product's workspace holds what. No call of fewer rows needs more.
@@ -2905,10 +2920,8 @@ RowSpace row_space(const ctox_hip_matrix *m, uint64_t rows, int32_t x_dtype) {
         for (const ctox_quant_segment &seg : m->segments) any = any || (seg.dtype == CTOX_DTYPE_Q4B64) == (q4 == 1);
         w.staged[q4] = take(any ? one : 0);
     }
-    const std::vector<uint64_t> &before = m->row_partials[w.parts - 1];
-    const size_t whole = std::min<size_t>((rows - 1) / 32, before.size());
-    uint64_t partial = row_partial_bytes(m, (uint32_t)rows, w.parts);
-    if (whole) partial = std::max(partial, before[whole - 1]);
+    const uint64_t partial = std::max(row_partial_bytes(m, (uint32_t)rows, w.parts, true),
+                                      row_partials_up_to(m, (rows - 1) / 32, w.parts));
     w.exps = take(w.parts == 2 ? rows * sizeof(int32_t) : 0);
     w.partial = take(partial);
     w.total = at;
@@ -2916,7 +2929,6 @@ RowSpace row_space(const ctox_hip_matrix *m, uint64_t rows, int32_t x_dtype) {
 }
 
 bool row_dtype(int32_t d) { return d == CTOX_DTYPE_F32 || d == CTOX_DTYPE_F16; }
-constexpr uint64_t kMostRows = 1u << 20;
 }  // namespace
 
 extern "C" ctox_status ctox_hip_matrix_rows_workspace(const ctox_hip_matrix *m, size_t rows, int32_t x_dtype,

@@ -375,3 +375,27 @@ def test_f16_activations_below_the_normal_range(hip, dtype):
     x = (rng.standard_normal((40, 256)) * 10.0 ** rng.uniform(-7.5, -4, (40, 1))).astype(np.float16)
     x[7] = np.uint16(1).view(np.float16)
     check(run(m, x), *expect(d, x, None), False)
+
+
+@pytest.mark.parametrize("kinds", [("F32", "F16Le"), ("F16Le", "F16Le"), ("F32", "F32")])
+@pytest.mark.parametrize("half", [False, True])
+def test_scale_types_of_mixed_segments(hip, kinds, half):
+    import ctox_hip as ch
+    say(f"case rows product scales {kinds} half={half}")
+    rng = np.random.default_rng(67)
+    cols, rows_each, dtypes = 448, (41, 90), (Q2, Q4)
+    parts = [pack(rng, d, r, cols) for d, r in zip(dtypes, rows_each)]
+    types = dict(F32=np.float32, F16Le=np.float16)
+    si = rng.uniform(0.5, 1.5, cols).astype(types[kinds[0]])
+    so = rng.uniform(0.5, 1.5, 131).astype(types[kinds[1]])
+    bias = (rng.standard_normal(131) * 0.1).astype(np.float32)
+    segs = [ch.QuantSegment(0, 0, 41, ch.TensorDType(Q2), 0, parts[0].size),
+            ch.QuantSegment(1, 41, 131, ch.TensorDType(Q4), parts[0].size, parts[1].size)]
+    m = hip.prepare(ch.FusedMatVec(ch.TensorDType.MixedQ2Q4B64, np.concatenate([p.reshape(-1) for p in parts]), 131, cols,
+                                   segments=segs, s_in=getattr(ch.ScaleSlice, kinds[0])(si),
+                                   s_out=getattr(ch.ScaleSlice, kinds[1])(so), bias=bias, activation=ch.Activation.Silu))
+    d = dict(W=np.concatenate([values(p, t) for p, t in zip(parts, dtypes)]), s_in=si.astype(np.float64), s_out=so.astype(np.float64),
+             bias=bias, silu=True)
+    for rows in (5, 80):
+        x = rng.standard_normal((rows, cols)).astype(np.float16 if half else np.float32)
+        check(run(m, x, y_half=half), *expect(d, x, None), half)
