@@ -239,7 +239,7 @@ def _inputs_tree(c, seed):
             "tokens": _int32([a + n for a, n in zip(cached, nodes)]), "rows": rows,
             "masks": torch.zeros(rows, dtype=torch.int64, device=DEV),
             "positions": torch.zeros(rows, dtype=torch.int32, device=DEV),
-            "status": torch.zeros(2, dtype=torch.int32, device=DEV)}
+            "depths": torch.zeros(c["requests"], dtype=torch.int32, device=DEV)}
 
 
 def _mask_words(forest):
@@ -344,7 +344,7 @@ def _inputs_pages(c, seed):
             "free4": torch.zeros(n4, dtype=torch.int32, device=DEV), "free2": torch.zeros(n2, dtype=torch.int32, device=DEV),
             "free_counts": torch.zeros(2, dtype=torch.int32, device=DEV), "most": max(nodes),
             "source": _int32([rng.choice(going) for _ in ended]), "target": _int32(ended),
-            "commit_status": torch.zeros(2, dtype=torch.int32, device=DEV),
+            "commit_status": torch.zeros(R, dtype=torch.int32, device=DEV),
             "fork_status": torch.zeros(2, dtype=torch.int32, device=DEV), "token_bytes": token_bytes}
 
 
@@ -419,7 +419,7 @@ def _keep(s):
     if op == "tree":
         s["call"] = ctox.TreePlan(
             d_row_starts=ptr("row_starts"), d_tokens=ptr("tokens"), d_parents=ptr("parents"), d_masks=ptr("masks"),
-            d_positions=ptr("positions"), d_status=ptr("status"), requests=R, rows=s["rows"])
+            d_positions=ptr("positions"), d_depths=ptr("depths"), requests=R, rows=s["rows"])
     elif op == "attention":
         KV, page, cv = c["kv_heads"], c["page"], c["kv_heads"] * HD
         b4, b2 = s["q4"].shape[1], s["q2"].shape[1]
@@ -466,8 +466,8 @@ def _keep(s):
             d_dt_bias=ptr("dt_bias"), d_state_in=ptr("state"), d_row_starts=ptr("row_starts"),
             d_parents=ptr("parents"), d_out=ptr("out"), d_counts=ptr("counts"), d_path=ptr("path"),
             d_conv_out=ptr("windows_out"), d_state_out=ptr("state_out"), proj_stride=s["proj"].shape[1],
-            a_off=C + H * dv, b_off=C + H * dv + H, requests=R, rows=s["proj"].shape[0], heads=H, key_heads=KH,
-            key_dim=dk, value_dim=dv, kernel=c["kernel"], blocked=c["blocked"])
+            a_off=C + H * dv, b_off=C + H * dv + H, requests=R, rows=s["proj"].shape[0], max_rows=s["most"], heads=H,
+            key_heads=KH, key_dim=dk, value_dim=dv, kernel=c["kernel"], blocked=c["blocked"])
         s["workspace"] = _bytes(hip().gdn_tree_workspace(s["call"]))
         s["call"].bind_workspace(s["workspace"].data_ptr(), s["workspace"].numel())
 
@@ -477,7 +477,7 @@ def _run_own(s):
     op = c["op"]
     if op == "tree":
         hip().tree_plan_device(s["call"], st)
-        return {k: s[k] for k in ("masks", "positions", "status")}
+        return {k: s[k] for k in ("masks", "positions", "depths")}
     if op == "attention":
         cv = c["kv_heads"] * HD
         hip().kv_append_q4_device(s["q4"].data_ptr(), s["keys"].data_ptr(), s["values"].data_ptr(),
@@ -551,10 +551,10 @@ def _plain_tree(s):
     bits = torch.where(seen, torch.ones(1, dtype=torch.int64, device=DEV) << torch.arange(NODES, device=DEV), 0)
     past = s["tokens"].long() - (starts[1:] - starts[:-1])
     zero = torch.zeros_like(depth)
-    deepest = torch.where(inside, depth + 1, zero).amax()
+    depths = torch.zeros_like(past).scatter_reduce(0, r, torch.where(inside, depth + 1, zero), "amax")
     return {"masks": torch.where(inside, bits.sum(1), zero),
             "positions": torch.where(inside, past[r] + depth, zero).to(torch.int32),
-            "status": torch.stack([torch.zeros_like(deepest), deepest]).to(torch.int32)}
+            "depths": depths.to(torch.int32)}
 
 
 def _plain_attention(s):
@@ -709,7 +709,7 @@ def _plain_pages(s):
     zero = torch.zeros_like(found[0])
     return {"pool": s["pool"], "descriptors": desc, "live": length.to(torch.int32), "free4": lists[0],
             "free2": lists[1], "free_counts": torch.stack(found).to(torch.int32),
-            "commit_status": torch.stack([zero, live.sum()]).to(torch.int32),
+            "commit_status": torch.zeros(R, dtype=torch.int32, device=DEV),
             "fork_status": torch.stack([zero, (part > 0).sum()]).to(torch.int32)}
 
 
