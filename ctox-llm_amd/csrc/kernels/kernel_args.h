@@ -684,6 +684,146 @@ struct GqaRowsArgs {
     uint32_t page_magic;     // token / page_tokens = token * page_magic >> page_shift, tokens < 2^30
     uint32_t page_shift;
     uint32_t pad;
+    const uint64_t *masks;   // trees: [rows], bit j: the row sees its request's node j
+};
+
+// Trees of drafted tokens (tree_ops.hip, tree_verify.hip, gated_delta_tree.hip).
+#define CTOX_TREE_NODES 64
+#define CTOX_TREE_RELEASE 0xffffffffu
+#define CTOX_TREE_FAILED 0xfffffffeu
+#define CTOX_TREE_POOLS 64  // layers of one commit or fork
+struct TreePlanArgs {
+    const uint32_t *row_starts;  // [requests + 1]
+    const uint32_t *tokens;      // [requests]
+    const uint32_t *parents;     // [rows]
+    uint64_t *masks;             // [rows]
+    uint32_t *positions;         // [rows]
+    uint32_t *depths;            // [requests]
+    uint32_t requests;
+    uint32_t rows;
+};
+
+struct PagedCommitArgs {
+    uint8_t *pools[CTOX_TREE_POOLS];
+    PagedKvDesc *desc;           // [requests][max_pages]
+    const uint32_t *row_starts;
+    const uint32_t *tokens;
+    const uint32_t *counts;      // [requests]: kept nodes, or CTOX_TREE_RELEASE
+    const uint32_t *path;        // [rows]
+    uint32_t *new_tokens;        // [requests]
+    uint32_t *status;            // [requests]
+    uint64_t q4_page_bytes;
+    uint32_t requests;
+    uint32_t rows;
+    uint32_t max_pages;
+    uint32_t page_tokens;
+    uint32_t q4_slots;
+    uint32_t token_bytes;
+    uint32_t layers;
+    uint32_t unit;               // bytes of an access: 16 or 4
+};
+
+struct FreeSlotsArgs {
+    const PagedKvDesc *desc;
+    const uint32_t *tokens;      // [requests]
+    uint32_t *used;              // workspace: a bit a slot, the Q4 pool's words, then the Q2 pool's
+    uint32_t *lists[2];          // Q4, Q2
+    uint32_t *counts;            // [2]
+    uint32_t slots[2];
+    uint32_t words[2];
+    uint32_t requests;
+    uint32_t max_pages;
+    uint32_t page_tokens;
+    uint32_t pad;
+};
+
+struct PagedForkArgs {
+    uint8_t *pools[CTOX_TREE_POOLS];
+    PagedKvDesc *desc;
+    uint32_t *tokens;            // [requests]
+    const uint32_t *sources;     // [forks]
+    const uint32_t *targets;     // [forks]
+    const uint32_t *free_slots;
+    const uint32_t *free_count;  // one word
+    uint32_t *status;            // [2]
+    uint64_t q4_page_bytes;
+    uint32_t requests;
+    uint32_t forks;
+    uint32_t max_pages;
+    uint32_t page_tokens;
+    uint32_t q4_slots;
+    uint32_t token_bytes;
+    uint32_t layers;
+    uint32_t unit;
+};
+
+struct TreeStat {                // of a part of a row
+    double sum;                  // of exp((x - top) / T); greedy: the largest logit's token
+    float top;
+    uint32_t bad;                // holds a logit that is no number or +inf
+};
+struct TreeVerifyArgs {
+    const float *target;         // [rows][target_stride]
+    const float *draft;          // [rows][draft_stride] or NULL
+    const uint32_t *inverse;     // [vocab]: a token's place in a draft row, or NULL
+    const uint32_t *tokens;      // [rows]
+    const uint32_t *parents;     // [rows]
+    const uint32_t *row_starts;
+    const float *accept;         // [rows]
+    const float *sample;         // [requests]
+    uint32_t *counts;            // [requests]
+    uint32_t *path;              // [rows]
+    uint32_t *next;              // [requests]
+    TreeStat *stats;             // [rows][parts]
+    TreeStat *draft_stats;       // [rows][draft_parts]
+    double *rest;                // [width][rows][parts]
+    uint64_t target_stride;
+    uint64_t draft_stride;
+    double inv_t;
+    uint32_t requests;
+    uint32_t rows;
+    uint32_t vocab;
+    uint32_t draft_vocab;
+    uint32_t parts;              // at most 64
+    uint32_t draft_parts;
+    uint32_t part;               // tokens of one, a multiple of 4096
+    uint32_t draft_part;
+    uint32_t width;              // children that are offered
+    uint32_t round;
+    uint32_t without;            // siblings drawn without replacement
+    uint32_t greedy;
+};
+
+struct GdnTreeArgs {
+    const float *proj;           // [rows][proj_stride]
+    const float *conv_w;         // [channels][kernel]
+    const float *conv_in;        // [requests][conv_stride]
+    float *conv_out;
+    const float *a_log;          // [heads]
+    const float *dt_bias;
+    const float *state_in;       // [requests][state_stride]
+    float *state_out;
+    const uint32_t *row_starts;
+    const uint32_t *parents;     // [rows]
+    const uint32_t *counts;      // [requests]
+    const uint32_t *path;        // [rows]
+    float *out;                  // [rows][heads][value_dim]
+    float *keys;                 // workspace: [rows][key_heads][128], dims i at (i % 16) * 8 + i / 16
+    float *deltas;               // workspace: [rows][heads][value_dim]
+    float *decays;               // workspace: [rows][heads], log decays
+    uint64_t proj_stride;
+    uint64_t conv_stride;
+    uint64_t state_stride;
+    uint32_t a_off;
+    uint32_t b_off;
+    uint32_t requests;
+    uint32_t rows;
+    uint32_t heads;
+    uint32_t key_heads;
+    uint32_t key_dim;
+    uint32_t value_dim;
+    uint32_t kernel;
+    uint32_t blocked;
 };
 
 // Decode engine helpers (engine_ops.hip).

@@ -11,6 +11,9 @@
 //    32 queries a workgroup.
 //  * ctox_gqa_few16_gfx950: the same for batches in which no request has more than 16 (decoded tokens).
 //  * ctox_gqa_join_gfx950: joins the parts of a split token range.
+//  * ctox_gqa_tree_rows_gfx950, _few_, _few16_: the same three for trees of drafted tokens. A request's rows are the
+//    at most 64 nodes of a tree, the last cached tokens; a row sees the tokens before them and the nodes
+//    that its 64-bit mask names (GrTree).
 //
 // Which workgroup takes what is decided on the device from row_starts and tokens, so the
 // host needs no lengths and a captured launch stays right for other lengths: every workgroup
@@ -50,6 +53,15 @@
 typedef float gr_v16 __attribute__((ext_vector_type(16)));
 
 #define GR_MOVE 6.0f  // base-2 slack before the running maximum moves
+
+// What a query of a tree sees of tile t's 32 tokens, one bit each: what lies before the nodes, and the nodes of its
+// mask (bit j: token past + j). Masks are kept in LDS, only the last tiles need them.
+__device__ __forceinline__ uint32_t gr_tree_word(uint64_t mask, uint32_t t, int32_t past) {
+    const int32_t d = (int32_t)(t * 32) - past;
+    if (d <= -32) return ~0u;
+    if (d < 0) return (uint32_t)(mask << -d) | ((1u << -d) - 1);
+    return d < 64 ? (uint32_t)(mask >> d) : 0u;
+}
 
 struct __attribute__((packed, aligned(2))) GrBytes16 {
     uint32_t w[4];
@@ -382,7 +394,7 @@ struct GrLoad {
 // ---------------------------------------------------------------------------
 // LDS of a workgroup of QS query subtiles x TS token shares: queries and the shares' tiles (while
 // tiles run; the joined sums afterwards).
-template <int QS, int TS>
+template <int QS, int TS, bool TREE>
 struct GrLds {
     union {
         struct {
@@ -399,14 +411,15 @@ struct GrLds {
         GrScratch scratch;
     } u;
     float stat[QS * TS][2][32];  // (maximum, denominator) of a publishing wave
+    uint64_t mask[TREE ? 32 * QS : 1];  // of a query
 };
 
-template <int QS, int TS>
+template <int QS, int TS, bool TREE>
 __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     constexpr int NT = 64 * QS * TS;
     constexpr bool FEW = QS == 1;
     constexpr uint32_t kQueries = 32 * QS;
-    __shared__ GrLds<QS, TS> L;
+    __shared__ GrLds<QS, TS, TREE> L;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t li = lane & 31, h = lane >> 5, qsub = wave % QS, ts = wave / QS;
     const uint32_t range = gr_range<NT>(a, FEW, L.u.scratch);
@@ -424,7 +437,7 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     const uint32_t kvh = it.local % a.kv_heads, rest = it.local / a.kv_heads;
     const uint32_t part = rest % it.ranges, q0 = (nqt - 1 - rest / it.ranges) * kQueries;
     const int32_t past = (int32_t)rq.tokens - (int32_t)rq.rows;  // tokens before the first row
-    const int32_t seen = past + (int32_t)(min(q0 + kQueries - 1, nq - 1) / a.group) + 1;
+    const int32_t seen = TREE ? (int32_t)rq.tokens : past + (int32_t)(min(q0 + kQueries - 1, nq - 1) / a.group) + 1;
     const uint32_t vis = (uint32_t)max(seen, 0);
     const uint32_t units = (vis + 32 * TS - 1) / (32 * TS), per = (units + it.ranges - 1) / it.ranges;
     // Tiles of 32 tokens: this wave's are t0, t0 + TS, ... below t1 (a last one may have no tokens).
@@ -433,7 +446,8 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     const uint32_t qi = q0 + 32 * qsub + li;  // this lane's query
     const bool valid = qi < nq;
     const int32_t lim = valid ? past + (int32_t)(qi / a.group) : -1;
-    const int32_t lim0 = past + (int32_t)(min(q0 + 32 * qsub, nq - 1) / a.group);  // the subtile's first query's
+    // (the subtile's first query's; in a tree the last token that all see)
+    const int32_t lim0 = TREE ? past - 1 : past + (int32_t)(min(q0 + 32 * qsub, nq - 1) / a.group);
     const uint32_t qrow = valid ? qi / a.group : 0, qg = valid ? qi - qrow * a.group : 0;
     const size_t qat = ((size_t)(rq.row0 + qrow) * a.query_heads + kvh * a.group + qg) * 256;
 
@@ -499,6 +513,7 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
             L.u.t.q[qsub][1][s][lane] = hi;
         }
     }
+    if (TREE && ts == 0 && h == 0) L.mask[32 * qsub + li] = valid ? a.masks[rq.row0 + qrow] : 0;
     if (QS == 1) __syncthreads();
 
     gr_v16 o[4][2];  // [dim block][even, odd dims]
@@ -586,12 +601,13 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
         }
         // ---- masks: a tile that ends past the first query's last token, or has absent tokens ----
         if ((int32_t)((t + 1) * 32) - 1 > lim0 || ld.here != ~0u) {
-            const uint32_t on = ld.here >> (4 * h);
+            const uint32_t word = TREE ? gr_tree_word(L.mask[32 * qsub + li], t, past) : ~0u;
+            const uint32_t on = (ld.here & word) >> (4 * h);
             const int32_t left = lim - (int32_t)(t * 32 + 4 * h);  // tokens up to this one
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int c = 8 * (r >> 2) + (r & 3);
-                if (c > left || !(on >> c & 1)) s[r] = -INFINITY;
+                if ((!TREE && c > left) || !(on >> c & 1)) s[r] = -INFINITY;
             }
         }
         // ---- softmax ----
@@ -651,14 +667,15 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
         if (mark & 1) {
             const uint4 bad4 = *(const uint4 *)L.u.t.bad[ts];
             const uint32_t bads[4] = {bad4.x, bad4.y, bad4.z, bad4.w};
+            const uint32_t word = TREE ? gr_tree_word(L.mask[32 * qsub + li], t, past) : ~0u;
 #pragma unroll
             for (int b = 0; b < 4; b++) {
-                const uint32_t bad = bads[b] >> (4 * h);
+                const uint32_t bad = (bads[b] & word) >> (4 * h);
                 bool any = false;
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int c = 8 * (r >> 2) + (r & 3);
-                    any |= (bad >> c & 1) && c <= lim - (int32_t)(t * 32 + 4 * h);
+                    any |= (bad >> c & 1) && (TREE || c <= lim - (int32_t)(t * 32 + 4 * h));
                 }
                 any |= __shfl_xor((int)any, 32) != 0;
 #pragma unroll
@@ -795,8 +812,10 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
             d[1] = make_float4(x[4 * j + 2] * f, y[4 * j + 2] * f, x[4 * j + 3] * f, y[4 * j + 3] * f);
         }
 }
-extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_rows_gfx950(GqaRowsArgs a) { gqa_rows<4, 2>(a); }
-extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few_gfx950(GqaRowsArgs a) { gqa_rows<1, 4>(a); }
+extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_rows_gfx950(GqaRowsArgs a) { gqa_rows<4, 2, false>(a); }
+extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few_gfx950(GqaRowsArgs a) { gqa_rows<1, 4, false>(a); }
+extern "C" __global__ __launch_bounds__(512, 2) void ctox_gqa_tree_rows_gfx950(GqaRowsArgs a) { gqa_rows<4, 2, true>(a); }
+extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_tree_few_gfx950(GqaRowsArgs a) { gqa_rows<1, 4, true>(a); }
 
 // ---------------------------------------------------------------------------
 // at most 16 queries a KV head
@@ -820,7 +839,8 @@ struct GrLds16 {
     float stat[2][2][16];
 };
 
-extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRowsArgs a) {
+template <bool TREE>
+__device__ __forceinline__ void gqa_few16(const GqaRowsArgs &a) {
     __shared__ GrLds16 L;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t li = lane & 15, g = lane >> 4;
@@ -841,6 +861,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
     const int32_t lim = valid ? past + (int32_t)(li / a.group) : -1;
     const uint32_t qrow = valid ? li / a.group : 0, qg = valid ? li - qrow * a.group : 0;
     const size_t qat = ((size_t)(rq.row0 + qrow) * a.query_heads + kvh * a.group + qg) * 256;
+    const uint64_t mask = TREE && valid ? a.masks[rq.row0 + qrow] : 0;
 
     GrLoad<4> ld{a, it.request, kvh, vis, t1, lane, 0};
     ld.desc_load(t0);
@@ -943,14 +964,15 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
         }
         // ---- masks ----
         if ((int32_t)((t + 1) * 32) - 1 > past || ld.here != ~0u) {
-            const uint32_t on = ld.here >> (4 * g);
+            const uint32_t word = TREE ? gr_tree_word(mask, t, past) : ~0u;
+            const uint32_t on = (ld.here & word) >> (4 * g);
             const int32_t left = lim - (int32_t)(t * 32 + 4 * g);  // tokens up to this one
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int c = 16 * n + r;
-                    if (c > left || !(on >> c & 1)) s[n][r] = -INFINITY;
+                    if ((!TREE && c > left) || !(on >> c & 1)) s[n][r] = -INFINITY;
                 }
         }
         // ---- softmax ----
@@ -999,14 +1021,15 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
         if (mark & 1) {
             const uint4 bad4 = *(const uint4 *)L.u.t.bad[wave];
             const uint32_t bads[4] = {bad4.x, bad4.y, bad4.z, bad4.w};
+            const uint32_t word = TREE ? gr_tree_word(mask, t, past) : ~0u;
 #pragma unroll
             for (int b = 0; b < 4; b++) {
-                const uint32_t bad = bads[b] >> (4 * g);
+                const uint32_t bad = (bads[b] & word) >> (4 * g);
                 bool any = false;
 #pragma unroll
                 for (int r = 0; r < 8; r++) {
                     const int c = 16 * (r >> 2) + (r & 3);
-                    any |= (bad >> c & 1) && c <= lim - (int32_t)(t * 32 + 4 * g);
+                    any |= (bad >> c & 1) && (TREE || c <= lim - (int32_t)(t * 32 + 4 * g));
                 }
                 any |= __shfl_xor((int)any, 16) != 0;
                 any |= __shfl_xor((int)any, 32) != 0;
@@ -1116,6 +1139,9 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
             d[1] = make_float4(x[2] * f, y[2] * f, x[3] * f, y[3] * f);
         }
 }
+
+extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRowsArgs a) { gqa_few16<false>(a); }
+extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_tree_few16_gfx950(GqaRowsArgs a) { gqa_few16<true>(a); }
 
 // ---------------------------------------------------------------------------
 // join: grid (rows, quarters of the query heads), 64 lanes x 4 dims

@@ -163,7 +163,11 @@ struct ctox_hip_backend {
                   prep_x = nullptr, finite = nullptr, gather = nullptr, topk_part = nullptr, topk_final = nullptr, stream_read = nullptr,
                   write_segments = nullptr, rope_axes[2] = {}, plan = nullptr, kv_append = nullptr,
                   rows_max[2] = {}, rows_stage[2] = {}, rows_stage_few[2] = {}, rows_reduce = nullptr,
-                  gqa_rows = nullptr, gqa_few = nullptr, gqa_few16 = nullptr, gqa_join = nullptr;
+                  gqa_rows = nullptr, gqa_few = nullptr, gqa_few16 = nullptr, gqa_join = nullptr,
+                  gqa_tree_rows = nullptr, gqa_tree_few = nullptr, gqa_tree_few16 = nullptr, tree_plan = nullptr,
+                  paged_commit = nullptr, free_clear = nullptr, free_mark = nullptr, free_list = nullptr,
+                  paged_fork = nullptr, tree_stats = nullptr, tree_rest = nullptr, tree_walk = nullptr,
+                  gdn_tree[3] = {}, gdn_tree_commit = nullptr;
     // Row products: [q4][parts - 1][shape], shapes as kRowShapes.
     hipFunction_t rows_mul[2][2][4] = {};
     // Batch-1 slice kernels per dtype [Q2, Q4]: [0] walks the slices, [n]
@@ -963,7 +967,15 @@ extern "C" ctox_status ctox_hip_backend_create(int device, ctox_hip_backend **ou
                {&b->rows_stage_few[1], "ctox_rows_stage_few_vec_gfx950"},
                {&b->rows_reduce, "ctox_rows_reduce_gfx950"},
                {&b->gqa_rows, "ctox_gqa_rows_gfx950"}, {&b->gqa_few, "ctox_gqa_few_gfx950"},
-               {&b->gqa_few16, "ctox_gqa_few16_gfx950"}, {&b->gqa_join, "ctox_gqa_join_gfx950"}};
+               {&b->gqa_few16, "ctox_gqa_few16_gfx950"}, {&b->gqa_join, "ctox_gqa_join_gfx950"},
+               {&b->gqa_tree_rows, "ctox_gqa_tree_rows_gfx950"}, {&b->gqa_tree_few, "ctox_gqa_tree_few_gfx950"},
+               {&b->gqa_tree_few16, "ctox_gqa_tree_few16_gfx950"}, {&b->tree_plan, "ctox_tree_plan_gfx950"},
+               {&b->paged_commit, "ctox_paged_commit_gfx950"}, {&b->free_clear, "ctox_free_clear_gfx950"},
+               {&b->free_mark, "ctox_free_mark_gfx950"}, {&b->free_list, "ctox_free_list_gfx950"},
+               {&b->paged_fork, "ctox_paged_fork_gfx950"}, {&b->tree_stats, "ctox_tree_stats_gfx950"},
+               {&b->tree_rest, "ctox_tree_rest_gfx950"}, {&b->tree_walk, "ctox_tree_walk_gfx950"},
+               {&b->gdn_tree[0], "ctox_gdn_tree1_gfx950"}, {&b->gdn_tree[1], "ctox_gdn_tree2_gfx950"},
+               {&b->gdn_tree[2], "ctox_gdn_tree4_gfx950"}, {&b->gdn_tree_commit, "ctox_gdn_tree_commit_gfx950"}};
     for (auto &f : fns) {
         if (le != hipSuccess) break;
         le = hipModuleGetFunction(f.f, b->module, f.name);
@@ -3122,7 +3134,9 @@ extern "C" ctox_status ctox_hip_paged_gqa_rows_workspace(const ctox_hip_backend 
     return CTOX_OK;
 }
 
-extern "C" ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *b, const ctox_paged_gqa_rows *op, void *stream) {
+namespace {
+// masks: the rows are trees' nodes.
+ctox_status gqa_rows_impl(ctox_hip_backend *b, const ctox_paged_gqa_rows *op, const uint64_t *masks, void *stream) {
     if (ctox_status st = check_gqa_rows(op)) return st;
     if (!b || !op->q2_pages || !op->q4_pages || !op->descriptors || !op->row_starts || !op->tokens ||
         (op->rows && (!op->query || !op->out)))
@@ -3175,13 +3189,433 @@ extern "C" ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *b, const
     while (l < 31 && (1u << l) < p.page_tokens) l++;
     a.page_shift = 30 + l;
     a.page_magic = (uint32_t)(((1ull << a.page_shift) + p.page_tokens - 1) / p.page_tokens);
+    a.masks = masks;
+    const hipFunction_t rows = masks ? b->gqa_tree_rows : b->gqa_rows;
+    const hipFunction_t few = g.few == 16 ? (masks ? b->gqa_tree_few16 : b->gqa_few16) : masks ? b->gqa_tree_few : b->gqa_few;
     OnDevice on(b);
     hipStream_t s = (hipStream_t)stream;
     ctox_status st = CTOX_OK;
-    if (g.wide) st = launch(b->gqa_rows, dim3(g.items), dim3(512), s, a, "ctox_gqa_rows_gfx950");
-    if (!st && g.few)
-        st = launch(g.few == 16 ? b->gqa_few16 : b->gqa_few, dim3(g.few_items), dim3(256), s, a, "ctox_gqa_few_gfx950");
+    if (g.wide) st = launch(rows, dim3(g.items), dim3(512), s, a, "ctox_gqa_rows_gfx950");
+    if (!st && g.few) st = launch(few, dim3(g.few_items), dim3(256), s, a, "ctox_gqa_few_gfx950");
     if (!st && g.cut && (g.few || g.split))
         st = launch(b->gqa_join, dim3(a.rows, (p.query_heads + 3) / 4), dim3(256), s, a, "ctox_gqa_join_gfx950");
     return st;
+}
+}  // namespace
+
+extern "C" ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *b, const ctox_paged_gqa_rows *op, void *stream) {
+    return gqa_rows_impl(b, op, nullptr, stream);
+}
+
+// ======================================================================
+// trees of drafted tokens
+// ======================================================================
+namespace {
+ctox_status check_gqa_tree(const ctox_paged_gqa_tree *op, ctox_paged_gqa_rows *rows) {
+    if (!op) return fail(CTOX_ERR_SHAPE, "null argument");
+    *rows = op->rows;
+    if (rows->max_rows > CTOX_TREE_NODES)
+        return fail(CTOX_ERR_SHAPE, "trees of %u nodes, %d at most", rows->max_rows, CTOX_TREE_NODES);
+    if (rows->max_rows == 0) rows->max_rows = CTOX_TREE_NODES;
+    return CTOX_OK;
+}
+
+// Geometry that commits and forks share; *unit: bytes of an access.
+ctox_status check_pools(uint8_t *const *pools, uint32_t layers, uint32_t requests, uint32_t max_pages,
+                        uint32_t page_tokens, uint32_t q4_slots, uint32_t token_bytes, uint32_t page_bytes,
+                        uint8_t *out[CTOX_TREE_POOLS], uint32_t *unit) {
+    if (requests == 0 || requests > CTOX_PLAN_REQUESTS)
+        return fail(CTOX_ERR_SHAPE, "%u requests outside 1..%d", requests, CTOX_PLAN_REQUESTS);
+    if (layers == 0 || layers > CTOX_TREE_POOLS) return fail(CTOX_ERR_SHAPE, "%u layers outside 1..%d", layers, CTOX_TREE_POOLS);
+    if (page_tokens == 0 || max_pages == 0 || (uint64_t)max_pages * page_tokens > 0xffffffffull ||
+        (uint64_t)requests * max_pages > 0xffffffffull || (uint64_t)q4_slots * page_tokens > 0xffffffffull)
+        return fail(CTOX_ERR_SHAPE, "page geometry is empty or too large");
+    if (token_bytes == 0 || token_bytes % 4 || token_bytes > (1u << 24) || (uint64_t)page_tokens * token_bytes > page_bytes || page_bytes % 4)
+        return fail(CTOX_ERR_SHAPE, "KV tokens do not fit the Q4 page");
+    if (!pools) return fail(CTOX_ERR_SHAPE, "null argument");
+    bool wide = token_bytes % 16 == 0 && page_bytes % 16 == 0;
+    for (uint32_t i = 0; i < layers; i++) {
+        if (!pools[i]) return fail(CTOX_ERR_SHAPE, "null argument");
+        if (!aligned(pools[i], 4)) return fail(CTOX_ERR_SHAPE, "the Q4 pools need 4-byte alignment");
+        wide = wide && aligned(pools[i], 16);
+        out[i] = pools[i];
+    }
+    *unit = wide ? 16 : 4;
+    return CTOX_OK;
+}
+}  // namespace
+
+extern "C" ctox_status ctox_hip_tree_plan_device(ctox_hip_backend *b, const ctox_tree_plan *op, void *stream) {
+    if (!op) return fail(CTOX_ERR_SHAPE, "null argument");
+    if (op->requests == 0 || op->requests > CTOX_PLAN_REQUESTS)
+        return fail(CTOX_ERR_SHAPE, "plan of %u requests outside 1..%d", op->requests, CTOX_PLAN_REQUESTS);
+    if (op->rows > kMostGroups256) return fail(CTOX_ERR_SHAPE, "%u rows reach 2^24", op->rows);
+    if (!b || !op->row_starts || !op->tokens || !op->depths || (op->rows && (!op->parents || !op->masks || !op->positions)))
+        return fail(CTOX_ERR_SHAPE, "null argument");
+    if (!aligned(op->masks, 8)) return fail(CTOX_ERR_SHAPE, "masks need 8-byte alignment");
+    TreePlanArgs a{op->row_starts, op->tokens, op->parents, op->masks, op->positions, op->depths, op->requests, op->rows};
+    OnDevice on(b);
+    return launch(b->tree_plan, dim3((op->requests + 3) / 4), dim3(256), (hipStream_t)stream, a, "ctox_tree_plan_gfx950");
+}
+
+extern "C" ctox_status ctox_hip_paged_gqa_tree_workspace(const ctox_hip_backend *b, const ctox_paged_gqa_tree *op,
+                                                         size_t *bytes) {
+    if (!bytes) return fail(CTOX_ERR_SHAPE, "null argument");
+    *bytes = 0;
+    ctox_paged_gqa_rows rows;
+    if (ctox_status st = check_gqa_tree(op, &rows)) return st;
+    return ctox_hip_paged_gqa_rows_workspace(b, &rows, bytes);
+}
+
+extern "C" ctox_status ctox_hip_paged_gqa_tree_device(ctox_hip_backend *b, const ctox_paged_gqa_tree *op, void *stream) {
+    ctox_paged_gqa_rows rows;
+    if (ctox_status st = check_gqa_tree(op, &rows)) return st;
+    if (!op->masks) return fail(CTOX_ERR_SHAPE, "null argument");
+    if (!aligned(op->masks, 8)) return fail(CTOX_ERR_SHAPE, "masks need 8-byte alignment");
+    return gqa_rows_impl(b, &rows, op->masks, stream);
+}
+
+namespace {
+ctox_status check_verify_tree(const ctox_verify_tree *op) {
+    if (!op) return fail(CTOX_ERR_SHAPE, "null argument");
+    if (op->requests == 0 || op->requests > CTOX_PLAN_REQUESTS)
+        return fail(CTOX_ERR_SHAPE, "verification of %u requests outside 1..%d", op->requests, CTOX_PLAN_REQUESTS);
+    if (op->rows > 65535) return fail(CTOX_ERR_SHAPE, "%u rows reach 2^16", op->rows);
+    if (op->vocab == 0 || op->vocab > 0x7fffffffu || op->max_children == 0 || op->max_children > CTOX_TREE_NODES)
+        return fail(CTOX_ERR_SHAPE, "vocabulary or children are empty or too large");
+    if (!std::isfinite(op->temperature) || op->temperature < 0.0f)
+        return fail(CTOX_ERR_INVALID_ARTIFACT, "temperature must be finite and non-negative");
+    if (op->draft && (op->draft_vocab == 0 || op->draft_vocab > op->vocab || (!op->draft_inverse && op->draft_vocab != op->vocab)))
+        return fail(CTOX_ERR_SHAPE, "a restricted draft vocabulary needs its inverse");
+    if ((op->target_stride && op->target_stride < op->vocab) || (op->draft && op->draft_stride && op->draft_stride < op->draft_vocab) ||
+        !spans(op->rows, op->target_stride) || !spans(op->rows, op->draft_stride))
+        return fail(CTOX_ERR_SHAPE, "logit rows overlap or are too far apart");
+    return CTOX_OK;
+}
+// Parts of a row: of 4096 tokens, or as many times that as leave 64 (a lane each).
+uint32_t tree_part(uint32_t vocab) { return ((vocab + 63) / 64 + 4095) / 4096 * 4096; }
+struct TreeVerifyPlan {
+    uint32_t part, parts, draft_part, draft_parts, rounds;
+    uint64_t stats, draft_stats, need;
+};
+TreeVerifyPlan tree_verify_plan(const ctox_verify_tree *op) {
+    TreeVerifyPlan p{};
+    const bool greedy = op->temperature == 0.0f, draft = op->draft && !greedy;
+    p.part = tree_part(op->vocab);
+    p.parts = (op->vocab + p.part - 1) / p.part;
+    if (draft) {
+        p.draft_part = tree_part(op->draft_vocab);
+        p.draft_parts = (op->draft_vocab + p.draft_part - 1) / p.draft_part;
+    }
+    p.rounds = greedy ? 0 : op->max_children;
+    p.stats = (uint64_t)op->rows * p.parts * sizeof(TreeStat);
+    p.draft_stats = (uint64_t)op->rows * p.draft_parts * sizeof(TreeStat);
+    p.need = p.stats + p.draft_stats + (uint64_t)p.rounds * op->rows * p.parts * sizeof(double);
+    return p;
+}
+// Workspace of every call of at most so many rows, tokens and children: a smaller vocabulary may have more parts.
+uint64_t tree_verify_need(const ctox_verify_tree *op) {
+    const uint64_t most = op->vocab > 64 * 4096 ? 64 : (op->vocab + 4095) / 4096;
+    return (uint64_t)op->rows * most * (2 * sizeof(TreeStat) + op->max_children * sizeof(double));
+}
+}  // namespace
+
+extern "C" ctox_status ctox_hip_verify_tree_workspace(const ctox_hip_backend *b, const ctox_verify_tree *op, size_t *bytes) {
+    if (!bytes) return fail(CTOX_ERR_SHAPE, "null argument");
+    *bytes = 0;
+    if (ctox_status st = check_verify_tree(op)) return st;
+    if (!b) return fail(CTOX_ERR_SHAPE, "null argument");
+    *bytes = (size_t)tree_verify_need(op);
+    return CTOX_OK;
+}
+
+extern "C" ctox_status ctox_hip_verify_tree_device(ctox_hip_backend *b, const ctox_verify_tree *op, void *stream) {
+    if (ctox_status st = check_verify_tree(op)) return st;
+    const bool greedy = op->temperature == 0.0f;
+    if (!b || !op->row_starts || !op->counts || !op->next ||
+        (op->rows && (!op->target || !op->tokens || !op->parents || !op->path)) || (!greedy && (!op->accept_draws || !op->sample_draws)))
+        return fail(CTOX_ERR_SHAPE, "null argument");
+    const TreeVerifyPlan p = tree_verify_plan(op);
+    const uint64_t need = tree_verify_need(op);
+    if (op->workspace_bytes < need || (need && (!op->workspace || !aligned(op->workspace, 16))))
+        return fail(CTOX_ERR_MEMORY_BUDGET, "workspace of %llu bytes, %llu needed, 16-byte aligned",
+                    (unsigned long long)op->workspace_bytes, (unsigned long long)need);
+    TreeVerifyArgs a{};
+    a.target = op->target;
+    a.draft = greedy ? nullptr : op->draft;
+    a.inverse = op->draft_inverse;
+    a.tokens = op->tokens;
+    a.parents = op->parents;
+    a.row_starts = op->row_starts;
+    a.accept = op->accept_draws;
+    a.sample = op->sample_draws;
+    a.counts = op->counts;
+    a.path = op->path;
+    a.next = op->next;
+    uint8_t *ws = (uint8_t *)op->workspace;
+    a.stats = (TreeStat *)ws;
+    a.draft_stats = (TreeStat *)(ws + p.stats);
+    a.rest = (double *)(ws + p.stats + p.draft_stats);
+    a.target_stride = op->target_stride ? op->target_stride : op->vocab;
+    a.draft_stride = op->draft_stride ? op->draft_stride : op->draft_vocab;
+    a.inv_t = greedy ? 1.0 : 1.0 / (double)op->temperature;
+    a.requests = op->requests;
+    a.rows = op->rows;
+    a.vocab = op->vocab;
+    a.draft_vocab = op->draft_vocab;
+    a.parts = p.parts;
+    a.draft_parts = p.draft_parts;
+    a.part = p.part;
+    a.draft_part = p.draft_part;
+    a.width = op->max_children;
+    a.without = op->without_replacement != 0;
+    a.greedy = greedy;
+    OnDevice on(b);
+    hipStream_t s = (hipStream_t)stream;
+    ctox_status st = CTOX_OK;
+    if (op->rows) {
+        st = launch(b->tree_stats, dim3(std::max(p.parts, p.draft_parts), op->rows, a.draft ? 2 : 1), dim3(256), s, a,
+                    "ctox_tree_stats_gfx950");
+        for (a.round = 1; !st && a.round <= p.rounds; a.round++)
+            st = launch(b->tree_rest, dim3(p.parts, op->rows), dim3(256), s, a, "ctox_tree_rest_gfx950");
+    }
+    if (!st) st = launch(b->tree_walk, dim3(op->requests), dim3(1024), s, a, "ctox_tree_walk_gfx950");
+    return st;
+}
+
+extern "C" ctox_status ctox_hip_paged_commit_device(ctox_hip_backend *b, const ctox_paged_commit *op, void *stream) {
+    if (!op) return fail(CTOX_ERR_SHAPE, "null argument");
+    PagedCommitArgs a{};
+    if (ctox_status st = check_pools(op->q4_pools, op->layers, op->requests, op->max_pages, op->page_tokens, op->q4_slots,
+                                     op->token_bytes, op->q4_page_bytes, a.pools, &a.unit))
+        return st;
+    if (op->rows > 0x7fffffffu) return fail(CTOX_ERR_SHAPE, "%u rows are too many", op->rows);
+    if (!b || !op->descriptors || !op->row_starts || !op->tokens || !op->counts || !op->new_tokens || !op->status ||
+        (op->rows && !op->path))
+        return fail(CTOX_ERR_SHAPE, "null argument");
+    if (!aligned(op->descriptors, 16)) return fail(CTOX_ERR_SHAPE, "descriptors need 16-byte alignment");
+    a.desc = (PagedKvDesc *)op->descriptors;
+    a.row_starts = op->row_starts;
+    a.tokens = op->tokens;
+    a.counts = op->counts;
+    a.path = op->path;
+    a.new_tokens = op->new_tokens;
+    a.status = op->status;
+    a.q4_page_bytes = op->q4_page_bytes;
+    a.requests = op->requests;
+    a.rows = op->rows;
+    a.max_pages = op->max_pages;
+    a.page_tokens = op->page_tokens;
+    a.q4_slots = op->q4_slots;
+    a.token_bytes = op->token_bytes;
+    a.layers = op->layers;
+    const uint64_t columns = (uint64_t)op->token_bytes / a.unit * op->layers;
+    OnDevice on(b);
+    return launch(b->paged_commit, dim3((unsigned)((columns + 255) / 256), op->requests), dim3(256), (hipStream_t)stream, a,
+                  "ctox_paged_commit_gfx950");
+}
+
+namespace {
+ctox_status check_free_slots(const ctox_paged_free_slots *op) {
+    if (!op) return fail(CTOX_ERR_SHAPE, "null argument");
+    if (op->requests == 0 || op->requests > CTOX_PLAN_REQUESTS)
+        return fail(CTOX_ERR_SHAPE, "%u requests outside 1..%d", op->requests, CTOX_PLAN_REQUESTS);
+    if (op->page_tokens == 0 || op->max_pages == 0 || (uint64_t)op->max_pages * op->page_tokens > 0xffffffffull ||
+        (uint64_t)op->requests * op->max_pages > 0xffffffffull || op->q4_slots > (1u << 24) || op->q2_slots > (1u << 24))
+        return fail(CTOX_ERR_SHAPE, "page geometry is empty or too large");
+    return CTOX_OK;
+}
+}  // namespace
+
+extern "C" ctox_status ctox_hip_paged_free_slots_workspace(const ctox_hip_backend *b, const ctox_paged_free_slots *op,
+                                                           size_t *bytes) {
+    if (!bytes) return fail(CTOX_ERR_SHAPE, "null argument");
+    *bytes = 0;
+    if (ctox_status st = check_free_slots(op)) return st;
+    if (!b) return fail(CTOX_ERR_SHAPE, "null argument");
+    *bytes = ((op->q4_slots + 31) / 32 + (op->q2_slots + 31) / 32) * sizeof(uint32_t);
+    return CTOX_OK;
+}
+
+extern "C" ctox_status ctox_hip_paged_free_slots_device(ctox_hip_backend *b, const ctox_paged_free_slots *op, void *stream) {
+    if (ctox_status st = check_free_slots(op)) return st;
+    if (!b || !op->descriptors || !op->tokens || !op->counts || (op->q4_slots && !op->q4_free) || (op->q2_slots && !op->q2_free))
+        return fail(CTOX_ERR_SHAPE, "null argument");
+    if (!aligned(op->descriptors, 16)) return fail(CTOX_ERR_SHAPE, "descriptors need 16-byte alignment");
+    FreeSlotsArgs a{};
+    a.desc = (const PagedKvDesc *)op->descriptors;
+    a.tokens = op->tokens;
+    a.used = (uint32_t *)op->workspace;
+    a.lists[0] = op->q4_free;
+    a.lists[1] = op->q2_free;
+    a.counts = op->counts;
+    a.slots[0] = op->q4_slots;
+    a.slots[1] = op->q2_slots;
+    for (int i = 0; i < 2; i++) a.words[i] = (a.slots[i] + 31) / 32;
+    a.requests = op->requests;
+    a.max_pages = op->max_pages;
+    a.page_tokens = op->page_tokens;
+    const uint64_t need = ((uint64_t)a.words[0] + a.words[1]) * sizeof(uint32_t);
+    if (op->workspace_bytes < need || (need && (!op->workspace || !aligned(op->workspace, 4))))
+        return fail(CTOX_ERR_MEMORY_BUDGET, "workspace of %llu bytes, %llu needed, 4-byte aligned",
+                    (unsigned long long)op->workspace_bytes, (unsigned long long)need);
+    const uint32_t most = std::max(a.words[0], a.words[1]), cus = (uint32_t)b->cus;
+    OnDevice on(b);
+    hipStream_t s = (hipStream_t)stream;
+    ctox_status st = CTOX_OK;
+    if (need) {
+        st = launch(b->free_clear, dim3(std::min<uint32_t>(cus, (uint32_t)(need / 4 + 255) / 256)), dim3(256), s, a,
+                    "ctox_free_clear_gfx950");
+        const uint32_t groups = std::min<uint32_t>((op->max_pages + 255) / 256, std::max<uint32_t>(1, 2048 / op->requests));
+        if (!st) st = launch(b->free_mark, dim3(groups, op->requests), dim3(256), s, a, "ctox_free_mark_gfx950");
+    }
+    if (!st)
+        st = launch(b->free_list, dim3(std::max<uint32_t>(1, (most + 255) / 256), 2), dim3(256), s, a, "ctox_free_list_gfx950");
+    return st;
+}
+
+extern "C" ctox_status ctox_hip_paged_fork_device(ctox_hip_backend *b, const ctox_paged_fork *op, void *stream) {
+    if (!op) return fail(CTOX_ERR_SHAPE, "null argument");
+    PagedForkArgs a{};
+    if (ctox_status st = check_pools(op->q4_pools, op->layers, op->requests, op->max_pages, op->page_tokens, op->q4_slots,
+                                     op->token_bytes, op->q4_page_bytes, a.pools, &a.unit))
+        return st;
+    if (op->forks > CTOX_PLAN_REQUESTS) return fail(CTOX_ERR_SHAPE, "%u forks are too many", op->forks);
+    if (!b || !op->descriptors || !op->tokens || !op->status || !op->free_count || (op->q4_slots && !op->free_slots) ||
+        (op->forks && (!op->sources || !op->targets)))
+        return fail(CTOX_ERR_SHAPE, "null argument");
+    if (!aligned(op->descriptors, 16)) return fail(CTOX_ERR_SHAPE, "descriptors need 16-byte alignment");
+    a.desc = (PagedKvDesc *)op->descriptors;
+    a.tokens = op->tokens;
+    a.sources = op->sources;
+    a.targets = op->targets;
+    a.free_slots = op->free_slots;
+    a.free_count = op->free_count;
+    a.status = op->status;
+    a.q4_page_bytes = op->q4_page_bytes;
+    a.requests = op->requests;
+    a.forks = op->forks;
+    a.max_pages = op->max_pages;
+    a.page_tokens = op->page_tokens;
+    a.q4_slots = op->q4_slots;
+    a.token_bytes = op->token_bytes;
+    a.layers = op->layers;
+    // A few accesses a thread; the whole chip for a few forks.
+    const uint64_t units = (uint64_t)op->page_tokens * op->token_bytes / a.unit * op->layers;
+    const uint64_t pieces = std::min<uint64_t>((units + 1023) / 1024, std::max<uint64_t>(1, 4096 / std::max(1u, op->forks)));
+    OnDevice on(b);
+    return launch(b->paged_fork, dim3((unsigned)pieces, std::max(1u, op->forks)), dim3(256), (hipStream_t)stream, a,
+                  "ctox_paged_fork_gfx950");
+}
+
+namespace {
+ctox_status check_gdn_tree(const ctox_gdn_tree *op) {
+    if (!op) return fail(CTOX_ERR_SHAPE, "null argument");
+    if (op->requests == 0 || op->requests > CTOX_PLAN_REQUESTS)
+        return fail(CTOX_ERR_SHAPE, "%u requests outside 1..%d", op->requests, CTOX_PLAN_REQUESTS);
+    if (op->rows > kMostGroups256) return fail(CTOX_ERR_SHAPE, "%u rows reach 2^24", op->rows);
+    if (op->max_rows > CTOX_TREE_NODES) return fail(CTOX_ERR_SHAPE, "trees of %u nodes, %d at most", op->max_rows, CTOX_TREE_NODES);
+    if (op->heads == 0 || op->key_heads == 0 || op->heads % op->key_heads || op->heads > 4096 || op->key_dim == 0 ||
+        op->key_dim > 128 || op->value_dim == 0 || op->value_dim > 4096 || op->kernel == 0 || op->kernel > 8)
+        return fail(CTOX_ERR_SHAPE, "gated delta shapes");
+    const uint64_t channels = 2ull * op->key_heads * op->key_dim + (uint64_t)op->heads * op->value_dim;
+    const uint64_t state = op->blocked ? (uint64_t)op->heads * ((op->value_dim + 15) / 16) * 2048
+                                       : (uint64_t)op->heads * op->key_dim * op->value_dim;
+    if (op->proj_stride < channels || op->proj_stride > 0x7fffffffu || op->a_off + op->heads > op->proj_stride ||
+        op->b_off + op->heads > op->proj_stride || op->a_off > 0x7fffffffu || op->b_off > 0x7fffffffu)
+        return fail(CTOX_ERR_SHAPE, "gated delta rows do not hold their channels");
+    if ((op->conv_stride && op->conv_stride < channels * op->kernel) || (op->state_stride && op->state_stride < state) ||
+        op->conv_stride > 0x7fffffffu || op->state_stride > 0x7fffffffu || state > 0x7fffffffu)
+        return fail(CTOX_ERR_SHAPE, "gated delta states overlap or are too far apart");
+    if (op->blocked && op->state_stride % 4) return fail(CTOX_ERR_SHAPE, "blocked gated delta state needs 16-byte alignment");
+    return CTOX_OK;
+}
+uint64_t gdn_tree_need(const ctox_gdn_tree *op) {
+    return (uint64_t)op->rows * 4 * ((uint64_t)op->key_heads * 128 + (uint64_t)op->heads * op->value_dim + op->heads);
+}
+GdnTreeArgs gdn_tree_args(const ctox_gdn_tree *op) {
+    GdnTreeArgs a{};
+    a.proj = op->proj;
+    a.conv_w = op->conv_w;
+    a.conv_in = op->conv_in;
+    a.conv_out = op->conv_out;
+    a.a_log = op->a_log;
+    a.dt_bias = op->dt_bias;
+    a.state_in = op->state_in;
+    a.state_out = op->state_out;
+    a.row_starts = op->row_starts;
+    a.parents = op->parents;
+    a.counts = op->counts;
+    a.path = op->path;
+    a.out = op->out;
+    a.keys = (float *)op->workspace;
+    a.deltas = a.keys + (size_t)op->rows * op->key_heads * 128;
+    a.decays = a.deltas + (size_t)op->rows * op->heads * op->value_dim;
+    a.proj_stride = op->proj_stride;
+    const uint64_t channels = 2ull * op->key_heads * op->key_dim + (uint64_t)op->heads * op->value_dim;
+    const uint64_t state = op->blocked ? (uint64_t)op->heads * ((op->value_dim + 15) / 16) * 2048
+                                       : (uint64_t)op->heads * op->key_dim * op->value_dim;
+    a.conv_stride = op->conv_stride ? op->conv_stride : channels * op->kernel;
+    a.state_stride = op->state_stride ? op->state_stride : state;
+    a.a_off = (uint32_t)op->a_off;
+    a.b_off = (uint32_t)op->b_off;
+    a.requests = op->requests;
+    a.rows = op->rows;
+    a.heads = op->heads;
+    a.key_heads = op->key_heads;
+    a.key_dim = op->key_dim;
+    a.value_dim = op->value_dim;
+    a.kernel = op->kernel;
+    a.blocked = op->blocked != 0;
+    return a;
+}
+ctox_status gdn_tree_workspace_ok(const ctox_gdn_tree *op) {
+    const uint64_t need = gdn_tree_need(op);
+    if (op->workspace_bytes < need || (need && (!op->workspace || !aligned(op->workspace, 16))))
+        return fail(CTOX_ERR_MEMORY_BUDGET, "workspace of %llu bytes, %llu needed, 16-byte aligned",
+                    (unsigned long long)op->workspace_bytes, (unsigned long long)need);
+    return CTOX_OK;
+}
+}  // namespace
+
+extern "C" ctox_status ctox_hip_gdn_tree_workspace(const ctox_hip_backend *b, const ctox_gdn_tree *op, size_t *bytes) {
+    if (!bytes) return fail(CTOX_ERR_SHAPE, "null argument");
+    *bytes = 0;
+    if (ctox_status st = check_gdn_tree(op)) return st;
+    if (!b) return fail(CTOX_ERR_SHAPE, "null argument");
+    *bytes = (size_t)gdn_tree_need(op);
+    return CTOX_OK;
+}
+
+extern "C" ctox_status ctox_hip_gdn_tree_device(ctox_hip_backend *b, const ctox_gdn_tree *op, void *stream) {
+    if (ctox_status st = check_gdn_tree(op)) return st;
+    if (!b || !op->conv_w || !op->conv_in || !op->a_log || !op->dt_bias || !op->state_in || !op->row_starts ||
+        (op->rows && (!op->proj || !op->parents || !op->out)))
+        return fail(CTOX_ERR_SHAPE, "null argument");
+    if (op->blocked && !aligned(op->state_in, 16)) return fail(CTOX_ERR_SHAPE, "blocked gated delta state needs 16-byte alignment");
+    if (ctox_status st = gdn_tree_workspace_ok(op)) return st;
+    if (op->rows == 0) return CTOX_OK;
+    const GdnTreeArgs a = gdn_tree_args(op);
+    const uint32_t most = std::min<uint32_t>(op->max_rows ? op->max_rows : CTOX_TREE_NODES, op->rows);
+    const dim3 grid(op->heads * ((op->value_dim + 63) / 64), op->requests);
+    OnDevice on(b);
+    ctox_status st = CTOX_OK;
+    for (int i = 0; !st && i < 3; i++)
+        if (i == 0 || most > 16u * i) st = launch(b->gdn_tree[i], grid, dim3(256), (hipStream_t)stream, a, "ctox_gdn_tree_gfx950");
+    return st;
+}
+
+extern "C" ctox_status ctox_hip_gdn_tree_commit_device(ctox_hip_backend *b, const ctox_gdn_tree *op, void *stream) {
+    if (ctox_status st = check_gdn_tree(op)) return st;
+    if (!b || !op->conv_in || !op->conv_out || !op->state_in || !op->state_out || !op->row_starts || !op->counts ||
+        (op->rows && (!op->proj || !op->path)))
+        return fail(CTOX_ERR_SHAPE, "null argument");
+    if (op->blocked && !(aligned(op->state_in, 16) && aligned(op->state_out, 16)))
+        return fail(CTOX_ERR_SHAPE, "blocked gated delta state needs 16-byte alignment");
+    if (ctox_status st = gdn_tree_workspace_ok(op)) return st;
+    const GdnTreeArgs a = gdn_tree_args(op);
+    const uint32_t channels = 2 * op->key_heads * op->key_dim + op->heads * op->value_dim;
+    OnDevice on(b);
+    return launch(b->gdn_tree_commit, dim3(op->heads * ((op->value_dim + 15) / 16) + (channels + 255) / 256, op->requests),
+                  dim3(256), (hipStream_t)stream, a, "ctox_gdn_tree_commit_gfx950");
 }

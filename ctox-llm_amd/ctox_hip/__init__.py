@@ -291,6 +291,132 @@ class PagedGqaRows(_Op):
         self.workspace, self.workspace_bytes = d_workspace, workspace_bytes
 
 
+NO_PARENT = 0xffffffff      # a root's parent
+TREE_NODES = 64             # of one request's tree
+TREE_RELEASE = 0xffffffff   # a commit's count of a request that has ended
+TREE_FAILED = 0xfffffffe    # next token of a request whose logits are no numbers
+
+
+def _fields(pointers, words, tail=()):
+    return [(n, ctypes.c_void_p) for n in pointers] + [(n, ctypes.c_uint32) for n in words] + list(tail)
+
+
+class TreePlan(_Op):
+    """ctox_tree_plan (all pointers are device addresses)."""
+    _fields_ = _fields(("row_starts", "tokens", "parents", "masks", "positions", "depths"), ("requests", "rows"))
+    _bits = _bits(_fields_)
+
+    def __init__(self, d_row_starts, d_tokens, d_parents, d_masks, d_positions, d_depths, requests, rows):
+        super().__init__(d_row_starts, d_tokens, d_parents, d_masks, d_positions, d_depths, requests, rows)
+
+
+class PagedGqaTree(ctypes.Structure):
+    """ctox_paged_gqa_tree: `rows` is the PagedGqaRows of the nodes (max_rows 0: TREE_NODES)."""
+    _fields_ = [("rows", PagedGqaRows), ("masks", ctypes.c_void_p)]
+
+    def __init__(self, d_query, d_out, d_q2_pages, d_q4_pages, d_descriptors, d_row_starts, d_tokens, d_masks, rows,
+                 requests, params, max_rows=0, d_workspace=None, workspace_bytes=0):
+        super().__init__(PagedGqaRows(d_query, d_out, d_q2_pages, d_q4_pages, d_descriptors, d_row_starts, d_tokens,
+                                      rows, requests, params, max_rows, d_workspace, workspace_bytes), d_masks)
+
+    def bind_workspace(self, d_workspace: int, workspace_bytes: int) -> None:
+        self.rows.bind_workspace(d_workspace, workspace_bytes)
+
+
+class _Workspace(_Op):
+    def bind_workspace(self, d_workspace: int, workspace_bytes: int) -> None:
+        self.workspace, self.workspace_bytes = d_workspace, workspace_bytes
+
+
+_WORKSPACE = (("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64))
+
+
+class VerifyTree(_Workspace):
+    """ctox_verify_tree. Strides are in values (0: dense rows); d_draft None: children were chosen outright."""
+    _fields_ = _fields(("target", "draft", "draft_inverse", "tokens", "parents", "row_starts", "accept_draws",
+                        "sample_draws", "counts", "path", "next"), (), [
+        ("target_stride", ctypes.c_uint64), ("draft_stride", ctypes.c_uint64)] + [
+        (n, ctypes.c_uint32) for n in ("requests", "rows", "vocab", "draft_vocab", "max_children")] + [
+        ("without_replacement", ctypes.c_int32), ("temperature", ctypes.c_float), *_WORKSPACE])
+    _bits = _bits(_fields_)
+
+    def __init__(self, d_target, d_tokens, d_parents, d_row_starts, d_counts, d_path, d_next, requests, rows, vocab,
+                 max_children, temperature, d_draft=None, d_draft_inverse=None, d_accept_draws=None,
+                 d_sample_draws=None, draft_vocab=None, without_replacement=True, target_stride=0, draft_stride=0,
+                 d_workspace=None, workspace_bytes=0):
+        super().__init__(d_target, d_draft, d_draft_inverse, d_tokens, d_parents, d_row_starts, d_accept_draws,
+                         d_sample_draws, d_counts, d_path, d_next, target_stride, draft_stride, requests, rows, vocab,
+                         vocab if draft_vocab is None else draft_vocab, max_children, int(bool(without_replacement)),
+                         temperature, d_workspace, workspace_bytes)
+
+
+class _Pooled(_Op):
+    """A call whose first field is a host array of pools, one device address a layer."""
+
+    def _pools(self, pools):
+        self._kept = (ctypes.c_void_p * max(1, len(pools)))(*pools)
+        return ctypes.addressof(self._kept)
+
+
+class PagedCommit(_Pooled):
+    """ctox_paged_commit. q4_pools: the layers' Q4 pools (device addresses)."""
+    _fields_ = _fields(("q4_pools", "descriptors", "row_starts", "tokens", "counts", "path", "new_tokens", "status"),
+                       ("layers", "requests", "rows", "max_pages", "page_tokens", "q4_slots", "token_bytes",
+                        "q4_page_bytes"))
+    _bits = _bits(_fields_)
+
+    def __init__(self, q4_pools, d_descriptors, d_row_starts, d_tokens, d_counts, d_path, d_new_tokens, d_status,
+                 requests, rows, max_pages, page_tokens, q4_slots, token_bytes, q4_page_bytes):
+        super().__init__(self._pools(q4_pools), d_descriptors, d_row_starts, d_tokens, d_counts, d_path, d_new_tokens,
+                         d_status, len(q4_pools), requests, rows, max_pages, page_tokens, q4_slots, token_bytes,
+                         q4_page_bytes)
+
+
+class PagedFreeSlots(_Workspace):
+    """ctox_paged_free_slots (device addresses)."""
+    _fields_ = _fields(("descriptors", "tokens", "q4_free", "q2_free", "counts"),
+                       ("requests", "max_pages", "page_tokens", "q4_slots", "q2_slots"), _WORKSPACE)
+    _bits = _bits(_fields_)
+
+    def __init__(self, d_descriptors, d_tokens, d_q4_free, d_q2_free, d_counts, requests, max_pages, page_tokens,
+                 q4_slots, q2_slots, d_workspace=None, workspace_bytes=0):
+        super().__init__(d_descriptors, d_tokens, d_q4_free, d_q2_free, d_counts, requests, max_pages, page_tokens,
+                         q4_slots, q2_slots, d_workspace, workspace_bytes)
+
+
+class PagedFork(_Pooled):
+    """ctox_paged_fork. q4_pools: the layers' Q4 pools (device addresses)."""
+    _fields_ = _fields(("q4_pools", "descriptors", "tokens", "sources", "targets", "free_slots", "free_count", "status"),
+                       ("layers", "requests", "forks", "max_pages", "page_tokens", "q4_slots", "token_bytes",
+                        "q4_page_bytes"))
+    _bits = _bits(_fields_)
+
+    def __init__(self, q4_pools, d_descriptors, d_tokens, d_sources, d_targets, d_free_slots, d_free_count, d_status,
+                 requests, forks, max_pages, page_tokens, q4_slots, token_bytes, q4_page_bytes):
+        super().__init__(self._pools(q4_pools), d_descriptors, d_tokens, d_sources, d_targets, d_free_slots,
+                         d_free_count, d_status, len(q4_pools), requests, forks, max_pages, page_tokens, q4_slots,
+                         token_bytes, q4_page_bytes)
+
+
+class GdnTree(_Workspace):
+    """ctox_gdn_tree: one description serves the nodes' call and the commit of the accepted path."""
+    _fields_ = _fields(("proj", "conv_w", "conv_in", "a_log", "dt_bias", "state_in", "row_starts", "parents", "out",
+                        "counts", "path", "conv_out", "state_out"), (), [
+        (n, ctypes.c_uint64) for n in ("proj_stride", "a_off", "b_off", "conv_stride", "state_stride")] + [
+        (n, ctypes.c_uint32) for n in ("requests", "rows", "max_rows", "heads", "key_heads", "key_dim", "value_dim",
+                                       "kernel")] + [("blocked", ctypes.c_int32), *_WORKSPACE])
+    _bits = _bits(_fields_)
+
+    def __init__(self, d_proj, d_conv_w, d_conv_in, d_a_log, d_dt_bias, d_state_in, d_row_starts, d_parents, d_out,
+                 proj_stride, a_off, b_off, requests, rows, heads, key_heads, key_dim, value_dim, kernel, d_counts=None,
+                 d_path=None, d_conv_out=None, d_state_out=None, max_rows=0, blocked=False, conv_stride=0,
+                 state_stride=0, d_workspace=None, workspace_bytes=0):
+        super().__init__(d_proj, d_conv_w, d_conv_in, d_a_log, d_dt_bias, d_state_in, d_row_starts, d_parents, d_out,
+                         d_counts, d_path, d_conv_out, d_state_out, proj_stride, a_off, b_off, conv_stride,
+                         state_stride, requests, rows, max_rows, heads, key_heads, key_dim, value_dim, kernel,
+                         int(bool(blocked)), d_workspace, workspace_bytes)
+
+
 # Every symbol include/ctox_hip.h declares: name -> (restype, argtypes).
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
@@ -361,6 +487,18 @@ SIGNATURES = {
     "ctox_hip_paged_gqa_rows_workspace": (_I32, [_P, ctypes.POINTER(PagedGqaRows), ctypes.POINTER(_SZ)]),
     "ctox_hip_paged_gqa_rows_device": (_I32, [_P, ctypes.POINTER(PagedGqaRows), _P]),
     "ctox_hip_kv_append_q4_device": (_I32, [_P, _P, _P, _SZ, _P, _SZ, _P, _SZ, _SZ, _U32, _U32, _U32, _P]),
+    "ctox_hip_tree_plan_device": (_I32, [_P, ctypes.POINTER(TreePlan), _P]),
+    "ctox_hip_paged_gqa_tree_workspace": (_I32, [_P, ctypes.POINTER(PagedGqaTree), ctypes.POINTER(_SZ)]),
+    "ctox_hip_paged_gqa_tree_device": (_I32, [_P, ctypes.POINTER(PagedGqaTree), _P]),
+    "ctox_hip_verify_tree_workspace": (_I32, [_P, ctypes.POINTER(VerifyTree), ctypes.POINTER(_SZ)]),
+    "ctox_hip_verify_tree_device": (_I32, [_P, ctypes.POINTER(VerifyTree), _P]),
+    "ctox_hip_paged_commit_device": (_I32, [_P, ctypes.POINTER(PagedCommit), _P]),
+    "ctox_hip_paged_free_slots_workspace": (_I32, [_P, ctypes.POINTER(PagedFreeSlots), ctypes.POINTER(_SZ)]),
+    "ctox_hip_paged_free_slots_device": (_I32, [_P, ctypes.POINTER(PagedFreeSlots), _P]),
+    "ctox_hip_paged_fork_device": (_I32, [_P, ctypes.POINTER(PagedFork), _P]),
+    "ctox_hip_gdn_tree_workspace": (_I32, [_P, ctypes.POINTER(GdnTree), ctypes.POINTER(_SZ)]),
+    "ctox_hip_gdn_tree_device": (_I32, [_P, ctypes.POINTER(GdnTree), _P]),
+    "ctox_hip_gdn_tree_commit_device": (_I32, [_P, ctypes.POINTER(GdnTree), _P]),
     "ctox_hip_fill_random_device": (_I32, [_P, _P, ctypes.c_uint64, _U32, ctypes.c_uint64, ctypes.c_float,
                                            ctypes.c_float, _P]),
     "ctox_hip_embedding_rows_device": (_I32, [_P, _I32, _P, _P, _P, _P, _SZ, _SZ, _SZ, _P, _P]),
@@ -785,6 +923,56 @@ class HipBackend:
     def paged_gqa_rows_device(self, op: PagedGqaRows, stream: Optional[int] = None) -> None:
         """Attention of a ragged batch's new rows over the paged cache (Q/src/reference.rs:420-499)."""
         _check(load_library().ctox_hip_paged_gqa_rows_device(self.handle, ctypes.byref(op), stream))
+
+    # ---- trees of drafted tokens (device pointers) ----
+    def _workspace(self, name: str, op) -> int:
+        n = ctypes.c_size_t()
+        _check(getattr(load_library(), f"ctox_hip_{name}_workspace")(self.handle, ctypes.byref(op), ctypes.byref(n)))
+        return n.value
+
+    def tree_plan_device(self, op: TreePlan, stream: Optional[int] = None) -> None:
+        """Ancestor masks and positions of drafted nodes, from their parents."""
+        _check(load_library().ctox_hip_tree_plan_device(self.handle, ctypes.byref(op), stream))
+
+    def paged_gqa_tree_workspace(self, op: PagedGqaTree) -> int:
+        return self._workspace("paged_gqa_tree", op)
+
+    def paged_gqa_tree_device(self, op: PagedGqaTree, stream: Optional[int] = None) -> None:
+        """Attention of trees' nodes over the paged cache and their ancestors (Q/src/reference.rs:420-499)."""
+        _check(load_library().ctox_hip_paged_gqa_tree_device(self.handle, ctypes.byref(op), stream))
+
+    def verify_tree_workspace(self, op: VerifyTree) -> int:
+        return self._workspace("verify_tree", op)
+
+    def verify_tree_device(self, op: VerifyTree, stream: Optional[int] = None) -> None:
+        """The path of each tree that the target accepts, and the next token (Q/src/engine.rs:915-963 for trees)."""
+        _check(load_library().ctox_hip_verify_tree_device(self.handle, ctypes.byref(op), stream))
+
+    def paged_commit_device(self, op: PagedCommit, stream: Optional[int] = None) -> None:
+        """An accepted path's tokens closed up in all layers' pages; lengths and descriptors cut."""
+        _check(load_library().ctox_hip_paged_commit_device(self.handle, ctypes.byref(op), stream))
+
+    def paged_free_slots_workspace(self, op: PagedFreeSlots) -> int:
+        return self._workspace("paged_free_slots", op)
+
+    def paged_free_slots_device(self, op: PagedFreeSlots, stream: Optional[int] = None) -> None:
+        """Ascending lists of the slots that no live page holds."""
+        _check(load_library().ctox_hip_paged_free_slots_device(self.handle, ctypes.byref(op), stream))
+
+    def paged_fork_device(self, op: PagedFork, stream: Optional[int] = None) -> None:
+        """Requests' caches forked: full pages shared, a part-filled last page copied."""
+        _check(load_library().ctox_hip_paged_fork_device(self.handle, ctypes.byref(op), stream))
+
+    def gdn_tree_workspace(self, op: GdnTree) -> int:
+        return self._workspace("gdn_tree", op)
+
+    def gdn_tree_device(self, op: GdnTree, stream: Optional[int] = None) -> None:
+        """The GatedDeltaNet token mixer over trees' nodes (Q/src/decoder.rs:863-913)."""
+        _check(load_library().ctox_hip_gdn_tree_device(self.handle, ctypes.byref(op), stream))
+
+    def gdn_tree_commit_device(self, op: GdnTree, stream: Optional[int] = None) -> None:
+        """Conv windows and states behind the accepted paths, after gdn_tree_device."""
+        _check(load_library().ctox_hip_gdn_tree_commit_device(self.handle, ctypes.byref(op), stream))
 
     def synchronize(self) -> None:
         _check(load_library().ctox_hip_synchronize(self.handle))

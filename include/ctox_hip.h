@@ -737,6 +737,199 @@ ctox_status ctox_hip_paged_gqa_rows_workspace(const ctox_hip_backend *backend, c
                                               size_t *bytes);
 ctox_status ctox_hip_paged_gqa_rows_device(ctox_hip_backend *backend, const ctox_paged_gqa_rows *op, void *stream);
 
+/* ---- trees of drafted tokens (device buffers) ----
+ * A decode step in which every request has a tree of drafted tokens: one
+ * target pass over all nodes, then one path of the tree is kept. Request
+ * r's nodes are its rows row_starts[r] .. row_starts[r + 1] - 1 of the ragged
+ * batch (a plan's, with added[r] = nodes), at most CTOX_TREE_NODES. Node 0 is
+ * the root, the token that was chosen last (its K and V are not cached yet);
+ * parents[row] is the number of a node's parent in its request. A parent has a
+ * smaller number than its children; a node with any other parent (CTOX_NO_PARENT)
+ * is a root of its own. The crate drafts chains (Q/src/engine.rs:583-590,
+ * 915-963, Q/src/decoder.rs:1311-1375): a chain is the tree with parents 0, 1, 2 ..
+ * As the calls for ragged batches these allocate nothing, wait for nothing, use no
+ * scratch of the backend and read all lengths on the device. */
+#define CTOX_TREE_NODES 64
+#define CTOX_NO_PARENT 0xffffffffu
+
+/* Ancestor masks and positions of the nodes. masks[row]: bit j is set where node j of
+ * the request is the row's node or above it. positions[row]: tokens[r] - nodes + depth
+ * (a root's depth is 0), where rotary positions of the node come from. depths[r]: nodes
+ * on the longest path, 0 without nodes, 0xffffffff where a request has more than
+ * CTOX_TREE_NODES rows (their masks are 0). Rows from row_starts[requests] on get mask 0 and keep
+ * their positions. No output may overlap an input. rows < 2^24, requests <= 4096. */
+typedef struct {
+    const uint32_t *row_starts;  /* [requests + 1], not falling, at most rows */
+    const uint32_t *tokens;      /* [requests], the nodes included */
+    const uint32_t *parents;     /* [rows] */
+    uint64_t *masks;             /* [rows], 8-byte aligned */
+    uint32_t *positions;         /* [rows] */
+    uint32_t *depths;            /* [requests] */
+    uint32_t requests, rows;
+} ctox_tree_plan;
+ctox_status ctox_hip_tree_plan_device(ctox_hip_backend *backend, const ctox_tree_plan *op, void *stream);
+
+/* ctox_hip_paged_gqa_rows_device (Q/src/reference.rs:420-499) with each row seeing the tokens
+ * in front of its request's rows, 0 .. tokens[r] - n - 1, and of the n rows' own tokens those whose
+ * bit its mask has: row j's token is tokens[r] - n + j. Bits from n on do not
+ * count. Any mask may be given; a row that sees nothing gets zeros. rows.max_rows bounds the
+ * rows of any one request and is at most CTOX_TREE_NODES (0: CTOX_TREE_NODES). Everything
+ * else is as there, the workspace too (with its own ctox_hip_paged_gqa_tree_workspace). */
+typedef struct {
+    ctox_paged_gqa_rows rows;
+    const uint64_t *masks;       /* [rows], 8-byte aligned */
+} ctox_paged_gqa_tree;
+ctox_status ctox_hip_paged_gqa_tree_workspace(const ctox_hip_backend *backend, const ctox_paged_gqa_tree *op,
+                                              size_t *bytes);
+ctox_status ctox_hip_paged_gqa_tree_device(ctox_hip_backend *backend, const ctox_paged_gqa_tree *op, void *stream);
+
+/* Which path of each tree the target accepts, and the token after it. Row i of target
+ * holds the logits behind node i. From the root down a node's children are offered in the order of
+ * their numbers (the first max_children of them), each with its number accept_draws[child] in
+ * [0, 1); the first that is accepted is the next node of the path. p = softmax(target / temperature).
+ *  - draft given: siblings were drawn from q = softmax(draft / temperature), row i of draft holding the
+ *    logits that node i's children were drawn from, with replacement or (without_replacement) without.
+ *    A child with token t is accepted iff u q'(t) < r(t), q' the law it was drawn from (without the
+ *    siblings before it, renormalised) and r what the refusals before left of p: r = p at first, a
+ *    refusal makes it max(r - q', 0), renormalised. The tokens then follow p exactly, whatever q is.
+ *    Siblings drawn without replacement differ; where q has no undrawn mass left (below 2^-40) no
+ *    further child is offered. draft_inverse (or NULL) maps a token to its place in a draft row of draft_vocab
+ *    logits (0xffffffff: not among them), as ctox_hip_mtp_accept_restricted_device.
+ *  - draft NULL: children were chosen outright; a refusal takes the token out of p.
+ *  - temperature 0: the child whose token is the largest logit's (the later token wins ties, as
+ *    ctox_hip_greedy_tokens_device) is accepted; draft and the numbers are not read.
+ * Where no child is accepted next[r] is drawn with sample_draws[r] from r (from p where no child was
+ * refused): the first token whose running sum exceeds the number times the total. A chain is
+ * verified by the rule of ctox_hip_mtp_accept_device. Sums and laws are in 64 bits.
+ * counts[r]: nodes of the path, the root included; path[row_starts[r] + i]: its i-th node,
+ * 0xffffffff behind it. A request without rows: counts 0, next 0xffffffff. A token that is not below vocab is
+ * never accepted. -inf is a token that is ruled out; where a row on the path (or, with children, its
+ * draft row) has a logit that is +inf or no number, or none that is finite, the request fails
+ * closed: counts 0, next CTOX_TREE_FAILED. Strides of 0 stand for dense rows. rows <= 65535, vocab < 2^31.
+ * workspace holds ctox_hip_verify_tree_workspace bytes (of the same op; its device pointers are
+ * not read, but for draft being NULL or not), 16-byte aligned; one for the most rows, vocab, draft_vocab and
+ * max_children serves smaller calls. */
+#define CTOX_TREE_FAILED 0xfffffffeu
+typedef struct {
+    const float *target;            /* [rows][target_stride] */
+    const float *draft;             /* [rows][draft_stride] or NULL */
+    const uint32_t *draft_inverse;  /* [vocab] or NULL (draft_vocab == vocab) */
+    const uint32_t *tokens;         /* [rows] */
+    const uint32_t *parents;        /* [rows] */
+    const uint32_t *row_starts;     /* [requests + 1] */
+    const float *accept_draws;      /* [rows] */
+    const float *sample_draws;      /* [requests] */
+    uint32_t *counts;               /* [requests] */
+    uint32_t *path;                 /* [rows] */
+    uint32_t *next;                 /* [requests] */
+    uint64_t target_stride, draft_stride;
+    uint32_t requests, rows, vocab, draft_vocab, max_children;
+    int32_t without_replacement;
+    float temperature;
+    void *workspace;
+    uint64_t workspace_bytes;
+} ctox_verify_tree;
+ctox_status ctox_hip_verify_tree_workspace(const ctox_hip_backend *backend, const ctox_verify_tree *op, size_t *bytes);
+ctox_status ctox_hip_verify_tree_device(ctox_hip_backend *backend, const ctox_verify_tree *op, void *stream);
+
+/* What an accepted path leaves of the paged cache, for all layers that share a table: token path[j]
+ * of request r's rows moves to the place of row j (j < counts[r]) in the Q4 pages of every pool, the rest
+ * of the rows is dropped. new_tokens[r] = tokens[r] - rows + counts[r], and descriptors of pages past it are
+ * cut (tokens 0 where nothing is left; slots stay readable, see ctox_hip_paged_free_slots_device).
+ * counts[r] = CTOX_TREE_RELEASE drops the request's whole cache: new_tokens[r] = 0. path rises.
+ * status[r]: 0; 1 counts[r] is more than the rows or CTOX_TREE_NODES, or the lengths do not fit
+ * the table; 2 the path does not rise or names no row, or a token that moves is not in a Q4 page of its
+ * place. Such a request is left as it is (new_tokens[r] = tokens[r]). Pages that hold rows must be the request's
+ * own. No output may overlap an input, except that descriptors are changed in place. requests <= 4096, layers
+ * <= 64, token_bytes a multiple of 4, max_pages * page_tokens below 2^32. */
+#define CTOX_TREE_RELEASE 0xffffffffu
+typedef struct {
+    uint8_t *const *q4_pools;    /* HOST [layers]: device addresses, 4-byte aligned, copied by the call */
+    ctox_paged_kv_descriptor *descriptors;  /* [requests][max_pages] */
+    const uint32_t *row_starts;  /* [requests + 1] */
+    const uint32_t *tokens;      /* [requests], the rows included */
+    const uint32_t *counts;      /* [requests] */
+    const uint32_t *path;        /* [rows] */
+    uint32_t *new_tokens;        /* [requests] */
+    uint32_t *status;            /* [requests] */
+    uint32_t layers, requests, rows, max_pages, page_tokens, q4_slots, token_bytes, q4_page_bytes;
+} ctox_paged_commit;
+ctox_status ctox_hip_paged_commit_device(ctox_hip_backend *backend, const ctox_paged_commit *op, void *stream);
+
+/* Lists of the slots that no live page holds, ascending: page p of request r is live where
+ * p * page_tokens < tokens[r]. The tables are all that is read, so pages may be shared by any number of
+ * requests, and a request's pages become free by its length alone (PagedKvCache's free list,
+ * Q/src/kv_cache.rs:394-429, for many requests). q4_free [q4_slots], q2_free [q2_slots]: the list, then
+ * CTOX_NO_SLOT; counts[0], counts[1]: how many are free. A list may be NULL with 0 slots. requests <= 4096,
+ * slots <= 2^24 each. workspace holds ctox_hip_paged_free_slots_workspace bytes, 4-byte aligned. */
+typedef struct {
+    const ctox_paged_kv_descriptor *descriptors;
+    const uint32_t *tokens;      /* [requests] */
+    uint32_t *q4_free, *q2_free;
+    uint32_t *counts;            /* [2] */
+    uint32_t requests, max_pages, page_tokens, q4_slots, q2_slots;
+    void *workspace;
+    uint64_t workspace_bytes;
+} ctox_paged_free_slots;
+ctox_status ctox_hip_paged_free_slots_workspace(const ctox_hip_backend *backend, const ctox_paged_free_slots *op,
+                                                size_t *bytes);
+ctox_status ctox_hip_paged_free_slots_device(ctox_hip_backend *backend, const ctox_paged_free_slots *op, void *stream);
+
+/* Request targets[f] becomes a copy of request sources[f]: its table's live pages and its length. Full
+ * pages are shared; a last page that is part-filled is copied, in every pool, to the next of
+ * free_slots (taken from the front, in the order of the forks), so that both may go on. A source may
+ * be forked more than once. What a target held before is dropped (its slots
+ * show as free in the next list). status[0]: 0; 1 a source or target is no request, a target is also a
+ * source or another fork's target, or a source is longer than its table; 2 fewer than the slots needed are in
+ * *free_count; 3 a part-filled page is not a Q4 page of its place; 4 a free slot is past q4_slots. Then
+ * nothing is changed. status[1]: slots taken. forks <= 4096; the rest as ctox_paged_commit. */
+typedef struct {
+    uint8_t *const *q4_pools;    /* HOST [layers], as ctox_paged_commit */
+    ctox_paged_kv_descriptor *descriptors;
+    uint32_t *tokens;            /* [requests] */
+    const uint32_t *sources, *targets;  /* [forks], may be NULL with forks = 0 */
+    const uint32_t *free_slots;
+    const uint32_t *free_count;  /* device word */
+    uint32_t *status;            /* [2] */
+    uint32_t layers, requests, forks, max_pages, page_tokens, q4_slots, token_bytes, q4_page_bytes;
+} ctox_paged_fork;
+ctox_status ctox_hip_paged_fork_device(ctox_hip_backend *backend, const ctox_paged_fork *op, void *stream);
+
+/* The GatedDeltaNet token mixer of ctox_hip_gdn_fused_device over trees: every node goes on from its parent's
+ * convolution window and state, a root from its request's. The first call reads conv_in and state_in and writes
+ * out; the states stay as they are. The second, when the path is known, writes the windows and the
+ * state behind it: request r goes through its nodes path[row_starts[r] ..], counts[r] of them (0, or
+ * more than its nodes: none; a path ends at the first entry that is no node). It needs what the first left in
+ * workspace, and proj's q | k | v channels, unchanged; conv_out may be conv_in and state_out state_in. Layouts as
+ * ctox_hip_gdn_fused_snap_device (rows of proj [q | k | v] at 0, a at a_off, b at b_off; windows
+ * [channels][kernel], states [heads][key_dim][value_dim] or blocked), request r's windows at
+ * r * conv_stride, its state at r * state_stride floats (0: dense). max_rows bounds the nodes of any one
+ * request (0: CTOX_TREE_NODES), no request may have more. key_dim <= 128, kernel <= 8,
+ * requests <= 4096, rows < 2^24. workspace holds ctox_hip_gdn_tree_workspace bytes, 16-byte aligned, and
+ * is in use from the first call to the second: layers of a step need one each. */
+typedef struct {
+    const float *proj;           /* [rows][proj_stride] */
+    const float *conv_w;         /* [channels][kernel], channels = 2 key_heads key_dim + heads value_dim */
+    const float *conv_in;
+    const float *a_log, *dt_bias;  /* [heads] */
+    const float *state_in;
+    const uint32_t *row_starts;  /* [requests + 1] */
+    const uint32_t *parents;     /* [rows] */
+    float *out;                  /* [rows][heads][value_dim] */
+    const uint32_t *counts;      /* [requests], this and below: second call */
+    const uint32_t *path;        /* [rows] */
+    float *conv_out;
+    float *state_out;
+    uint64_t proj_stride, a_off, b_off, conv_stride, state_stride;
+    uint32_t requests, rows, max_rows, heads, key_heads, key_dim, value_dim, kernel;
+    int32_t blocked;
+    void *workspace;
+    uint64_t workspace_bytes;
+} ctox_gdn_tree;
+ctox_status ctox_hip_gdn_tree_workspace(const ctox_hip_backend *backend, const ctox_gdn_tree *op, size_t *bytes);
+ctox_status ctox_hip_gdn_tree_device(ctox_hip_backend *backend, const ctox_gdn_tree *op, void *stream);
+ctox_status ctox_hip_gdn_tree_commit_device(ctox_hip_backend *backend, const ctox_gdn_tree *op, void *stream);
+
 /* ---- decode engine helpers (device buffers) ---- */
 /* Seeded synthetic tensors (counter-based, reproducible for any sub-range):
  * kind 0 Q4_B64 blocks and 1 Q2_B64 blocks (uniform codes, fp16 scale
