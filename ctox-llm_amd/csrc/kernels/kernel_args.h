@@ -762,6 +762,16 @@ struct TreeStat {                // of a part of a row
     float top;
     uint32_t bad;                // holds a logit that is no number or +inf
 };
+struct TreeRow {                 // a row's tests so far
+    double lambda;
+    double undrawn;              // mass of the draft
+    double p_top, p_inv, q_top, q_inv;  // the laws, as TvLaw
+};
+struct alignas(8) TreeMark {
+    int32_t chosen;              // accepted child, -1 none yet, -2 no law
+    uint32_t refused;            // children before
+};
+#define CTOX_TREE_LANES 64       // rows that a round after the first takes at once
 struct TreeVerifyArgs {
     const float *target;         // [rows][target_stride]
     const float *draft;          // [rows][draft_stride] or NULL
@@ -774,12 +784,16 @@ struct TreeVerifyArgs {
     uint32_t *counts;            // [requests]
     uint32_t *path;              // [rows]
     uint32_t *next;              // [requests]
-    TreeStat *stats;             // [rows][parts]
+    TreeStat *stats;             // [rows][parts], of stat_parts; a leaf's that is accepted of parts
     TreeStat *draft_stats;       // [rows][draft_parts]
-    double *rest;                // [width][rows][parts]
+    double *rest;                // [width][rows][parts]: sums after so many refusals
+    TreeRow *states;             // [2][rows]: after even and odd rounds
+    uint64_t *marks;             // [rows]: TreeMark
+    uint32_t *lists;             // [2][rows]: rows that wait for an even, odd round's successor
+    uint32_t *waiting;           // [CTOX_TREE_NODES]: how many after a round
     uint64_t target_stride;
     uint64_t draft_stride;
-    double inv_t;
+    double c;                    // log2(e) / temperature
     uint32_t requests;
     uint32_t rows;
     uint32_t vocab;
@@ -787,11 +801,15 @@ struct TreeVerifyArgs {
     uint32_t parts;              // at most 64
     uint32_t draft_parts;
     uint32_t part;               // tokens of one, a multiple of 4096
+    uint32_t stat_parts;
+    uint32_t stat_part;
     uint32_t draft_part;
     uint32_t width;              // children that are offered
     uint32_t round;
     uint32_t without;            // siblings drawn without replacement
     uint32_t greedy;
+    uint32_t per;                // parts that a workgroup of the first round takes
+    uint32_t pad;
 };
 
 struct GdnTreeArgs {

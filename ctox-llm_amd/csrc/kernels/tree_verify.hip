@@ -12,22 +12,45 @@
 // of ctox_mtp_decide_gfx950.
 //
 // The results are whole numbers, and among 150 thousand tokens the borders of the running sum lie 1e-7 apart,
-// what 32 bits hold of it: logits are taken apart in 64 bits from the exponential on.
+// what 32 bits hold of it: logits are taken apart in 64 bits from the exponential on (tv_exp2).
 //
-//  * ctox_tree_stats_gfx950: maximum and sum of every part of 4096 tokens of a row (target, draft), or its largest
-//    logit where the temperature is 0.
-//  * ctox_tree_rest_gfx950, round k: sums of r_k (not yet divided by Z_k) by parts, of rows whose first k children
-//    are refused; every workgroup repeats its row's tests for itself.
-//  * ctox_tree_walk_gfx950: a workgroup a request: every row's tests, the walk down from the root, and the next
-//    token: the part where the running sum reaches the request's number, then that part's tokens.
+// Rows are cut into parts of 4096 tokens, counted from the 16-byte border in front of the row; the first statistics of
+// many rows into parts of a few times that, since a part's reductions cost as much as a third of its exponentials.
+//  * ctox_tree_stats_gfx950: maximum and sum of every part (target, draft) of the rows with children and of roots; its
+//    largest logit, of all rows, where the temperature is 0.
+//  * ctox_tree_first_gfx950, ctox_tree_round_gfx950: round k, the test of a row's k-th child: of every row, then of those
+//    that refused it and may still be on the path. Of a row that refuses, the parts' sums of
+//    r_k, not yet divided by Z_k; of a leaf that is accepted its own statistics (the others' are never read).
+//    Each workgroup repeats its row's test for itself; what it needs of the round before is a TreeRow.
+//  * ctox_tree_walk_gfx950: a workgroup a request: the walk down from the root, and the next token: the part where
+//    the running sum passes the request's number, then that part's tokens.
 #include <hip/hip_runtime.h>
 
 #include "kernel_args.h"
 #include "lds_barrier.h"
 #include "tree.h"
 
-#define TV_PART 4096
 #define TV_LEAST 0x1p-40  // undrawn mass of the draft below which its rounding errors would be offered
+
+// 2^y for y <= 0 (a hair above 0 at most), within 1.1e-12: 2^f, |f| <= 1/2, by its interpolation in the nine
+// Chebyshev points. A running sum is moved by as little, far below the distance of its borders. Whole numbers
+// are split off and put into the exponent by additions alone. What is below 2^-1000, -inf too, gives 2^-1000: nothing
+// beside a largest weight of 1, but not 0 (tv_none).
+__device__ __forceinline__ double tv_exp2(double y) {
+    y = fmax(y, -1000.0);
+    const double big = 6755399441055744.0, t = y + big, f = y - (t - big);  // 1.5 * 2^52
+    double p = 1.3255224887698904e-06;
+    p = fma(p, f, 1.5310079402479794e-05);
+    p = fma(p, f, 1.5403455852411408e-04);
+    p = fma(p, f, 1.3333450567999659e-03);
+    p = fma(p, f, 9.6181291594026191e-03);
+    p = fma(p, f, 5.5504109412059341e-02);
+    p = fma(p, f, 2.4022650695812989e-01);
+    p = fma(p, f, 6.9314718054593349e-01);
+    p = fma(p, f, 1.0);
+    return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
+}
+__device__ __forceinline__ bool tv_none(float x) { return x == -INFINITY; }
 
 __device__ __forceinline__ double tv_sum64(double x) {
 #pragma unroll
@@ -40,88 +63,66 @@ __device__ __forceinline__ float tv_max64(float x) {
     return x;
 }
 
-// A law: logits of a row, its maximum and 1 / (sum of exp((x - maximum) / T)).
+// A row of logits; `skew` floats lie between the 16-byte border in front of it and its first.
+struct TvRow {
+    const float *x;
+    uint32_t len, skew;
+    __device__ __forceinline__ TvRow(const float *x, uint32_t len)
+        : x(x), len(len), skew(((uint32_t)(uintptr_t)x >> 2) & 3) {}
+    // Four logits from place e (a multiple of 4 counted from the border); places outside the row give -inf.
+    __device__ __forceinline__ float4 four(uint32_t e) const {
+        if (e >= skew && e - skew + 4 <= len) return *(const float4 *)(x + (e - skew));
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t i = e + k - skew;  // (below 0: large)
+            v[k] = i < len ? x[i] : -INFINITY;
+        }
+        return make_float4(v[0], v[1], v[2], v[3]);
+    }
+    // The 4096 places from e0: four times four a thread.
+    __device__ __forceinline__ void piece(uint32_t e0, float4 (&v)[4]) const {
+        if (e0 >= skew && e0 - skew + 4096 <= len) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = *(const float4 *)(x + (e0 - skew + 1024 * k + 4 * threadIdx.x));
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = four(e0 + 1024 * k + 4 * threadIdx.x);
+        }
+    }
+};
+__device__ __forceinline__ TvRow tv_target(const TreeVerifyArgs &a, uint32_t row) {
+    return TvRow(a.target + (size_t)row * a.target_stride, a.vocab);
+}
+__device__ __forceinline__ TvRow tv_draft(const TreeVerifyArgs &a, uint32_t row) {
+    return TvRow(a.draft + (size_t)row * a.draft_stride, a.draft_vocab);
+}
+
+// Its law: probability of a logit x is 2^(x c - top) inv.
 struct TvLaw {
-    const float *row;
-    double top, inv;  // inv 0: no law (a logit that is no number or +inf, or no finite one)
-    __device__ __forceinline__ double at(float x, double inv_t) const { return exp(((double)x - top) * inv_t) * inv; }
+    double top, inv;  // inv 0: no law (a logit that is no number or +inf, or none that is finite)
+    __device__ __forceinline__ double at(const TreeVerifyArgs &a, float x) const {
+        return tv_none(x) ? 0.0 : tv_exp2(fma((double)x, a.c, -top)) * inv;
+    }
 };
 
-// Parts' statistics of one row joined by a wave: TreeStat of `parts` parts.
-__device__ __forceinline__ TvLaw tv_law(const float *row, const TreeStat *s, uint32_t parts, double inv_t) {
+// Parts' statistics of one row joined by a wave.
+__device__ __forceinline__ TvLaw tv_law(const TreeVerifyArgs &a, const TreeStat *s, uint32_t parts) {
     const uint32_t lane = threadIdx.x & 63;
     TreeStat x{0.0, -INFINITY, 0};
     if (lane < parts) x = s[lane];
     const float top = tv_max64(x.top);
     const bool bad = __builtin_amdgcn_ballot_w64(x.bad) || !(fabsf(top) < INFINITY);
-    const double sum = tv_sum64(x.sum > 0.0 ? x.sum * exp(((double)x.top - (double)top) * inv_t) : 0.0);
-    return {row, (double)top, bad ? 0.0 : 1.0 / sum};
+    const double tops = (double)top * a.c;
+    const double sum = tv_sum64(x.sum > 0.0 ? x.sum * tv_exp2(fma((double)x.top, a.c, -tops)) : 0.0);
+    return {tops, bad ? 0.0 : 1.0 / sum};
 }
-
-// What the tests of one row leave, in every lane of the wave that makes them.
-struct TvTests {
-    double lambda, left;   // of the refusals so far; left = Z
-    int chosen;            // the accepted child (its number in the request), or -1
-    uint32_t refused;      // how many were
-    bool bad, stuck;       // stuck: the next test waits for the sum of round `refused`
-};
-
-struct TvRow {
-    uint32_t row;        // in the batch
-    uint64_t children;   // of the node, by their numbers
-};
 
 __device__ __forceinline__ bool tv_point(const TreeVerifyArgs &a) { return a.draft == nullptr; }
 
-__device__ __forceinline__ double tv_draft_at(const TreeVerifyArgs &a, const TvLaw &q, uint32_t token) {
-    uint32_t i = token;
-    if (a.inverse) i = a.inverse[token];
-    return i < a.draft_vocab ? q.at(q.row[i], a.inv_t) : 0.0;
-}
-
-// Tests the children of a row as far as the sums of rounds 1 .. rounds go. All lanes of a wave call it.
-__device__ __forceinline__ TvTests tv_tests(const TreeVerifyArgs &a, const TreeRows &q, const TvRow &n, const TvLaw &p,
-                                            const TvLaw &d, uint32_t rounds) {
-    const uint32_t lane = threadIdx.x & 63;
-    TvTests t{0.0, 1.0, -1, 0, p.inv == 0.0 || (n.children && !tv_point(a) && d.inv == 0.0), false};
-    if (t.bad) return t;
-    double undrawn = 1.0;
-    uint64_t rest = n.children;
-    for (uint32_t k = 0; rest && k < a.width; k++) {
-        if (!(undrawn > TV_LEAST)) break;
-        if (k) {  // the sum after k refusals
-            if (k > rounds) {
-                t.stuck = true;
-                break;
-            }
-            const double *z = a.rest + ((size_t)(k - 1) * a.rows + n.row) * a.parts;
-            t.left = tv_sum64(lane < a.parts ? z[lane] : 0.0);
-        }
-        const int child = __ffsll((unsigned long long)rest) - 1;
-        rest &= rest - 1;
-        const uint32_t token = a.tokens[q.row0 + child];
-        double pt = 0.0, qt = tv_point(a) ? 1.0 : 0.0;
-        bool tried = false;
-        if (token < a.vocab) {
-            pt = p.at(p.row[token], a.inv_t);
-            if (!tv_point(a)) qt = tv_draft_at(a, d, token);
-        }
-        if (tv_point(a)) {  // a token that was tried is left with nothing
-            uint64_t m = n.children & ((1ull << child) - 1);
-            for (; m; m &= m - 1) tried |= a.tokens[q.row0 + __ffsll((unsigned long long)m) - 1] == token;
-        }
-        const double r = tv_point(a) ? (tried ? 0.0 : pt) : fmax(pt - t.lambda * qt, 0.0);
-        if ((double)a.accept[q.row0 + child] * (qt / undrawn) * t.left < r) {
-            t.chosen = child;
-            break;
-        }
-        t.refused = k + 1;
-        if (!tv_point(a)) {
-            t.lambda += t.left / undrawn;
-            if (a.without) undrawn -= qt;
-        }
-    }
-    return t;
+__device__ __forceinline__ double tv_draft_at(const TreeVerifyArgs &a, const TvLaw &q, const float *x, uint32_t token) {
+    const uint32_t i = a.inverse ? a.inverse[token] : token;
+    return i < a.draft_vocab ? q.at(a, x[i]) : 0.0;
 }
 
 // Children of node `local`: lanes hold the nodes' parents.
@@ -129,122 +130,300 @@ __device__ __forceinline__ uint64_t tv_children(int parent, uint32_t local) {
     return __builtin_amdgcn_ballot_w64(parent == (int)local);
 }
 
-// ---------------------------------------------------------------------------
-// statistics of a part
-// ---------------------------------------------------------------------------
 // Order of f32 numbers, as f32::total_cmp.
 __device__ __forceinline__ int32_t tv_key(float v) {
     const int32_t b = __float_as_int(v);
     return b ^ (int32_t)(((uint32_t)(b >> 31)) >> 1);
 }
+__device__ __forceinline__ void tv_larger(float &top, uint32_t &id, float t, uint32_t i) {  // the later one wins ties
+    if (tv_key(t) > tv_key(top) || (tv_key(t) == tv_key(top) && i > id)) {
+        top = t;
+        id = i;
+    }
+}
+
+// Marks are written and read in one round: whole 64-bit words.
+__device__ __forceinline__ TreeMark tv_mark(const TreeVerifyArgs &a, uint32_t row) {
+    return __builtin_bit_cast(TreeMark, __hip_atomic_load(a.marks + row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+__device__ __forceinline__ void tv_set_mark(const TreeVerifyArgs &a, uint32_t row, TreeMark m) {
+    __hip_atomic_store(a.marks + row, __builtin_bit_cast(uint64_t, m), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+struct TvScratch {
+    double sums[4];
+    float tops[4];
+    uint32_t ids[4], bads[4];
+};
+
+// Statistics of parts first .. last - 1 of a row, by a workgroup of 256.
+__device__ __forceinline__ void tv_stats(const TreeVerifyArgs &a, const TvRow &row, uint32_t first, uint32_t last,
+                                         uint32_t size, TreeStat *out, TvScratch &L) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t end = min(last * size, row.len + row.skew);
+    float top = -INFINITY;  // of the wave; greedy: of the thread
+    double sum = 0.0;
+    uint32_t id = 0;
+    bool bad = false;
+    float4 v[4], next[4];
+    row.piece(first * size, next);
+    for (uint32_t e0 = first * size; e0 < end; e0 += 4096) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = next[k];
+        if (e0 + 4096 < end) row.piece(e0 + 4096, next);  // (under way during this piece's exponentials)
+        const float *x = (const float *)v;
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 16; k++) {
+            bad |= !(x[k] < INFINITY);
+            m = fmaxf(m, x[k]);
+        }
+        if (a.greedy) {
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const uint32_t i = e0 + 1024 * (k >> 2) + 4 * tid + (k & 3) - row.skew;
+                if (i < row.len) tv_larger(top, id, x[k], i);
+            }
+        } else {
+            m = tv_max64(m);
+            if (m > top) {
+                sum = top > -INFINITY ? sum * tv_exp2(((double)top - (double)m) * a.c) : 0.0;
+                top = m;
+            }
+            const double t = (double)top * a.c;
+            double s[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+            for (int k = 0; k < 16; k++) s[k & 3] += tv_exp2(fma((double)x[k], a.c, -t));
+            if (top > -INFINITY) sum += (s[0] + s[1]) + (s[2] + s[3]);
+        }
+        if ((e0 + 4096) % size && e0 + 4096 < end) continue;
+        // ---- the part's end ----
+        const uint32_t any = __builtin_amdgcn_ballot_w64(bad) != 0;
+        if (a.greedy) {
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) tv_larger(top, id, __shfl_xor(top, o), __shfl_xor(id, o));
+        } else {
+            sum = tv_sum64(sum);
+        }
+        if (lane == 0) {
+            L.sums[wave] = sum;
+            L.tops[wave] = top;
+            L.ids[wave] = id;
+            L.bads[wave] = any;
+        }
+        lds_barrier();
+        if (tid == 0) {
+            if (a.greedy) {
+                for (int w = 1; w < 4; w++) tv_larger(top, id, L.tops[w], L.ids[w]);
+                sum = (double)id;
+            } else {
+                const float t = fmaxf(fmaxf(L.tops[0], L.tops[1]), fmaxf(L.tops[2], L.tops[3]));
+                sum = 0.0;
+                for (int w = 0; w < 4; w++)
+                    if (L.sums[w] > 0.0) sum += L.sums[w] * tv_exp2(((double)L.tops[w] - (double)t) * a.c);
+                top = t;
+            }
+            out[e0 / size] = TreeStat{sum, top, L.bads[0] | L.bads[1] | L.bads[2] | L.bads[3]};
+        }
+        lds_barrier();
+        top = -INFINITY, sum = 0.0, id = 0, bad = false;
+    }
+}
 
 // grid (parts, rows, 1 or 2: target, draft)
 extern "C" __global__ __launch_bounds__(256) void ctox_tree_stats_gfx950(TreeVerifyArgs a) {
-    __shared__ float tops[4];
-    __shared__ double sums[4];
-    __shared__ uint32_t ids[4], bads[4];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y, part = blockIdx.x;
+    __shared__ TvScratch L;
+    const uint32_t row = blockIdx.y, part = blockIdx.x;
+    if (!a.greedy && blockIdx.x + blockIdx.y + blockIdx.z == 0 && threadIdx.x < CTOX_TREE_NODES) a.waiting[threadIdx.x] = 0;
     if (row >= min(a.row_starts[a.requests], a.rows) || row < a.row_starts[0]) return;
     const bool draft = blockIdx.z != 0;
-    const uint32_t len = draft ? a.draft_vocab : a.vocab, parts = draft ? a.draft_parts : a.parts;
-    const uint32_t size = draft ? a.draft_part : a.part;
-    if (part >= parts) return;
-    if (draft) {  // of nodes with children only
+    if (part >= (draft ? a.draft_parts : a.stat_parts)) return;
+    if (!a.greedy) {  // a leaf is read when it is accepted
         const uint32_t r = tree_request(a.row_starts, a.requests, row);
         const TreeRows q = tree_rows(a.row_starts, r, a.rows);
-        if (!tv_children(tree_parent(a.parents, q, lane), row - q.row0)) return;
+        const bool any = tv_children(tree_parent(a.parents, q, threadIdx.x & 63), row - q.row0) != 0;
+        if (!any && (draft || row != q.row0)) return;
     }
-    const float *x = (draft ? a.draft + (size_t)row * a.draft_stride : a.target + (size_t)row * a.target_stride);
-    TreeStat *out = (draft ? a.draft_stats + (size_t)row * a.draft_parts : a.stats + (size_t)row * a.parts) + part;
-    const uint32_t b = part * size, e = min(len, b + size);
-    float top = -INFINITY;
-    uint32_t id = 0;
-    bool bad = false;
-    for (uint32_t i = b + tid; i < e; i += 256) {
-        const float v = x[i];
-        bad |= !(v < INFINITY);
-        if (tv_key(v) >= tv_key(top)) {  // (a later one wins)
-            top = v;
-            id = i;
-        }
-    }
-    const float mine = top;
+    if (draft) tv_stats(a, tv_draft(a, row), part, part + 1, a.draft_part, a.draft_stats + (size_t)row * a.draft_parts, L);
+    else tv_stats(a, tv_target(a, row), part, part + 1, a.stat_part, a.stats + (size_t)row * a.parts, L);
+}
+
+// ---------------------------------------------------------------------------
+// a round of tests
+// ---------------------------------------------------------------------------
+// Weights of tokens after `refused` refusals; tried: the tokens of the first `refused` children (point laws).
+struct TvRest {
+    const TreeVerifyArgs &a;
+    const TvRow p;
+    const float *q;
+    const TvLaw pl, ql;
+    const double lambda;
+    const uint32_t refused;
+    const uint32_t *tried;
+    // of the four places from e, whose logits are v
+    __device__ __forceinline__ void four(uint32_t e, const float4 &v, double (&w)[4]) const {
+        const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float t = __shfl_xor(top, o);
-        const uint32_t j = __shfl_xor(id, o);
-        if (tv_key(t) > tv_key(top) || (tv_key(t) == tv_key(top) && j > id)) {
-            top = t;
-            id = j;
+        for (int k = 0; k < 4; k++) w[k] = pl.at(a, x[k]);
+        if (!refused) return;
+        const uint32_t i0 = e - p.skew;
+        if (tv_point(a)) {
+            for (uint32_t t = 0; t < refused; t++) {
+                const uint32_t k = tried[t] - i0;
+                w[0] = k == 0 ? 0.0 : w[0];
+                w[1] = k == 1 ? 0.0 : w[1];
+                w[2] = k == 2 ? 0.0 : w[2];
+                w[3] = k == 3 ? 0.0 : w[3];
+            }
+            return;
         }
-    }
-    (void)mine;
-    const uint32_t any = __builtin_amdgcn_ballot_w64(bad) != 0;
-    if (lane == 0) tops[wave] = top, ids[wave] = id, bads[wave] = any;
-    __syncthreads();
-    top = tops[0];
-    id = ids[0];
-    for (int w = 1; w < 4; w++)
-        if (tv_key(tops[w]) > tv_key(top) || (tv_key(tops[w]) == tv_key(top) && ids[w] > id)) {
-            top = tops[w];
-            id = ids[w];
+        float y[4];
+        if (!a.inverse && i0 + 4 <= p.len && i0 < p.len && ((uintptr_t)(q + i0) & 15) == 0) {
+            const float4 u = *(const float4 *)(q + i0);
+            y[0] = u.x, y[1] = u.y, y[2] = u.z, y[3] = u.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                uint32_t i = i0 + k;
+                if (i < p.len && a.inverse) i = a.inverse[i];
+                y[k] = i0 + k < p.len && i < a.draft_vocab ? q[i] : -INFINITY;
+            }
         }
-    const bool some_bad = bads[0] | bads[1] | bads[2] | bads[3];
-    double sum = 0.0;
-    if (a.greedy) {
-        if (tid == 0) *out = TreeStat{(double)id, top, some_bad};
-        return;
+#pragma unroll
+        for (int k = 0; k < 4; k++) w[k] = fmax(fma(-lambda, ql.at(a, y[k]), w[k]), 0.0);
     }
-    if (top > -INFINITY && !some_bad)
-        for (uint32_t i = b + tid; i < e; i += 256) sum += exp(((double)x[i] - (double)top) * a.inv_t);
-    sum = tv_sum64(sum);
-    if (lane == 0) sums[wave] = sum;
-    __syncthreads();
-    if (tid == 0) *out = TreeStat{(sums[0] + sums[1]) + (sums[2] + sums[3]), top, some_bad};
-}
+};
 
-// ---------------------------------------------------------------------------
-// what k refusals leave
-// ---------------------------------------------------------------------------
-// The weight of token i after `refused` refusals; tried: the tokens of the first `refused` children (point laws).
-__device__ __forceinline__ double tv_weight(const TreeVerifyArgs &a, const TvLaw &p, const TvLaw &d, uint32_t i,
-                                            double lambda, uint32_t refused, const uint32_t *tried) {
-    double w = p.at(p.row[i], a.inv_t);
-    if (!refused) return w;
-    if (!tv_point(a)) return fmax(w - lambda * tv_draft_at(a, d, i), 0.0);
-    for (uint32_t k = 0; k < refused; k++)
-        if (tried[k] == i) w = 0.0;
-    return w;
-}
-
-// grid (parts, rows)
-extern "C" __global__ __launch_bounds__(256) void ctox_tree_rest_gfx950(TreeVerifyArgs a) {
-    __shared__ double sums[4];
-    __shared__ uint32_t tried[CTOX_TREE_NODES];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y, part = blockIdx.x;
-    if (row >= min(a.row_starts[a.requests], a.rows) || row < a.row_starts[0]) return;
+// The test of a row's child number k = a.round - 1 and what follows it, in parts first .. last - 1.
+__device__ __forceinline__ void tv_round(const TreeVerifyArgs &a, uint32_t row, uint32_t first, uint32_t last,
+                                         TvScratch &L, uint32_t (&tried)[CTOX_TREE_NODES]) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.round - 1;
+    const bool chief = first == 0 && tid == 0;  // keeps the row's records
     const uint32_t r = tree_request(a.row_starts, a.requests, row);
     const TreeRows q = tree_rows(a.row_starts, r, a.rows);
-    const TvRow n{row, tv_children(tree_parent(a.parents, q, lane), row - q.row0)};
-    if ((uint32_t)__popcll(n.children) < a.round) return;
-    const TvLaw p = tv_law(a.target + (size_t)row * a.target_stride, a.stats + (size_t)row * a.parts, a.parts, a.inv_t);
-    TvLaw d{nullptr, 0.0, 0.0};
-    if (!tv_point(a))
-        d = tv_law(a.draft + (size_t)row * a.draft_stride, a.draft_stats + (size_t)row * a.draft_parts, a.draft_parts, a.inv_t);
-    const TvTests t = tv_tests(a, q, n, p, d, a.round - 1);
-    if (t.bad || t.chosen >= 0 || t.refused != a.round) return;
-    if (tid == 0) {
-        uint64_t m = n.children;
-        for (uint32_t k = 0; k < t.refused; k++, m &= m - 1) tried[k] = a.tokens[q.row0 + __ffsll((unsigned long long)m) - 1];
+    const int parent = tree_parent(a.parents, q, lane);
+    const uint64_t children = tv_children(parent, row - q.row0);
+    TreeRow s{0.0, 1.0, 0.0, 0.0, 0.0, 0.0};
+    if (k) {
+        s = a.states[(size_t)(k & 1) * a.rows + row];
+    } else if (!children) {
+        if (chief) tv_set_mark(a, row, TreeMark{-1, 0});
+        return;
     }
-    __syncthreads();
-    const uint32_t b = part * a.part, e = min(a.vocab, b + a.part);
-    double sum = 0.0;
-    for (uint32_t i = b + tid; i < e; i += 256) sum += tv_weight(a, p, d, i, t.lambda, t.refused, tried);
-    sum = tv_sum64(sum);
-    if (lane == 0) sums[wave] = sum;
-    __syncthreads();
-    if (tid == 0) a.rest[((size_t)(a.round - 1) * a.rows + row) * a.parts + part] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    uint64_t rest = children;
+    for (uint32_t i = 0; i < k; i++) rest &= rest - 1;
+    const TvRow p = tv_target(a, row);
+    const float *x = tv_point(a) ? nullptr : a.draft + (size_t)row * a.draft_stride;
+    const int child = __ffsll((unsigned long long)rest) - 1;
+    rest &= rest - 1;
+    const uint32_t token = a.tokens[q.row0 + child];
+    const float px = p.x[min(token, a.vocab - 1)];
+    double left = 1.0;
+    TvLaw pl, ql{0.0, 0.0};
+    if (k) {
+        left = tv_sum64(lane < a.parts ? a.rest[((size_t)(k - 1) * a.rows + row) * a.parts + lane] : 0.0);
+        pl = {s.p_top, s.p_inv};
+        ql = {s.q_top, s.q_inv};
+    } else {
+        pl = tv_law(a, a.stats + (size_t)row * a.parts, a.stat_parts);
+        if (!tv_point(a)) ql = tv_law(a, a.draft_stats + (size_t)row * a.draft_parts, a.draft_parts);
+        s.p_top = pl.top, s.p_inv = pl.inv, s.q_top = ql.top, s.q_inv = ql.inv;
+        if (pl.inv == 0.0 || (!tv_point(a) && ql.inv == 0.0)) {
+            if (chief) tv_set_mark(a, row, TreeMark{-2, 0});
+            return;
+        }
+    }
+    double pt = 0.0, qt = tv_point(a) ? 1.0 : 0.0;
+    if (token < a.vocab) {
+        pt = pl.at(a, px);
+        if (!tv_point(a)) qt = tv_draft_at(a, ql, x, token);
+    }
+    if (tv_point(a)) {  // a token that was tried is left with nothing
+        const uint64_t before = children & ((1ull << child) - 1);
+        if (__builtin_amdgcn_ballot_w64((before >> lane & 1) && a.tokens[q.row0 + lane] == token)) pt = 0.0;
+    } else {
+        pt = fmax(pt - s.lambda * qt, 0.0);
+    }
+    const bool accepted = (double)a.accept[q.row0 + child] * (qt / s.undrawn) * left < pt;
+    if (accepted) {
+        if (chief) tv_set_mark(a, row, TreeMark{child, k});
+        if (tv_children(parent, (uint32_t)child)) return;
+        const uint32_t leaf = q.row0 + child;
+        tv_stats(a, tv_target(a, leaf), first, last, a.part, a.stats + (size_t)leaf * a.parts, L);
+        return;
+    }
+    if (!tv_point(a)) {
+        s.lambda += left / s.undrawn;
+        if (a.without) s.undrawn -= qt;
+    }
+    if (chief) {
+        tv_set_mark(a, row, TreeMark{-1, k + 1});
+        a.states[(size_t)(a.round & 1) * a.rows + row] = s;
+        // The next round's rows; in which order does not matter.
+        if (rest && a.round < a.width && s.undrawn > TV_LEAST) {
+            const uint32_t at = atomicAdd(&a.waiting[a.round], 1u);
+            a.lists[(size_t)(a.round & 1) * a.rows + at] = row;
+        }
+    }
+    if (tv_point(a)) {
+        if (wave == 0 && (children >> lane & 1)) {
+            const uint32_t at = __popcll(children & ((1ull << lane) - 1));
+            tried[at] = a.tokens[q.row0 + lane];
+        }
+        lds_barrier();
+    }
+    const TvRest f{a, p, x, pl, ql, s.lambda, k + 1, tried};
+    for (uint32_t part = first; part < last; part++) {
+        double sum = 0.0;
+        for (uint32_t e0 = part * a.part; e0 < (part + 1) * a.part && e0 < p.len + p.skew; e0 += 4096) {
+            float4 v[4];
+            p.piece(e0, v);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                double w[4];
+                f.four(e0 + 1024 * i + 4 * tid, v[i], w);
+                sum += (w[0] + w[1]) + (w[2] + w[3]);
+            }
+        }
+        sum = tv_sum64(sum);
+        if (lane == 0) L.sums[wave] = sum;
+        lds_barrier();
+        if (tid == 0)
+            a.rest[((size_t)k * a.rows + row) * a.parts + part] = (L.sums[0] + L.sums[1]) + (L.sums[2] + L.sums[3]);
+        lds_barrier();
+    }
+}
+
+// Round 1: grid (groups of a.per parts, rows)
+extern "C" __global__ __launch_bounds__(256) void ctox_tree_first_gfx950(TreeVerifyArgs a) {
+    __shared__ TvScratch L;
+    __shared__ uint32_t tried[CTOX_TREE_NODES];
+    const uint32_t row = blockIdx.y, first = blockIdx.x * a.per;
+    if (row >= min(a.row_starts[a.requests], a.rows) || row < a.row_starts[0]) return;
+    tv_round(a, row, first, min(first + a.per, a.parts), L, tried);
+}
+
+// The rounds after it: grid (parts, CTOX_TREE_LANES), which take the rows that wait in turn.
+extern "C" __global__ __launch_bounds__(256) void ctox_tree_round_gfx950(TreeVerifyArgs a) {
+    __shared__ TvScratch L;
+    __shared__ uint32_t tried[CTOX_TREE_NODES];
+    const uint32_t waiting = a.waiting[a.round - 1];
+    for (uint32_t i = blockIdx.y; i < waiting; i += CTOX_TREE_LANES) {
+        const uint32_t row = a.lists[(size_t)((a.round - 1) & 1) * a.rows + i];
+        // Where another child was accepted above it the row is not on the path, whatever it accepts. Marks of this
+        // round may be there already or not, so they do not count: every workgroup decides the same.
+        const uint32_t lane = threadIdx.x & 63;
+        const TreeRows q = tree_rows(a.row_starts, tree_request(a.row_starts, a.requests, row), a.rows);
+        const int parent = tree_parent(a.parents, q, lane);
+        TreeMark m{-1, 0};
+        if (lane < q.n) m = tv_mark(a, q.row0 + lane);
+        const int accepted = m.refused < a.round - 1 ? m.chosen : -1;
+        const int above = __shfl(accepted, parent < 0 ? (int)lane : parent);
+        const uint64_t line = __shfl(tree_lineage(parent, lane, lane < q.n), (int)((row - q.row0) & 63));
+        if (__builtin_amdgcn_ballot_w64((line >> lane & 1) && parent >= 0 && above != -1 && above != (int)lane)) continue;
+        tv_round(a, row, blockIdx.x, blockIdx.x + 1, L, tried);
+        lds_barrier();
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -253,14 +432,12 @@ extern "C" __global__ __launch_bounds__(256) void ctox_tree_rest_gfx950(TreeVeri
 // grid (requests), 1024 threads
 extern "C" __global__ __launch_bounds__(1024) void ctox_tree_walk_gfx950(TreeVerifyArgs a) {
     __shared__ int chosen[CTOX_TREE_NODES];
-    __shared__ uint32_t refused[CTOX_TREE_NODES], best[CTOX_TREE_NODES], tried[CTOX_TREE_NODES];
-    __shared__ double lambda[CTOX_TREE_NODES], sums[16];
-    __shared__ uint32_t end, total_nodes, pick, found;
-    __shared__ double want;
+    __shared__ uint32_t best[CTOX_TREE_NODES], tried[CTOX_TREE_NODES];
+    __shared__ double sums[16];
+    __shared__ uint32_t found;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x;
     const TreeRows all = tree_rows(a.row_starts, r, a.rows);
     const TreeRows q{all.row0, min(all.n, (uint32_t)CTOX_TREE_NODES)};
-    for (uint32_t i = tid; i < all.n; i += 1024) a.path[all.row0 + i] = CTOX_NO_SLOT;
     if (q.n == 0) {
         if (tid == 0) {
             a.counts[r] = 0;
@@ -269,95 +446,79 @@ extern "C" __global__ __launch_bounds__(1024) void ctox_tree_walk_gfx950(TreeVer
         return;
     }
     const int parent = tree_parent(a.parents, q, lane);
-    for (uint32_t i = wave; i < q.n; i += 16) {
-        const TvRow n{q.row0 + i, tv_children(parent, i)};
-        if (a.greedy) {
+    if (a.greedy) {
+        for (uint32_t i = wave; i < q.n; i += 16) {
             TreeStat x{0.0, -INFINITY, 0};
-            if (lane < a.parts) x = a.stats[(size_t)n.row * a.parts + lane];
+            if (lane < a.stat_parts) x = a.stats[(size_t)(q.row0 + i) * a.parts + lane];
             float top = x.top;
             uint32_t id = (uint32_t)x.sum;
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) {
-                const float t = __shfl_xor(top, o);
-                const uint32_t j = __shfl_xor(id, o);
-                if (tv_key(t) > tv_key(top) || (tv_key(t) == tv_key(top) && j > id)) {
-                    top = t;
-                    id = j;
-                }
-            }
+            for (int o = 32; o > 0; o >>= 1) tv_larger(top, id, __shfl_xor(top, o), __shfl_xor(id, o));
             const bool bad = __builtin_amdgcn_ballot_w64(x.bad) || !(fabsf(top) < INFINITY);
-            uint64_t m = n.children;
-            int c = -1;
-            for (uint32_t k = 0; m && k < a.width && c < 0; k++, m &= m - 1) {
-                const int child = __ffsll((unsigned long long)m) - 1;
-                if (a.tokens[q.row0 + child] == id) c = child;
-            }
+            const uint64_t children = tv_children(parent, i);
+            // the first of the children that are offered
+            const bool offered = (children >> lane & 1) && (uint32_t)__popcll(children & ((1ull << lane) - 1)) < a.width;
+            const uint64_t same = __builtin_amdgcn_ballot_w64(offered && a.tokens[q.row0 + lane] == id);
             if (lane == 0) {
-                chosen[i] = bad ? -2 : c;
+                chosen[i] = bad ? -2 : __ffsll((unsigned long long)same) - 1;
                 best[i] = id;
             }
-            continue;
         }
-        const TvLaw p = tv_law(a.target + (size_t)n.row * a.target_stride, a.stats + (size_t)n.row * a.parts, a.parts, a.inv_t);
-        TvLaw d{nullptr, 0.0, 0.0};
-        if (!tv_point(a) && n.children)
-            d = tv_law(a.draft + (size_t)n.row * a.draft_stride, a.draft_stats + (size_t)n.row * a.draft_parts,
-                       a.draft_parts, a.inv_t);
-        const TvTests t = tv_tests(a, q, n, p, d, a.width);
-        if (lane == 0) {
-            chosen[i] = t.bad ? -2 : t.chosen;
-            refused[i] = t.refused;
-            lambda[i] = t.lambda;
-        }
+    } else if (tid < q.n) {
+        chosen[tid] = tv_mark(a, q.row0 + tid).chosen;
     }
+    if (tid == 0) found = ~0u;
     __syncthreads();
-    if (tid == 0) {
-        uint32_t at = 0, count = 1;
-        a.path[q.row0] = 0;
-        while (chosen[at] >= 0) {  // (children have larger numbers: it ends)
-            at = (uint32_t)chosen[at];
-            a.path[q.row0 + count++] = at;
-        }
-        end = at;
-        total_nodes = chosen[at] == -2 ? 0 : count;
+    // Every thread walks for itself (children have larger numbers: it ends).
+    uint32_t node = 0, count = 1;
+    uint64_t on = 1;
+    while (chosen[node] >= 0) {
+        node = (uint32_t)chosen[node];
+        on |= 1ull << node;
+        count++;
     }
-    __syncthreads();
-    if (total_nodes == 0) {  // logits that are no numbers on the path: nothing is accepted
-        for (uint32_t i = tid; i < q.n; i += 1024) a.path[q.row0 + i] = CTOX_NO_SLOT;
-        if (tid == 0) {
-            a.counts[r] = 0;
-            a.next[r] = CTOX_TREE_FAILED;
-        }
-        return;
-    }
-    if (tid == 0) a.counts[r] = total_nodes;
-    if (a.greedy) {
-        if (tid == 0) a.next[r] = best[end];
-        return;
-    }
-    const uint32_t node = end, row = q.row0 + node;
-    uint32_t gone = refused[node];
+    const uint32_t row = q.row0 + node;
+    bool failed = chosen[node] == -2;
+    TreeRow s{0.0, 1.0, 0.0, 0.0, 0.0, 0.0};
+    TvLaw pl{0.0, 0.0}, ql{0.0, 0.0};
     const uint64_t children = tv_children(parent, node);
-    const TvLaw p = tv_law(a.target + (size_t)row * a.target_stride, a.stats + (size_t)row * a.parts, a.parts, a.inv_t);
-    TvLaw d{nullptr, 0.0, 0.0};
-    if (gone && !tv_point(a))
-        d = tv_law(a.draft + (size_t)row * a.draft_stride, a.draft_stats + (size_t)row * a.draft_parts, a.draft_parts, a.inv_t);
-    if (tid == 0) {
-        uint64_t m = children;
-        for (uint32_t k = 0; k < gone; k++, m &= m - 1) tried[k] = a.tokens[q.row0 + __ffsll((unsigned long long)m) - 1];
-        found = ~0u;
+    // A leaf below the root has the statistics that the round of its test made.
+    const bool late = !children && node;
+    const uint32_t stats = late ? a.parts : a.stat_parts;
+    uint32_t gone = 0;
+    if (!a.greedy && !failed) {
+        if (children) {
+            gone = tv_mark(a, row).refused;  // (one at least: a child was offered, and none accepted)
+            s = a.states[(size_t)(gone & 1) * a.rows + row];
+            pl = {s.p_top, s.p_inv};
+            ql = {s.q_top, s.q_inv};
+        } else {
+            pl = tv_law(a, a.stats + (size_t)row * a.parts, stats);
+            failed = pl.inv == 0.0;
+        }
     }
+    // (the path rises: a node's place is the number of its nodes in front)
+    if (failed) on = 0, count = 0;
+    for (uint32_t i = tid; i < all.n; i += 1024)
+        if (i >= count) a.path[all.row0 + i] = CTOX_NO_SLOT;
+    if (tid < 64 && (on >> tid & 1)) a.path[q.row0 + __popcll(on & ((1ull << tid) - 1))] = tid;
+    if (tid == 0) a.counts[r] = count;
+    if (failed || a.greedy) {
+        if (tid == 0) a.next[r] = failed ? CTOX_TREE_FAILED : best[node];
+        return;
+    }
+    if (wave == 0 && (children >> lane & 1)) tried[__popcll(children & ((1ull << lane) - 1))] = a.tokens[q.row0 + lane];
     // The part where the running sum passes the number. Where nothing is left of the target (only rounding could have
     // refused then) the target itself is drawn from.
     double mass = 0.0, in = 0.0;
     for (int again = 0; again < 2; again++) {
         mass = 0.0;
-        if (lane < a.parts) {
+        if (lane < (gone ? a.parts : stats)) {
             if (gone) {
                 mass = a.rest[((size_t)(gone - 1) * a.rows + row) * a.parts + lane];
             } else {
-                const TreeStat s = a.stats[(size_t)row * a.parts + lane];
-                mass = s.sum > 0.0 ? s.sum * exp(((double)s.top - p.top) * a.inv_t) * p.inv : 0.0;
+                const TreeStat x = a.stats[(size_t)row * a.parts + lane];
+                mass = x.sum > 0.0 ? x.sum * tv_exp2(fma((double)x.top, a.c, -pl.top)) * pl.inv : 0.0;
             }
         }
         in = mass;
@@ -374,24 +535,24 @@ extern "C" __global__ __launch_bounds__(1024) void ctox_tree_walk_gfx950(TreeVer
     const uint64_t past = __builtin_amdgcn_ballot_w64(in > goal), massive = __builtin_amdgcn_ballot_w64(mass > 0.0);
     const uint32_t part = past ? (uint32_t)__ffsll((unsigned long long)past) - 1
                                : massive ? 63 - (uint32_t)__clzll((long long)massive) : 0;
-    if (tid == part) want = goal - (in - mass);
-    if (tid == 0) pick = part;
+    const double want = goal - __shfl(in - mass, part);
     __syncthreads();
-    // That part's tokens, 4 a thread and round.
-    const uint32_t b = pick * a.part, e = min(a.vocab, b + a.part);
+    // That part's tokens, four a thread and round.
+    const TvRow p = tv_target(a, row);
+    const TvRest f{a, p, tv_point(a) ? nullptr : a.draft + (size_t)row * a.draft_stride, pl, ql, s.lambda, gone, tried};
+    const uint32_t size = gone || late ? a.part : a.stat_part;
     double before = 0.0;
-    uint32_t last = b;  // the last token with a weight, of this thread
+    uint32_t last = 0;  // the last token with a weight, of this thread
     bool has = false;
-    for (uint32_t i0 = b; i0 < e; i0 += 4096) {
-        double w[4], s = 0.0;
+    for (uint32_t e0 = part * size; e0 < (part + 1) * size && e0 < p.len + p.skew; e0 += 4096) {
+        double w[4];
+        f.four(e0 + 4 * tid, p.four(e0 + 4 * tid), w);
+        const uint32_t i0 = e0 + 4 * tid - p.skew;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const uint32_t i = i0 + 4 * tid + k;
-            w[k] = i < e ? tv_weight(a, p, d, i, lambda[node], gone, tried) : 0.0;
-            if (w[k] > 0.0) last = i, has = true;
-            s += w[k];
-        }
-        double run = s;
+        for (int k = 0; k < 4; k++)
+            if (w[k] > 0.0) last = i0 + k, has = true;
+        const double sum = (w[0] + w[1]) + (w[2] + w[3]);
+        double run = sum;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const double x = __shfl_up(run, o);
@@ -399,7 +560,8 @@ extern "C" __global__ __launch_bounds__(1024) void ctox_tree_walk_gfx950(TreeVer
         }
         if (lane == 63) sums[wave] = run;
         __syncthreads();
-        double at = before + run - s;
+        double at = before + run - sum;
+#pragma unroll
         for (uint32_t v = 0; v < 16; v++) {
             if (v < wave) at += sums[v];
             before += sums[v];
@@ -408,7 +570,7 @@ extern "C" __global__ __launch_bounds__(1024) void ctox_tree_walk_gfx950(TreeVer
         for (int k = 0; k < 4; k++) {
             at += w[k];
             if (w[k] > 0.0 && at > want) {
-                atomicMin(&found, i0 + 4 * tid + k);
+                atomicMin(&found, i0 + k);
                 break;
             }
         }
@@ -416,7 +578,7 @@ extern "C" __global__ __launch_bounds__(1024) void ctox_tree_walk_gfx950(TreeVer
         if (found != ~0u) break;
     }
     if (found == ~0u) {  // rounding: the last token with a weight
-        __syncthreads();
+        __shared__ uint32_t pick;
         if (tid == 0) pick = 0;
         __syncthreads();
         if (has) atomicMax(&pick, last);

@@ -166,7 +166,7 @@ struct ctox_hip_backend {
                   gqa_rows = nullptr, gqa_few = nullptr, gqa_few16 = nullptr, gqa_join = nullptr,
                   gqa_tree_rows = nullptr, gqa_tree_few = nullptr, gqa_tree_few16 = nullptr, tree_plan = nullptr,
                   paged_commit = nullptr, free_clear = nullptr, free_mark = nullptr, free_list = nullptr,
-                  paged_fork = nullptr, tree_stats = nullptr, tree_rest = nullptr, tree_walk = nullptr,
+                  paged_fork = nullptr, tree_stats = nullptr, tree_first = nullptr, tree_round = nullptr, tree_walk = nullptr,
                   gdn_tree[3] = {}, gdn_tree_commit = nullptr;
     // Row products: [q4][parts - 1][shape], shapes as kRowShapes.
     hipFunction_t rows_mul[2][2][4] = {};
@@ -973,7 +973,7 @@ extern "C" ctox_status ctox_hip_backend_create(int device, ctox_hip_backend **ou
                {&b->paged_commit, "ctox_paged_commit_gfx950"}, {&b->free_clear, "ctox_free_clear_gfx950"},
                {&b->free_mark, "ctox_free_mark_gfx950"}, {&b->free_list, "ctox_free_list_gfx950"},
                {&b->paged_fork, "ctox_paged_fork_gfx950"}, {&b->tree_stats, "ctox_tree_stats_gfx950"},
-               {&b->tree_rest, "ctox_tree_rest_gfx950"}, {&b->tree_walk, "ctox_tree_walk_gfx950"},
+               {&b->tree_first, "ctox_tree_first_gfx950"}, {&b->tree_round, "ctox_tree_round_gfx950"}, {&b->tree_walk, "ctox_tree_walk_gfx950"},
                {&b->gdn_tree[0], "ctox_gdn_tree1_gfx950"}, {&b->gdn_tree[1], "ctox_gdn_tree2_gfx950"},
                {&b->gdn_tree[2], "ctox_gdn_tree4_gfx950"}, {&b->gdn_tree_commit, "ctox_gdn_tree_commit_gfx950"}};
     for (auto &f : fns) {
@@ -3292,31 +3292,45 @@ ctox_status check_verify_tree(const ctox_verify_tree *op) {
         return fail(CTOX_ERR_SHAPE, "logit rows overlap or are too far apart");
     return CTOX_OK;
 }
-// Parts of a row: of 4096 tokens, or as many times that as leave 64 (a lane each).
-uint32_t tree_part(uint32_t vocab) { return ((vocab + 63) / 64 + 4095) / 4096 * 4096; }
+// Parts of a row: of `pieces` times 4096 tokens, or as many as leave 64 parts (a lane each). A row begins up to
+// three tokens behind its first part's start.
+uint32_t tree_part(uint32_t vocab, uint32_t pieces) {
+    const uint64_t all = ((uint64_t)vocab + 3 + 4095) / 4096;
+    return 4096 * (uint32_t)std::max<uint64_t>(pieces, (all + 63) / 64);
+}
+uint32_t tree_parts(uint32_t vocab, uint32_t part) { return (uint32_t)(((uint64_t)vocab + 3 + part - 1) / part); }
 struct TreeVerifyPlan {
-    uint32_t part, parts, draft_part, draft_parts, rounds;
-    uint64_t stats, draft_stats, need;
+    uint32_t part, parts, stat_part, stat_parts, draft_part, draft_parts, rounds, per;
+    uint64_t stats, draft_stats, rest;
 };
-TreeVerifyPlan tree_verify_plan(const ctox_verify_tree *op) {
+TreeVerifyPlan tree_verify_plan(uint32_t cus, const ctox_verify_tree *op) {
     TreeVerifyPlan p{};
     const bool greedy = op->temperature == 0.0f, draft = op->draft && !greedy;
-    p.part = tree_part(op->vocab);
-    p.parts = (op->vocab + p.part - 1) / p.part;
+    p.part = tree_part(op->vocab, 1);
+    p.parts = tree_parts(op->vocab, p.part);
+    // Statistics: 32 parts a CU or fewer, half of them leaves' that are not read. (Measured us, 315 rows of 151936
+    // tokens, pieces of 1, 2, 3, 4: STATS_MEASURED; 5 rows 6.2 with 1.)
+    const uint32_t pieces = (uint32_t)std::min<uint64_t>(4, 1 + (uint64_t)op->rows * p.parts * (draft ? 2 : 1) / (32 * cus));
+    p.stat_part = tree_part(op->vocab, pieces);
+    p.stat_parts = tree_parts(op->vocab, p.stat_part);
     if (draft) {
-        p.draft_part = tree_part(op->draft_vocab);
-        p.draft_parts = (op->draft_vocab + p.draft_part - 1) / p.draft_part;
+        p.draft_part = tree_part(op->draft_vocab, pieces);
+        p.draft_parts = tree_parts(op->draft_vocab, p.draft_part);
     }
+    // A workgroup of the first round makes its row's test once for several parts.
+    p.per = (uint32_t)(1 + (uint64_t)op->rows * p.parts / (16 * cus));
     p.rounds = greedy ? 0 : op->max_children;
     p.stats = (uint64_t)op->rows * p.parts * sizeof(TreeStat);
     p.draft_stats = (uint64_t)op->rows * p.draft_parts * sizeof(TreeStat);
-    p.need = p.stats + p.draft_stats + (uint64_t)p.rounds * op->rows * p.parts * sizeof(double);
+    p.rest = (uint64_t)p.rounds * op->rows * p.parts * sizeof(double);
     return p;
 }
 // Workspace of every call of at most so many rows, tokens and children: a smaller vocabulary may have more parts.
 uint64_t tree_verify_need(const ctox_verify_tree *op) {
-    const uint64_t most = op->vocab > 64 * 4096 ? 64 : (op->vocab + 4095) / 4096;
-    return (uint64_t)op->rows * most * (2 * sizeof(TreeStat) + op->max_children * sizeof(double));
+    const uint64_t most = std::min<uint64_t>(64, ((uint64_t)op->vocab + 3 + 4095) / 4096);
+    return (uint64_t)op->rows * (most * (2 * sizeof(TreeStat) + op->max_children * sizeof(double)) +
+                                  2 * sizeof(TreeRow) + sizeof(TreeMark) + 2 * sizeof(uint32_t)) +
+           CTOX_TREE_NODES * sizeof(uint32_t);
 }
 }  // namespace
 
@@ -3335,7 +3349,7 @@ extern "C" ctox_status ctox_hip_verify_tree_device(ctox_hip_backend *b, const ct
     if (!b || !op->row_starts || !op->counts || !op->next ||
         (op->rows && (!op->target || !op->tokens || !op->parents || !op->path)) || (!greedy && (!op->accept_draws || !op->sample_draws)))
         return fail(CTOX_ERR_SHAPE, "null argument");
-    const TreeVerifyPlan p = tree_verify_plan(op);
+    const TreeVerifyPlan p = tree_verify_plan((uint32_t)b->cus, op);
     const uint64_t need = tree_verify_need(op);
     if (op->workspace_bytes < need || (need && (!op->workspace || !aligned(op->workspace, 16))))
         return fail(CTOX_ERR_MEMORY_BUDGET, "workspace of %llu bytes, %llu needed, 16-byte aligned",
@@ -3356,9 +3370,13 @@ extern "C" ctox_status ctox_hip_verify_tree_device(ctox_hip_backend *b, const ct
     a.stats = (TreeStat *)ws;
     a.draft_stats = (TreeStat *)(ws + p.stats);
     a.rest = (double *)(ws + p.stats + p.draft_stats);
+    a.states = (TreeRow *)(ws + p.stats + p.draft_stats + p.rest);
+    a.marks = (uint64_t *)(a.states + 2 * (size_t)op->rows);
+    a.lists = (uint32_t *)(a.marks + op->rows);
+    a.waiting = a.lists + 2 * (size_t)op->rows;
     a.target_stride = op->target_stride ? op->target_stride : op->vocab;
     a.draft_stride = op->draft_stride ? op->draft_stride : op->draft_vocab;
-    a.inv_t = greedy ? 1.0 : 1.0 / (double)op->temperature;
+    a.c = greedy ? 1.0 : 1.4426950408889634074 / (double)op->temperature;
     a.requests = op->requests;
     a.rows = op->rows;
     a.vocab = op->vocab;
@@ -3366,6 +3384,9 @@ extern "C" ctox_status ctox_hip_verify_tree_device(ctox_hip_backend *b, const ct
     a.parts = p.parts;
     a.draft_parts = p.draft_parts;
     a.part = p.part;
+    a.stat_parts = p.stat_parts;
+    a.stat_part = p.stat_part;
+    a.per = p.per;
     a.draft_part = p.draft_part;
     a.width = op->max_children;
     a.without = op->without_replacement != 0;
@@ -3374,10 +3395,13 @@ extern "C" ctox_status ctox_hip_verify_tree_device(ctox_hip_backend *b, const ct
     hipStream_t s = (hipStream_t)stream;
     ctox_status st = CTOX_OK;
     if (op->rows) {
-        st = launch(b->tree_stats, dim3(std::max(p.parts, p.draft_parts), op->rows, a.draft ? 2 : 1), dim3(256), s, a,
+        st = launch(b->tree_stats, dim3(std::max(p.stat_parts, p.draft_parts), op->rows, a.draft ? 2 : 1), dim3(256), s, a,
                     "ctox_tree_stats_gfx950");
         for (a.round = 1; !st && a.round <= p.rounds; a.round++)
-            st = launch(b->tree_rest, dim3(p.parts, op->rows), dim3(256), s, a, "ctox_tree_rest_gfx950");
+            st = a.round == 1 ? launch(b->tree_first, dim3((p.parts + a.per - 1) / a.per, op->rows), dim3(256), s, a,
+                                       "ctox_tree_first_gfx950")
+                              : launch(b->tree_round, dim3(p.parts, std::min<uint32_t>(CTOX_TREE_LANES, op->rows)),
+                                       dim3(256), s, a, "ctox_tree_round_gfx950");
     }
     if (!st) st = launch(b->tree_walk, dim3(op->requests), dim3(1024), s, a, "ctox_tree_walk_gfx950");
     return st;
