@@ -167,7 +167,7 @@ struct ctox_hip_backend {
                   gqa_tree_rows = nullptr, gqa_tree_few = nullptr, gqa_tree_few16 = nullptr, tree_plan = nullptr,
                   paged_commit = nullptr, free_clear = nullptr, free_mark = nullptr, free_list = nullptr,
                   paged_fork = nullptr, tree_stats = nullptr, tree_first = nullptr, tree_round = nullptr, tree_walk = nullptr,
-                  gdn_tree[3] = {}, gdn_tree_commit = nullptr;
+                  gdn_tree[2][2][3] = {}, gdn_tree_commit = nullptr;
     // Row products: [q4][parts - 1][shape], shapes as kRowShapes.
     hipFunction_t rows_mul[2][2][4] = {};
     // Batch-1 slice kernels per dtype [Q2, Q4]: [0] walks the slices, [n]
@@ -974,8 +974,7 @@ extern "C" ctox_status ctox_hip_backend_create(int device, ctox_hip_backend **ou
                {&b->free_mark, "ctox_free_mark_gfx950"}, {&b->free_list, "ctox_free_list_gfx950"},
                {&b->paged_fork, "ctox_paged_fork_gfx950"}, {&b->tree_stats, "ctox_tree_stats_gfx950"},
                {&b->tree_first, "ctox_tree_first_gfx950"}, {&b->tree_round, "ctox_tree_round_gfx950"}, {&b->tree_walk, "ctox_tree_walk_gfx950"},
-               {&b->gdn_tree[0], "ctox_gdn_tree1_gfx950"}, {&b->gdn_tree[1], "ctox_gdn_tree2_gfx950"},
-               {&b->gdn_tree[2], "ctox_gdn_tree4_gfx950"}, {&b->gdn_tree_commit, "ctox_gdn_tree_commit_gfx950"}};
+               {&b->gdn_tree_commit, "ctox_gdn_tree_commit_gfx950"}};
     for (auto &f : fns) {
         if (le != hipSuccess) break;
         le = hipModuleGetFunction(f.f, b->module, f.name);
@@ -1000,6 +999,14 @@ extern "C" ctox_status ctox_hip_backend_create(int device, ctox_hip_backend **ou
                                     hipGetErrorString(le));
                     }
                 }
+    // Gated delta over trees: by inputs of the convolution (4, 8), value columns (64, 128) and tiles of nodes.
+    for (int k = 0; k < 2 && le == hipSuccess; k++)
+        for (int w = 0; w < 2 && le == hipSuccess; w++)
+            for (int t = 0; t < 3 && le == hipSuccess; t++) {
+                char name[64];
+                std::snprintf(name, sizeof name, "ctox_gdn_tree%d%c%d_gfx950", 1 << t, w ? 'w' : 'n', k ? 8 : 4);
+                le = hipModuleGetFunction(&b->gdn_tree[k][w][t], b->module, name);
+            }
     // The small-M kernels for staged rows, one per row count 2..8.
     for (int q = 0; q < 2 && le == hipSuccess; q++)
         for (int m = 0; m < 7 && le == hipSuccess; m++)
@@ -3621,12 +3628,16 @@ extern "C" ctox_status ctox_hip_gdn_tree_device(ctox_hip_backend *b, const ctox_
     if (op->rows == 0) return CTOX_OK;
     const GdnTreeArgs a = gdn_tree_args(op);
     const uint32_t most = std::min<uint32_t>(op->max_rows ? op->max_rows : CTOX_TREE_NODES, op->rows);
-    const dim3 grid(op->heads * ((op->value_dim + 63) / 64), op->requests);
+    // 128 columns a workgroup where that still leaves the CUs one each: a head's convolution and products of nodes
+    // are then made once. (Measured, 16 trees of up to 64 nodes,
+    // 48 heads: 109 us, with 64 columns 114; one tree of 12 nodes with 64 columns 13.6.)
+    const int tiles = most <= 16 ? 0 : most <= 32 ? 1 : 2;
+    const bool wide = op->value_dim > 64 && (uint64_t)op->heads * op->requests >= (uint64_t)b->cus;
+    const uint32_t columns = wide ? 128 : 64;
     OnDevice on(b);
-    ctox_status st = CTOX_OK;
-    for (int i = 0; !st && i < 3; i++)
-        if (i == 0 || most > 16u * i) st = launch(b->gdn_tree[i], grid, dim3(256), (hipStream_t)stream, a, "ctox_gdn_tree_gfx950");
-    return st;
+    return launch(b->gdn_tree[op->kernel > 4][wide][tiles],
+                  dim3(op->heads * ((op->value_dim + columns - 1) / columns), op->requests), dim3(wide ? 512 : 256),
+                  (hipStream_t)stream, a, "ctox_gdn_tree_gfx950");
 }
 
 extern "C" ctox_status ctox_hip_gdn_tree_commit_device(ctox_hip_backend *b, const ctox_gdn_tree *op, void *stream) {
