@@ -723,6 +723,8 @@ struct PagedCommitArgs {
     uint32_t unit;               // bytes of an access: 16 or 4
 };
 
+#define CTOX_FREE_WORDS 8192     // slots / 32 of both pools that one workgroup's LDS takes
+#define CTOX_FREE_ENTRIES 16384  // and table entries that it reads in a few round trips
 struct FreeSlotsArgs {
     const PagedKvDesc *desc;
     const uint32_t *tokens;      // [requests]

@@ -10,7 +10,7 @@
 //  * ctox_free_mark_gfx950, ctox_free_list_gfx950: slots that no live page of any request holds, ascending. The tables
 //    themselves say what is in use, so shared pages need no counts: every live page sets its slot's bit
 //    (whole words, their order does not matter), then a workgroup takes 8192 slots and counts the free ones in
-//    front of them for itself.
+//    front of them for itself. ctox_free_small_gfx950 does it in one launch.
 //  * ctox_paged_fork_gfx950: a request's table copied to another's place; a last page that is part-filled is copied
 //    to a free slot in all layers. Every workgroup counts for itself how many slots the forks before its own take.
 // All are bound by launch latency and a few dependent loads.
@@ -195,6 +195,59 @@ extern "C" __global__ __launch_bounds__(256) void ctox_free_list_gfx950(FreeSlot
     if (me < words)
         for (uint32_t i = max(32 * me, total); i < min(32 * me + 32, slots); i++) list[i] = CTOX_NO_SLOT;
     if (me == 0) a.counts[kind] = total;
+}
+
+// The same by one workgroup of 1024, the bits in LDS: small tables and pools.
+extern "C" __global__ __launch_bounds__(1024) void ctox_free_small_gfx950(FreeSlotsArgs a) {
+    __shared__ uint32_t used[CTOX_FREE_WORDS], sums[16];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, all = a.requests * a.max_pages;
+    for (uint32_t i = tid; i < a.words[0] + a.words[1]; i += 1024) used[i] = 0;
+    __syncthreads();
+    for (uint32_t i0 = tid; i0 < all; i0 += 4096) {
+        PagedKvDesc d[4];
+        bool live[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {  // (four entries' loads under way at once, those of dead pages too)
+            const uint32_t i = min(i0 + 1024 * k, all - 1), r = i / a.max_pages;
+            live[k] = i0 + 1024 * k < all && (uint64_t)(i - r * a.max_pages) * a.page_tokens < a.tokens[r];
+            d[k] = a.desc[i];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t kind = d[k].precision ? 0 : 1, slot = d[k].physical_slot;
+            if (live[k] && slot < a.slots[kind]) atomicOr(&used[(kind ? a.words[0] : 0) + slot / 32], 1u << (slot & 31));
+        }
+    }
+    for (uint32_t kind = 0; kind < 2; kind++) {
+        const uint32_t words = a.words[kind], slots = a.slots[kind], per = (words + 1023) / 1024;
+        const uint32_t *bits = used + (kind ? a.words[0] : 0);
+        const uint32_t w0 = min(tid * per, words), w1 = min(w0 + per, words);
+        auto free_of = [&](uint32_t w) {
+            const uint32_t left = slots - 32 * w;
+            return ~bits[w] & (left < 32 ? (1u << left) - 1 : ~0u);
+        };
+        __syncthreads();
+        uint32_t n = 0;
+        for (uint32_t w = w0; w < w1; w++) n += __popc(free_of(w));
+        uint32_t in = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t x = __shfl_up(in, o);
+            if ((int)lane >= o) in += x;
+        }
+        if (lane == 63) sums[wave] = in;
+        __syncthreads();
+        uint32_t at = in - n, total = 0;
+        for (uint32_t w = 0; w < 16; w++) {
+            if (w < wave) at += sums[w];
+            total += sums[w];
+        }
+        uint32_t *list = a.lists[kind];
+        for (uint32_t w = w0; w < w1; w++)
+            for (uint32_t m = free_of(w); m; m &= m - 1) list[at++] = 32 * w + (uint32_t)__ffs((int)m) - 1;
+        for (uint32_t i = total + tid; i < slots; i += 1024) list[i] = CTOX_NO_SLOT;
+        if (tid == 0) a.counts[kind] = total;
+    }
 }
 
 // ---------------------------------------------------------------------------

@@ -165,7 +165,7 @@ struct ctox_hip_backend {
                   rows_max[2] = {}, rows_stage[2] = {}, rows_stage_few[2] = {}, rows_reduce = nullptr,
                   gqa_rows = nullptr, gqa_few = nullptr, gqa_few16 = nullptr, gqa_join = nullptr,
                   gqa_tree_rows = nullptr, gqa_tree_few = nullptr, gqa_tree_few16 = nullptr, tree_plan = nullptr,
-                  paged_commit = nullptr, free_clear = nullptr, free_mark = nullptr, free_list = nullptr,
+                  paged_commit = nullptr, free_clear = nullptr, free_mark = nullptr, free_list = nullptr, free_small = nullptr,
                   paged_fork = nullptr, tree_stats = nullptr, tree_first = nullptr, tree_round = nullptr, tree_walk = nullptr,
                   gdn_tree[2][2][3] = {}, gdn_tree_commit = nullptr;
     // Row products: [q4][parts - 1][shape], shapes as kRowShapes.
@@ -972,6 +972,7 @@ extern "C" ctox_status ctox_hip_backend_create(int device, ctox_hip_backend **ou
                {&b->gqa_tree_few16, "ctox_gqa_tree_few16_gfx950"}, {&b->tree_plan, "ctox_tree_plan_gfx950"},
                {&b->paged_commit, "ctox_paged_commit_gfx950"}, {&b->free_clear, "ctox_free_clear_gfx950"},
                {&b->free_mark, "ctox_free_mark_gfx950"}, {&b->free_list, "ctox_free_list_gfx950"},
+               {&b->free_small, "ctox_free_small_gfx950"},
                {&b->paged_fork, "ctox_paged_fork_gfx950"}, {&b->tree_stats, "ctox_tree_stats_gfx950"},
                {&b->tree_first, "ctox_tree_first_gfx950"}, {&b->tree_round, "ctox_tree_round_gfx950"}, {&b->tree_walk, "ctox_tree_walk_gfx950"},
                {&b->gdn_tree_commit, "ctox_gdn_tree_commit_gfx950"}};
@@ -3494,6 +3495,9 @@ extern "C" ctox_status ctox_hip_paged_free_slots_device(ctox_hip_backend *b, con
     OnDevice on(b);
     hipStream_t s = (hipStream_t)stream;
     ctox_status st = CTOX_OK;
+    // (128 requests of up to 50 pages: SMALL_MEASURED)
+    if ((uint64_t)op->requests * op->max_pages <= CTOX_FREE_ENTRIES && a.words[0] + a.words[1] <= CTOX_FREE_WORDS)
+        return launch(b->free_small, dim3(1), dim3(1024), s, a, "ctox_free_small_gfx950");
     if (need) {
         st = launch(b->free_clear, dim3(std::min<uint32_t>(cus, (uint32_t)(need / 4 + 255) / 256)), dim3(256), s, a,
                     "ctox_free_clear_gfx950");
