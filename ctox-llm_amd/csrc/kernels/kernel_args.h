@@ -683,7 +683,7 @@ struct GqaRowsArgs {
     float scale;
     uint32_t page_magic;     // token / page_tokens = token * page_magic >> page_shift, tokens < 2^30
     uint32_t page_shift;
-    uint32_t pad;
+    uint32_t join_heads;     // heads that a workgroup of the join takes: 4 or 1
     const uint64_t *masks;   // trees: [rows], bit j: the row sees its request's node j
 };
 

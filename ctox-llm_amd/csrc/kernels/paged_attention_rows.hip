@@ -477,35 +477,36 @@ __device__ __forceinline__ void gqa_rows(const GqaRowsArgs &a) {
     {
         const float *q = a.query + qat + 32 * h;
         const float pre = valid ? a.scale * 1.44269504088896341f : 0.0f;
-        // Eight dims of k step s in the key operand's order (read twice rather than kept).
-        auto load = [&](int s, float (&x)[8]) {
+        // Eight dims of each k step in the key operand's order (the sums' registers are free yet).
+        float x[16][8];
+#pragma unroll
+        for (int s = 0; s < 16; s++) {
             const float4 u = *(const float4 *)(q + 64 * (s >> 2) + 8 * (s & 3));
             const float4 v = *(const float4 *)(q + 64 * (s >> 2) + 8 * (s & 3) + 4);
             const float y[8] = {u.x, v.x, u.y, v.y, u.z, v.z, u.w, v.w};
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = y[i] * pre;
-        };
+            for (int i = 0; i < 8; i++) x[s][i] = y[i];
+        }
+        __builtin_amdgcn_sched_barrier(0);  // all of them under way at once
         float mx = 0.0f;
 #pragma unroll
-        for (int s = 0; s < 16; s++) {
-            float x[8];
-            load(s, x);
+        for (int s = 0; s < 16; s++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[i]) < INFINITY ? fabsf(x[i]) : 0.0f);
-        }
+            for (int i = 0; i < 8; i++) {
+                x[s][i] *= pre;
+                mx = fmaxf(mx, fabsf(x[s][i]) < INFINITY ? fabsf(x[s][i]) : 0.0f);
+            }
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const int e = gr_query_exponent(mx);
         qs = ldexpf(1.0f, e - 15);
         // The waves of a subtile write a share of it each.
 #pragma unroll
-        for (int k = 0; k < 16 / TS; k++) {
-            const int s = ts * (16 / TS) + k;
-            float x[8];
-            load(s, x);
+        for (int s = 0; s < 16; s++) {
+            if ((int)ts != s / (16 / TS)) continue;
             rm_h8 hi, lo;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float v = ldexpf(x[i], 15 - e);
+                const float v = ldexpf(x[s][i], 15 - e);
                 hi[i] = (_Float16)v;
                 lo[i] = fabsf(v) < INFINITY ? (_Float16)(v - (float)hi[i]) : (_Float16)0.0f;
             }
@@ -1144,7 +1145,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_few16_gfx950(GqaRo
 extern "C" __global__ __launch_bounds__(256, 2) void ctox_gqa_tree_few16_gfx950(GqaRowsArgs a) { gqa_few16<true>(a); }
 
 // ---------------------------------------------------------------------------
-// join: grid (rows, quarters of the query heads), 64 lanes x 4 dims
+// join: grid (rows, query heads in groups of a.join_heads), 64 lanes x 4 dims
 // ---------------------------------------------------------------------------
 // A wave takes a head of its own, or, where there are more than GR_ALONE parts, every fourth part of one head after the
 // other. (A mixed batch of 36 thousand row heads: 19 us, 38 us with four waves a head throughout.)
@@ -1213,13 +1214,13 @@ extern "C" __global__ __launch_bounds__(256) void ctox_gqa_join_gfx950(GqaRowsAr
             make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
     };
     if (alone) {
-        const uint32_t head = 4 * blockIdx.y + wave;
-        if (head >= a.query_heads) return;
+        const uint32_t head = a.join_heads * blockIdx.y + wave;
+        if (wave >= a.join_heads || head >= a.query_heads) return;
         sum(head, 0, 1);
         write(head, acc, den);
         return;
     }
-    for (uint32_t head = 4 * blockIdx.y; head < min(4 * blockIdx.y + 4, a.query_heads); head++) {
+    for (uint32_t head = a.join_heads * blockIdx.y; head < min(a.join_heads * (blockIdx.y + 1), a.query_heads); head++) {
         sum(head, wave, 4);
         acc4[wave][lane] = acc;
         if (lane == 0) {

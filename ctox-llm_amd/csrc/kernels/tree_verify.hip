@@ -98,11 +98,12 @@ __device__ __forceinline__ TvRow tv_draft(const TreeVerifyArgs &a, uint32_t row)
     return TvRow(a.draft + (size_t)row * a.draft_stride, a.draft_vocab);
 }
 
-// Its law: probability of a logit x is 2^(x c - top) inv.
+// Its law: probability of a logit x is 2^((x - top) c) inv. (The difference is formed first: whatever the logits and the
+// temperature, the largest weight is 1.)
 struct TvLaw {
     double top, inv;  // inv 0: no law (a logit that is no number or +inf, or none that is finite)
     __device__ __forceinline__ double at(const TreeVerifyArgs &a, float x) const {
-        return tv_none(x) ? 0.0 : tv_exp2(fma((double)x, a.c, -top)) * inv;
+        return tv_none(x) ? 0.0 : tv_exp2(((double)x - top) * a.c) * inv;
     }
 };
 
@@ -113,9 +114,8 @@ __device__ __forceinline__ TvLaw tv_law(const TreeVerifyArgs &a, const TreeStat 
     if (lane < parts) x = s[lane];
     const float top = tv_max64(x.top);
     const bool bad = __builtin_amdgcn_ballot_w64(x.bad) || !(fabsf(top) < INFINITY);
-    const double tops = (double)top * a.c;
-    const double sum = tv_sum64(x.sum > 0.0 ? x.sum * tv_exp2(fma((double)x.top, a.c, -tops)) : 0.0);
-    return {tops, bad ? 0.0 : 1.0 / sum};
+    const double sum = tv_sum64(x.sum > 0.0 ? x.sum * tv_exp2(((double)x.top - (double)top) * a.c) : 0.0);
+    return {(double)top, bad ? 0.0 : 1.0 / sum};
 }
 
 __device__ __forceinline__ bool tv_point(const TreeVerifyArgs &a) { return a.draft == nullptr; }
@@ -190,10 +190,10 @@ __device__ __forceinline__ void tv_stats(const TreeVerifyArgs &a, const TvRow &r
                 sum = top > -INFINITY ? sum * tv_exp2(((double)top - (double)m) * a.c) : 0.0;
                 top = m;
             }
-            const double t = (double)top * a.c;
+            const double t = top > -INFINITY ? (double)top : 0.0;
             double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-            for (int k = 0; k < 16; k++) s[k & 3] += tv_exp2(fma((double)x[k], a.c, -t));
+            for (int k = 0; k < 16; k++) s[k & 3] += tv_exp2(((double)x[k] - t) * a.c);
             if (top > -INFINITY) sum += (s[0] + s[1]) + (s[2] + s[3]);
         }
         if ((e0 + 4096) % size && e0 + 4096 < end) continue;
@@ -518,7 +518,7 @@ extern "C" __global__ __launch_bounds__(1024) void ctox_tree_walk_gfx950(TreeVer
                 mass = a.rest[((size_t)(gone - 1) * a.rows + row) * a.parts + lane];
             } else {
                 const TreeStat x = a.stats[(size_t)row * a.parts + lane];
-                mass = x.sum > 0.0 ? x.sum * tv_exp2(fma((double)x.top, a.c, -pl.top)) * pl.inv : 0.0;
+                mass = x.sum > 0.0 ? x.sum * tv_exp2(((double)x.top - pl.top) * a.c) * pl.inv : 0.0;
             }
         }
         in = mass;

@@ -3198,6 +3198,7 @@ ctox_status gqa_rows_impl(ctox_hip_backend *b, const ctox_paged_gqa_rows *op, co
     a.page_shift = 30 + l;
     a.page_magic = (uint32_t)(((1ull << a.page_shift) + p.page_tokens - 1) / p.page_tokens);
     a.masks = masks;
+    a.join_heads = (uint64_t)a.rows * p.query_heads <= 4 * (uint64_t)b->cus ? 1 : 4;
     const hipFunction_t rows = masks ? b->gqa_tree_rows : b->gqa_rows;
     const hipFunction_t few = g.few == 16 ? (masks ? b->gqa_tree_few16 : b->gqa_few16) : masks ? b->gqa_tree_few : b->gqa_few;
     OnDevice on(b);
@@ -3206,7 +3207,8 @@ ctox_status gqa_rows_impl(ctox_hip_backend *b, const ctox_paged_gqa_rows *op, co
     if (g.wide) st = launch(rows, dim3(g.items), dim3(512), s, a, "ctox_gqa_rows_gfx950");
     if (!st && g.few) st = launch(few, dim3(g.few_items), dim3(256), s, a, "ctox_gqa_few_gfx950");
     if (!st && g.cut && (g.few || g.split))
-        st = launch(b->gqa_join, dim3(a.rows, (p.query_heads + 3) / 4), dim3(256), s, a, "ctox_gqa_join_gfx950");
+        st = launch(b->gqa_join, dim3(a.rows, (p.query_heads + a.join_heads - 1) / a.join_heads), dim3(256), s, a,
+                    "ctox_gqa_join_gfx950");
     return st;
 }
 }  // namespace
