@@ -35,7 +35,7 @@
 // 2^y for y <= 0 (a hair above 0 at most), within 1.1e-12: 2^f, |f| <= 1/2, by its interpolation in the nine
 // Chebyshev points. A running sum is moved by as little, far below the distance of its borders. Whole numbers
 // are split off and put into the exponent by additions alone. What is below 2^-1000, -inf too, gives 2^-1000: nothing
-// beside a largest weight of 1, but not 0 (tv_none).
+// in a sum whose largest term is 1; as a token's weight (TvLaw) it is 0.
 __device__ __forceinline__ double tv_exp2(double y) {
     y = fmax(y, -1000.0);
     const double big = 6755399441055744.0, t = y + big, f = y - (t - big);  // 1.5 * 2^52
@@ -50,7 +50,6 @@ __device__ __forceinline__ double tv_exp2(double y) {
     p = fma(p, f, 1.0);
     return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
 }
-__device__ __forceinline__ bool tv_none(float x) { return x == -INFINITY; }
 
 __device__ __forceinline__ double tv_sum64(double x) {
 #pragma unroll
@@ -103,7 +102,8 @@ __device__ __forceinline__ TvRow tv_draft(const TreeVerifyArgs &a, uint32_t row)
 struct TvLaw {
     double top, inv;  // inv 0: no law (a logit that is no number or +inf, or none that is finite)
     __device__ __forceinline__ double at(const TreeVerifyArgs &a, float x) const {
-        return tv_none(x) ? 0.0 : tv_exp2(((double)x - top) * a.c) * inv;
+        const double y = ((double)x - top) * a.c;
+        return y < -1000.0 ? 0.0 : tv_exp2(y) * inv;
     }
 };
 
@@ -161,6 +161,9 @@ __device__ __forceinline__ void tv_stats(const TreeVerifyArgs &a, const TvRow &r
                                          uint32_t size, TreeStat *out, TvScratch &L) {
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t end = min(last * size, row.len + row.skew);
+    // A row that begins at its border may have no token in its last part.
+    for (uint32_t p = first; p < last; p++)
+        if (p * size >= end && tid == 0) out[p] = TreeStat{0.0, -INFINITY, 0};
     float top = -INFINITY;  // of the wave; greedy: of the thread
     double sum = 0.0;
     uint32_t id = 0;
