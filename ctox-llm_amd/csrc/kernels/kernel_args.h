@@ -810,8 +810,6 @@ struct TreeVerifyArgs {
     uint32_t round;
     uint32_t without;            // siblings drawn without replacement
     uint32_t greedy;
-    uint32_t per;                // parts that a workgroup of the first round takes
-    uint32_t pad;
 };
 
 struct GdnTreeArgs {

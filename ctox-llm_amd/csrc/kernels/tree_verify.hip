@@ -22,6 +22,8 @@
 //    that refused it and may still be on the path. Of a row that refuses, the parts' sums of
 //    r_k, not yet divided by Z_k; of a leaf that is accepted its own statistics (the others' are never read).
 //    Each workgroup repeats its row's test for itself; what it needs of the round before is a TreeRow.
+//    ctox_tree_test_gfx950, ctox_tree_rest_gfx950: the first round of many rows, every test made once and the sums only where
+//    the tests above still lead.
 //  * ctox_tree_walk_gfx950: a workgroup a request: the walk down from the root, and the next token: the part where
 //    the running sum passes the request's number, then that part's tokens.
 #include <hip/hip_runtime.h>
@@ -297,30 +299,32 @@ struct TvRest {
     }
 };
 
-// The test of a row's child number k = a.round - 1 and what follows it, in parts first .. last - 1.
-__device__ __forceinline__ void tv_round(const TreeVerifyArgs &a, uint32_t row, uint32_t first, uint32_t last,
-                                         TvScratch &L, uint32_t (&tried)[CTOX_TREE_NODES]) {
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.round - 1;
-    const bool chief = first == 0 && tid == 0;  // keeps the row's records
-    const uint32_t r = tree_request(a.row_starts, a.requests, row);
-    const TreeRows q = tree_rows(a.row_starts, r, a.rows);
-    const int parent = tree_parent(a.parents, q, lane);
-    const uint64_t children = tv_children(parent, row - q.row0);
-    TreeRow s{0.0, 1.0, 0.0, 0.0, 0.0, 0.0};
+// What a row's test of its child number k = a.round - 1 leaves.
+struct TvTest {
+    TreeRow s;
+    uint64_t children;
+    int leaf;      // row of a child without children that was accepted, else -1
+    bool refused;  // else accepted, or nothing to test
+};
+
+// By whole waves; the chief's lane 0 keeps the row's records.
+__device__ __forceinline__ TvTest tv_test(const TreeVerifyArgs &a, uint32_t row, const TreeRows &q, int parent, bool chief) {
+    const uint32_t lane = threadIdx.x & 63, k = a.round - 1;
+    TvTest t{{0.0, 1.0, 0.0, 0.0, 0.0, 0.0}, tv_children(parent, row - q.row0), -1, false};
+    TreeRow &s = t.s;
     if (k) {
         s = a.states[(size_t)(k & 1) * a.rows + row];
-    } else if (!children) {
+    } else if (!t.children) {
         if (chief) tv_set_mark(a, row, TreeMark{-1, 0});
-        return;
+        return t;
     }
-    uint64_t rest = children;
+    uint64_t rest = t.children;
     for (uint32_t i = 0; i < k; i++) rest &= rest - 1;
-    const TvRow p = tv_target(a, row);
-    const float *x = tv_point(a) ? nullptr : a.draft + (size_t)row * a.draft_stride;
     const int child = __ffsll((unsigned long long)rest) - 1;
     rest &= rest - 1;
+    const float *x = tv_point(a) ? nullptr : a.draft + (size_t)row * a.draft_stride;
     const uint32_t token = a.tokens[q.row0 + child];
-    const float px = p.x[min(token, a.vocab - 1)];
+    const float px = (a.target + (size_t)row * a.target_stride)[min(token, a.vocab - 1)];
     double left = 1.0;
     TvLaw pl, ql{0.0, 0.0};
     if (k) {
@@ -333,7 +337,7 @@ __device__ __forceinline__ void tv_round(const TreeVerifyArgs &a, uint32_t row, 
         s.p_top = pl.top, s.p_inv = pl.inv, s.q_top = ql.top, s.q_inv = ql.inv;
         if (pl.inv == 0.0 || (!tv_point(a) && ql.inv == 0.0)) {
             if (chief) tv_set_mark(a, row, TreeMark{-2, 0});
-            return;
+            return t;
         }
     }
     double pt = 0.0, qt = tv_point(a) ? 1.0 : 0.0;
@@ -342,19 +346,17 @@ __device__ __forceinline__ void tv_round(const TreeVerifyArgs &a, uint32_t row, 
         if (!tv_point(a)) qt = tv_draft_at(a, ql, x, token);
     }
     if (tv_point(a)) {  // a token that was tried is left with nothing
-        const uint64_t before = children & ((1ull << child) - 1);
+        const uint64_t before = t.children & ((1ull << child) - 1);
         if (__builtin_amdgcn_ballot_w64((before >> lane & 1) && a.tokens[q.row0 + lane] == token)) pt = 0.0;
     } else {
         pt = fmax(pt - s.lambda * qt, 0.0);
     }
-    const bool accepted = (double)a.accept[q.row0 + child] * (qt / s.undrawn) * left < pt;
-    if (accepted) {
+    if ((double)a.accept[q.row0 + child] * (qt / s.undrawn) * left < pt) {
         if (chief) tv_set_mark(a, row, TreeMark{child, k});
-        if (tv_children(parent, (uint32_t)child)) return;
-        const uint32_t leaf = q.row0 + child;
-        tv_stats(a, tv_target(a, leaf), first, last, a.part, a.stats + (size_t)leaf * a.parts, L);
-        return;
+        if (!tv_children(parent, (uint32_t)child)) t.leaf = (int)(q.row0 + child);
+        return t;
     }
+    t.refused = true;
     if (!tv_point(a)) {
         s.lambda += left / s.undrawn;
         if (a.without) s.undrawn -= qt;
@@ -368,14 +370,23 @@ __device__ __forceinline__ void tv_round(const TreeVerifyArgs &a, uint32_t row, 
             a.lists[(size_t)(a.round & 1) * a.rows + at] = row;
         }
     }
+    return t;
+}
+
+// A row that refused children 0 .. k: sums of what is left in parts first .. last - 1, by a workgroup.
+__device__ __forceinline__ void tv_rest(const TreeVerifyArgs &a, uint32_t row, const TreeRows &q, const TvTest &t, uint32_t k,
+                                        uint32_t first, uint32_t last, TvScratch &L, uint32_t (&tried)[CTOX_TREE_NODES]) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (tv_point(a)) {
-        if (wave == 0 && (children >> lane & 1)) {
-            const uint32_t at = __popcll(children & ((1ull << lane) - 1));
+        if (wave == 0 && (t.children >> lane & 1)) {
+            const uint32_t at = __popcll(t.children & ((1ull << lane) - 1));
             tried[at] = a.tokens[q.row0 + lane];
         }
         lds_barrier();
     }
-    const TvRest f{a, p, x, pl, ql, s.lambda, k + 1, tried};
+    const TvRow p = tv_target(a, row);
+    const TvRest f{a, p, tv_point(a) ? nullptr : a.draft + (size_t)row * a.draft_stride, {t.s.p_top, t.s.p_inv},
+                   {t.s.q_top, t.s.q_inv}, t.s.lambda, k + 1, tried};
     for (uint32_t part = first; part < last; part++) {
         double sum = 0.0;
         for (uint32_t e0 = part * a.part; e0 < (part + 1) * a.part && e0 < p.len + p.skew; e0 += 4096) {
@@ -397,34 +408,80 @@ __device__ __forceinline__ void tv_round(const TreeVerifyArgs &a, uint32_t row, 
     }
 }
 
-// Round 1: grid (groups of a.per parts, rows)
+// Whether another child was accepted where the row's path branches off, by marks of fewer than `rounds` refusals.
+__device__ __forceinline__ bool tv_off(const TreeVerifyArgs &a, const TreeRows &q, int parent, uint32_t row, uint32_t rounds) {
+    const uint32_t lane = threadIdx.x & 63;
+    TreeMark m{-1, 0};
+    if (lane < q.n) m = tv_mark(a, q.row0 + lane);
+    const int accepted = m.refused < rounds ? m.chosen : -1;
+    const int above = __shfl(accepted, parent < 0 ? (int)lane : parent);
+    const uint64_t line = __shfl(tree_lineage(parent, lane, lane < q.n), (int)((row - q.row0) & 63));
+    return __builtin_amdgcn_ballot_w64((line >> lane & 1) && parent >= 0 && above != -1 && above != (int)lane) != 0;
+}
+
+__device__ __forceinline__ bool tv_has(const TreeVerifyArgs &a, uint32_t row) {
+    return row < min(a.row_starts[a.requests], a.rows) && row >= a.row_starts[0];
+}
+
+// Round 1 of few rows: grid (parts, rows)
 extern "C" __global__ __launch_bounds__(256) void ctox_tree_first_gfx950(TreeVerifyArgs a) {
     __shared__ TvScratch L;
     __shared__ uint32_t tried[CTOX_TREE_NODES];
-    const uint32_t row = blockIdx.y, first = blockIdx.x * a.per;
-    if (row >= min(a.row_starts[a.requests], a.rows) || row < a.row_starts[0]) return;
-    tv_round(a, row, first, min(first + a.per, a.parts), L, tried);
+    const uint32_t row = blockIdx.y, part = blockIdx.x;
+    if (!tv_has(a, row)) return;
+    const TreeRows q = tree_rows(a.row_starts, tree_request(a.row_starts, a.requests, row), a.rows);
+    const int parent = tree_parent(a.parents, q, threadIdx.x & 63);
+    const TvTest t = tv_test(a, row, q, parent, part == 0 && threadIdx.x == 0);
+    if (t.refused) tv_rest(a, row, q, t, 0, part, part + 1, L, tried);
+    else if (t.leaf >= 0)
+        tv_stats(a, tv_target(a, t.leaf), part, part + 1, a.part, a.stats + (size_t)t.leaf * a.parts, L);
+}
+
+// Round 1 of many: a wave a row tests, ...
+#define TV_LEAF 0x80000000u
+extern "C" __global__ __launch_bounds__(256) void ctox_tree_test_gfx950(TreeVerifyArgs a) {
+    const uint32_t row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (!tv_has(a, row)) return;
+    const TreeRows q = tree_rows(a.row_starts, tree_request(a.row_starts, a.requests, row), a.rows);
+    const TvTest t = tv_test(a, row, q, tree_parent(a.parents, q, lane), lane == 0);
+    if (lane == 0 && (t.refused || t.leaf >= 0))
+        a.lists[atomicAdd(&a.waiting[0], 1u)] = t.refused ? row : (uint32_t)t.leaf | TV_LEAF;
+}
+// ... and what may still be on the path is summed: grid (parts, CTOX_TREE_LANES).
+extern "C" __global__ __launch_bounds__(256) void ctox_tree_rest_gfx950(TreeVerifyArgs a) {
+    __shared__ TvScratch L;
+    __shared__ uint32_t tried[CTOX_TREE_NODES];
+    const uint32_t waiting = a.waiting[0], part = blockIdx.x;
+    for (uint32_t i = blockIdx.y; i < waiting; i += CTOX_TREE_LANES) {
+        const uint32_t entry = a.lists[i], row = entry & ~TV_LEAF;
+        const TreeRows q = tree_rows(a.row_starts, tree_request(a.row_starts, a.requests, row), a.rows);
+        const int parent = tree_parent(a.parents, q, threadIdx.x & 63);
+        if (tv_off(a, q, parent, row, 1)) continue;
+        if (entry & TV_LEAF) {
+            tv_stats(a, tv_target(a, row), part, part + 1, a.part, a.stats + (size_t)row * a.parts, L);
+        } else {
+            const TvTest t{a.states[a.rows + row], tv_children(parent, row - q.row0), -1, true};
+            tv_rest(a, row, q, t, 0, part, part + 1, L, tried);
+        }
+        lds_barrier();
+    }
 }
 
 // The rounds after it: grid (parts, CTOX_TREE_LANES), which take the rows that wait in turn.
 extern "C" __global__ __launch_bounds__(256) void ctox_tree_round_gfx950(TreeVerifyArgs a) {
     __shared__ TvScratch L;
     __shared__ uint32_t tried[CTOX_TREE_NODES];
-    const uint32_t waiting = a.waiting[a.round - 1];
+    const uint32_t waiting = a.waiting[a.round - 1], part = blockIdx.x;
     for (uint32_t i = blockIdx.y; i < waiting; i += CTOX_TREE_LANES) {
         const uint32_t row = a.lists[(size_t)((a.round - 1) & 1) * a.rows + i];
-        // Where another child was accepted above it the row is not on the path, whatever it accepts. Marks of this
-        // round may be there already or not, so they do not count: every workgroup decides the same.
-        const uint32_t lane = threadIdx.x & 63;
         const TreeRows q = tree_rows(a.row_starts, tree_request(a.row_starts, a.requests, row), a.rows);
-        const int parent = tree_parent(a.parents, q, lane);
-        TreeMark m{-1, 0};
-        if (lane < q.n) m = tv_mark(a, q.row0 + lane);
-        const int accepted = m.refused < a.round - 1 ? m.chosen : -1;
-        const int above = __shfl(accepted, parent < 0 ? (int)lane : parent);
-        const uint64_t line = __shfl(tree_lineage(parent, lane, lane < q.n), (int)((row - q.row0) & 63));
-        if (__builtin_amdgcn_ballot_w64((line >> lane & 1) && parent >= 0 && above != -1 && above != (int)lane)) continue;
-        tv_round(a, row, blockIdx.x, blockIdx.x + 1, L, tried);
+        const int parent = tree_parent(a.parents, q, threadIdx.x & 63);
+        // Marks of this round may be there already or not, so they do not count: every workgroup decides the same.
+        if (tv_off(a, q, parent, row, a.round - 1)) continue;
+        const TvTest t = tv_test(a, row, q, parent, part == 0 && threadIdx.x == 0);
+        if (t.refused) tv_rest(a, row, q, t, a.round - 1, part, part + 1, L, tried);
+        else if (t.leaf >= 0)
+            tv_stats(a, tv_target(a, t.leaf), part, part + 1, a.part, a.stats + (size_t)t.leaf * a.parts, L);
         lds_barrier();
     }
 }

@@ -166,7 +166,7 @@ struct ctox_hip_backend {
                   gqa_rows = nullptr, gqa_few = nullptr, gqa_few16 = nullptr, gqa_join = nullptr,
                   gqa_tree_rows = nullptr, gqa_tree_few = nullptr, gqa_tree_few16 = nullptr, tree_plan = nullptr,
                   paged_commit = nullptr, free_clear = nullptr, free_mark = nullptr, free_list = nullptr, free_small = nullptr,
-                  paged_fork = nullptr, tree_stats = nullptr, tree_first = nullptr, tree_round = nullptr, tree_walk = nullptr,
+                  paged_fork = nullptr, tree_stats = nullptr, tree_first = nullptr, tree_test = nullptr, tree_rest = nullptr, tree_round = nullptr, tree_walk = nullptr,
                   gdn_tree[2][2][3] = {}, gdn_tree_commit = nullptr;
     // Row products: [q4][parts - 1][shape], shapes as kRowShapes.
     hipFunction_t rows_mul[2][2][4] = {};
@@ -974,7 +974,8 @@ extern "C" ctox_status ctox_hip_backend_create(int device, ctox_hip_backend **ou
                {&b->free_mark, "ctox_free_mark_gfx950"}, {&b->free_list, "ctox_free_list_gfx950"},
                {&b->free_small, "ctox_free_small_gfx950"},
                {&b->paged_fork, "ctox_paged_fork_gfx950"}, {&b->tree_stats, "ctox_tree_stats_gfx950"},
-               {&b->tree_first, "ctox_tree_first_gfx950"}, {&b->tree_round, "ctox_tree_round_gfx950"}, {&b->tree_walk, "ctox_tree_walk_gfx950"},
+               {&b->tree_first, "ctox_tree_first_gfx950"},
+               {&b->tree_test, "ctox_tree_test_gfx950"}, {&b->tree_rest, "ctox_tree_rest_gfx950"}, {&b->tree_round, "ctox_tree_round_gfx950"}, {&b->tree_walk, "ctox_tree_walk_gfx950"},
                {&b->gdn_tree_commit, "ctox_gdn_tree_commit_gfx950"}};
     for (auto &f : fns) {
         if (le != hipSuccess) break;
@@ -3310,7 +3311,8 @@ uint32_t tree_part(uint32_t vocab, uint32_t pieces) {
 }
 uint32_t tree_parts(uint32_t vocab, uint32_t part) { return (uint32_t)(((uint64_t)vocab + 3 + part - 1) / part); }
 struct TreeVerifyPlan {
-    uint32_t part, parts, stat_part, stat_parts, draft_part, draft_parts, rounds, per;
+    uint32_t part, parts, stat_part, stat_parts, draft_part, draft_parts, rounds;
+    bool many;
     uint64_t stats, draft_stats, rest;
 };
 TreeVerifyPlan tree_verify_plan(uint32_t cus, const ctox_verify_tree *op) {
@@ -3327,8 +3329,10 @@ TreeVerifyPlan tree_verify_plan(uint32_t cus, const ctox_verify_tree *op) {
         p.draft_part = tree_part(op->draft_vocab, pieces);
         p.draft_parts = tree_parts(op->draft_vocab, p.draft_part);
     }
-    // A workgroup of the first round makes its row's test once for several parts.
-    p.per = (uint32_t)(1 + (uint64_t)op->rows * p.parts / (16 * cus));
+    // A test is a chain of loads, some 8 us: workgroups of a part each repeat it while they fill the chip, beyond that it
+    // is made once, in a launch of its own. (Measured us of the first round: 5 rows of 151936 tokens 9 repeated; 315 rows
+    // 50 repeated, three parts a workgroup, 6.7 + 22.6 made once.)
+    p.many = (uint64_t)op->rows * p.parts > 8 * cus;
     p.rounds = greedy ? 0 : op->max_children;
     p.stats = (uint64_t)op->rows * p.parts * sizeof(TreeStat);
     p.draft_stats = (uint64_t)op->rows * p.draft_parts * sizeof(TreeStat);
@@ -3396,7 +3400,6 @@ extern "C" ctox_status ctox_hip_verify_tree_device(ctox_hip_backend *b, const ct
     a.part = p.part;
     a.stat_parts = p.stat_parts;
     a.stat_part = p.stat_part;
-    a.per = p.per;
     a.draft_part = p.draft_part;
     a.width = op->max_children;
     a.without = op->without_replacement != 0;
@@ -3407,11 +3410,17 @@ extern "C" ctox_status ctox_hip_verify_tree_device(ctox_hip_backend *b, const ct
     if (op->rows) {
         st = launch(b->tree_stats, dim3(std::max(p.stat_parts, p.draft_parts), op->rows, a.draft ? 2 : 1), dim3(256), s, a,
                     "ctox_tree_stats_gfx950");
-        for (a.round = 1; !st && a.round <= p.rounds; a.round++)
-            st = a.round == 1 ? launch(b->tree_first, dim3((p.parts + a.per - 1) / a.per, op->rows), dim3(256), s, a,
-                                       "ctox_tree_first_gfx950")
-                              : launch(b->tree_round, dim3(p.parts, std::min<uint32_t>(CTOX_TREE_LANES, op->rows)),
-                                       dim3(256), s, a, "ctox_tree_round_gfx950");
+        const dim3 lanes(p.parts, std::min<uint32_t>(CTOX_TREE_LANES, op->rows));
+        for (a.round = 1; !st && a.round <= p.rounds; a.round++) {
+            if (a.round > 1) {
+                st = launch(b->tree_round, lanes, dim3(256), s, a, "ctox_tree_round_gfx950");
+            } else if (p.many) {
+                st = launch(b->tree_test, dim3((op->rows + 3) / 4), dim3(256), s, a, "ctox_tree_test_gfx950");
+                if (!st) st = launch(b->tree_rest, lanes, dim3(256), s, a, "ctox_tree_rest_gfx950");
+            } else {
+                st = launch(b->tree_first, dim3(p.parts, op->rows), dim3(256), s, a, "ctox_tree_first_gfx950");
+            }
+        }
     }
     if (!st) st = launch(b->tree_walk, dim3(op->requests), dim3(1024), s, a, "ctox_tree_walk_gfx950");
     return st;

@@ -189,9 +189,13 @@ def test_many_refusals(hip):
             v.check(hip, max_children=2)
 
 
-def test_many_requests_and_long_rows(hip):
-    v = Verify(3, [int(x) for x in np.random.default_rng(1).integers(0, 12, 150)], 20000, 4, 0.8, "without", 5000)
-    v.check(hip)
+@pytest.mark.parametrize("drawn,draft_vocab,noise", [("without", 5000, 0.9), ("with", None, 2.5), ("point", None, 0.9),
+                                                     ("without", None, 2.5)])
+def test_many_requests_and_long_rows(hip, drawn, draft_vocab, noise):
+    """Enough rows that the first round's tests have a launch of their own."""
+    say("many", drawn, draft_vocab)
+    nodes = [int(x) for x in np.random.default_rng(1).integers(0, 14, 100)]
+    Verify(3, nodes, 20000, 4, 0.8, drawn, draft_vocab, noise=noise).check(hip)
 
 
 def test_a_chain_is_the_chain_rule(hip):
