@@ -3,17 +3,14 @@
 Against the formula in float64 over the values that the pages stand for, with the tolerance that is derived in
 test_gpu_paged_attention_rows.py: the arithmetic of a (row, token) pair is the same, only which pairs there are differs.
 """
-import ctypes
-import math
-
 import numpy as np
 import pytest
 import torch
 
 import ctox_hip as ch
 import test_gpu_paged_attention_rows as rows
-from test_gpu_paged_attention_rows import HD, Q2, Q4, dev
-from tree_model import lines, masks, random_tree
+from test_gpu_paged_attention_rows import HD, dev
+from tree_model import masks, random_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -58,11 +55,10 @@ class Trees(rows.Batch):
         return want, tol
 
     def tree_op(self, hip, max_rows=0):
-        op = self.op(hip)
-        inner = getattr(op, "rows_op", op)
-        fields = {n: getattr(inner, n) for n in ("query", "out", "q2_pages", "q4_pages", "descriptors", "row_starts", "tokens")}
+        inner = self.op(hip)
+        pointers = [getattr(inner, n) for n in ("query", "out", "q2_pages", "q4_pages", "descriptors", "row_starts", "tokens")]
         self.d["masks"] = dev(self.masks.view(np.int64))
-        t = ch.PagedGqaTree(*fields.values(), self.d["masks"].data_ptr(), rows=inner.rows, requests=inner.requests,
+        t = ch.PagedGqaTree(*pointers, self.d["masks"].data_ptr(), rows=inner.rows, requests=inner.requests,
                             params=inner.params, max_rows=max_rows)
         self.ws = torch.full((max(16, hip.paged_gqa_tree_workspace(t)),), 255, dtype=torch.uint8, device="cuda")
         t.bind_workspace(self.ws.data_ptr(), self.ws.numel())

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import ctox_hip as ch
-from tree_model import NO, flat, lines, random_tree, starts
+from tree_model import NO, flat, random_tree, starts
 from test_gpu_tree_ops import dev, host, stream
 
 pytestmark = pytest.mark.gpu
@@ -117,7 +117,7 @@ class Verify:
             out.append((path, token))
         return out
 
-    def op(self, hip, width=None, max_children=None):
+    def op(self, hip, max_children=None):
         t, k = self.skew, self.width if max_children is None else max_children
         self.d = {"target": self.padded(self.target), "draft": None if self.drawn == "point" else self.padded(self.draft),
                   "inverse": None if self.DV == self.V else dev(self.inverse), "tokens": dev(self.tokens),
