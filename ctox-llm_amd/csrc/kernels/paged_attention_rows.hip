@@ -964,8 +964,8 @@ __device__ __forceinline__ void gqa_few16(const GqaRowsArgs &a) {
                 s[n][3] = fmaf(f.w, x[n][3], s[n][3]);
             }
         }
-        // ---- masks ----
-        if ((int32_t)((t + 1) * 32) - 1 > past || ld.here != ~0u) {
+        // ---- masks: past the first query's last token, in a tree past the last token that all see ----
+        if ((int32_t)((t + 1) * 32) - 1 > (TREE ? past - 1 : past) || ld.here != ~0u) {
             const uint32_t word = TREE ? gr_tree_word(mask, t, past) : ~0u;
             const uint32_t on = (ld.here & word) >> (4 * g);
             const int32_t left = lim - (int32_t)(t * 32 + 4 * g);  // tokens up to this one

@@ -182,3 +182,18 @@ def test_workspace_serves_smaller_calls(hip):
     t.bind_workspace(big.ws.data_ptr(), 16)
     with pytest.raises(ch.MemoryBudget):
         hip.paged_gqa_tree_device(t, None)
+
+
+@pytest.mark.parametrize("heads,kv,most", [(6, 1, 2), (24, 4, 2), (8, 8, 16), (4, 2, 8)])
+@pytest.mark.parametrize("cached", [30, 31, 32, 63, 95, 96])
+def test_a_hidden_first_node(hip, heads, kv, most, cached):
+    """At most 16 queries a KV head: rows that do not see node 0, which may be a full tile's last token."""
+    say("hidden first node", heads, kv, most, cached)
+    rng = np.random.default_rng(cached + heads)
+    requests = [(cached, most), (cached + 1, most), (cached - 1, most)]
+    free = rng.integers(0, 2 ** most, 3 * most, dtype=np.uint64)
+    free[:most] &= np.uint64(2 ** most - 2)
+    Trees(cached, requests, 16, heads, kv, masks_=free).check(hip, most)
+    # several roots: every other node is one
+    parent = [i - 1 if i % 2 else -1 for i in range(most)]
+    Trees(cached + 1, requests, 16, heads, kv, masks_=np.concatenate([masks(parent)] * 3)).check(hip, most)
