@@ -582,8 +582,10 @@ extern "C" __global__ __launch_bounds__(1024) void ctox_tree_walk_gfx950(TreeVer
             if (gone) {
                 mass = a.rest[((size_t)(gone - 1) * a.rows + row) * a.parts + lane];
             } else {
+                // (of a part without a token of weight, by the border of TvLaw: 0)
                 const TreeStat x = a.stats[(size_t)row * a.parts + lane];
-                mass = x.sum > 0.0 ? x.sum * tv_exp2(((double)x.top - pl.top) * a.c) * pl.inv : 0.0;
+                const double y = ((double)x.top - pl.top) * a.c;
+                mass = x.sum > 0.0 && y >= -1000.0 ? x.sum * tv_exp2(y) * pl.inv : 0.0;
             }
         }
         in = mass;
@@ -596,8 +598,9 @@ extern "C" __global__ __launch_bounds__(1024) void ctox_tree_walk_gfx950(TreeVer
         gone = 0;
     }
     const double total = __shfl(in, 63), goal = (double)a.sample[r] * total;
-    // (the last part with mass where rounding leaves none past the number)
-    const uint64_t past = __builtin_amdgcn_ballot_w64(in > goal), massive = __builtin_amdgcn_ballot_w64(mass > 0.0);
+    // (of the parts with mass, since a running sum may grow by a rounding where there is none; the last of them where
+    // rounding leaves none past the number)
+    const uint64_t massive = __builtin_amdgcn_ballot_w64(mass > 0.0), past = __builtin_amdgcn_ballot_w64(in > goal) & massive;
     const uint32_t part = past ? (uint32_t)__ffsll((unsigned long long)past) - 1
                                : massive ? 63 - (uint32_t)__clzll((long long)massive) : 0;
     const double want = goal - __shfl(in - mass, part);

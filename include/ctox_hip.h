@@ -800,7 +800,8 @@ ctox_status ctox_hip_paged_gqa_tree_device(ctox_hip_backend *backend, const ctox
  *    ctox_hip_greedy_tokens_device) is accepted; draft and the numbers are not read.
  * Where no child is accepted next[r] is drawn with sample_draws[r] from r (from p where no child was
  * refused): the first token whose running sum exceeds the number times the total. A chain is
- * verified by the rule of ctox_hip_mtp_accept_device. Sums and laws are in 64 bits.
+ * verified by the rule of ctox_hip_mtp_accept_device. Sums and laws are in 64 bits; a token below 2^-1000 of
+ * its row's most probable one counts as ruled out.
  * counts[r]: nodes of the path, the root included; path[row_starts[r] + i]: its i-th node,
  * 0xffffffff behind it. A request without rows: counts 0, next 0xffffffff. A token that is not below vocab is
  * never accepted. -inf is a token that is ruled out; where a row on the path (or, with children, its

@@ -328,3 +328,24 @@ def test_workspace(hip):
     op.bind_workspace(big.data_ptr(), big.numel() - 1)
     with pytest.raises(ch.MemoryBudget):
         hip.verify_tree_device(op, stream())
+
+
+@pytest.mark.parametrize("drawn", ["without", "with", "point"])
+@pytest.mark.parametrize("skew", [0, 3])
+def test_draw_of_nothing_passes_parts_without_a_weight(hip, drawn, skew):
+    """The draw 0 takes the first token that weighs anything. Here everything in front of token 9000 lies 30 / 0.01 below
+    the largest logit, e^-3000 of it, and token 0 is ruled out: a root alone, an accepted leaf, a refused child."""
+    v = Verify(41, [1, 2, 2], 20000, 2, 0.01, drawn, std=0.05, skew=skew, forest=[[-1], [-1, 0], [-1, 0]])
+    for x in (v.target, v.draft):
+        x[:, :9000] -= 30.0
+        x[:, 0] = -np.inf
+    v.tokens[2] = 15000
+    v.u[:] = [0.0, 0.0, 0.0, 0.0, 1 - 2.0 ** -24]
+    v.tokens[4] = 77  # of no weight: never accepted
+    v.s[:] = 0.0
+    v.target[1, 15000] = 2.0  # so that request 1's child is accepted
+    hip.verify_tree_device(v.op(hip), stream())
+    got = v.got()
+    assert [p for p, _ in got] == [[0], [0, 1], [0]], got
+    # (std 0.05 over T = 0.01 is at most 2^-60 of the largest weight; only r = max(p - q, 0) may leave out more)
+    assert got[0][1] == 9000 and got[1][1] == 9000 and 9000 <= got[2][1] < 20000, got
