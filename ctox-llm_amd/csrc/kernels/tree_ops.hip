@@ -255,8 +255,8 @@ extern "C" __global__ __launch_bounds__(1024) void ctox_free_small_gfx950(FreeSl
 // forks
 // ---------------------------------------------------------------------------
 // grid (pieces of a page of all layers, forks). Codes: 1 a source or target is no request, a target is a source or
-// another fork's target, or the source is longer than its table; 2 too few free slots; 3 a part-filled page is
-// not a Q4 page of its request; 4 a free slot past q4_slots.
+// another fork's target, or the source is longer than its table; 2 too few free slots, by the count or by the pool; 3 a
+// part-filled page is not a Q4 page of its request; 4 a free slot past q4_slots.
 extern "C" __global__ __launch_bounds__(256) void ctox_paged_fork_gfx950(PagedForkArgs a) {
     __shared__ uint32_t sources[CTOX_PLAN_REQUESTS / 32], targets[CTOX_PLAN_REQUESTS / 32];
     __shared__ uint32_t bad[5], before, all;
@@ -292,8 +292,10 @@ extern "C" __global__ __launch_bounds__(256) void ctox_paged_fork_gfx950(PagedFo
     __syncthreads();
     for (uint32_t i = tid; i < CTOX_PLAN_REQUESTS / 32; i += 256)
         if (sources[i] & targets[i]) bad[1] = 1;
-    if (tid == 0 && all > room) bad[2] = 1;
-    for (uint32_t i = tid; i < min(all, min(room, a.q4_slots)); i += 256)
+    // (the list has q4_slots entries, whatever the count says: every slot that is used below is checked here)
+    const uint32_t there = min(room, a.q4_slots);
+    if (tid == 0 && all > there) bad[2] = 1;
+    for (uint32_t i = tid; i < min(all, there); i += 256)
         if (a.free_slots[i] >= a.q4_slots) bad[4] = 1;
     __syncthreads();
     uint32_t code = 0;

@@ -881,9 +881,10 @@ ctox_status ctox_hip_paged_free_slots_device(ctox_hip_backend *backend, const ct
  * free_slots (taken from the front, in the order of the forks), so that both may go on. A source may
  * be forked more than once. What a target held before is dropped (its slots
  * show as free in the next list). status[0]: 0; 1 a source or target is no request, a target is also a
- * source or another fork's target, or a source is longer than its table; 2 fewer than the slots needed are in
- * *free_count; 3 a part-filled page is not a Q4 page of its place; 4 a free slot is past q4_slots. Then
- * nothing is changed. status[1]: slots taken. forks <= 4096; the rest as ctox_paged_commit. */
+ * source or another fork's target, or a source is longer than its table; 2 more slots are needed than
+ * *free_count or q4_slots; 3 a part-filled page is not a Q4 page of its place; 4 a free slot is past q4_slots. Then
+ * nothing is changed. status[1]: slots taken. free_slots holds min(*free_count, q4_slots) slots that differ from
+ * each other and from those in use. forks <= 4096; the rest as ctox_paged_commit. */
 typedef struct {
     uint8_t *const *q4_pools;    /* HOST [layers], as ctox_paged_commit */
     ctox_paged_kv_descriptor *descriptors;

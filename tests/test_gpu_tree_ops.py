@@ -267,3 +267,14 @@ def test_workspace_is_checked(hip):
                            p.d["tokens"].data_ptr(), q2_slots=0, **p.geometry())
     with pytest.raises(ch.MemoryBudget):
         hip.paged_free_slots_device(op, stream())
+
+
+def test_fork_of_more_pages_than_the_pool_has(hip):
+    """A count of free slots that is larger than the pool does not make room: nothing is changed."""
+    p = Pages(14, [5, 0, 0, 0], [0] * 4, 16, 2, 272, q2=0, spare=1)
+    assert p.n4 == 2
+    p.free(hip)
+    spare = p.lists[0][0]
+    p.fork(hip, [(0, 1), (0, 2), (0, 3)], None, code=2, free=[spare, spare], count=9)
+    p.fork(hip, [(0, 1), (0, 2), (0, 3)], None, code=2, free=[spare, spare], count=NO)
+    p.fork(hip, [(0, 3)], None, free=[spare], count=1)
