@@ -501,12 +501,12 @@ extern "C" __global__ __launch_bounds__(1024) void ctox_tree_walk_gfx950(TreeVer
     __shared__ double sums[16];
     __shared__ uint32_t found;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x;
-    const TreeRows all = tree_rows(a.row_starts, r, a.rows);
-    const TreeRows q{all.row0, min(all.n, (uint32_t)CTOX_TREE_NODES)};
-    if (q.n == 0) {
+    const TreeRows q = tree_rows(a.row_starts, r, a.rows);
+    if (q.n == 0 || q.n > CTOX_TREE_NODES) {  // no nodes, or not a tree of these kernels
+        for (uint32_t i = tid; i < q.n; i += 1024) a.path[q.row0 + i] = CTOX_NO_SLOT;
         if (tid == 0) {
             a.counts[r] = 0;
-            a.next[r] = CTOX_NO_SLOT;
+            a.next[r] = q.n ? CTOX_TREE_FAILED : CTOX_NO_SLOT;
         }
         return;
     }
@@ -564,8 +564,7 @@ extern "C" __global__ __launch_bounds__(1024) void ctox_tree_walk_gfx950(TreeVer
     }
     // (the path rises: a node's place is the number of its nodes in front)
     if (failed) on = 0, count = 0;
-    for (uint32_t i = tid; i < all.n; i += 1024)
-        if (i >= count) a.path[all.row0 + i] = CTOX_NO_SLOT;
+    if (tid >= count && tid < q.n) a.path[q.row0 + tid] = CTOX_NO_SLOT;
     if (tid < 64 && (on >> tid & 1)) a.path[q.row0 + __popcll(on & ((1ull << tid) - 1))] = tid;
     if (tid == 0) a.counts[r] = count;
     if (failed || a.greedy) {

@@ -805,8 +805,8 @@ ctox_status ctox_hip_paged_gqa_tree_device(ctox_hip_backend *backend, const ctox
  * counts[r]: nodes of the path, the root included; path[row_starts[r] + i]: its i-th node,
  * 0xffffffff behind it. A request without rows: counts 0, next 0xffffffff. A token that is not below vocab is
  * never accepted. -inf is a token that is ruled out; where a row on the path (or, with children, its
- * draft row) has a logit that is +inf or no number, or none that is finite, the request fails
- * closed: counts 0, next CTOX_TREE_FAILED. Strides of 0 stand for dense rows. rows <= 65535, vocab < 2^31.
+ * draft row) has a logit that is +inf or no number, or none that is finite, or where it has more than
+ * CTOX_TREE_NODES rows, the request fails closed: counts 0, next CTOX_TREE_FAILED. Strides of 0 stand for dense rows. rows <= 65535, vocab < 2^31.
  * workspace holds ctox_hip_verify_tree_workspace bytes (of the same op; its device pointers are
  * not read, but for draft being NULL or not), 16-byte aligned; one for the most rows, vocab, draft_vocab and
  * max_children serves smaller calls. */

@@ -349,3 +349,14 @@ def test_draw_of_nothing_passes_parts_without_a_weight(hip, drawn, skew):
     assert [p for p, _ in got] == [[0], [0, 1], [0]], got
     # (std 0.05 over T = 0.01 is at most 2^-60 of the largest weight; only r = max(p - q, 0) may leave out more)
     assert got[0][1] == 9000 and got[1][1] == 9000 and 9000 <= got[2][1] < 20000, got
+
+
+@pytest.mark.parametrize("T", [0.0, 1.0])
+def test_more_nodes_than_a_tree_has_fail_closed(hip, T):
+    """65 rows and more are no tree of these calls: nothing of that request is accepted, the others stand."""
+    for n in (65, 70, 200):
+        v = Verify(n, [3, n, 64, 5], 700, 4, T, "without", std=1.5)
+        want = v.expect()
+        want[1] = ([], FAILED)
+        hip.verify_tree_device(v.op(hip), stream())
+        assert v.got() == want
