@@ -71,9 +71,14 @@ __device__ __forceinline__ void gdn_tree(const GdnTreeArgs &a) {
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m = lane & 15;
     const uint32_t groups = (a.value_dim + 16 * W - 1) / (16 * W), head = blockIdx.x / groups, group = blockIdx.x % groups;
     const uint32_t r = blockIdx.y;
-    const TreeRows all = tree_rows(a.row_starts, r, a.rows);
-    const TreeRows q{all.row0, min(all.n, (uint32_t)N)};
+    const TreeRows q = tree_rows(a.row_starts, r, a.rows);
     if (q.n == 0) return;
+    if (q.n > N) {  // not a tree of this kernel
+        for (uint32_t i = wave; i < q.n; i += W)
+            for (uint32_t c = group * 16 * W + lane; c < min((group + 1) * 16 * W, a.value_dim); c += 64)
+                a.out[((size_t)(q.row0 + i) * a.heads + head) * a.value_dim + c] = 0.0f;
+        return;
+    }
     const int nt = (int)(q.n + 15) / 16;  // tiles that have nodes
     const uint32_t dk = a.key_dim, dv = a.value_dim, rep = a.heads / a.key_heads, kh = head / rep, kw = a.key_heads * dk;
     const float *window = a.conv_in + (size_t)r * a.conv_stride;
@@ -451,7 +456,7 @@ extern "C" __global__ __launch_bounds__(256) void ctox_gdn_tree_commit_gfx950(Gd
     const uint32_t tid = threadIdx.x, r = blockIdx.y;
     const uint32_t slices = (a.value_dim + 15) / 16, parts = a.heads * slices;
     const TreeRows all = tree_rows(a.row_starts, r, a.rows);
-    const uint32_t n = min(all.n, (uint32_t)CTOX_TREE_NODES);
+    const uint32_t n = all.n > a.nodes ? 0 : all.n;  // (more: the rows' kernel took it for no tree)
     if (tid < 64) {  // the path as far as it names nodes
         const uint32_t count = a.counts[r];
         const bool mine = tid < n && count <= n && tid < count;

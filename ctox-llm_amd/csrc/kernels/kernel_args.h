@@ -842,6 +842,8 @@ struct GdnTreeArgs {
     uint32_t value_dim;
     uint32_t kernel;
     uint32_t blocked;
+    uint32_t nodes;              // of one request that the rows' kernel takes: 16, 32 or 64
+    uint32_t pad;
 };
 
 // Decode engine helpers (engine_ops.hip).

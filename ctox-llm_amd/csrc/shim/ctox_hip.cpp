@@ -3579,6 +3579,11 @@ ctox_status check_gdn_tree(const ctox_gdn_tree *op) {
 uint64_t gdn_tree_need(const ctox_gdn_tree *op) {
     return (uint64_t)op->rows * 4 * ((uint64_t)op->key_heads * 128 + (uint64_t)op->heads * op->value_dim + op->heads);
 }
+// Tiles of 16 nodes of the rows' kernel: 1, 2 or 4, as 0, 1, 2.
+int gdn_tree_tiles(const ctox_gdn_tree *op) {
+    const uint32_t most = std::min<uint32_t>(op->max_rows ? op->max_rows : CTOX_TREE_NODES, op->rows);
+    return most <= 16 ? 0 : most <= 32 ? 1 : 2;
+}
 GdnTreeArgs gdn_tree_args(const ctox_gdn_tree *op) {
     GdnTreeArgs a{};
     a.proj = op->proj;
@@ -3613,6 +3618,7 @@ GdnTreeArgs gdn_tree_args(const ctox_gdn_tree *op) {
     a.value_dim = op->value_dim;
     a.kernel = op->kernel;
     a.blocked = op->blocked != 0;
+    a.nodes = 16u << gdn_tree_tiles(op);
     return a;
 }
 ctox_status gdn_tree_workspace_ok(const ctox_gdn_tree *op) {
@@ -3642,15 +3648,13 @@ extern "C" ctox_status ctox_hip_gdn_tree_device(ctox_hip_backend *b, const ctox_
     if (ctox_status st = gdn_tree_workspace_ok(op)) return st;
     if (op->rows == 0) return CTOX_OK;
     const GdnTreeArgs a = gdn_tree_args(op);
-    const uint32_t most = std::min<uint32_t>(op->max_rows ? op->max_rows : CTOX_TREE_NODES, op->rows);
     // 128 columns a workgroup where that still leaves the CUs one each: a head's convolution and products of nodes
     // are then made once. (Measured, 16 trees of up to 64 nodes,
     // 48 heads: 109 us, with 64 columns 114; one tree of 12 nodes with 64 columns 13.6.)
-    const int tiles = most <= 16 ? 0 : most <= 32 ? 1 : 2;
     const bool wide = op->value_dim > 64 && (uint64_t)op->heads * op->requests >= (uint64_t)b->cus;
     const uint32_t columns = wide ? 128 : 64;
     OnDevice on(b);
-    return launch(b->gdn_tree[op->kernel > 4][wide][tiles],
+    return launch(b->gdn_tree[op->kernel > 4][wide][gdn_tree_tiles(op)],
                   dim3(op->heads * ((op->value_dim + columns - 1) / columns), op->requests), dim3(wide ? 512 : 256),
                   (hipStream_t)stream, a, "ctox_gdn_tree_gfx950");
 }

@@ -906,7 +906,8 @@ ctox_status ctox_hip_paged_fork_device(ctox_hip_backend *backend, const ctox_pag
  * ctox_hip_gdn_fused_snap_device (rows of proj [q | k | v] at 0, a at a_off, b at b_off; windows
  * [channels][kernel], states [heads][key_dim][value_dim] or blocked), request r's windows at
  * r * conv_stride, its state at r * state_stride floats (0: dense). max_rows bounds the nodes of any one
- * request (0: CTOX_TREE_NODES), no request may have more. key_dim <= 128, kernel <= 8,
+ * request (0: CTOX_TREE_NODES); one with more rows than that, rounded up to 16, 32 or 64, is no tree: its rows of out
+ * are zeros, the second call leaves its windows and state (as counts 0). key_dim <= 128, kernel <= 8,
  * requests <= 4096, rows < 2^24. workspace holds ctox_hip_gdn_tree_workspace bytes, 16-byte aligned, and
  * is in use from the first call to the second: layers of a step need one each. */
 typedef struct {

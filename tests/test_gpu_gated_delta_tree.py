@@ -256,3 +256,36 @@ def test_workspace_is_checked(hip):
     for call in (hip.gdn_tree_device, hip.gdn_tree_commit_device):
         with pytest.raises(ch.MemoryBudget):
             call(op, stream())
+
+
+@pytest.mark.parametrize("max_rows,nodes,over", [(0, [5, 70, 64, 20], [1]), (64, [65, 1], [0]), (16, [16, 17, 3, 40], [1, 3]),
+                                                 (20, [32, 33, 7], [1]), (12, [12, 16, 64], [2])])
+@pytest.mark.parametrize("batch", [False, True])
+def test_more_nodes_than_the_bound(hip, max_rows, nodes, over, batch):
+    """Requests past the bound (rounded up to 16, 32 or 64) are no trees of the call: rows of zeros, windows and
+    states as they were; the others stand."""
+    say("delta", max_rows, nodes, batch)
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    count = -(-cus // (6 * len(nodes))) if batch else 1  # (128 value columns a workgroup from a head a CU on)
+    L = Layer(max_rows + 3, nodes * count, chain=0.5, blocked=batch)
+    over = [r for r in range(len(L.nodes)) if r % len(nodes) in over]
+    for r in over:  # paths that run into the rows past the bound
+        L.kept[r] = max(lines(L.forest[r]), key=lambda x: x[-1])
+    op = L.op(hip, max_rows=max_rows)
+    hip.gdn_tree_device(op, stream())
+    hip.gdn_tree_commit_device(op, stream())
+    out, after, slid = L.expect()
+    got, state = L.d["out"].cpu().numpy(), L.d["state2"].cpu().numpy()
+    before = block(L.state) if L.blocked else L.state
+    after = block(after) if L.blocked else after
+    for r, n in enumerate(L.nodes):
+        a = int(L.starts[r])
+        windows = L.d["win2"].cpu().numpy()[r].reshape(slid[r].shape)
+        if r in over:
+            assert not got[a:a + n].any(), r
+            assert np.array_equal(state[r], before[r].reshape(-1)) and np.array_equal(windows, L.windows[r]), r
+            continue
+        big = max(np.abs(L.state[r]).max() * 4, np.linalg.norm(out[a:a + n], axis=-1).max(), 1.0)
+        assert np.linalg.norm(got[a:a + n] - out[a:a + n], axis=-1).max() <= 512 * E * big, r
+        assert np.abs(state[r] - after[r].reshape(-1)).max() <= 512 * E * max(1.0, np.abs(after[r]).max()), r
+        assert np.array_equal(windows, slid[r].astype(np.float32)), r
