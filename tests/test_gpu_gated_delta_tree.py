@@ -289,3 +289,19 @@ def test_more_nodes_than_the_bound(hip, max_rows, nodes, over, batch):
         assert np.linalg.norm(got[a:a + n] - out[a:a + n], axis=-1).max() <= 512 * E * big, r
         assert np.abs(state[r] - after[r].reshape(-1)).max() <= 512 * E * max(1.0, np.abs(after[r]).max()), r
         assert np.array_equal(windows, slid[r].astype(np.float32)), r
+
+
+@pytest.mark.parametrize("heads,key_heads,dk,dv", [(2, 2, 17, 130), (3, 1, 96, 80), (6, 2, 64, 128), (4, 2, 128, 65)])
+@pytest.mark.parametrize("K", [1, 3, 4, 5, 8])
+@pytest.mark.parametrize("most", [16, 32, 64])
+def test_shapes_of_batches(hip, heads, key_heads, dk, dv, K, most):
+    """Enough heads that a workgroup takes 128 value columns: part-filled groups of them, short keys, all convolutions,
+    both orders of the state."""
+    say("delta", heads, key_heads, dk, dv, K, most)
+    R = -(-torch.cuda.get_device_properties(0).multi_processor_count // heads)
+    assert dv > 64  # (with fewer columns it takes 64 whatever the batch)
+    rng = np.random.default_rng(most + K)
+    nodes = [int(x) for x in rng.integers(0, 12, R)]
+    nodes[0], nodes[R // 2], nodes[-1] = most, most - 1, most // 2 + 1
+    for blocked in (False, True):
+        Layer(dk + K, nodes, heads, key_heads, dk, dv, K, blocked, chain=0.6, pad=1).check(hip, max_rows=most, gap=8 if blocked else 0)
