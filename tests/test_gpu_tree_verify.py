@@ -360,3 +360,23 @@ def test_more_nodes_than_a_tree_has_fail_closed(hip, T):
         want[1] = ([], FAILED)
         hip.verify_tree_device(v.op(hip), stream())
         assert v.got() == want
+
+
+@pytest.mark.parametrize("drawn,vocab,draft_vocab,T,requests,skew,pieces", [
+    ("without", 60000, None, 1.0, 60, 1, 2), ("with", 60001, 20000, 0.8, 70, 0, 2), ("point", 60000, None, 1.0, 110, 3, 2),
+    ("without", 60000, None, 0.0, 110, 2, 2), ("without", 90000, None, 1.2, 60, 0, 3), ("without", 130000, 129999, 1.0, 66, 1, 4)])
+def test_statistics_of_longer_parts(hip, drawn, vocab, draft_vocab, T, requests, skew, pieces):
+    """Rows enough that the first statistics take parts of several times the later rounds' 4096 tokens: roots alone, leaves
+    that are accepted, nodes whose children are refused."""
+    say("parts", drawn, vocab, draft_vocab, T, requests, skew, pieces)
+    nodes = [int(x) for x in np.random.default_rng(requests).integers(0, 13, requests)]
+    nodes[:4] = [1, 12, 1, 12]
+    v = Verify(vocab + pieces, nodes, vocab, 4, T, drawn, draft_vocab, skew=skew)
+    # (what follows restates when the library takes longer parts, so that this test does not lose its subject)
+    chunks, cus = -(-(vocab + 3) // 4096), torch.cuda.get_device_properties(0).multi_processor_count
+    reads = v.M * chunks * (2 if T and drawn != "point" else 1)
+    assert min(4, 1 + reads // (32 * cus)) == pieces
+    want = v.check(hip)
+    ends = [len(parent) > 1 and path[-1] in parent for parent, (path, _) in zip(v.forest, want) if parent]
+    leaves = [len(path) > 1 and path[-1] not in parent for parent, (path, _) in zip(v.forest, want) if parent]
+    assert any(ends) and any(leaves)
