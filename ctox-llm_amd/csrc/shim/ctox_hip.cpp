@@ -3281,7 +3281,7 @@ extern "C" ctox_status ctox_hip_paged_gqa_tree_workspace(const ctox_hip_backend 
 extern "C" ctox_status ctox_hip_paged_gqa_tree_device(ctox_hip_backend *b, const ctox_paged_gqa_tree *op, void *stream) {
     ctox_paged_gqa_rows rows;
     if (ctox_status st = check_gqa_tree(op, &rows)) return st;
-    if (!op->masks) return fail(CTOX_ERR_SHAPE, "null argument");
+    if (rows.rows && !op->masks) return fail(CTOX_ERR_SHAPE, "null argument");
     if (!aligned(op->masks, 8)) return fail(CTOX_ERR_SHAPE, "masks need 8-byte alignment");
     return gqa_rows_impl(b, &rows, op->masks, stream);
 }

@@ -197,3 +197,12 @@ def test_a_hidden_first_node(hip, heads, kv, most, cached):
     # several roots: every other node is one
     parent = [i - 1 if i % 2 else -1 for i in range(most)]
     Trees(cached + 1, requests, 16, heads, kv, masks_=np.concatenate([masks(parent)] * 3)).check(hip, most)
+
+
+def test_no_rows_need_no_buffers(hip):
+    """A step without nodes: addresses of empty buffers are null, as in the ragged batch's call."""
+    b = Trees(15, [(20, 0), (5, 0)], 16, 6, 1)
+    t = b.tree_op(hip)
+    t.rows.rows, t.rows.query, t.rows.out, t.masks = 0, None, None, None
+    t.bind_workspace(None, 0)
+    hip.paged_gqa_tree_device(t, torch.cuda.current_stream().cuda_stream)
