@@ -20,9 +20,9 @@
 //    product with 0 would carry it: such waves take sums over ancestors alone (the second form of the solve).
 //  * ctox_gdn_tree_commit_gfx950: the state and the conv windows behind the path; bound by reading and writing the state.
 //
-// Measured, 48 heads over 16, 128 x 128: a tree of 12 nodes 13.8 us and 4.1 for the commit; 16 trees of up to 64 nodes 110 us
-// (672 workgroups of 8 waves, two a CU: f32 MFMA 21 us, VALU 20, LDS 25 of the CUs' time, in phases between barriers) and
-// 23 us (91 MB of state, 3.9 TB/s).
+// Measured, 48 heads over 16, 128 x 128: a tree of 12 nodes 13.4 us and 4.1 for the commit; 16 trees of up to 64 nodes 106 us
+// (110 in the first launches on an idle card; 672 workgroups of 8 waves, two a CU: f32 MFMA 21 us, VALU 20, LDS 25 of the
+// CUs' time, in phases between barriers) and 23 us (101 MB of states and 5 of windows, read and written: 4.6 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "kernel_args.h"

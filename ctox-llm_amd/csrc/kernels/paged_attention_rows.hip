@@ -40,8 +40,8 @@
 // Measured, 24 query heads over 4 KV heads, pages of 16 tokens, old ones of 2-bit codes: a prompt of 4096 tokens
 // 584 us (206 G score and value operations, each twice for the two parts: 706 TFLOP/s of products, where a large
 // f16 matrix product of the card reaches 1108), 512 rows behind 32768 tokens 1038 us, 32 decoded tokens over up to 8192
-// cached ones 70 us (1.23 TB/s); trees: 4 of 64 nodes behind 32768 tokens 590 us (206 G, 698 TFLOP/s of
-// products), 12 nodes behind 8192 38 us and 6 for the join. Bound by vector operations (about 840 a tile and wave, 56 % of all issue,
+// cached ones 70 us (1.23 TB/s); trees: 4 of 64 nodes behind 32768 tokens 537 us (206 G, 768 TFLOP/s of
+// products; 626 to 696 in the first launches on an idle card), 12 nodes behind 8192 37 us and 6 for the join. Bound by vector operations (about 840 a tile and wave, 56 % of all issue,
 // beside 30 % of the matrix units' time): 352 of them turn codes into f16 operands, 192 split P s_v. All 256 registers
 // are taken; the 7 (128 queries) and 8 (32) spilled ones are read outside the tile loop and in its rare branches.
 // With four subtiles K is stored while V is in use and V while K is, so that one buffer each is

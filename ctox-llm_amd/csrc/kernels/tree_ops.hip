@@ -14,7 +14,8 @@
 //  * ctox_paged_fork_gfx950: a request's table copied to another's place; a last page that is part-filled is copied
 //    to a free slot in all layers. Every workgroup counts for itself how many slots the forks before its own take.
 // All are bound by launch latency and a few dependent loads: plan 3.0 us (512 trees of 64), commit 6.3 (128 requests, 8
-// layers), free slots 7.5, fork 8.0 (32 forks of 8 layers).
+// layers), free slots 7.6 in one launch, 1.7 + 6.6 + 7.2 in three (16 requests of up to 2048 pages), fork 8.0 (32 forks
+// of 8 layers).
 #include <hip/hip_runtime.h>
 
 #include "kernel_args.h"

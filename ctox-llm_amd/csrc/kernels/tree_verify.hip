@@ -28,9 +28,9 @@
 //    the running sum passes the request's number, then that part's tokens.
 //
 // Measured, 151936 tokens, a draft row a node with children: 16 trees of up to 32 nodes (315 rows, 146 with children)
-// 131 us, 51 of it the statistics (177 MB, 3.5 TB/s; 20 operations a logit, the exponential 15: both bound it), the first
-// round 6.7 + 22, three more 10-14 each, the walk 11; a chain of five 23.6 us in three launches; greedy, 8 trees of up
-// to 16 nodes, 17.8 us (47 MB).
+// 130 to 132 us, 48 of it the statistics (177 MB, 3.7 TB/s; 20 operations a logit, the exponential 15: both bound it), the
+// first round 6.7 + 21, three more 10-13 each, the walk 11; a chain of five 23 to 24 us in three launches; greedy, 8 trees of
+// up to 16 nodes, 17.9 us (47 MB).
 #include <hip/hip_runtime.h>
 
 #include "kernel_args.h"
